@@ -42,6 +42,12 @@ from .core import (
     unpack_signed_int4,
 )
 
+# Extensions beyond the reference's names (``__all__`` stays the reference's list).
+from .activation import gelu_tanh_saved8
+from .int8 import Int8Linear, int8_linear, int8_matmul, quantize_int8_weight, quantize_signed_int8_rowwise
+from .norm import layer_norm, modulated_layer_norm
+from .rotary import axial_rotary
+
 __version__ = "0.1.0"
 
 __all__ = [

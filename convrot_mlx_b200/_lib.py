@@ -48,6 +48,16 @@ SIGNATURES: dict[str, tuple] = {
     "convrot_peer_barrier": (_I, [ctypes.POINTER(_P), _I, _I, ctypes.c_uint32, _P]),
     "convrot_copy_2d": (_I, [_P, _I64, _P, _I64, _I64, _I64, _P]),
     "convrot_w4a4_linear_static": (_I, [_P, _I, _I, _P, _I, _P, _P, _P, _I, _I64, _I64, _I64, _P]),
+    "convrot_quantize_i8": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _P, _P]),
+    "convrot_i8_gemm": (_I, [_P, _I64, _P, _I64, _I, _P, _P, _P, _P, _I, _I64, _I64, _I64, _P]),
+    "convrot_axial_rotary": (_I, [_I, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _I64, _I, _P,
+                                  ctypes.c_double, _I, _I, _P]),
+    "convrot_layer_norm": (_I, [_P, _I, _I64, _I64, _P, _P, _I, _I64, _I64, _I, ctypes.c_float, _P, _P, _P, _P]),
+    "convrot_layer_norm_workspace": (_I64, [_I64, _I64, _I64]),
+    "convrot_layer_norm_backward": (_I, [_P, _P, _I, _I64, _I64, _P, _I, _I64, _I64, _I, _P, _P, _P, _P, _P, _P, _I64,
+                                         _P]),
+    "convrot_gelu_saved8": (_I, [_P, _I, _I64, _I64, _P, _P, _P, _P]),
+    "convrot_gelu_saved8_backward": (_I, [_P, _I, _I64, _I64, _P, _P, _P, _P]),
     "convrot_set_gemm_route": (_I, [_I]),
     "convrot_take_device_error": (_I, [ctypes.POINTER(_I)]),
 }
@@ -99,6 +109,19 @@ def stream_of(t: torch.Tensor):
 
 def ptr(t: torch.Tensor | None):
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
+
+
+def call(name: str, on: torch.Tensor, *args) -> None:
+    """Call entry point ``name`` with ``args`` and the current stream of ``on``'s device, with that device current."""
+
+    fn = getattr(load(), name)
+    index = on.device.index
+    if index == torch.cuda.current_device():
+        status = fn(*args, stream_of(on))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, stream_of(on))
+    check(status, name)
 
 
 def take_device_error() -> int:

@@ -19,6 +19,7 @@ import torch
 from torch import nn
 
 from .core import CONVROT_GROUP_SIZE, ConvRotLinear, eligible_linear, quantize_convrot_weight, repack_nk_weight_for_mpp
+from .int8 import Int8Linear
 
 
 def _set_module(root: nn.Module, name: str, module: nn.Module) -> None:
@@ -50,3 +51,14 @@ def replace_convrot_linears(model: nn.Module, *, backend: str = "mpp-w4a4", prep
         _set_module(model, name, layer)
         names.append(name)
     return names
+
+
+def replace_int8_linears(model: nn.Module, *, keep=()) -> list[str]:
+    """Replace every ``nn.Linear`` in ``model`` but those named in ``keep`` by its frozen 8-bit form
+    (``Int8Linear.from_linear``); returns the replaced names in module order."""
+
+    targets = [(name, m) for name, m in model.named_modules()
+               if name and name not in keep and isinstance(m, nn.Linear)]
+    for name, linear in targets:
+        _set_module(model, name, Int8Linear.from_linear(linear))
+    return [name for name, _ in targets]

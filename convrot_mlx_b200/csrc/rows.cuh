@@ -1,0 +1,57 @@
+// Helpers shared by the row-wise 8-bit and training kernels (int8_quant.cu,
+// layer_norm.cu, gelu_saved8.cu): typed loads, reductions, and the 8-bit
+// quantizer's arithmetic.
+#pragma once
+
+#include "common.cuh"
+
+namespace convrot {
+
+// Bits of |v|: as unsigned integers they order like the values, infinity
+// above every finite value and NaN above infinity, so one integer maximum
+// finds a row's largest magnitude and whether the row holds anything that is
+// not finite (fmaxf would drop NaN).
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+__device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+
+// Symmetric 8-bit quantizer of values whose largest magnitude is `top`:
+//   code = rne(127 x / top) in [-127, 127], scale = top / 127.
+// x and top are first scaled by the power of two that brings top near 1, so
+// that 127 x cannot overflow; q = p r then misses p / top by at most two
+// ulps, and one step of residual correction, q += (p - q top) r with the
+// residual exact in one FMA, makes it the correctly rounded quotient.  Ties
+// (x = top / 2 gives 63.5 exactly) therefore round as in exact arithmetic.
+// Adding 1.5 * 2^23 rounds to the integer (nearest even) in the low bits.
+// top = 0: codes 0 and scale 0.  top infinite or NaN: codes 0, scale NaN.
+struct Quant8 {
+  float k127, top, r;
+  __device__ __forceinline__ explicit Quant8(uint32_t top_bits) {
+    const bool live = top_bits != 0 && top_bits < kInfBits;
+    int e = static_cast<int>(top_bits >> 23) - 127;
+    e = e < -100 ? -100 : (e > 126 ? 126 : e);
+    const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);  // 2^-e
+    k127 = live ? 127.0f * f : 0.0f;
+    top = live ? __uint_as_float(top_bits) * f : 1.0f;
+    r = __frcp_rn(top);
+  }
+  // low byte of the result: the code in two's complement
+  __device__ __forceinline__ uint32_t code(float x) const {
+    const float p = __fmul_rn(x, k127);
+    const float q = __fmul_rn(p, r);
+    const float c = __fmaf_rn(__fmaf_rn(-q, top, p), r, q);
+    return __float_as_uint(__fadd_rn(c, 12582912.0f));
+  }
+  static __device__ __forceinline__ float scale(uint32_t top_bits) {
+    return top_bits < kInfBits ? __fdiv_rn(__uint_as_float(top_bits), 127.0f) : __uint_as_float(0x7FC00000u);
+  }
+};
+
+}  // namespace convrot

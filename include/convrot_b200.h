@@ -283,6 +283,94 @@ int convrot_set_gemm_route(int route);
  */
 int convrot_take_device_error(int* code);
 
+/*
+ * 8-bit row quantizer: for each row, top = max |v|, scale = top / 127 and
+ * codes rne(127 v / top) in [-127, 127], with v = x, or the float32 product
+ * x[r, c] * col_scale[c] when col_scale is not NULL (the gradient of the
+ * 8-bit linear folds its weight scales in).  A zero row has codes 0 and scale
+ * 0; a row that holds an infinity or a NaN has codes 0 and scale NaN, so that
+ * what is computed from it is NaN.  Row r of x starts at r * x_stride
+ * elements, of the codes at r * q_stride bytes.  No reference counterpart
+ * (the 4-bit form is convrot_prepare_packed with group_size 1).
+ */
+int convrot_quantize_i8(const void* x, int dtype, int64_t rows, int64_t features, int64_t x_stride,
+                        const float* col_scale, int8_t* q, int64_t q_stride, float* scales, void* stream);
+
+/*
+ * 8-bit linear: out[i, j] = T(fl(fl(fl(dot[i, j]) * xscales[i]) * wscales[j])
+ * + bias[j]) with dot[i, j] = sum over k of act[i, k] w[j, k], exact in int32
+ * (k <= 131072; tcgen05 kind::i8).  act: (m, k) int8 codes, row i at
+ * i * act_stride bytes.  weight: int8, layout CONVROT_LAYOUT_NK = (n, k) rows
+ * or CONVROT_LAYOUT_KN = (k, n) rows (the same matrix contracted over its
+ * rows: the gradient of the input), row r at r * weight_stride bytes.
+ * Strides are multiples of 16 and cover the rows.  wscales and bias may be
+ * NULL (ones, zeros).  Codes are in [-127, 127].  No reference counterpart.
+ */
+int convrot_i8_gemm(const int8_t* act, int64_t act_stride, const int8_t* weight, int64_t weight_stride, int layout,
+                    const float* xscales, const float* wscales, const float* bias, void* out, int out_dtype,
+                    int64_t m, int64_t n, int64_t k, void* stream);
+
+/*
+ * Rotary positions with several axes for queries and keys, in one launch.
+ * Tensors are (batch, heads, tokens, dim) with element strides {batch, head,
+ * token} and unit stride along dim (dim <= 256); k_heads (or q_heads) may be
+ * 0.  The first sum(widths) values of a head are pairs, adjacent
+ * (interleaved) or sum(widths) / 2 apart; pair j of axis a turns by
+ * positions[token, a] * theta^(-2 j / widths[a]); the rest is copied.
+ * inverse turns back: the gradient of the input from that of the output.
+ * positions: (tokens, axes) float32, that of sample b at b *
+ * position_batch_stride elements (0: shared).  widths: host array, positive
+ * and even.  Outputs may not overlap inputs, except that each may be exactly
+ * its own input.  No reference counterpart.
+ */
+int convrot_axial_rotary(int dtype, int64_t batch, int64_t tokens, int64_t dim, const void* q, int64_t q_heads,
+                         const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, const void* k,
+                         int64_t k_heads, const int64_t* k_strides, void* k_out, const int64_t* k_out_strides,
+                         const float* positions, int64_t position_batch_stride, int axes, const int32_t* widths,
+                         double theta, int interleaved, int inverse, void* stream);
+
+/*
+ * Layer norm of the rows of x (rows, features), packed:
+ * y = (x - mean) * rsqrt(var + eps) * w + bias in float32, one rounding; w =
+ * weight, or 1 + weight with add_one.  Rows r with the same r /
+ * rows_per_weight share a weight and a bias vector, at weight_stride elements
+ * from one another: all rows (affine norm), or those of a sample (modulated
+ * norm).  weight_dtype: that of x, or CONVROT_F32.  weight and bias may be
+ * NULL (w = 1, bias 0).  mean and rstd: (rows,) float32 for the backward
+ * pass, or both NULL.  No reference counterpart.
+ */
+int convrot_layer_norm(const void* x, int dtype, int64_t rows, int64_t features, const void* weight,
+                       const void* bias, int weight_dtype, int64_t rows_per_weight, int64_t weight_stride,
+                       int add_one, float eps, void* y, float* mean, float* rstd, void* stream);
+
+/*
+ * Gradients of convrot_layer_norm: dx (rows, features) of x's dtype, and the
+ * sums over the rows that share a weight, dweight = sum dy h and dbias = sum
+ * dy with h the normalized row, (rows / rows_per_weight, features) packed, of
+ * weight_dtype, either NULL when not wanted.  Sums are float32, in an order
+ * fixed by the shape.  mean, rstd: from the forward pass.  workspace:
+ * convrot_layer_norm_workspace bytes, 16-byte aligned (not used when neither
+ * sum is wanted).  With 0 rows nothing is written.
+ */
+int64_t convrot_layer_norm_workspace(int64_t rows, int64_t features, int64_t rows_per_weight);
+int convrot_layer_norm_backward(const void* x, const void* dy, int dtype, int64_t rows, int64_t features,
+                                const void* weight, int weight_dtype, int64_t rows_per_weight,
+                                int64_t weight_stride, int add_one, const float* mean, const float* rstd, void* dx,
+                                void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Tanh GELU whose input is saved in 8 bits for the backward pass.  Forward:
+ * y = gelu_tanh(x) (rows, features), and the codes (rows, features) int8 with
+ * scales (rows, ceil(features / 128)) float32 of x in groups of 128 features,
+ * as convrot_quantize_i8 forms them; codes and scales may both be NULL (no
+ * backward pass wanted).  Backward: dx = dy * gelu_tanh'(codes * scale).  All
+ * packed; y, dy and dx have x's dtype.  No reference counterpart.
+ */
+int convrot_gelu_saved8(const void* x, int dtype, int64_t rows, int64_t features, void* y, int8_t* codes,
+                        float* scales, void* stream);
+int convrot_gelu_saved8_backward(const void* dy, int dtype, int64_t rows, int64_t features, const int8_t* codes,
+                                 const float* scales, void* dx, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
