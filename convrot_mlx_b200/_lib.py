@@ -50,6 +50,7 @@ SIGNATURES: dict[str, tuple] = {
     "convrot_w4a4_linear_static": (_I, [_P, _I, _I, _P, _I, _P, _P, _P, _I, _I64, _I64, _I64, _P]),
     "convrot_quantize_i8": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _P, _P]),
     "convrot_i8_gemm": (_I, [_P, _I64, _P, _I64, _I, _P, _P, _P, _P, _I, _I64, _I64, _I64, _P]),
+    "convrot_i8_linear": (_I, [_P, _I, _I64, _P, _P, _I64, _I, _P, _P, _P, _I, _I64, _I64, _I64, _P, _I64, _P, _P]),
     "convrot_axial_rotary": (_I, [_I, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _I64, _I, _P,
                                   ctypes.c_double, _I, _I, _P]),
     "convrot_layer_norm": (_I, [_P, _I, _I64, _I64, _P, _P, _I, _I64, _I64, _I, ctypes.c_float, _P, _P, _P, _P]),

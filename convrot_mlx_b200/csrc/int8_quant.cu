@@ -3,49 +3,159 @@
 // column (the gradient of the 8-bit linear folds the weight scales in).
 //
 // Memory-bound: a row is read once from HBM and its codes are written once.
+// One CTA for each row, which stays in registers between the maximum and the
+// codes; wide loads where address and pitch allow, else one element a lane
+// (consecutive lanes on consecutive elements).  Rows that do not fit the
+// registers are read a second time, through L2.
 #include "rows.cuh"
 
 namespace convrot {
 namespace {
 
-template <typename T>
-__device__ __forceinline__ float scaled(const T* x, const float* col_scale, int64_t c) {
-  const float v = Elem<T>::to_f(x[c]);
-  return col_scale ? __fmul_rn(v, col_scale[c]) : v;
+constexpr int kThreads = 256;
+
+struct QuantParams {
+  const void* x;
+  const float* col_scale;
+  int8_t* q;
+  float* scales;
+  int64_t rows, features, x_stride, q_stride;
+};
+
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
+  v = warp_max(v);
+  if (blockDim.x > 32) {
+    __syncthreads();  // red may still be read by the previous row
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = (threadIdx.x & 31) < (blockDim.x >> 5) ? red[threadIdx.x & 31] : 0u;
+    v = warp_max(v);
+  }
+  return v;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) quantize_i8_kernel(const T* __restrict__ x, int64_t rows, int64_t features,
-                                                          int64_t x_stride, const float* __restrict__ col_scale,
-                                                          int8_t* __restrict__ q, int64_t q_stride,
-                                                          float* __restrict__ scales) {
-  __shared__ uint32_t red[8];
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T* xr = x + row * x_stride;
-    uint32_t top = 0;
-    for (int64_t c = threadIdx.x; c < features; c += 256) top = max(top, abs_bits(scaled(xr, col_scale, c)));
-    top = warp_max(top);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
-    __syncthreads();
-    top = red[0];
+// VEC consecutive elements at column c as float32; columns past the end read 0.
+template <typename T, int VEC>
+__device__ __forceinline__ void load(const QuantParams& p, int64_t row, int64_t c, float (&v)[VEC]) {
+  const T* src = static_cast<const T*>(p.x) + row * p.x_stride + c;
+  if (c + VEC <= p.features) {
+    load_vec<T, VEC>(src, v);
+  } else {
 #pragma unroll
-    for (int w = 1; w < 8; ++w) top = max(top, red[w]);
-    const Quant8 quant(top);
-    if (threadIdx.x == 0) scales[row] = Quant8::scale(top);
-    for (int64_t c = threadIdx.x; c < features; c += 256)
-      q[row * q_stride + c] = top < kInfBits ? static_cast<int8_t>(quant.code(scaled(xr, col_scale, c))) : 0;
+    for (int i = 0; i < VEC; ++i) v[i] = c + i < p.features ? Elem<T>::to_f(src[i]) : 0.0f;
+  }
+  if (p.col_scale) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = c + i < p.features ? __fmul_rn(v[i], __ldg(p.col_scale + c + i)) : 0.0f;
   }
 }
 
-template <typename T>
-int launch(const void* x, int64_t rows, int64_t features, int64_t x_stride, const float* col_scale, int8_t* q,
-           int64_t q_stride, float* scales, cudaStream_t stream) {
-  const int64_t ctas = 8LL * device_sm_count();
-  const int64_t grid = rows < ctas ? rows : ctas;
-  quantize_i8_kernel<T><<<static_cast<unsigned>(grid), 256, 0, stream>>>(static_cast<const T*>(x), rows, features,
-                                                                        x_stride, col_scale, q, q_stride, scales);
+template <int VEC>
+__device__ __forceinline__ void store(const QuantParams& p, int64_t row, int64_t c, const Quant8& quant,
+                                      const float (&v)[VEC]) {
+  int8_t* dst = p.q + row * p.q_stride + c;
+  uint32_t code[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) code[i] = quant.code(v[i]);
+  if constexpr (VEC % 4 == 0) {
+    if (c + VEC <= p.features) {
+      store_codes<VEC>(dst, code, quant.mask);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+    if (c + i < p.features) dst[i] = static_cast<int8_t>(code[i] & quant.mask);
+}
+
+// NV vectors of VEC elements a thread in registers; NV = 0: any length, in
+// two passes over the row.
+template <typename T, int VEC, int NV>
+__global__ void __launch_bounds__(kThreads) quantize_i8_kernel(const QuantParams p) {
+  __shared__ uint32_t red[kThreads / 32];
+  grid_dependency_wait();  // x may come from the previous kernel of the stream
+  grid_dependents_launch();
+  const int step = blockDim.x * VEC;
+  const int64_t c0 = static_cast<int64_t>(threadIdx.x) * VEC;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    uint32_t top = 0;
+    if constexpr (NV > 0) {
+      float v[NV][VEC];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int64_t c = c0 + static_cast<int64_t>(j) * step;
+        if (c < p.features) {
+          load<T, VEC>(p, row, c, v[j]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[j][i] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) top = max(top, abs_bits(v[j][i]));
+      top = block_max(top, red);
+      const Quant8 quant(top);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int64_t c = c0 + static_cast<int64_t>(j) * step;
+        if (c < p.features) store<VEC>(p, row, c, quant, v[j]);
+      }
+    } else {
+      for (int64_t c = c0; c < p.features; c += step) {
+        float v[VEC];
+        load<T, VEC>(p, row, c, v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) top = max(top, abs_bits(v[i]));
+      }
+      top = block_max(top, red);
+      const Quant8 quant(top);
+      for (int64_t c = c0; c < p.features; c += step) {
+        float v[VEC];
+        load<T, VEC>(p, row, c, v);
+        store<VEC>(p, row, c, quant, v);
+      }
+    }
+    if (threadIdx.x == 0) p.scales[row] = Quant8::scale(top);
+  }
+}
+
+template <typename T, int VEC, int NV>
+int launch_nv(const QuantParams& p, int threads, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.rows < (1LL << 30) ? p.rows : (1LL << 30)), 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CONVROT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, quantize_i8_kernel<T, VEC, NV>, p));
   return check_launch("convrot_quantize_i8");
+}
+
+template <typename T, int VEC>
+int launch_vec(const QuantParams& p, cudaStream_t stream) {
+  // as many threads as give each one vector, at most 256; then more vectors
+  const int64_t vectors = (p.features + VEC - 1) / VEC;
+  const int threads = vectors >= kThreads ? kThreads : static_cast<int>((vectors + 31) / 32 * 32);
+  const int64_t nv = (vectors + threads - 1) / threads;
+  constexpr int kScale = VEC == 1 ? 4 : 1;  // registers hold 32 or 64 elements a thread
+  if (nv <= 1 * kScale) return launch_nv<T, VEC, 1 * kScale>(p, threads, stream);
+  if (nv <= 2 * kScale) return launch_nv<T, VEC, 2 * kScale>(p, threads, stream);
+  if (nv <= 4 * kScale) return launch_nv<T, VEC, 4 * kScale>(p, threads, stream);
+  if (nv <= 8 * kScale) return launch_nv<T, VEC, 8 * kScale>(p, threads, stream);
+  return launch_nv<T, VEC, 0>(p, threads, stream);
+}
+
+template <typename T>
+int launch(const QuantParams& p, cudaStream_t stream) {
+  constexpr int kWide = 16 / sizeof(T);
+  const bool wide = aligned_to(p.x, 16) && p.x_stride * static_cast<int64_t>(sizeof(T)) % 16 == 0 &&
+                    aligned_to(p.q, 8) && p.q_stride % 8 == 0;
+  return wide ? launch_vec<T, kWide>(p, stream) : launch_vec<T, 1>(p, stream);
 }
 
 }  // namespace
@@ -64,11 +174,12 @@ int convrot_quantize_i8(const void* x, int dtype, int64_t rows, int64_t features
                   static_cast<long long>(q_stride));
   if (rows == 0) return CONVROT_OK;
   CONVROT_REQUIRE(x && q && scales, CONVROT_ERR_INVALID, "null pointer");
+  const QuantParams p{x, col_scale, q, scales, rows, features, x_stride, q_stride};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case CONVROT_BF16: return launch<__nv_bfloat16>(x, rows, features, x_stride, col_scale, q, q_stride, scales, s);
-    case CONVROT_F16: return launch<__half>(x, rows, features, x_stride, col_scale, q, q_stride, scales, s);
-    default: return launch<float>(x, rows, features, x_stride, col_scale, q, q_stride, scales, s);
+    case CONVROT_BF16: return launch<__nv_bfloat16>(p, s);
+    case CONVROT_F16: return launch<__half>(p, s);
+    default: return launch<float>(p, s);
   }
 }
 

@@ -22,6 +22,54 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// VEC packed elements of T to float32.
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const uint32_t* w, float (&v)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      v[i] = __uint_as_float(w[i]);
+    } else {
+      const typename Elem<T>::Pair h = *reinterpret_cast<const typename Elem<T>::Pair*>(&w[i / 2]);
+      v[i] = Elem<T>::to_f(i % 2 ? Elem<T>::hi(h) : Elem<T>::lo(h));
+    }
+  }
+}
+
+// VEC consecutive elements as float32, in one load of up to 16 bytes (the
+// address is a multiple of its size).
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* src, float (&v)[VEC]) {
+  constexpr int kBytes = VEC * sizeof(T);
+  if constexpr (kBytes == 16 || kBytes == 8) {
+    uint32_t w[kBytes / 4];
+    if constexpr (kBytes == 16) {
+      const uint4 r = *reinterpret_cast<const uint4*>(src);
+      w[0] = r.x, w[1] = r.y, w[2] = r.z, w[3] = r.w;
+    } else {
+      const uint2 r = *reinterpret_cast<const uint2*>(src);
+      w[0] = r.x, w[1] = r.y;
+    }
+    unpack<T, VEC>(w, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = Elem<T>::to_f(src[i]);
+  }
+}
+
+// The low bytes of VEC words as VEC consecutive bytes under `mask` (VEC 4 or
+// 8, address a multiple of VEC).
+template <int VEC>
+__device__ __forceinline__ void store_codes(int8_t* dst, const uint32_t (&code)[VEC], uint32_t mask) {
+  uint32_t w[VEC / 4];
+#pragma unroll
+  for (int i = 0; i < VEC / 4; ++i)
+    w[i] = __byte_perm(__byte_perm(code[4 * i], code[4 * i + 1], 0x0040),
+                       __byte_perm(code[4 * i + 2], code[4 * i + 3], 0x0040), 0x5410) & mask;
+  if constexpr (VEC == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(dst) = w[0];
+}
+
 // Symmetric 8-bit quantizer of values whose largest magnitude is `top`:
 //   code = rne(127 x / top) in [-127, 127], scale = top / 127.
 // x and top are first scaled by the power of two that brings top near 1, so
@@ -30,14 +78,17 @@ __device__ __forceinline__ float warp_sum(float v) {
 // residual exact in one FMA, makes it the correctly rounded quotient.  Ties
 // (x = top / 2 gives 63.5 exactly) therefore round as in exact arithmetic.
 // Adding 1.5 * 2^23 rounds to the integer (nearest even) in the low bits.
-// top = 0: codes 0 and scale 0.  top infinite or NaN: codes 0, scale NaN.
+// top = 0: codes 0 and scale 0.  top infinite or NaN: codes 0 (their bits may
+// be those of a NaN: `mask` clears them), scale NaN.
 struct Quant8 {
   float k127, top, r;
+  uint32_t mask;
   __device__ __forceinline__ explicit Quant8(uint32_t top_bits) {
     const bool live = top_bits != 0 && top_bits < kInfBits;
     int e = static_cast<int>(top_bits >> 23) - 127;
     e = e < -100 ? -100 : (e > 126 ? 126 : e);
     const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);  // 2^-e
+    mask = live ? 0xFFFFFFFFu : 0u;
     k127 = live ? 127.0f * f : 0.0f;
     top = live ? __uint_as_float(top_bits) * f : 1.0f;
     r = __frcp_rn(top);

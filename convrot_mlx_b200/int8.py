@@ -113,26 +113,40 @@ def int8_matmul(codes, qweight, xscales, wscales, bias=None, *, output_dtype) ->
                  None if bias is None else _f32_vec(bias), output_dtype, n)
 
 
+def _product(x2, col_scale, qweight, layout, wscales, bias, n) -> torch.Tensor:
+    """The quantizer and the product in one call; x2 as ``_rows`` gives it."""
+
+    m, k = x2.shape
+    pitch = -(-k // _PITCH) * _PITCH
+    out = torch.empty((m, n), dtype=x2.dtype, device=x2.device)
+    codes = torch.empty((m, pitch), dtype=torch.int8, device=x2.device)
+    scales = torch.empty((m,), dtype=torch.float32, device=x2.device)
+    dtype = _dtype_code(x2.dtype)
+    _lib.call("convrot_i8_linear", x2, _lib.ptr(x2), dtype, x2.stride(0), _lib.ptr(col_scale), _lib.ptr(qweight),
+              qweight.stride(0), layout, _lib.ptr(wscales), _lib.ptr(bias), _lib.ptr(out), dtype, m, n, k,
+              _lib.ptr(codes), pitch, _lib.ptr(scales))
+    return out
+
+
 def _forward(x, qweight, wscales, bias):
-    codes, xscales = _quantize(_rows(x))
-    out = _gemm(codes, qweight, _lib.LAYOUT_NK, xscales, wscales, bias, x.dtype, qweight.shape[0])
-    return out.reshape(*x.shape[:-1], qweight.shape[0])
+    n = qweight.shape[0]
+    out = _product(_rows(x), None, qweight, _lib.LAYOUT_NK, wscales, bias, n)
+    return out.view(*x.shape[:-1], n)
 
 
 class _Int8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, qweight, wscales, bias):
         ctx.save_for_backward(qweight, wscales)
-        ctx.lead = x.shape
         return _forward(x, qweight, wscales, bias)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         qweight, wscales = ctx.saved_tensors
-        codes, scales = _quantize(_rows(dy), wscales)
-        dx = _gemm(codes, qweight, _lib.LAYOUT_KN, scales, None, None, dy.dtype, qweight.shape[1])
-        return dx.reshape(ctx.lead), None, None, None
+        k = qweight.shape[1]
+        dx = _product(_rows(dy), wscales, qweight, _lib.LAYOUT_KN, None, None, k)
+        return dx.view(*dy.shape[:-1], k), None, None, None
 
 
 def int8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor,

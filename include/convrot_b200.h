@@ -279,7 +279,10 @@ int convrot_set_gemm_route(int route);
  * 41 staged prep row copy; 51-57 swap-AB small-m GEMM (51 packed-weight
  * slot free, 52 activation stage landed, 53 expanded weights ready, 54
  * packed weights landed, 55 expanded-weight slot free, 56 final MMA drain,
- * 57 activation slot free).
+ * 57 activation slot free); 61-65 8-bit pair GEMM (61 copy slot free, 62
+ * accumulator buffer free, 63 stage landed, 64 final MMA drain, 65
+ * accumulator ready); 71-74 8-bit swap GEMM (71 copy slot free, 72 weight
+ * stage landed, 73 activation stage landed, 74 final MMA drain).
  */
 int convrot_take_device_error(int* code);
 
@@ -309,6 +312,18 @@ int convrot_quantize_i8(const void* x, int dtype, int64_t rows, int64_t features
 int convrot_i8_gemm(const int8_t* act, int64_t act_stride, const int8_t* weight, int64_t weight_stride, int layout,
                     const float* xscales, const float* wscales, const float* bias, void* out, int out_dtype,
                     int64_t m, int64_t n, int64_t k, void* stream);
+
+/*
+ * convrot_quantize_i8 of x into `codes` (m, k) and `scales` (m,), then
+ * convrot_i8_gemm of them, in one call: the 8-bit linear (layout NK), or with
+ * col_scale and layout KN the gradient of its input.  The product starts
+ * reading the weight while the quantizer runs: `codes` and `scales` may not
+ * overlap the weight.
+ */
+int convrot_i8_linear(const void* x, int x_dtype, int64_t x_stride, const float* col_scale, const int8_t* weight,
+                      int64_t weight_stride, int layout, const float* wscales, const float* bias, void* out,
+                      int out_dtype, int64_t m, int64_t n, int64_t k, int8_t* codes, int64_t codes_stride,
+                      float* scales, void* stream);
 
 /*
  * Rotary positions with several axes for queries and keys, in one launch.

@@ -87,7 +87,9 @@ def _linear64(x, qweight, wscales, bias):
 
 SIZES = [(1, 1, 1), (1, 4096, 4096), (2, 33, 17), (5, 512, 640), (8, 1000, 264), (16, 2048, 96), (17, 129, 257),
          (64, 3000, 200), (65, 160, 1211), (127, 128, 128), (128, 256, 256), (129, 144, 259), (333, 1997, 1211),
-         (257, 4160, 520), (600, 96, 2050), (1100, 1536, 1024)]
+         (257, 4160, 520), (600, 96, 2050), (1100, 1536, 1024),
+         (1300, 300, 2100), (1300, 2103, 333), (300, 1997, 5001), (300, 5008, 1040), (2500, 130, 1000), (2500, 1000, 129),
+         (4000, 1216, 1216)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -48,6 +48,16 @@ def test_gemm_arguments(lib):
     assert run(m=0) == 0
 
 
+def test_linear_arguments(lib):
+    def run(dtype=2, m=4, k=16, codes=FAKE, pitch=16, x=FAKE, stride=16):
+        return lib.convrot_i8_linear(x, dtype, stride, None, FAKE, 16, 0, FAKE, None, FAKE, dtype, m, 8, k, codes,
+                                     pitch, FAKE, None)
+
+    assert run(dtype=3) == -1 and run(pitch=24) == -1 and run(codes=None) == -1
+    assert run(x=None) == -1 and run(stride=8) == -1 and run(k=131073) == -2
+    assert run(m=0) == 0
+
+
 def test_rotary_arguments(lib):
     strides = (ctypes.c_int64 * 3)(0, 0, 0)
 
