@@ -51,7 +51,7 @@ SIGNATURES: dict[str, tuple] = {
     "convrot_quantize_i8": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _P, _P]),
     "convrot_i8_gemm": (_I, [_P, _I64, _P, _I64, _I, _P, _P, _P, _P, _I, _I64, _I64, _I64, _P]),
     "convrot_i8_linear": (_I, [_P, _I, _I64, _P, _P, _I64, _I, _P, _P, _P, _I, _I64, _I64, _I64, _P, _I64, _P, _P]),
-    "convrot_axial_rotary": (_I, [_I, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _I64, _I, _P,
+    "convrot_axial_rotary": (_I, [_I, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _P, _P, _I64, _I, _P,
                                   ctypes.c_double, _I, _I, _P]),
     "convrot_layer_norm": (_I, [_P, _I, _I64, _I64, _P, _P, _I, _I64, _I64, _I, ctypes.c_float, _P, _P, _P, _P]),
     "convrot_layer_norm_workspace": (_I64, [_I64, _I64, _I64]),
@@ -112,17 +112,23 @@ def ptr(t: torch.Tensor | None):
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 
 
-def call(name: str, on: torch.Tensor, *args) -> None:
-    """Call entry point ``name`` with ``args`` and the current stream of ``on``'s device, with that device current."""
+# The raw handle of a device's current stream, without a Stream object around it where torch offers that.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-    fn = getattr(load(), name)
-    index = on.device.index
+
+def call(name: str, index: int, *args) -> None:
+    """Call entry point ``name`` with ``args`` and the current stream of CUDA device ``index``, with that device
+    current.  Pointers are plain addresses (``Tensor.data_ptr()``) or None."""
+
+    fn = getattr(_lib or load(), name)
     if index == torch.cuda.current_device():
-        status = fn(*args, stream_of(on))
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            status = fn(*args, stream_of(on))
-    check(status, name)
+            status = fn(*args, _raw_stream(index))
+    if status:
+        check(status, name)
 
 
 def take_device_error() -> int:

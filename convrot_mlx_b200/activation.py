@@ -14,13 +14,13 @@ SAVED_GROUP = 128  # features of a row that share one scale
 def _forward(x, save: bool):
     features = x.shape[-1]
     rows = x.numel() // features
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x)
     codes = scales = None
     if save:
         codes = torch.empty((rows, features), dtype=torch.int8, device=x.device)
         scales = torch.empty((rows, -(-features // SAVED_GROUP)), dtype=torch.float32, device=x.device)
-    _lib.call("convrot_gelu_saved8", x, _lib.ptr(x), _dtype_code(x.dtype), rows, features, _lib.ptr(y),
-              _lib.ptr(codes), _lib.ptr(scales))
+    _lib.call("convrot_gelu_saved8", x.get_device(), x.data_ptr(), _dtype_code(x.dtype), rows, features, y.data_ptr(),
+              codes.data_ptr() if save else None, scales.data_ptr() if save else None)
     return y, codes, scales
 
 
@@ -37,8 +37,8 @@ class _GeluSaved8(torch.autograd.Function):
         codes, scales = ctx.saved_tensors
         dy = dy.contiguous()
         dx = torch.empty_like(dy)
-        _lib.call("convrot_gelu_saved8_backward", dy, _lib.ptr(dy), _dtype_code(dy.dtype), codes.shape[0],
-                  codes.shape[1], _lib.ptr(codes), _lib.ptr(scales), _lib.ptr(dx))
+        _lib.call("convrot_gelu_saved8_backward", dy.get_device(), dy.data_ptr(), _dtype_code(dy.dtype), codes.shape[0],
+                  codes.shape[1], codes.data_ptr(), scales.data_ptr(), dx.data_ptr())
         return dx
 
 

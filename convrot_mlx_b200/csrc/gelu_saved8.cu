@@ -7,8 +7,8 @@
 // u), and with x^ the restored input
 //   dx = dy (s + x^ s (1 - s) 2 c (1 + 3 * 0.044715 x^2)).
 //
-// Memory-bound: forward e + e + 1 + 4 / 128 bytes an element, backward the
-// same, for e bytes in the type of x.
+// Memory-bound: forward 2 e + 1 + 4 / 128 bytes an element, backward the same,
+// for e bytes in the type of x.
 #include "rows.cuh"
 
 namespace convrot {
@@ -26,78 +26,216 @@ __device__ __forceinline__ float gate(float x, float x2) {
   return __fdividef(1.0f, 1.0f + __expf(-kC2 * x * (1.0f + kA * x2)));
 }
 
-// One warp for each group of 128 features of a row.
-template <typename T>
-__global__ void __launch_bounds__(256) gelu_fwd_kernel(const T* __restrict__ x, int64_t rows, int64_t features,
-                                                       T* __restrict__ y, int8_t* __restrict__ codes,
-                                                       float* __restrict__ scales) {
-  const int lane = threadIdx.x & 31;
-  const int64_t groups = (features + kGroup - 1) / kGroup;
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < rows * groups; i += warps) {
-    const int64_t row = i / groups, c0 = i % groups * kGroup;
-    float v[4];
+// A group is spread over LANES lanes, NV vectors of VEC elements each; a CTA
+// of 256 threads takes kUnroll groups for each of its 256 / LANES lane sets,
+// all loaded before the first is used.
+template <int VEC>
+struct Spread {
+  static constexpr int kLanes = kGroup / VEC < 32 ? kGroup / VEC : 32;
+  static constexpr int kVectors = kGroup / (VEC * kLanes);
+  static constexpr int kSets = 256 / kLanes;
+};
+constexpr int kUnroll = 4;
+
+struct GeluParams {
+  const void* in;  // x, or dy
+  void* out;       // y, or dx
+  int8_t* codes;
+  float* scales;
+  uint32_t total, groups;  // groups of all rows, and of a row
+  int64_t features;
+};
+
+// Element offset of a group's first value and its length.
+__device__ __forceinline__ void locate(const GeluParams& p, uint32_t group, int64_t& base, int& length) {
+  if (p.features % kGroup == 0) {  // groups follow one another in memory
+    base = static_cast<int64_t>(group) * kGroup;
+    length = kGroup;
+  } else {
+    const uint32_t row = group / p.groups, g = group - row * p.groups;
+    base = static_cast<int64_t>(row) * p.features + static_cast<int64_t>(g) * kGroup;
+    const int64_t left = p.features - static_cast<int64_t>(g) * kGroup;
+    length = left < kGroup ? static_cast<int>(left) : kGroup;
+  }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) gelu_fwd_kernel(const GeluParams p) {
+  using S = Spread<VEC>;
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const int lane = threadIdx.x % S::kLanes;
+  const uint32_t first = blockIdx.x * (S::kSets * kUnroll) + threadIdx.x / S::kLanes;
+  const T* x = static_cast<const T*>(p.in);
+  Pack<T, VEC> raw[kUnroll][S::kVectors];
+  int64_t base[kUnroll];
+  int length[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const uint32_t group = first + u * S::kSets;
+    length[u] = 0;
+    if (group < p.total) locate(p, group, base[u], length[u]);
+#pragma unroll
+    for (int j = 0; j < S::kVectors; ++j) {
+      const int c = (lane + j * S::kLanes) * VEC;
+      if (c < length[u]) raw[u][j].load(x + base[u] + c);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    float v[S::kVectors][VEC];
     uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t c = c0 + lane + 32 * j;
-      v[j] = c < features ? Elem<T>::to_f(x[row * features + c]) : 0.0f;
-      top = max(top, abs_bits(v[j]));
-    }
-    top = warp_max(top);
-    const Quant8 quant(top);
-    if (lane == 0 && scales) scales[i] = Quant8::scale(top);
+    for (int j = 0; j < S::kVectors; ++j) {
+      const int c = (lane + j * S::kLanes) * VEC;
+      if (c < length[u]) {
+        raw[u][j].get(v[j]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t c = c0 + lane + 32 * j;
-      if (c >= features) break;
-      y[row * features + c] = Elem<T>::from_f(v[j] * gate(v[j], square(v[j])));
-      if (codes) codes[row * features + c] = top < kInfBits ? static_cast<int8_t>(quant.code(v[j])) : 0;
+        for (int i = 0; i < VEC; ++i) top = max(top, abs_bits(v[j][i]));
+      }
+    }
+    if constexpr (S::kLanes == 32) {
+      top = warp_max(top);
+    } else {
+#pragma unroll
+      for (int o = S::kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    }
+    const Quant8 quant(top);
+    if (lane == 0 && length[u] > 0 && p.scales) p.scales[first + u * S::kSets] = Quant8::scale(top);
+#pragma unroll
+    for (int j = 0; j < S::kVectors; ++j) {
+      const int c = (lane + j * S::kLanes) * VEC;
+      if (c < length[u]) {
+        float y[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) y[i] = v[j][i] * gate(v[j][i], square(v[j][i]));
+        Pack<T, VEC> out;
+        out.set(y);
+        out.store(static_cast<T*>(p.out) + base[u] + c);
+        if (p.codes) {
+          uint32_t code[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) code[i] = quant.code(v[j][i]);
+          store_codes<VEC>(p.codes + base[u] + c, code, quant.mask);
+        }
+      }
     }
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) gelu_bwd_kernel(const T* __restrict__ dy, int64_t rows, int64_t features,
-                                                       const int8_t* __restrict__ codes,
-                                                       const float* __restrict__ scales, T* __restrict__ dx) {
-  const int64_t groups = (features + kGroup - 1) / kGroup;
-  const int64_t total = rows * features;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    const float x = static_cast<float>(codes[i]) * scales[i / features * groups + i % features / kGroup];
-    const float x2 = square(x), s = gate(x, x2);
-    const float slope = s + x * s * (1.0f - s) * kC2 * (1.0f + 3.0f * kA * x2);
-    dx[i] = Elem<T>::from_f(Elem<T>::to_f(dy[i]) * slope);
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) gelu_bwd_kernel(const GeluParams p) {
+  using S = Spread<VEC>;
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const int lane = threadIdx.x % S::kLanes;
+  const uint32_t first = blockIdx.x * (S::kSets * kUnroll) + threadIdx.x / S::kLanes;
+  const T* dy = static_cast<const T*>(p.in);
+  Pack<T, VEC> raw[kUnroll][S::kVectors];
+  Pack<uint8_t, VEC> codes[kUnroll][S::kVectors];
+  float scale[kUnroll];
+  int64_t base[kUnroll];
+  int length[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const uint32_t group = first + u * S::kSets;
+    length[u] = 0;
+    scale[u] = 0.0f;
+    if (group < p.total) {
+      locate(p, group, base[u], length[u]);
+      scale[u] = __ldg(p.scales + group);
+    }
+#pragma unroll
+    for (int j = 0; j < S::kVectors; ++j) {
+      const int c = (lane + j * S::kLanes) * VEC;
+      if (c < length[u]) {
+        raw[u][j].load(dy + base[u] + c);
+        codes[u][j].load(reinterpret_cast<const uint8_t*>(p.codes) + base[u] + c);
+      }
+    }
   }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+    for (int j = 0; j < S::kVectors; ++j) {
+      const int c = (lane + j * S::kLanes) * VEC;
+      if (c < length[u]) {
+        float d[VEC];
+        raw[u][j].get(d);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float x = signed_byte(codes[u][j].w[i / 4], i % 4) * scale[u];
+          const float x2 = square(x), s = gate(x, x2);
+          d[i] *= s + x * s * (1.0f - s) * kC2 * (1.0f + 3.0f * kA * x2);
+        }
+        Pack<T, VEC> out;
+        out.set(d);
+        out.store(static_cast<T*>(p.out) + base[u] + c);
+      }
+    }
 }
 
 int check_shape(int dtype, int64_t rows, int64_t features) {
   CONVROT_REQUIRE(valid_dtype(dtype), CONVROT_ERR_INVALID, "unknown dtype %d", dtype);
   CONVROT_REQUIRE(rows >= 0 && features > 0, CONVROT_ERR_INVALID, "invalid shape (%lld, %lld)",
                   static_cast<long long>(rows), static_cast<long long>(features));
+  CONVROT_REQUIRE(features <= (1LL << 31) && rows <= (1LL << 31) / ((features + kGroup - 1) / kGroup),
+                  CONVROT_ERR_UNSUPPORTED, "more than 2^31 groups of %d", kGroup);
   return CONVROT_OK;
 }
 
-unsigned grid_of(int64_t items) {
-  const int64_t most = 8LL * device_sm_count();
-  return static_cast<unsigned>(items < most ? items : most);
+template <int VEC>
+int enqueue(void (*kernel)(GeluParams), const GeluParams& p, const char* what, cudaStream_t s) {
+  constexpr uint32_t kPerCta = Spread<VEC>::kSets * kUnroll;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((p.total + kPerCta - 1) / kPerCta, 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CONVROT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
+  return check_launch(what);
+}
+
+// Elements of a vector: 16 bytes' worth, or the most for which every row's
+// start is aligned in all three arrays.
+template <typename T>
+int vector_of(const GeluParams& p) {
+  for (int vec = 16 / sizeof(T); vec > 1; vec /= 2)
+    if (p.features % vec == 0 && aligned_to(p.in, vec * sizeof(T)) && aligned_to(p.out, vec * sizeof(T)) &&
+        aligned_to(p.codes, vec))
+      return vec;
+  return 1;
 }
 
 template <typename T>
-int forward(const void* x, int64_t rows, int64_t features, void* y, int8_t* codes, float* scales, cudaStream_t s) {
-  const int64_t groups = rows * ((features + kGroup - 1) / kGroup);
-  gelu_fwd_kernel<T><<<grid_of((groups + 7) / 8), 256, 0, s>>>(static_cast<const T*>(x), rows, features,
-                                                              static_cast<T*>(y), codes, scales);
-  return check_launch("convrot_gelu_saved8");
+int forward(const GeluParams& p, cudaStream_t s) {
+  const char* what = "convrot_gelu_saved8";
+  const int vec = vector_of<T>(p);
+  if constexpr (sizeof(T) == 2)
+    if (vec == 8) return enqueue<8>(gelu_fwd_kernel<T, 8>, p, what, s);
+  if (vec == 4) return enqueue<4>(gelu_fwd_kernel<T, 4>, p, what, s);
+  if (vec == 2) return enqueue<2>(gelu_fwd_kernel<T, 2>, p, what, s);
+  return enqueue<1>(gelu_fwd_kernel<T, 1>, p, what, s);
 }
 
 template <typename T>
-int backward(const void* dy, int64_t rows, int64_t features, const int8_t* codes, const float* scales, void* dx,
-             cudaStream_t s) {
-  gelu_bwd_kernel<T><<<grid_of((rows * features + 255) / 256), 256, 0, s>>>(
-      static_cast<const T*>(dy), rows, features, codes, scales, static_cast<T*>(dx));
-  return check_launch("convrot_gelu_saved8_backward");
+int backward(const GeluParams& p, cudaStream_t s) {
+  const char* what = "convrot_gelu_saved8_backward";
+  const int vec = vector_of<T>(p);
+  if constexpr (sizeof(T) == 2)
+    if (vec == 8) return enqueue<8>(gelu_bwd_kernel<T, 8>, p, what, s);
+  if (vec == 4) return enqueue<4>(gelu_bwd_kernel<T, 4>, p, what, s);
+  if (vec == 2) return enqueue<2>(gelu_bwd_kernel<T, 2>, p, what, s);
+  return enqueue<1>(gelu_bwd_kernel<T, 1>, p, what, s);
+}
+
+GeluParams params(const void* in, void* out, int8_t* codes, float* scales, int64_t rows, int64_t features) {
+  const int64_t groups = (features + kGroup - 1) / kGroup;
+  return {in, out, codes, scales, static_cast<uint32_t>(rows * groups), static_cast<uint32_t>(groups), features};
 }
 
 }  // namespace
@@ -111,11 +249,12 @@ int convrot_gelu_saved8(const void* x, int dtype, int64_t rows, int64_t features
   const int rc = check_shape(dtype, rows, features);
   if (rc != CONVROT_OK || rows == 0) return rc;
   CONVROT_REQUIRE(x && y && (codes != nullptr) == (scales != nullptr), CONVROT_ERR_INVALID, "null pointer");
+  const GeluParams p = params(x, y, codes, scales, rows, features);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case CONVROT_BF16: return forward<__nv_bfloat16>(x, rows, features, y, codes, scales, s);
-    case CONVROT_F16: return forward<__half>(x, rows, features, y, codes, scales, s);
-    default: return forward<float>(x, rows, features, y, codes, scales, s);
+    case CONVROT_BF16: return forward<__nv_bfloat16>(p, s);
+    case CONVROT_F16: return forward<__half>(p, s);
+    default: return forward<float>(p, s);
   }
 }
 
@@ -125,11 +264,13 @@ int convrot_gelu_saved8_backward(const void* dy, int dtype, int64_t rows, int64_
   const int rc = check_shape(dtype, rows, features);
   if (rc != CONVROT_OK || rows == 0) return rc;
   CONVROT_REQUIRE(dy && dx && codes && scales, CONVROT_ERR_INVALID, "null pointer");
+  const GeluParams p =
+      params(dy, dx, const_cast<int8_t*>(codes), const_cast<float*>(scales), rows, features);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case CONVROT_BF16: return backward<__nv_bfloat16>(dy, rows, features, codes, scales, dx, s);
-    case CONVROT_F16: return backward<__half>(dy, rows, features, codes, scales, dx, s);
-    default: return backward<float>(dy, rows, features, codes, scales, dx, s);
+    case CONVROT_BF16: return backward<__nv_bfloat16>(p, s);
+    case CONVROT_F16: return backward<__half>(p, s);
+    default: return backward<float>(p, s);
   }
 }
 

@@ -94,16 +94,6 @@ __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorM
       : "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (sizeof(T) == 4) {
-    return 0;
-  } else {
-    const typename Elem<T>::Pair h = Elem<T>::make(Elem<T>::from_f(a), Elem<T>::from_f(b));
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-
 // ===========================================================================
 // Pair kernel.  Each CTA of a pair holds 128 tokens and 128 channels of the
 // 256 x 256 tile:
@@ -291,12 +281,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int q = 0; q < 4; ++q) {
             const uint32_t at = sb + lane * 64 + (((q + (lane >> 1)) & 3) << 4);
             const int o = part * kCols + q * (kCols / 4);
-            if constexpr (sizeof(TOut) == 2)
-              sts128(at, pack2<TOut>(v[o], v[o + 1]), pack2<TOut>(v[o + 2], v[o + 3]), pack2<TOut>(v[o + 4], v[o + 5]),
-                     pack2<TOut>(v[o + 6], v[o + 7]));
-            else
-              sts128(at, __float_as_uint(v[o]), __float_as_uint(v[o + 1]), __float_as_uint(v[o + 2]),
-                     __float_as_uint(v[o + 3]));
+            float piece[kCols / 4];
+#pragma unroll
+            for (int e = 0; e < kCols / 4; ++e) piece[e] = v[o + e];
+            Pack<TOut, kCols / 4> pk;
+            pk.set(piece);
+            sts128(at, pk.w[0], pk.w[1], pk.w[2], pk.w[3]);
           }
           __syncwarp();
           const int col = col0 + c * 32 + part * kCols;

@@ -12,14 +12,16 @@
 namespace convrot {
 namespace {
 
-constexpr int kThreads = 256;
+// Most threads of a CTA: more for single elements, which are narrow loads.
+template <int VEC> constexpr int kThreads = VEC == 1 ? 1024 : 512;
 
 struct QuantParams {
   const void* x;
   const float* col_scale;
   int8_t* q;
   float* scales;
-  int64_t rows, features, x_stride, q_stride;
+  int64_t rows, x_stride, q_stride;
+  int features;
 };
 
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
@@ -36,10 +38,12 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
 
 // VEC consecutive elements at column c as float32; columns past the end read 0.
 template <typename T, int VEC>
-__device__ __forceinline__ void load(const QuantParams& p, int64_t row, int64_t c, float (&v)[VEC]) {
+__device__ __forceinline__ void load(const QuantParams& p, int64_t row, int c, float (&v)[VEC]) {
   const T* src = static_cast<const T*>(p.x) + row * p.x_stride + c;
   if (c + VEC <= p.features) {
-    load_vec<T, VEC>(src, v);
+    Pack<T, VEC> pk;
+    pk.load(src);
+    pk.get(v);
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) v[i] = c + i < p.features ? Elem<T>::to_f(src[i]) : 0.0f;
@@ -51,7 +55,7 @@ __device__ __forceinline__ void load(const QuantParams& p, int64_t row, int64_t 
 }
 
 template <int VEC>
-__device__ __forceinline__ void store(const QuantParams& p, int64_t row, int64_t c, const Quant8& quant,
+__device__ __forceinline__ void store(const QuantParams& p, int64_t row, int c, const Quant8& quant,
                                       const float (&v)[VEC]) {
   int8_t* dst = p.q + row * p.q_stride + c;
   uint32_t code[VEC];
@@ -71,19 +75,19 @@ __device__ __forceinline__ void store(const QuantParams& p, int64_t row, int64_t
 // NV vectors of VEC elements a thread in registers; NV = 0: any length, in
 // two passes over the row.
 template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(kThreads) quantize_i8_kernel(const QuantParams p) {
-  __shared__ uint32_t red[kThreads / 32];
+__global__ void __launch_bounds__(kThreads<VEC>) quantize_i8_kernel(const QuantParams p) {
+  __shared__ uint32_t red[32];
   grid_dependency_wait();  // x may come from the previous kernel of the stream
   grid_dependents_launch();
   const int step = blockDim.x * VEC;
-  const int64_t c0 = static_cast<int64_t>(threadIdx.x) * VEC;
+  const int c0 = threadIdx.x * VEC;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     uint32_t top = 0;
     if constexpr (NV > 0) {
       float v[NV][VEC];
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int64_t c = c0 + static_cast<int64_t>(j) * step;
+        const int c = c0 + j * step;
         if (c < p.features) {
           load<T, VEC>(p, row, c, v[j]);
         } else {
@@ -99,11 +103,11 @@ __global__ void __launch_bounds__(kThreads) quantize_i8_kernel(const QuantParams
       const Quant8 quant(top);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int64_t c = c0 + static_cast<int64_t>(j) * step;
+        const int c = c0 + j * step;
         if (c < p.features) store<VEC>(p, row, c, quant, v[j]);
       }
     } else {
-      for (int64_t c = c0; c < p.features; c += step) {
+      for (int c = c0; c < p.features; c += step) {
         float v[VEC];
         load<T, VEC>(p, row, c, v);
 #pragma unroll
@@ -111,7 +115,7 @@ __global__ void __launch_bounds__(kThreads) quantize_i8_kernel(const QuantParams
       }
       top = block_max(top, red);
       const Quant8 quant(top);
-      for (int64_t c = c0; c < p.features; c += step) {
+      for (int c = c0; c < p.features; c += step) {
         float v[VEC];
         load<T, VEC>(p, row, c, v);
         store<VEC>(p, row, c, quant, v);
@@ -138,16 +142,17 @@ int launch_nv(const QuantParams& p, int threads, cudaStream_t stream) {
 
 template <typename T, int VEC>
 int launch_vec(const QuantParams& p, cudaStream_t stream) {
-  // as many threads as give each one vector, at most 256; then more vectors
-  const int64_t vectors = (p.features + VEC - 1) / VEC;
-  const int threads = vectors >= kThreads ? kThreads : static_cast<int>((vectors + 31) / 32 * 32);
-  const int64_t nv = (vectors + threads - 1) / threads;
-  constexpr int kScale = VEC == 1 ? 4 : 1;  // registers hold 32 or 64 elements a thread
-  if (nv <= 1 * kScale) return launch_nv<T, VEC, 1 * kScale>(p, threads, stream);
-  if (nv <= 2 * kScale) return launch_nv<T, VEC, 2 * kScale>(p, threads, stream);
-  if (nv <= 4 * kScale) return launch_nv<T, VEC, 4 * kScale>(p, threads, stream);
-  if (nv <= 8 * kScale) return launch_nv<T, VEC, 8 * kScale>(p, threads, stream);
-  return launch_nv<T, VEC, 0>(p, threads, stream);
+  // two vectors (four single elements) a thread, more where the CTA is full
+  constexpr int kLeast = VEC == 1 ? 4 : 2;
+  const int vectors = (p.features + VEC - 1) / VEC;
+  int nv = kLeast;
+  while (nv < 4 * kLeast && vectors > nv * kThreads<VEC>) nv *= 2;
+  const int64_t per = (vectors + nv - 1) / nv;
+  if (per > kThreads<VEC>) return launch_nv<T, VEC, 0>(p, kThreads<VEC>, stream);
+  const int threads = static_cast<int>((per + 31) / 32 * 32);
+  if (nv == kLeast) return launch_nv<T, VEC, kLeast>(p, threads, stream);
+  if (nv == 2 * kLeast) return launch_nv<T, VEC, 2 * kLeast>(p, threads, stream);
+  return launch_nv<T, VEC, 4 * kLeast>(p, threads, stream);
 }
 
 template <typename T>
@@ -169,12 +174,13 @@ int convrot_quantize_i8(const void* x, int dtype, int64_t rows, int64_t features
   CONVROT_REQUIRE(valid_dtype(dtype), CONVROT_ERR_INVALID, "unknown dtype %d", dtype);
   CONVROT_REQUIRE(rows >= 0 && features > 0, CONVROT_ERR_INVALID, "invalid shape (%lld, %lld)",
                   static_cast<long long>(rows), static_cast<long long>(features));
+  CONVROT_REQUIRE(features <= (1 << 30), CONVROT_ERR_UNSUPPORTED, "too many features");
   CONVROT_REQUIRE(x_stride >= features && q_stride >= features, CONVROT_ERR_INVALID,
                   "row strides must cover the features (%lld, %lld)", static_cast<long long>(x_stride),
                   static_cast<long long>(q_stride));
   if (rows == 0) return CONVROT_OK;
   CONVROT_REQUIRE(x && q && scales, CONVROT_ERR_INVALID, "null pointer");
-  const QuantParams p{x, col_scale, q, scales, rows, features, x_stride, q_stride};
+  const QuantParams p{x, col_scale, q, scales, rows, x_stride, q_stride, static_cast<int>(features)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case CONVROT_BF16: return launch<__nv_bfloat16>(p, s);

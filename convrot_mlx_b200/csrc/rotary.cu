@@ -35,50 +35,173 @@ struct RotaryParams {
   int64_t pos_b;
   int64_t tokens;
   int batch, dim, pairs, axes, adjacent;
+  int units;   // threads that a head's values are spread over
   float sign;  // 1, or -1 for the gradient
   double turns[kMaxPairs];  // frequency of each pair in turns a position
   uint8_t axis[kMaxPairs];
 };
 
-// One thread for each pair (or pair of copied values) of a head.
-template <typename T>
-__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  const int half = (p.dim + 1) / 2;
-  const int heads = p.t[0].heads + p.t[1].heads;
-  const int64_t total = static_cast<int64_t>(p.batch) * p.tokens * heads * half;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int j = static_cast<int>(i % half);
-    int h = static_cast<int>(i / half % heads);
-    const int64_t bt = i / half / heads, token = bt % p.tokens, b = bt / p.tokens;
-    const int which = h >= p.t[0].heads;
-    h -= which ? p.t[0].heads : 0;
-    const RotaryTensor& t = p.t[which];
-    const T* in = static_cast<const T*>(t.in) + b * t.in_b + h * t.in_h + token * t.in_t;
-    T* out = static_cast<T*>(t.out) + b * t.out_b + h * t.out_h + token * t.out_t;
-    if (j < p.pairs) {
-      const double turn = static_cast<double>(p.positions[b * p.pos_b + token * p.axes + p.axis[j]]) * p.turns[j];
-      float s, c;
-      sincospif(2.0f * static_cast<float>(turn - rint(turn)), &s, &c);
-      s *= p.sign;
-      const int i0 = p.adjacent ? 2 * j : j, i1 = p.adjacent ? 2 * j + 1 : j + p.pairs;
-      const float x0 = Elem<T>::to_f(in[i0]), x1 = Elem<T>::to_f(in[i1]);
-      out[i0] = Elem<T>::from_f(x0 * c - x1 * s);
-      out[i1] = Elem<T>::from_f(x0 * s + x1 * c);
+// One thread keeps the sines and cosines of its pairs of one token and applies
+// them to the same place of every head of its share of the heads, kUnroll
+// heads in flight.  Units of a head, adjacent pairs: unit u is the VEC values
+// from VEC u on (values past the pairs are copied).  Pairs half apart: unit u
+// is the VEC values from VEC u on and the VEC from pairs + VEC u on; further
+// units copy VEC values each.  WIDE: VEC values move in one access; else one
+// value an access.
+constexpr int kUnroll = 4;
+
+template <typename T, int VEC, bool WIDE>
+struct Unit {
+  float v[VEC];
+  __device__ __forceinline__ void load(const T* src, int left) {
+    if constexpr (WIDE) {
+      Pack<T, VEC> pk;
+      pk.load(src);
+      pk.get(v);
     } else {
-      out[2 * j] = in[2 * j];
-      if (2 * j + 1 < p.dim) out[2 * j + 1] = in[2 * j + 1];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = i < left ? Elem<T>::to_f(src[i]) : 0.0f;
+    }
+  }
+  __device__ __forceinline__ void store(T* dst, int left) const {
+    if constexpr (WIDE) {
+      Pack<T, VEC> pk;
+      pk.set(v);
+      pk.store(dst);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (i < left) dst[i] = Elem<T>::from_f(v[i]);
+    }
+  }
+};
+
+template <typename T, int VEC, bool WIDE, bool ADJACENT>
+__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  constexpr int NP = ADJACENT ? VEC / 2 : VEC;  // pairs of a unit
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t bt = id / p.units;
+  if (bt >= p.batch * p.tokens) return;
+  const int u = static_cast<int>(id - bt * p.units);
+  const int64_t b = bt / p.tokens, token = bt - b * p.tokens;
+  const int turning = ADJACENT ? p.units : p.pairs / VEC;  // units that turn
+  const bool turns = u < turning;
+  const int e0 = ADJACENT || turns ? u * VEC : 2 * p.pairs + (u - turning) * VEC;  // first value of the unit
+  const int left = p.dim - e0;
+
+  float cs[NP], sn[NP];
+  if (turns) {
+    const float* pos = p.positions + b * p.pos_b + token * p.axes;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int j = u * NP + i;
+      cs[i] = 1.0f;
+      sn[i] = 0.0f;
+      if (j < p.pairs) {
+        const double turn = static_cast<double>(__ldg(pos + p.axis[j])) * p.turns[j];
+        sincospif(2.0f * static_cast<float>(turn - rint(turn)), &sn[i], &cs[i]);
+        sn[i] *= p.sign;
+      }
+    }
+  }
+  const int heads = p.t[0].heads + p.t[1].heads;
+  const int h0 = static_cast<int>(static_cast<int64_t>(heads) * blockIdx.y / gridDim.y);
+  const int h1 = static_cast<int>(static_cast<int64_t>(heads) * (blockIdx.y + 1) / gridDim.y);
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const RotaryTensor& t = p.t[which];
+    const int lo = which ? p.t[0].heads : 0, hi = min(h1, lo + t.heads);
+    const T* in = static_cast<const T*>(t.in) + b * t.in_b + token * t.in_t + e0;
+    T* out = static_cast<T*>(t.out) + b * t.out_b + token * t.out_t + e0;
+#pragma unroll 1
+    for (int h = max(h0, lo); h < hi; h += kUnroll) {
+      Unit<T, VEC, WIDE> x[kUnroll], y[ADJACENT ? 1 : kUnroll];
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k)
+        if (h + k < hi) {
+          const T* src = in + (h + k - lo) * t.in_h;
+          x[k].load(src, left);
+          if constexpr (!ADJACENT)
+            if (turns) y[k].load(src + p.pairs, VEC);
+        }
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k)
+        if (h + k < hi) {
+          T* dst = out + (h + k - lo) * t.out_h;
+          if constexpr (ADJACENT) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+              if (u * NP + i < p.pairs) {
+                const float x0 = x[k].v[2 * i], x1 = x[k].v[2 * i + 1];
+                x[k].v[2 * i] = x0 * cs[i] - x1 * sn[i];
+                x[k].v[2 * i + 1] = x0 * sn[i] + x1 * cs[i];
+              }
+          } else if (turns) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+              const float x0 = x[k].v[i], x1 = y[k].v[i];
+              x[k].v[i] = x0 * cs[i] - x1 * sn[i];
+              y[k].v[i] = x0 * sn[i] + x1 * cs[i];
+            }
+            y[k].store(dst + p.pairs, VEC);
+          }
+          x[k].store(dst, left);
+        }
     }
   }
 }
 
-template <typename T>
-int launch(const RotaryParams& p, cudaStream_t stream) {
-  const int64_t total =
-      static_cast<int64_t>(p.batch) * p.tokens * (p.t[0].heads + p.t[1].heads) * ((p.dim + 1) / 2);
-  const int64_t blocks = (total + 255) / 256, most = 16LL * device_sm_count();
-  rotary_kernel<T><<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, stream>>>(p);
+template <typename T, int VEC, bool WIDE, bool ADJACENT>
+int launch(RotaryParams& p, cudaStream_t stream) {
+  p.units = ADJACENT ? (p.dim + VEC - 1) / VEC : p.pairs / VEC + (p.dim - 2 * p.pairs + VEC - 1) / VEC;
+  const int64_t blocks = (static_cast<int64_t>(p.batch) * p.tokens * p.units + 255) / 256;
+  CONVROT_REQUIRE(blocks < (1LL << 31), CONVROT_ERR_UNSUPPORTED, "shape too large");
+  // Few tokens: the heads are shared out until there are about 4 CTAs for
+  // each SM, each with kUnroll heads at least.
+  const int heads = p.t[0].heads + p.t[1].heads;
+  int64_t shares = (4LL * device_sm_count() + blocks - 1) / blocks;
+  const int most = (heads + kUnroll - 1) / kUnroll;
+  if (shares > most) shares = most;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(shares), 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CONVROT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, rotary_kernel<T, VEC, WIDE, ADJACENT>, p));
   return check_launch("convrot_axial_rotary");
+}
+
+// Whether every vector of `vec` values is aligned: addresses, strides, and
+// for pairs half apart the second half's start and the copied tail's.
+template <typename T>
+bool aligned_for(const RotaryParams& p, int vec) {
+  if (p.dim % vec || (!p.adjacent && p.pairs % vec)) return false;
+  const int64_t bytes = vec * static_cast<int64_t>(sizeof(T));
+  for (const RotaryTensor& t : p.t) {
+    if (t.heads == 0) continue;
+    const int64_t strides = t.in_b | t.in_h | t.in_t | t.out_b | t.out_h | t.out_t;
+    if (strides % vec || !aligned_to(t.in, bytes) || !aligned_to(t.out, bytes)) return false;
+  }
+  return true;
+}
+
+template <typename T>
+int launch_type(RotaryParams& p, cudaStream_t s) {
+  constexpr int W = 16 / sizeof(T);
+  if (p.adjacent) {
+    if (aligned_for<T>(p, W)) return launch<T, W, true, true>(p, s);
+    if (aligned_for<T>(p, 2)) return launch<T, 2, true, true>(p, s);
+    return launch<T, 2, false, true>(p, s);
+  }
+  if (aligned_for<T>(p, W)) return launch<T, W, true, false>(p, s);
+  if (aligned_for<T>(p, 2)) return launch<T, 2, true, false>(p, s);
+  return launch<T, 1, false, false>(p, s);
 }
 
 }  // namespace
@@ -86,9 +209,8 @@ int launch(const RotaryParams& p, cudaStream_t stream) {
 
 extern "C" {
 
-int convrot_axial_rotary(int dtype, int64_t batch, int64_t tokens, int64_t dim, const void* q, int64_t q_heads,
-                         const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, const void* k,
-                         int64_t k_heads, const int64_t* k_strides, void* k_out, const int64_t* k_out_strides,
+int convrot_axial_rotary(int dtype, int64_t batch, int64_t tokens, int64_t dim, const void* q, void* q_out,
+                         int64_t q_heads, const void* k, void* k_out, int64_t k_heads, const int64_t* strides,
                          const float* positions, int64_t position_batch_stride, int axes, const int32_t* widths,
                          double theta, int interleaved, int inverse, void* stream) {
   using namespace convrot;
@@ -107,21 +229,22 @@ int convrot_axial_rotary(int dtype, int64_t batch, int64_t tokens, int64_t dim, 
     CONVROT_REQUIRE(widths[a] > 0 && widths[a] % 2 == 0 && 2 * pairs + widths[a] <= dim, CONVROT_ERR_INVALID,
                     "axis widths must be positive, even and sum to at most the head dimension %lld",
                     static_cast<long long>(dim));
-    for (int j = 0; j < widths[a] / 2; ++j, ++pairs) {
-      p.turns[pairs] = std::exp2(-2.0 * j / widths[a] * std::log2(theta)) * 0.15915494309189533577;  // 1 / (2 pi)
+    const double ratio = std::pow(theta, -2.0 / widths[a]);
+    double turns = 0.15915494309189533577;  // 1 / (2 pi): pair 0 turns by one radian a position
+    for (int j = 0; j < widths[a] / 2; ++j, ++pairs, turns *= ratio) {
+      p.turns[pairs] = turns;
       p.axis[pairs] = static_cast<uint8_t>(a);
     }
   }
   if (batch == 0 || tokens == 0 || q_heads + k_heads == 0) return CONVROT_OK;
-  CONVROT_REQUIRE(positions != nullptr && (q_heads == 0 || (q && q_out && q_strides && q_out_strides)) &&
-                      (k_heads == 0 || (k && k_out && k_strides && k_out_strides)),
+  CONVROT_REQUIRE(positions && strides && (q_heads == 0 || (q && q_out)) && (k_heads == 0 || (k && k_out)),
                   CONVROT_ERR_INVALID, "null pointer");
   if (q_heads > 0)
-    p.t[0] = RotaryTensor{q,           q_out, q_strides[0], q_strides[1], q_strides[2], q_out_strides[0], q_out_strides[1],
-                          q_out_strides[2], static_cast<int>(q_heads)};
+    p.t[0] = RotaryTensor{q,          q_out,      strides[0], strides[1], strides[2], strides[3], strides[4],
+                          strides[5], static_cast<int>(q_heads)};
   if (k_heads > 0)
-    p.t[1] = RotaryTensor{k,           k_out, k_strides[0], k_strides[1], k_strides[2], k_out_strides[0], k_out_strides[1],
-                          k_out_strides[2], static_cast<int>(k_heads)};
+    p.t[1] = RotaryTensor{k,           k_out,       strides[6], strides[7], strides[8], strides[9], strides[10],
+                          strides[11], static_cast<int>(k_heads)};
   p.positions = positions;
   p.pos_b = position_batch_stride;
   p.tokens = tokens;
@@ -133,9 +256,9 @@ int convrot_axial_rotary(int dtype, int64_t batch, int64_t tokens, int64_t dim, 
   p.sign = inverse ? -1.0f : 1.0f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case CONVROT_BF16: return launch<__nv_bfloat16>(p, s);
-    case CONVROT_F16: return launch<__half>(p, s);
-    default: return launch<float>(p, s);
+    case CONVROT_BF16: return launch_type<__nv_bfloat16>(p, s);
+    case CONVROT_F16: return launch_type<__half>(p, s);
+    default: return launch_type<float>(p, s);
   }
 }
 

@@ -22,6 +22,14 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// Two float32 values rounded to a pair of a 16-bit type, in one conversion.
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::Pair pair_of(float a, float b);
+template <>
+__device__ __forceinline__ __nv_bfloat162 pair_of<__nv_bfloat16>(float a, float b) { return __floats2bfloat162_rn(a, b); }
+template <>
+__device__ __forceinline__ __half2 pair_of<__half>(float a, float b) { return __floats2half2_rn(a, b); }
+
 // VEC packed elements of T to float32.
 template <typename T, int VEC>
 __device__ __forceinline__ void unpack(const uint32_t* w, float (&v)[VEC]) {
@@ -36,38 +44,85 @@ __device__ __forceinline__ void unpack(const uint32_t* w, float (&v)[VEC]) {
   }
 }
 
-// VEC consecutive elements as float32, in one load of up to 16 bytes (the
-// address is a multiple of its size).
+// VEC consecutive elements as they lie in memory, moved in accesses of at
+// most 16 bytes (the address is a multiple of that, or of VEC elements where
+// those are fewer bytes).
 template <typename T, int VEC>
-__device__ __forceinline__ void load_vec(const T* src, float (&v)[VEC]) {
-  constexpr int kBytes = VEC * sizeof(T);
-  if constexpr (kBytes == 16 || kBytes == 8) {
-    uint32_t w[kBytes / 4];
-    if constexpr (kBytes == 16) {
-      const uint4 r = *reinterpret_cast<const uint4*>(src);
-      w[0] = r.x, w[1] = r.y, w[2] = r.z, w[3] = r.w;
-    } else {
+struct Pack {
+  static constexpr int kBytes = VEC * static_cast<int>(sizeof(T));
+  static constexpr int kWords = kBytes < 4 ? 1 : kBytes / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* src) {
+    if constexpr (kBytes >= 16) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) {
+        const uint4 r = reinterpret_cast<const uint4*>(src)[i];
+        w[4 * i] = r.x, w[4 * i + 1] = r.y, w[4 * i + 2] = r.z, w[4 * i + 3] = r.w;
+      }
+    } else if constexpr (kBytes == 8) {
       const uint2 r = *reinterpret_cast<const uint2*>(src);
       w[0] = r.x, w[1] = r.y;
+    } else if constexpr (kBytes == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(src);
+    } else if constexpr (kBytes == 2) {
+      w[0] = *reinterpret_cast<const uint16_t*>(src);
+    } else {
+      w[0] = *reinterpret_cast<const uint8_t*>(src);
     }
-    unpack<T, VEC>(w, v);
-  } else {
+  }
+  __device__ __forceinline__ void store(T* dst) const {
+    if constexpr (kBytes >= 16) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = Elem<T>::to_f(src[i]);
+      for (int i = 0; i < kBytes / 16; ++i)
+        reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    } else if constexpr (kBytes == 8) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    } else if constexpr (kBytes == 4) {
+      *reinterpret_cast<uint32_t*>(dst) = w[0];
+    } else {
+      *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(w[0]);
+    }
+  }
+  __device__ __forceinline__ void get(float (&v)[VEC]) const { unpack<T, VEC>(w, v); }
+  __device__ __forceinline__ void set(const float (&v)[VEC]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) w[i] = __float_as_uint(v[i]);
+    } else if constexpr (VEC == 1) {
+      const T h = Elem<T>::from_f(v[0]);
+      w[0] = *reinterpret_cast<const uint16_t*>(&h);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        const typename Elem<T>::Pair h = pair_of<T>(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+  }
+};
+
+// The low bytes of VEC words as VEC consecutive bytes under `mask` (VEC 1, 2,
+// 4 or 8, address a multiple of VEC).
+template <int VEC>
+__device__ __forceinline__ void store_codes(int8_t* dst, const uint32_t (&code)[VEC], uint32_t mask) {
+  if constexpr (VEC == 1) {
+    *dst = static_cast<int8_t>(code[0] & mask);
+  } else if constexpr (VEC == 2) {
+    *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(__byte_perm(code[0], code[1], 0x0040) & mask);
+  } else {
+    uint32_t w[VEC / 4];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i)
+      w[i] = __byte_perm(__byte_perm(code[4 * i], code[4 * i + 1], 0x0040),
+                         __byte_perm(code[4 * i + 2], code[4 * i + 3], 0x0040), 0x5410) & mask;
+    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(dst) = w[0];
   }
 }
 
-// The low bytes of VEC words as VEC consecutive bytes under `mask` (VEC 4 or
-// 8, address a multiple of VEC).
-template <int VEC>
-__device__ __forceinline__ void store_codes(int8_t* dst, const uint32_t (&code)[VEC], uint32_t mask) {
-  uint32_t w[VEC / 4];
-#pragma unroll
-  for (int i = 0; i < VEC / 4; ++i)
-    w[i] = __byte_perm(__byte_perm(code[4 * i], code[4 * i + 1], 0x0040),
-                       __byte_perm(code[4 * i + 2], code[4 * i + 3], 0x0040), 0x5410) & mask;
-  if constexpr (VEC == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-  else *reinterpret_cast<uint32_t*>(dst) = w[0];
+// Byte i of a word as a signed value.
+__device__ __forceinline__ float signed_byte(uint32_t w, int i) {
+  return static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
 }
 
 // Symmetric 8-bit quantizer of values whose largest magnitude is `top`:

@@ -25,12 +25,16 @@ _PITCH = 16  # rows of codes start on multiples of 16 bytes
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x as (rows, features) with unit stride along the features and rows that do not overlap."""
 
-    x2 = x.reshape(-1, x.shape[-1])
+    x2 = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
     if x2.stride(1) != 1 or x2.stride(0) < x2.shape[1]:
         x2 = x2.contiguous()
         if x2.stride(0) < x2.shape[1]:  # a single row of a stride that was never needed
             x2 = x2.as_strided(x2.shape, (x2.shape[1], 1))
     return x2
+
+
+def _f32(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype is torch.float32 and t.is_contiguous() else _f32_vec(t)
 
 
 def _padded_rows(codes: torch.Tensor) -> torch.Tensor:
@@ -44,12 +48,12 @@ def _padded_rows(codes: torch.Tensor) -> torch.Tensor:
     return out.copy_(codes)
 
 
-def _quantize(x2: torch.Tensor, col_scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+def _quantize(x2: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     rows, features = x2.shape
     codes = torch.empty((rows, -(-features // _PITCH) * _PITCH), dtype=torch.int8, device=x2.device)
     scales = torch.empty((rows,), dtype=torch.float32, device=x2.device)
-    _lib.call("convrot_quantize_i8", x2, _lib.ptr(x2), _dtype_code(x2.dtype), rows, features, x2.stride(0),
-              _lib.ptr(col_scale), _lib.ptr(codes), codes.shape[1], _lib.ptr(scales))
+    _lib.call("convrot_quantize_i8", x2.get_device(), x2.data_ptr(), _dtype_code(x2.dtype), rows, features,
+              x2.stride(0), None, codes.data_ptr(), codes.shape[1], scales.data_ptr())
     return codes[:, :features], scales
 
 
@@ -72,14 +76,6 @@ def quantize_int8_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tens
     if weight.ndim != 2:
         raise ValueError(f"int8 weight must be 2D, got {tuple(weight.shape)}")
     return quantize_signed_int8_rowwise(weight)
-
-
-def _gemm(codes, qweight, layout, xscales, wscales, bias, dtype, n) -> torch.Tensor:
-    m, k = codes.shape
-    out = torch.empty((m, n), dtype=dtype, device=codes.device)
-    _lib.call("convrot_i8_gemm", codes, _lib.ptr(codes), codes.stride(0), _lib.ptr(qweight), qweight.stride(0), layout,
-              _lib.ptr(xscales), _lib.ptr(wscales), _lib.ptr(bias), _lib.ptr(out), _dtype_code(dtype), m, n, k)
-    return out
 
 
 def _validate(k: int, qweight, wscales, bias) -> int:
@@ -109,8 +105,14 @@ def int8_matmul(codes, qweight, xscales, wscales, bias=None, *, output_dtype) ->
         raise ValueError(f"int8 activation scales must have shape {(codes.shape[0],)}, got {tuple(xscales.shape)}")
     _dtype_code(output_dtype)
     _require_cuda(codes, qweight, xscales, wscales, bias)
-    return _gemm(_padded_rows(codes), _padded_rows(qweight), _lib.LAYOUT_NK, _f32_vec(xscales), _f32_vec(wscales),
-                 None if bias is None else _f32_vec(bias), output_dtype, n)
+    codes, qweight, xscales, wscales = _padded_rows(codes), _padded_rows(qweight), _f32(xscales), _f32(wscales)
+    bias = None if bias is None else _f32(bias)
+    m, k = codes.shape
+    out = torch.empty((m, n), dtype=output_dtype, device=codes.device)
+    _lib.call("convrot_i8_gemm", codes.get_device(), codes.data_ptr(), codes.stride(0), qweight.data_ptr(),
+              qweight.stride(0), _lib.LAYOUT_NK, xscales.data_ptr(), wscales.data_ptr(),
+              None if bias is None else bias.data_ptr(), out.data_ptr(), _dtype_code(output_dtype), m, n, k)
+    return out
 
 
 def _product(x2, col_scale, qweight, layout, wscales, bias, n) -> torch.Tensor:
@@ -118,20 +120,21 @@ def _product(x2, col_scale, qweight, layout, wscales, bias, n) -> torch.Tensor:
 
     m, k = x2.shape
     pitch = -(-k // _PITCH) * _PITCH
-    out = torch.empty((m, n), dtype=x2.dtype, device=x2.device)
-    codes = torch.empty((m, pitch), dtype=torch.int8, device=x2.device)
-    scales = torch.empty((m,), dtype=torch.float32, device=x2.device)
-    dtype = _dtype_code(x2.dtype)
-    _lib.call("convrot_i8_linear", x2, _lib.ptr(x2), dtype, x2.stride(0), _lib.ptr(col_scale), _lib.ptr(qweight),
-              qweight.stride(0), layout, _lib.ptr(wscales), _lib.ptr(bias), _lib.ptr(out), dtype, m, n, k,
-              _lib.ptr(codes), pitch, _lib.ptr(scales))
+    out = x2.new_empty((m, n))
+    # codes, then scales (16-byte aligned: the pitch is)
+    space = torch.empty((m * (pitch + 4),), dtype=torch.int8, device=x2.device)
+    codes, dtype = space.data_ptr(), _dtype_code(x2.dtype)
+    _lib.call("convrot_i8_linear", x2.get_device(), x2.data_ptr(), dtype, x2.stride(0),
+              None if col_scale is None else col_scale.data_ptr(), qweight.data_ptr(), qweight.stride(0), layout,
+              None if wscales is None else wscales.data_ptr(), None if bias is None else bias.data_ptr(),
+              out.data_ptr(), dtype, m, n, k, codes, pitch, codes + m * pitch)
     return out
 
 
 def _forward(x, qweight, wscales, bias):
     n = qweight.shape[0]
     out = _product(_rows(x), None, qweight, _lib.LAYOUT_NK, wscales, bias, n)
-    return out.view(*x.shape[:-1], n)
+    return out if x.ndim == 2 else out.view(*x.shape[:-1], n)
 
 
 class _Int8Linear(torch.autograd.Function):
@@ -146,7 +149,7 @@ class _Int8Linear(torch.autograd.Function):
         qweight, wscales = ctx.saved_tensors
         k = qweight.shape[1]
         dx = _product(_rows(dy), wscales, qweight, _lib.LAYOUT_KN, None, None, k)
-        return dx.view(*dy.shape[:-1], k), None, None, None
+        return dx if dy.ndim == 2 else dx.view(*dy.shape[:-1], k), None, None, None
 
 
 def int8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor,
@@ -166,8 +169,8 @@ def int8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor,
         raise ValueError("the weight scales and the bias of an int8 linear are frozen: they may not require gradients")
     _dtype_code(x.dtype)
     _require_cuda(x, qweight, wscales, bias)
-    qweight, wscales = _padded_rows(qweight), _f32_vec(wscales)
-    bias = None if bias is None else _f32_vec(bias)
+    qweight, wscales = _padded_rows(qweight), _f32(wscales)
+    bias = None if bias is None else _f32(bias)
     if torch.is_grad_enabled() and x.requires_grad:
         return _Int8Linear.apply(x, qweight, wscales, bias)
     return _forward(x, qweight, wscales, bias)

@@ -4,6 +4,7 @@ with their gradients.  No counterpart in the reference."""
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -11,33 +12,38 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .core import _dtype_code, _require_cuda
 
-MAX_HEAD_DIM = 256
+_Strides = ctypes.c_int64 * 12
 
 
-def _strides(t: torch.Tensor | None):
-    return None if t is None else (ctypes.c_int64 * 3)(*t.stride()[:3])
-
-
-def _unit(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(3) == 1 else t.contiguous()
+@functools.lru_cache(maxsize=64)
+def _widths(axes: tuple[int, ...]):
+    return (ctypes.c_int32 * len(axes))(*axes)
 
 
 def _turn(q, k, q_out, k_out, positions, axes, theta, interleaved, inverse) -> None:
     b, hq, t, d = q.shape
-    per_sample = positions.stride(0) if positions.ndim == 3 else 0
-    _lib.call("convrot_axial_rotary", q, _dtype_code(q.dtype), b, t, d, _lib.ptr(q), hq, _strides(q), _lib.ptr(q_out),
-              _strides(q_out), _lib.ptr(k), 0 if k is None else k.shape[1], _strides(k), _lib.ptr(k_out),
-              _strides(k_out), _lib.ptr(positions), per_sample, len(axes), (ctypes.c_int32 * len(axes))(*axes), theta,
-              int(interleaved), int(inverse))
+    if k is None:
+        kp = kop = None
+        hk, strides = 0, _Strides(*q.stride()[:3], *q_out.stride()[:3])
+    else:
+        kp, kop, hk = k.data_ptr(), k_out.data_ptr(), k.shape[1]
+        strides = _Strides(*q.stride()[:3], *q_out.stride()[:3], *k.stride()[:3], *k_out.stride()[:3])
+    _lib.call("convrot_axial_rotary", q.get_device(), _dtype_code(q.dtype), b, t, d, q.data_ptr(), q_out.data_ptr(), hq,
+              kp, kop, hk, strides, positions.data_ptr(), positions.stride(0) if positions.ndim == 3 else 0, len(axes),
+              _widths(axes), theta, interleaved, inverse)
+
+
+def _packed(t):
+    return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _unit(t):
+    return t if t is None or t.stride(3) == 1 else t.contiguous()
 
 
 def _forward(q, k, positions, axes, theta, interleaved):
-    q = _unit(q)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None
-    if k is not None:
-        k = _unit(k)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    q, k = _unit(q), _unit(k)
+    q_out, k_out = _packed(q), _packed(k)
     _turn(q, k, q_out, k_out, positions, axes, theta, interleaved, False)
     return q_out, k_out
 
@@ -46,28 +52,24 @@ class _AxialRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, axes, theta, interleaved):
         ctx.save_for_backward(positions)
-        ctx.how = (axes, theta, interleaved)
         # the gradients take the memory order of the inputs, often columns of one projection's output
-        ctx.like = q.stride(1) < q.stride(2)
+        ctx.how = (axes, theta, interleaved, q.stride(1) < q.stride(2))
         return _forward(q, k, positions, axes, theta, interleaved)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq, dk):
         (positions,) = ctx.saved_tensors
-        axes, theta, interleaved = ctx.how
+        axes, theta, interleaved, heads_inside = ctx.how
 
         def like(g):
+            if g is None or not heads_inside:
+                return _packed(g)
             b, h, t, d = g.shape
-            if ctx.like:
-                return torch.empty((b, t, h, d), dtype=g.dtype, device=g.device).transpose(1, 2)
-            return torch.empty(g.shape, dtype=g.dtype, device=g.device)
+            return torch.empty((b, t, h, d), dtype=g.dtype, device=g.device).transpose(1, 2)
 
-        dq = _unit(dq)
-        q_out, k_out = like(dq), None
-        if dk is not None:
-            dk = _unit(dk)
-            k_out = like(dk)
+        dq, dk = _unit(dq), _unit(dk)
+        q_out, k_out = like(dq), like(dk)
         _turn(dq, dk, q_out, k_out, positions, axes, theta, interleaved, True)
         return q_out, k_out, None, None, None, None
 
@@ -100,7 +102,8 @@ def axial_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
                          f"{tuple(positions.shape)}")
     _dtype_code(q.dtype)
     _require_cuda(q, k, positions)
-    positions = positions.detach().to(torch.float32).contiguous()
+    if positions.dtype is not torch.float32 or not positions.is_contiguous():
+        positions = positions.detach().to(torch.float32).contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _AxialRotary.apply(q, k, positions, axes, float(theta), bool(interleaved))
     return _forward(q, k, positions, axes, float(theta), bool(interleaved))

@@ -327,9 +327,9 @@ int convrot_i8_linear(const void* x, int x_dtype, int64_t x_stride, const float*
 
 /*
  * Rotary positions with several axes for queries and keys, in one launch.
- * Tensors are (batch, heads, tokens, dim) with element strides {batch, head,
- * token} and unit stride along dim (dim <= 256); k_heads (or q_heads) may be
- * 0.  The first sum(widths) values of a head are pairs, adjacent
+ * Tensors are (batch, heads, tokens, dim), dim <= 256, with unit stride along
+ * dim; strides: host array of the element strides {batch, head, token} of q,
+ * q_out, k and k_out in this order.  k_heads (or q_heads) may be 0.  The first sum(widths) values of a head are pairs, adjacent
  * (interleaved) or sum(widths) / 2 apart; pair j of axis a turns by
  * positions[token, a] * theta^(-2 j / widths[a]); the rest is copied.
  * inverse turns back: the gradient of the input from that of the output.
@@ -338,9 +338,8 @@ int convrot_i8_linear(const void* x, int x_dtype, int64_t x_stride, const float*
  * and even.  Outputs may not overlap inputs, except that each may be exactly
  * its own input.  No reference counterpart.
  */
-int convrot_axial_rotary(int dtype, int64_t batch, int64_t tokens, int64_t dim, const void* q, int64_t q_heads,
-                         const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, const void* k,
-                         int64_t k_heads, const int64_t* k_strides, void* k_out, const int64_t* k_out_strides,
+int convrot_axial_rotary(int dtype, int64_t batch, int64_t tokens, int64_t dim, const void* q, void* q_out,
+                         int64_t q_heads, const void* k, void* k_out, int64_t k_heads, const int64_t* strides,
                          const float* positions, int64_t position_batch_stride, int axes, const int32_t* widths,
                          double theta, int interleaved, int inverse, void* stream);
 

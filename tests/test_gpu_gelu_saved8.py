@@ -150,10 +150,11 @@ def test_unaligned_rows_through_the_c_entry():
     y = torch.empty((rows * f + 1,), dtype=torch.bfloat16, device=dev())[1:].view(rows, f)
     codes = torch.empty((rows * f + 3,), dtype=torch.int8, device=dev())[3:].view(rows, f)
     scales = torch.empty((rows, 3), device=dev())
-    _lib.call("convrot_gelu_saved8", x, _lib.ptr(x), _lib.BF16, rows, f, _lib.ptr(y), _lib.ptr(codes), _lib.ptr(scales))
+    _lib.call("convrot_gelu_saved8", 0, x.data_ptr(), _lib.BF16, rows, f, y.data_ptr(), codes.data_ptr(),
+              scales.data_ptr())
     dx = torch.empty_like(x)
-    _lib.call("convrot_gelu_saved8_backward", x, _lib.ptr(x), _lib.BF16, rows, f, _lib.ptr(codes), _lib.ptr(scales),
-              _lib.ptr(dx))
+    _lib.call("convrot_gelu_saved8_backward", 0, x.data_ptr(), _lib.BF16, rows, f, codes.data_ptr(), scales.data_ptr(),
+              dx.data_ptr())
     _check(x, y, x, dx)
     groups = torch.nn.functional.pad(x.double(), (0, -f % GROUP)).unflatten(-1, (-1, GROUP))
     assert torch.equal(codes.double(), codes64(groups)[1].flatten(-2)[:, :f])

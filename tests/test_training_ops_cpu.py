@@ -59,12 +59,12 @@ def test_linear_arguments(lib):
 
 
 def test_rotary_arguments(lib):
-    strides = (ctypes.c_int64 * 3)(0, 0, 0)
+    strides = (ctypes.c_int64 * 12)()
 
     def run(widths=(4, 4), dim=8, theta=10000.0, batch=1, tokens=1, dtype=2, heads=1, positions=FAKE):
         w = (ctypes.c_int32 * max(1, len(widths)))(*widths)
-        return lib.convrot_axial_rotary(dtype, batch, tokens, dim, FAKE, heads, strides, FAKE, strides, None, 0, None,
-                                        None, None, positions, 0, len(widths), w, theta, 1, 0, None)
+        return lib.convrot_axial_rotary(dtype, batch, tokens, dim, FAKE, FAKE, heads, None, None, 0, strides, positions,
+                                        0, len(widths), w, theta, 1, 0, None)
 
     assert run(dtype=3) == -1
     assert run(widths=()) == -1 and run(widths=(2,) * 9, dim=64) == -1 and "axes" in _err(lib)
