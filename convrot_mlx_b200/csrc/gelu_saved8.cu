@@ -17,13 +17,23 @@ namespace {
 constexpr int kGroup = 128;
 constexpr float kC2 = 1.5957691216057308f;  // 2 c
 constexpr float kA = 0.044715f;
+constexpr float kLog2e = 1.4426950408889634f;
 
-// x^2, bounded so that it stays finite: from |x| = 100 on the gate is exactly
-// 0 or 1 and its slope exactly 0 whatever the square.
-__device__ __forceinline__ float square(float x) { return fminf(x * x, 1.0e4f); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
+// s(x) from x and x^2: 1 / (1 + 2^(-x (k + k a x^2))), k = 2 c log2(e).  Where
+// the power overflows s is 0, and where x^2 does it is 0 or 1, as it should.
 __device__ __forceinline__ float gate(float x, float x2) {
-  return __fdividef(1.0f, 1.0f + __expf(-kC2 * x * (1.0f + kA * x2)));
+  return rcp(1.0f + ex2(x * fmaf(-kC2 * kLog2e * kA, x2, -kC2 * kLog2e)));
 }
 
 // A group is spread over LANES lanes, NV vectors of VEC elements each; a CTA
@@ -78,49 +88,60 @@ __global__ void __launch_bounds__(256) gelu_fwd_kernel(const GeluParams p) {
 #pragma unroll
     for (int j = 0; j < S::kVectors; ++j) {
       const int c = (lane + j * S::kLanes) * VEC;
-      if (c < length[u]) raw[u][j].load(x + base[u] + c);
+      if (c < length[u]) raw[u][j].load_nc(x + base[u] + c);
     }
   }
+  if (p.codes) {
+    // The groups' maxima; then lane u of a set forms the quantizer of group u,
+    // so that its divisions are done once, and the set takes it from there.
+    uint32_t mine = 0;
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    float v[S::kVectors][VEC];
-    uint32_t top = 0;
+    for (int u = 0; u < kUnroll; ++u) {
+      uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < S::kVectors; ++j) {
-      const int c = (lane + j * S::kLanes) * VEC;
-      if (c < length[u]) {
-        raw[u][j].get(v[j]);
+      for (int j = 0; j < S::kVectors; ++j)
+        if ((lane + j * S::kLanes) * VEC < length[u]) top = max(top, raw[u][j].top());
+      if constexpr (S::kLanes == 32) {
+        top = warp_max(top);
+      } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) top = max(top, abs_bits(v[j][i]));
+        for (int o = S::kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
       }
+      if (lane == u) mine = top;
     }
-    if constexpr (S::kLanes == 32) {
-      top = warp_max(top);
-    } else {
+    const Quant8<T> own(mine);
+    if (lane < kUnroll && first + lane * S::kSets < p.total) p.scales[first + lane * S::kSets] = scale8(mine);
 #pragma unroll
-      for (int o = S::kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    }
-    const Quant8 quant(top);
-    if (lane == 0 && length[u] > 0 && p.scales) p.scales[first + u * S::kSets] = Quant8::scale(top);
+    for (int u = 0; u < kUnroll; ++u) {
+      const Quant8<T> quant = own.from_lane(u, S::kLanes);
 #pragma unroll
-    for (int j = 0; j < S::kVectors; ++j) {
-      const int c = (lane + j * S::kLanes) * VEC;
-      if (c < length[u]) {
-        float y[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) y[i] = v[j][i] * gate(v[j][i], square(v[j][i]));
-        Pack<T, VEC> out;
-        out.set(y);
-        out.store(static_cast<T*>(p.out) + base[u] + c);
-        if (p.codes) {
+      for (int j = 0; j < S::kVectors; ++j) {
+        const int c = (lane + j * S::kLanes) * VEC;
+        if (c < length[u]) {
+          float v[VEC];
           uint32_t code[VEC];
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) code[i] = quant.code(v[j][i]);
-          store_codes<VEC>(p.codes + base[u] + c, code, quant.mask);
+          raw[u][j].get(v);
+          quant.codes(v, code);
+          store_codes<VEC>(p.codes + base[u] + c, code, quant.mask());
         }
       }
     }
   }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+    for (int j = 0; j < S::kVectors; ++j) {
+      const int c = (lane + j * S::kLanes) * VEC;
+      if (c < length[u]) {
+        float v[VEC];
+        raw[u][j].get(v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] *= gate(v[i], v[i] * v[i]);
+        Pack<T, VEC> out;
+        out.set(v);
+        out.store(static_cast<T*>(p.out) + base[u] + c);
+      }
+    }
 }
 
 template <typename T, int VEC>
@@ -149,8 +170,8 @@ __global__ void __launch_bounds__(256) gelu_bwd_kernel(const GeluParams p) {
     for (int j = 0; j < S::kVectors; ++j) {
       const int c = (lane + j * S::kLanes) * VEC;
       if (c < length[u]) {
-        raw[u][j].load(dy + base[u] + c);
-        codes[u][j].load(reinterpret_cast<const uint8_t*>(p.codes) + base[u] + c);
+        raw[u][j].load_nc(dy + base[u] + c);
+        codes[u][j].load_nc(reinterpret_cast<const uint8_t*>(p.codes) + base[u] + c);
       }
     }
   }
@@ -165,8 +186,10 @@ __global__ void __launch_bounds__(256) gelu_bwd_kernel(const GeluParams p) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           const float x = signed_byte(codes[u][j].w[i / 4], i % 4) * scale[u];
-          const float x2 = square(x), s = gate(x, x2);
-          d[i] *= s + x * s * (1.0f - s) * kC2 * (1.0f + 3.0f * kA * x2);
+          // x^2 bounded so that it stays finite: from |x| = 100 on s is
+          // exactly 0 or 1, and s - s^2 exactly 0 whatever it is multiplied by
+          const float x2 = fminf(x * x, 1.0e4f), s = gate(x, x2);
+          d[i] *= fmaf(x * fmaf(-s, s, s), fmaf(3.0f * kC2 * kA, x2, kC2), s);
         }
         Pack<T, VEC> out;
         out.set(d);

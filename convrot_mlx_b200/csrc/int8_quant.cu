@@ -36,99 +36,136 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
   return v;
 }
 
-// VEC consecutive elements at column c as float32; columns past the end read 0.
-template <typename T, int VEC>
-__device__ __forceinline__ void load(const QuantParams& p, int64_t row, int c, float (&v)[VEC]) {
-  const T* src = static_cast<const T*>(p.x) + row * p.x_stride + c;
-  if (c + VEC <= p.features) {
-    Pack<T, VEC> pk;
-    pk.load(src);
-    pk.get(v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = c + i < p.features ? Elem<T>::to_f(src[i]) : 0.0f;
-  }
-  if (p.col_scale) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = c + i < p.features ? __fmul_rn(v[i], __ldg(p.col_scale + c + i)) : 0.0f;
-  }
-}
+// The type whose quantizer applies: that of x, or float32 after the product
+// with the column scales.
+template <typename T, bool SCALED>
+using Quantized = Quant8<typename std::conditional<SCALED, float, T>::type>;
 
-template <int VEC>
-__device__ __forceinline__ void store(const QuantParams& p, int64_t row, int c, const Quant8& quant,
-                                      const float (&v)[VEC]) {
-  int8_t* dst = p.q + row * p.q_stride + c;
-  uint32_t code[VEC];
+// One thread's share of a row: NV vectors of VEC elements, `step` apart.
+template <typename T, int VEC, int NV, bool SCALED>
+struct Share {
+  Pack<T, VEC> raw[NV];
+  Pack<float, VEC> factor[SCALED ? NV : 1];
+
+  __device__ __forceinline__ void load(const QuantParams& p, int64_t row, int c0, int step) {
+    const T* src = static_cast<const T*>(p.x) + row * p.x_stride;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) code[i] = quant.code(v[i]);
-  if constexpr (VEC % 4 == 0) {
-    if (c + VEC <= p.features) {
-      store_codes<VEC>(dst, code, quant.mask);
-      return;
+    for (int j = 0; j < NV; ++j) {
+      const int c = c0 + j * step;
+      raw[j].clear();
+      if (c + VEC <= p.features) {
+        raw[j].load_nc(src + c);
+      } else if (VEC > 1 && c < p.features) {
+        raw[j].load_part(src + c, p.features - c);
+      }
+    }
+    if constexpr (SCALED) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = c0 + j * step;
+        factor[j].clear();
+        if (c + VEC <= p.features) {
+          factor[j].load_nc(p.col_scale + c);
+        } else if (VEC > 1 && c < p.features) {
+          factor[j].load_part(p.col_scale + c, p.features - c);
+        }
+      }
     }
   }
+  __device__ __forceinline__ void get(int j, float (&v)[VEC]) const {
+    raw[j].get(v);
+    if constexpr (SCALED) {
+      float f[VEC];
+      factor[j].get(f);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    if (c + i < p.features) dst[i] = static_cast<int8_t>(code[i] & quant.mask);
-}
+      for (int i = 0; i < VEC; ++i) v[i] = __fmul_rn(v[i], f[i]);
+    }
+  }
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if constexpr (SCALED) {
+        float v[VEC];
+        get(j, v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) m = max(m, abs_bits(v[i]));
+      } else {
+        m = max(m, raw[j].top());
+      }
+    }
+    return m;
+  }
+  __device__ __forceinline__ void store(const QuantParams& p, int64_t row, int c0, int step,
+                                        const Quantized<T, SCALED>& quant) const {
+    int8_t* dst = p.q + row * p.q_stride;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = c0 + j * step;
+      if (c < p.features) {
+        float v[VEC];
+        uint32_t code[VEC];
+        get(j, v);
+        quant.codes(v, code);
+        if (c + VEC <= p.features) {
+          store_codes<VEC>(dst + c, code, quant.mask());
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            if (c + i < p.features) dst[c + i] = static_cast<int8_t>(code[i] & quant.mask());
+        }
+      }
+    }
+  }
+};
 
-// NV vectors of VEC elements a thread in registers; NV = 0: any length, in
-// two passes over the row.
-template <typename T, int VEC, int NV>
-__global__ void __launch_bounds__(kThreads<VEC>) quantize_i8_kernel(const QuantParams p) {
+// WARP: a warp for each row, 4 in a CTA; else a CTA for each row.
+template <typename T, int VEC, int NV, bool SCALED, bool WARP>
+__global__ void __launch_bounds__(WARP ? 128 : kThreads<VEC>) quantize_i8_kernel(const QuantParams p) {
   __shared__ uint32_t red[32];
   grid_dependency_wait();  // x may come from the previous kernel of the stream
   grid_dependents_launch();
-  const int step = blockDim.x * VEC;
-  const int c0 = threadIdx.x * VEC;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    uint32_t top = 0;
-    if constexpr (NV > 0) {
-      float v[NV][VEC];
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int c = c0 + j * step;
-        if (c < p.features) {
-          load<T, VEC>(p, row, c, v[j]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) v[j][i] = 0.0f;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) top = max(top, abs_bits(v[j][i]));
-      top = block_max(top, red);
-      const Quant8 quant(top);
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int c = c0 + j * step;
-        if (c < p.features) store<VEC>(p, row, c, quant, v[j]);
-      }
-    } else {
-      for (int c = c0; c < p.features; c += step) {
-        float v[VEC];
-        load<T, VEC>(p, row, c, v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) top = max(top, abs_bits(v[i]));
-      }
-      top = block_max(top, red);
-      const Quant8 quant(top);
-      for (int c = c0; c < p.features; c += step) {
-        float v[VEC];
-        load<T, VEC>(p, row, c, v);
-        store<VEC>(p, row, c, quant, v);
-      }
-    }
-    if (threadIdx.x == 0) p.scales[row] = Quant8::scale(top);
+  const int c0 = (WARP ? threadIdx.x & 31 : threadIdx.x) * VEC, step = (WARP ? 32 : blockDim.x) * VEC;
+  const int64_t first = WARP ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  const int64_t stride = WARP ? static_cast<int64_t>(gridDim.x) * 4 : gridDim.x;
+  for (int64_t row = first; row < p.rows; row += stride) {
+    Share<T, VEC, NV, SCALED> x;
+    x.load(p, row, c0, step);
+    const uint32_t top = WARP ? warp_max(x.top()) : block_max(x.top(), red);
+    x.store(p, row, c0, step, Quantized<T, SCALED>(top));
+    if (c0 == 0) p.scales[row] = scale8(top);
   }
 }
 
-template <typename T, int VEC, int NV>
-int launch_nv(const QuantParams& p, int threads, cudaStream_t stream) {
+// Rows too long for the registers: two passes, the second through L2.
+template <typename T, int VEC, bool SCALED>
+__global__ void __launch_bounds__(kThreads<VEC>) quantize_i8_long_kernel(const QuantParams p) {
+  __shared__ uint32_t red[32];
+  grid_dependency_wait();
+  grid_dependents_launch();
+  const int step = blockDim.x * VEC;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    uint32_t top = 0;
+    for (int c = threadIdx.x * VEC; c < p.features; c += 4 * step) {
+      Share<T, VEC, 4, SCALED> x;
+      x.load(p, row, c, step);
+      top = max(top, x.top());
+    }
+    top = block_max(top, red);
+    const Quantized<T, SCALED> quant(top);
+    for (int c = threadIdx.x * VEC; c < p.features; c += 4 * step) {
+      Share<T, VEC, 4, SCALED> x;
+      x.load(p, row, c, step);
+      x.store(p, row, c, step, quant);
+    }
+    if (threadIdx.x == 0) p.scales[row] = scale8(top);
+  }
+}
+
+int enqueue(void (*kernel)(QuantParams), const QuantParams& p, int64_t rows_per_cta, int threads, cudaStream_t stream) {
+  const int64_t ctas = (p.rows + rows_per_cta - 1) / rows_per_cta;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.rows < (1LL << 30) ? p.rows : (1LL << 30)), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas < (1LL << 30) ? ctas : (1LL << 30)), 1, 1);
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -136,31 +173,38 @@ int launch_nv(const QuantParams& p, int threads, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  CONVROT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, quantize_i8_kernel<T, VEC, NV>, p));
+  CONVROT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
   return check_launch("convrot_quantize_i8");
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool SCALED>
 int launch_vec(const QuantParams& p, cudaStream_t stream) {
+  const int vectors = (p.features + VEC - 1) / VEC;
+  // Many rows of up to 16 vectors a lane (12 with column factors): a warp for
+  // each, which needs no barrier.  Few rows: a CTA for each.
+  if (VEC > 1 && p.rows >= 8LL * device_sm_count()) {
+    if (vectors <= 4 * 32) return enqueue(quantize_i8_kernel<T, VEC, 4, SCALED, true>, p, 4, 128, stream);
+    if (vectors <= 12 * 32) return enqueue(quantize_i8_kernel<T, VEC, 12, SCALED, true>, p, 4, 128, stream);
+  }
   // two vectors (four single elements) a thread, more where the CTA is full
   constexpr int kLeast = VEC == 1 ? 4 : 2;
-  const int vectors = (p.features + VEC - 1) / VEC;
   int nv = kLeast;
   while (nv < 4 * kLeast && vectors > nv * kThreads<VEC>) nv *= 2;
   const int64_t per = (vectors + nv - 1) / nv;
-  if (per > kThreads<VEC>) return launch_nv<T, VEC, 0>(p, kThreads<VEC>, stream);
+  if (per > kThreads<VEC>) return enqueue(quantize_i8_long_kernel<T, VEC, SCALED>, p, 1, kThreads<VEC>, stream);
   const int threads = static_cast<int>((per + 31) / 32 * 32);
-  if (nv == kLeast) return launch_nv<T, VEC, kLeast>(p, threads, stream);
-  if (nv == 2 * kLeast) return launch_nv<T, VEC, 2 * kLeast>(p, threads, stream);
-  return launch_nv<T, VEC, 4 * kLeast>(p, threads, stream);
+  if (nv == kLeast) return enqueue(quantize_i8_kernel<T, VEC, kLeast, SCALED, false>, p, 1, threads, stream);
+  if (nv == 2 * kLeast) return enqueue(quantize_i8_kernel<T, VEC, 2 * kLeast, SCALED, false>, p, 1, threads, stream);
+  return enqueue(quantize_i8_kernel<T, VEC, 4 * kLeast, SCALED, false>, p, 1, threads, stream);
 }
 
 template <typename T>
 int launch(const QuantParams& p, cudaStream_t stream) {
   constexpr int kWide = 16 / sizeof(T);
   const bool wide = aligned_to(p.x, 16) && p.x_stride * static_cast<int64_t>(sizeof(T)) % 16 == 0 &&
-                    aligned_to(p.q, 8) && p.q_stride % 8 == 0;
-  return wide ? launch_vec<T, kWide>(p, stream) : launch_vec<T, 1>(p, stream);
+                    aligned_to(p.q, 8) && p.q_stride % 8 == 0 && aligned_to(p.col_scale, 16);
+  if (p.col_scale) return wide ? launch_vec<T, kWide, true>(p, stream) : launch_vec<T, 1, true>(p, stream);
+  return wide ? launch_vec<T, kWide, false>(p, stream) : launch_vec<T, 1, false>(p, stream);
 }
 
 }  // namespace

@@ -63,7 +63,7 @@ struct Share {
   __device__ __forceinline__ void load(const T* row, int c0, int step, int features) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      if (c0 + j * step < features) v[j].load(row + c0 + j * step);
+      if (c0 + j * step < features) v[j].load_nc(row + c0 + j * step);
   }
 };
 
@@ -71,7 +71,7 @@ template <typename TW, int VEC>
 __device__ __forceinline__ void weights(const NormParams& p, const TW* w, int c, float (&out)[VEC]) {
   if (w) {
     Pack<TW, VEC> pk;
-    pk.load(w + c);
+    pk.load_nc(w + c);
     pk.get(out);
   } else {
 #pragma unroll
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) norm_fwd_kernel(const NormPa
         weights<TW, VEC>(p, weight, c, w);
         if (bias) {
           Pack<TW, VEC> pk;
-          pk.load(bias + c);
+          pk.load_nc(bias + c);
           pk.get(b);
         }
 #pragma unroll
@@ -226,11 +226,27 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) norm_bwd_kernel(const NormPa
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[j][i] = db[j][i] = 0.0f;
   const int64_t first = WARP ? r0 + warp : r0, stride = WARP ? 4 : 1;
+  // the next row's loads are in flight while this row is worked on, where the
+  // registers hold both
+  constexpr bool kAhead = NV * Pack<T, VEC>::kWords <= 8;
+  Share<T, VEC, NV> x, dy, next_x, next_dy;
+  float mean, rstd, next_mean = 0.0f, next_rstd = 0.0f;
+  auto fetch = [&](int64_t row) {
+    if (row < r1) {
+      next_x.load(xs + row * F, c0, step, F);
+      next_dy.load(dys + row * F, c0, step, F);
+      next_mean = __ldg(p.mean + row);
+      next_rstd = __ldg(p.rstd + row);
+    }
+  };
+  if (kAhead) fetch(first);
   for (int64_t row = first; row < r1; row += stride) {
-    Share<T, VEC, NV> x, dy;
-    x.load(xs + row * F, c0, step, F);
-    dy.load(dys + row * F, c0, step, F);
-    const float mean = __ldg(p.mean + row), rstd = __ldg(p.rstd + row);
+    if (!kAhead) fetch(row);
+    x = next_x;
+    dy = next_dy;
+    mean = next_mean;
+    rstd = next_rstd;
+    if (kAhead) fetch(row + stride);
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -460,8 +476,8 @@ int forward_rows(const NormParams& p, int vectors, cudaStream_t s) {
   // E: vectors that make 16 bytes' worth of elements (1 when wide)
   const int64_t most = 64LL * device_sm_count();
   if (vectors <= 32 * 4 * E) return enqueue(norm_fwd_kernel<T, TW, VEC, 4 * E, true>, rows_grid(p.rows, 4, most), 128, 0, p, s);
-  if (vectors <= 32 * 12 * E && p.rows >= 4LL * device_sm_count())
-    return enqueue(norm_fwd_kernel<T, TW, VEC, 12 * E, true>, rows_grid(p.rows, 4, most), 128, 0, p, s);
+  if (VEC > 1 && vectors <= 32 * 12 && p.rows >= 4LL * device_sm_count())
+    return enqueue(norm_fwd_kernel<T, TW, VEC, (VEC > 1 ? 12 : 4), true>, rows_grid(p.rows, 4, most), 128, 0, p, s);
   const int per = vectors <= 512 * E ? E : 4 * E;
   const int threads = (((vectors + per - 1) / per) + 31) / 32 * 32;
   if (vectors <= 512 * E) return enqueue(norm_fwd_kernel<T, TW, VEC, E, false>, rows_grid(p.rows, 1, most), threads, 0, p, s);

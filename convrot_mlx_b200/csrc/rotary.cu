@@ -35,40 +35,40 @@ struct RotaryParams {
   int64_t pos_b;
   int64_t tokens;
   int batch, dim, pairs, axes, adjacent;
-  int units;   // threads that a head's values are spread over
+  int units;       // threads that a head's values are spread over
+  uint32_t slots;  // tokens of a CTA
   float sign;  // 1, or -1 for the gradient
   double turns[kMaxPairs];  // frequency of each pair in turns a position
   uint8_t axis[kMaxPairs];
 };
 
 // One thread keeps the sines and cosines of its pairs of one token and applies
-// them to the same place of every head of its share of the heads, kUnroll
-// heads in flight.  Units of a head, adjacent pairs: unit u is the VEC values
+// them to the same place of every head of its share of the heads, kHeads
+// heads (64 bytes) in flight and as many being turned.  Units of a head, adjacent pairs: unit u is the VEC values
 // from VEC u on (values past the pairs are copied).  Pairs half apart: unit u
 // is the VEC values from VEC u on and the VEC from pairs + VEC u on; further
 // units copy VEC values each.  WIDE: VEC values move in one access; else one
 // value an access.
-constexpr int kUnroll = 4;
+template <bool ADJACENT> constexpr int kHeads = ADJACENT ? 4 : 2;
 
 template <typename T, int VEC, bool WIDE>
 struct Unit {
-  float v[VEC];
+  Pack<T, VEC> raw;
   __device__ __forceinline__ void load(const T* src, int left) {
     if constexpr (WIDE) {
-      Pack<T, VEC> pk;
-      pk.load(src);
-      pk.get(v);
+      raw.load(src);
+    } else if constexpr (VEC == 1) {
+      raw.load(src);
     } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = i < left ? Elem<T>::to_f(src[i]) : 0.0f;
+      raw.load_part(src, left < VEC ? left : VEC);
     }
   }
   __device__ __forceinline__ void store(T* dst, int left) const {
-    if constexpr (WIDE) {
-      Pack<T, VEC> pk;
-      pk.set(v);
-      pk.store(dst);
+    if constexpr (WIDE || VEC == 1) {
+      raw.store(dst);
     } else {
+      float v[VEC];
+      raw.get(v);
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
         if (i < left) dst[i] = Elem<T>::from_f(v[i]);
@@ -77,15 +77,17 @@ struct Unit {
 };
 
 template <typename T, int VEC, bool WIDE, bool ADJACENT>
-__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ RotaryParams p) {
   constexpr int NP = ADJACENT ? VEC / 2 : VEC;  // pairs of a unit
+  constexpr int kUnroll = kHeads<ADJACENT>;
   grid_dependency_wait();
   grid_dependents_launch();
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t bt = id / p.units;
-  if (bt >= p.batch * p.tokens) return;
-  const int u = static_cast<int>(id - bt * p.units);
-  const int64_t b = bt / p.tokens, token = bt - b * p.tokens;
+  const uint32_t slot = threadIdx.x / static_cast<uint32_t>(p.units);  // token of the CTA
+  const int u = static_cast<int>(threadIdx.x - slot * p.units);
+  const uint32_t bt = blockIdx.x * p.slots + slot;
+  if (slot >= p.slots || bt >= p.batch * static_cast<uint32_t>(p.tokens)) return;
+  const uint32_t sample = bt / static_cast<uint32_t>(p.tokens);
+  const int64_t b = sample, token = bt - sample * static_cast<uint32_t>(p.tokens);
   const int turning = ADJACENT ? p.units : p.pairs / VEC;  // units that turn
   const bool turns = u < turning;
   const int e0 = ADJACENT || turns ? u * VEC : 2 * p.pairs + (u - turning) * VEC;  // first value of the unit
@@ -115,36 +117,56 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
     const int lo = which ? p.t[0].heads : 0, hi = min(h1, lo + t.heads);
     const T* in = static_cast<const T*>(t.in) + b * t.in_b + token * t.in_t + e0;
     T* out = static_cast<T*>(t.out) + b * t.out_b + token * t.out_t + e0;
-#pragma unroll 1
-    for (int h = max(h0, lo); h < hi; h += kUnroll) {
-      Unit<T, VEC, WIDE> x[kUnroll], y[ADJACENT ? 1 : kUnroll];
+    // the next heads' values are in flight while these are turned
+    Unit<T, VEC, WIDE> x[kUnroll], y[ADJACENT ? 1 : kUnroll], nx[kUnroll], ny[ADJACENT ? 1 : kUnroll];
+    auto fetch = [&](int h) {
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k)
         if (h + k < hi) {
           const T* src = in + (h + k - lo) * t.in_h;
-          x[k].load(src, left);
+          nx[k].load(src, left);
           if constexpr (!ADJACENT)
-            if (turns) y[k].load(src + p.pairs, VEC);
+            if (turns) ny[k].load(src + p.pairs, VEC);
         }
+    };
+    const int begin = max(h0, lo);
+    fetch(begin);
+#pragma unroll 1
+    for (int h = begin; h < hi; h += kUnroll) {
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) {
+        x[k] = nx[k];
+        if constexpr (!ADJACENT) y[k] = ny[k];
+      }
+      fetch(h + kUnroll);
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k)
         if (h + k < hi) {
           T* dst = out + (h + k - lo) * t.out_h;
           if constexpr (ADJACENT) {
+            // values past the pairs keep their bits
+            float v[VEC];
+            x[k].raw.get(v);
 #pragma unroll
             for (int i = 0; i < NP; ++i)
               if (u * NP + i < p.pairs) {
-                const float x0 = x[k].v[2 * i], x1 = x[k].v[2 * i + 1];
-                x[k].v[2 * i] = x0 * cs[i] - x1 * sn[i];
-                x[k].v[2 * i + 1] = x0 * sn[i] + x1 * cs[i];
+                const float x0 = v[2 * i], x1 = v[2 * i + 1];
+                v[2 * i] = x0 * cs[i] - x1 * sn[i];
+                v[2 * i + 1] = x0 * sn[i] + x1 * cs[i];
               }
+            x[k].raw.set(v);
           } else if (turns) {
+            float v[VEC], w[VEC];
+            x[k].raw.get(v);
+            y[k].raw.get(w);
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-              const float x0 = x[k].v[i], x1 = y[k].v[i];
-              x[k].v[i] = x0 * cs[i] - x1 * sn[i];
-              y[k].v[i] = x0 * sn[i] + x1 * cs[i];
+              const float x0 = v[i], x1 = w[i];
+              v[i] = x0 * cs[i] - x1 * sn[i];
+              w[i] = x0 * sn[i] + x1 * cs[i];
             }
+            x[k].raw.set(v);
+            y[k].raw.set(w);
             y[k].store(dst + p.pairs, VEC);
           }
           x[k].store(dst, left);
@@ -156,13 +178,13 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
 template <typename T, int VEC, bool WIDE, bool ADJACENT>
 int launch(RotaryParams& p, cudaStream_t stream) {
   p.units = ADJACENT ? (p.dim + VEC - 1) / VEC : p.pairs / VEC + (p.dim - 2 * p.pairs + VEC - 1) / VEC;
-  const int64_t blocks = (static_cast<int64_t>(p.batch) * p.tokens * p.units + 255) / 256;
-  CONVROT_REQUIRE(blocks < (1LL << 31), CONVROT_ERR_UNSUPPORTED, "shape too large");
-  // Few tokens: the heads are shared out until there are about 4 CTAs for
-  // each SM, each with kUnroll heads at least.
+  p.slots = 256 / p.units;
+  const int64_t blocks = (static_cast<int64_t>(p.batch) * p.tokens + p.slots - 1) / p.slots;
+  // The heads are shared out until there are about 16 CTAs for each SM (some
+  // waves, for an even end), each with kHeads heads at least.
   const int heads = p.t[0].heads + p.t[1].heads;
-  int64_t shares = (4LL * device_sm_count() + blocks - 1) / blocks;
-  const int most = (heads + kUnroll - 1) / kUnroll;
+  int64_t shares = (16LL * device_sm_count() + blocks - 1) / blocks;
+  const int most = (heads + kHeads<ADJACENT> - 1) / kHeads<ADJACENT>;
   if (shares > most) shares = most;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(shares), 1);
@@ -221,7 +243,8 @@ int convrot_axial_rotary(int dtype, int64_t batch, int64_t tokens, int64_t dim, 
   CONVROT_REQUIRE(axes >= 1 && axes <= kMaxAxes && widths != nullptr, CONVROT_ERR_INVALID,
                   "the number of axes must be 1..%d, got %d", kMaxAxes, axes);
   CONVROT_REQUIRE(theta > 0.0 && std::isfinite(theta), CONVROT_ERR_INVALID, "theta must be positive and finite");
-  CONVROT_REQUIRE(batch < (1LL << 31) && tokens < (1LL << 31) && q_heads + k_heads < (1LL << 20),
+  CONVROT_REQUIRE(batch < (1LL << 31) && tokens < (1LL << 31) && batch * tokens < (1LL << 31) &&
+                      q_heads + k_heads < (1LL << 20),
                   CONVROT_ERR_UNSUPPORTED, "shape too large");
   RotaryParams p = {};
   int pairs = 0;

@@ -3,6 +3,8 @@
 // quantizer's arithmetic.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace convrot {
@@ -70,6 +72,60 @@ struct Pack {
       w[0] = *reinterpret_cast<const uint8_t*>(src);
     }
   }
+  // The same through the read-only path, for data that the kernel does not
+  // write: such loads may be moved above stores.
+  __device__ __forceinline__ void load_nc(const T* src) {
+    if constexpr (kBytes >= 16) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) {
+        const uint4 r = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        w[4 * i] = r.x, w[4 * i + 1] = r.y, w[4 * i + 2] = r.z, w[4 * i + 3] = r.w;
+      }
+    } else if constexpr (kBytes == 8) {
+      const uint2 r = __ldg(reinterpret_cast<const uint2*>(src));
+      w[0] = r.x, w[1] = r.y;
+    } else if constexpr (kBytes == 4) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(src));
+    } else if constexpr (kBytes == 2) {
+      w[0] = __ldg(reinterpret_cast<const uint16_t*>(src));
+    } else {
+      w[0] = __ldg(reinterpret_cast<const uint8_t*>(src));
+    }
+  }
+  // The first `count` < VEC elements, the rest 0.
+  __device__ __forceinline__ void load_part(const T* src, int count) {
+    float v[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = i < count ? Elem<T>::to_f(src[i]) : 0.0f;
+    set(v);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  // Bits of the largest magnitude, as abs_bits orders them.  16-bit types are
+  // compared in pairs, by a maximum that keeps NaN.
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (sizeof(T) == 2 && VEC > 1) {
+      using P = typename Elem<T>::Pair;
+      uint32_t m = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+      for (int i = 1; i < kWords; ++i) {
+        const uint32_t a = w[i] & 0x7FFF7FFFu;
+        const P r = __hmax2_nan(*reinterpret_cast<const P*>(&m), *reinterpret_cast<const P*>(&a));
+        m = *reinterpret_cast<const uint32_t*>(&r);
+      }
+      const P r = *reinterpret_cast<const P*>(&m);
+      return max(abs_bits(Elem<T>::to_f(Elem<T>::lo(r))), abs_bits(Elem<T>::to_f(Elem<T>::hi(r))));
+    } else {
+      float v[VEC];
+      unpack<T, VEC>(w, v);
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) m = max(m, abs_bits(v[i]));
+      return m;
+    }
+  }
   __device__ __forceinline__ void store(T* dst) const {
     if constexpr (kBytes >= 16) {
 #pragma unroll
@@ -120,44 +176,90 @@ __device__ __forceinline__ void store_codes(int8_t* dst, const uint32_t (&code)[
   }
 }
 
-// Byte i of a word as a signed value.
+// Byte i of a word, a two's complement value, as float32: the byte with its
+// sign bit turned over, as the low mantissa bits of 2^23, is 2^23 + 128 above
+// the value (no integer conversion, whose rate is a quarter of an addition's).
 __device__ __forceinline__ float signed_byte(uint32_t w, int i) {
-  return static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+  return __fsub_rn(__uint_as_float(__byte_perm(w ^ 0x80808080u, 0x4B000000u, 0x7440 | i)), 8388736.0f);
 }
 
 // Symmetric 8-bit quantizer of values whose largest magnitude is `top`:
-//   code = rne(127 x / top) in [-127, 127], scale = top / 127.
-// x and top are first scaled by the power of two that brings top near 1, so
-// that 127 x cannot overflow; q = p r then misses p / top by at most two
-// ulps, and one step of residual correction, q += (p - q top) r with the
-// residual exact in one FMA, makes it the correctly rounded quotient.  Ties
-// (x = top / 2 gives 63.5 exactly) therefore round as in exact arithmetic.
-// Adding 1.5 * 2^23 rounds to the integer (nearest even) in the low bits.
+//   code = rne(127 x / top) in [-127, 127], scale = top / 127,
+// the quotient rounded as in exact arithmetic: x = top / 2 is a tie (63.5)
+// that occurs in earnest.
+// * bfloat16 x: one FMA, x * f + 1.5 * 2^23, whose rounding is to the integer
+//   (nearest even, in the low bits), with f = 127 / top rounded up.  x f is
+//   above 127 x / top by less than 2^-23 of it, while a quotient that is not
+//   a half is at least 2^-16 of itself away from one (both significands have
+//   8 bits).  A half needs 254 x = (2 j + 1) top: since 127 is prime either
+//   2 j + 1 = 127, the tie 63.5, which rounding up sends to 64, the even one;
+//   or top's significand is 127, where f is a power of two and x f exact.
+//   (top below 2^-120, for which f overflows, goes the other way.)
+// * other types: x and top are first scaled by the power of two that brings
+//   top near 1, so that nothing overflows; q = p r with p = 127 x misses p / top by at most two ulps, and
+//   one step of residual correction, q += (p - q top) r with the residual
+//   exact in one FMA, makes it the correctly rounded quotient.
 // top = 0: codes 0 and scale 0.  top infinite or NaN: codes 0 (their bits may
-// be those of a NaN: `mask` clears them), scale NaN.
+// be those of a NaN: mask() clears them), scale NaN.
+template <typename T>
 struct Quant8 {
-  float k127, top, r;
-  uint32_t mask;
-  __device__ __forceinline__ explicit Quant8(uint32_t top_bits) {
-    const bool live = top_bits != 0 && top_bits < kInfBits;
-    int e = static_cast<int>(top_bits >> 23) - 127;
-    e = e < -100 ? -100 : (e > 126 ? 126 : e);
-    const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);  // 2^-e
-    mask = live ? 0xFFFFFFFFu : 0u;
-    k127 = live ? 127.0f * f : 0.0f;
-    top = live ? __uint_as_float(top_bits) * f : 1.0f;
-    r = __frcp_rn(top);
+  static constexpr bool kFast = std::is_same<T, __nv_bfloat16>::value;
+  static constexpr uint32_t kLeastFast = 7u << 23;  // 2^-120: from here on 127 / top is finite
+  uint32_t bits;
+  float k, top, r;
+
+  __device__ __forceinline__ explicit Quant8(uint32_t top_bits) : bits(top_bits) {
+    const bool live = mask() != 0;
+    if constexpr (kFast) {
+      top = r = 0.0f;
+      k = live ? __fdiv_ru(127.0f, __uint_as_float(bits)) : 0.0f;
+    } else {
+      int e = static_cast<int>(bits >> 23) - 127;
+      e = e < -100 ? -100 : (e > 126 ? 126 : e);
+      const float f = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);  // 2^-e
+      top = live ? __uint_as_float(bits) * f : 1.0f;
+      k = live ? 127.0f * f : 0.0f;
+      r = __frcp_rn(top);
+    }
   }
-  // low byte of the result: the code in two's complement
-  __device__ __forceinline__ uint32_t code(float x) const {
-    const float p = __fmul_rn(x, k127);
-    const float q = __fmul_rn(p, r);
-    const float c = __fmaf_rn(__fmaf_rn(-q, top, p), r, q);
-    return __float_as_uint(__fadd_rn(c, 12582912.0f));
+  __device__ __forceinline__ uint32_t mask() const { return bits - 1u < kInfBits - 1u ? 0xFFFFFFFFu : 0u; }
+
+  // The quantizer that lane `lane` of each set of `lanes` lanes holds.
+  __device__ __forceinline__ Quant8 from_lane(int lane, int lanes) const {
+    Quant8 q = *this;
+    q.bits = __shfl_sync(0xFFFFFFFFu, bits, lane, lanes);
+    q.k = __shfl_sync(0xFFFFFFFFu, k, lane, lanes);
+    if constexpr (!kFast) {
+      q.top = __shfl_sync(0xFFFFFFFFu, top, lane, lanes);
+      q.r = __shfl_sync(0xFFFFFFFFu, r, lane, lanes);
+    }
+    return q;
   }
-  static __device__ __forceinline__ float scale(uint32_t top_bits) {
-    return top_bits < kInfBits ? __fdiv_rn(__uint_as_float(top_bits), 127.0f) : __uint_as_float(0x7FC00000u);
+
+  // The codes in two's complement in the words' low bytes.
+  template <int VEC>
+  __device__ __forceinline__ void codes(const float (&x)[VEC], uint32_t (&code)[VEC]) const {
+    if constexpr (kFast) {
+      if (bits < kLeastFast && bits != 0) {
+        const Quant8<float> wide(bits);
+        wide.codes(x, code);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) code[i] = __float_as_uint(__fmaf_rn(x[i], k, 12582912.0f));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float p = __fmul_rn(x[i], k);
+        const float q = __fmul_rn(p, r);
+        code[i] = __float_as_uint(__fadd_rn(__fmaf_rn(__fmaf_rn(-q, top, p), r, q), 12582912.0f));
+      }
+    }
   }
 };
+
+__device__ __forceinline__ float scale8(uint32_t top_bits) {
+  return top_bits < kInfBits ? __fdiv_rn(__uint_as_float(top_bits), 127.0f) : __uint_as_float(0x7FC00000u);
+}
 
 }  // namespace convrot
