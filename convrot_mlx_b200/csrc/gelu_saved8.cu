@@ -56,9 +56,15 @@ struct GeluParams {
   int64_t features;
 };
 
-// Element offset of a group's first value and its length.
+// Element offset of a group's first value and its length (0 past the last
+// group).  FULL: the features are whole groups, which then follow one another
+// in memory.
+template <bool FULL>
 __device__ __forceinline__ void locate(const GeluParams& p, uint32_t group, int64_t& base, int& length) {
-  if (p.features % kGroup == 0) {  // groups follow one another in memory
+  base = 0;
+  length = 0;
+  if (group >= p.total) return;
+  if constexpr (FULL) {
     base = static_cast<int64_t>(group) * kGroup;
     length = kGroup;
   } else {
@@ -69,7 +75,7 @@ __device__ __forceinline__ void locate(const GeluParams& p, uint32_t group, int6
   }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool FULL>
 __global__ void __launch_bounds__(256) gelu_fwd_kernel(const GeluParams p) {
   using S = Spread<VEC>;
   grid_dependency_wait();
@@ -83,12 +89,11 @@ __global__ void __launch_bounds__(256) gelu_fwd_kernel(const GeluParams p) {
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const uint32_t group = first + u * S::kSets;
-    length[u] = 0;
-    if (group < p.total) locate(p, group, base[u], length[u]);
+    locate<FULL>(p, group, base[u], length[u]);
 #pragma unroll
     for (int j = 0; j < S::kVectors; ++j) {
       const int c = (lane + j * S::kLanes) * VEC;
-      if (c < length[u]) raw[u][j].load_nc(x + base[u] + c);
+      if (FULL ? length[u] > 0 : c < length[u]) raw[u][j].load_nc(x + base[u] + c);
     }
   }
   if (p.codes) {
@@ -100,7 +105,7 @@ __global__ void __launch_bounds__(256) gelu_fwd_kernel(const GeluParams p) {
       uint32_t top = 0;
 #pragma unroll
       for (int j = 0; j < S::kVectors; ++j)
-        if ((lane + j * S::kLanes) * VEC < length[u]) top = max(top, raw[u][j].top());
+        if (FULL ? length[u] > 0 : (lane + j * S::kLanes) * VEC < length[u]) top = max(top, raw[u][j].top());
       if constexpr (S::kLanes == 32) {
         top = warp_max(top);
       } else {
@@ -117,7 +122,7 @@ __global__ void __launch_bounds__(256) gelu_fwd_kernel(const GeluParams p) {
 #pragma unroll
       for (int j = 0; j < S::kVectors; ++j) {
         const int c = (lane + j * S::kLanes) * VEC;
-        if (c < length[u]) {
+        if (FULL ? length[u] > 0 : c < length[u]) {
           float v[VEC];
           uint32_t code[VEC];
           raw[u][j].get(v);
@@ -132,7 +137,7 @@ __global__ void __launch_bounds__(256) gelu_fwd_kernel(const GeluParams p) {
 #pragma unroll
     for (int j = 0; j < S::kVectors; ++j) {
       const int c = (lane + j * S::kLanes) * VEC;
-      if (c < length[u]) {
+      if (FULL ? length[u] > 0 : c < length[u]) {
         float v[VEC];
         raw[u][j].get(v);
 #pragma unroll
@@ -144,7 +149,7 @@ __global__ void __launch_bounds__(256) gelu_fwd_kernel(const GeluParams p) {
     }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool FULL>
 __global__ void __launch_bounds__(256) gelu_bwd_kernel(const GeluParams p) {
   using S = Spread<VEC>;
   grid_dependency_wait();
@@ -160,16 +165,12 @@ __global__ void __launch_bounds__(256) gelu_bwd_kernel(const GeluParams p) {
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
     const uint32_t group = first + u * S::kSets;
-    length[u] = 0;
-    scale[u] = 0.0f;
-    if (group < p.total) {
-      locate(p, group, base[u], length[u]);
-      scale[u] = __ldg(p.scales + group);
-    }
+    locate<FULL>(p, group, base[u], length[u]);
+    scale[u] = length[u] > 0 ? __ldg(p.scales + group) : 0.0f;
 #pragma unroll
     for (int j = 0; j < S::kVectors; ++j) {
       const int c = (lane + j * S::kLanes) * VEC;
-      if (c < length[u]) {
+      if (FULL ? length[u] > 0 : c < length[u]) {
         raw[u][j].load_nc(dy + base[u] + c);
         codes[u][j].load_nc(reinterpret_cast<const uint8_t*>(p.codes) + base[u] + c);
       }
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(256) gelu_bwd_kernel(const GeluParams p) {
 #pragma unroll
     for (int j = 0; j < S::kVectors; ++j) {
       const int c = (lane + j * S::kLanes) * VEC;
-      if (c < length[u]) {
+      if (FULL ? length[u] > 0 : c < length[u]) {
         float d[VEC];
         raw[u][j].get(d);
 #pragma unroll
@@ -238,22 +239,26 @@ template <typename T>
 int forward(const GeluParams& p, cudaStream_t s) {
   const char* what = "convrot_gelu_saved8";
   const int vec = vector_of<T>(p);
-  if constexpr (sizeof(T) == 2)
-    if (vec == 8) return enqueue<8>(gelu_fwd_kernel<T, 8>, p, what, s);
-  if (vec == 4) return enqueue<4>(gelu_fwd_kernel<T, 4>, p, what, s);
-  if (vec == 2) return enqueue<2>(gelu_fwd_kernel<T, 2>, p, what, s);
-  return enqueue<1>(gelu_fwd_kernel<T, 1>, p, what, s);
+  constexpr int W = 16 / sizeof(T);
+  if (vec == W && p.features % kGroup == 0) return enqueue<W>(gelu_fwd_kernel<T, W, true>, p, what, s);
+  if constexpr (W == 8)
+    if (vec == 8) return enqueue<8>(gelu_fwd_kernel<T, 8, false>, p, what, s);
+  if (vec == 4) return enqueue<4>(gelu_fwd_kernel<T, 4, false>, p, what, s);
+  if (vec == 2) return enqueue<2>(gelu_fwd_kernel<T, 2, false>, p, what, s);
+  return enqueue<1>(gelu_fwd_kernel<T, 1, false>, p, what, s);
 }
 
 template <typename T>
 int backward(const GeluParams& p, cudaStream_t s) {
   const char* what = "convrot_gelu_saved8_backward";
   const int vec = vector_of<T>(p);
-  if constexpr (sizeof(T) == 2)
-    if (vec == 8) return enqueue<8>(gelu_bwd_kernel<T, 8>, p, what, s);
-  if (vec == 4) return enqueue<4>(gelu_bwd_kernel<T, 4>, p, what, s);
-  if (vec == 2) return enqueue<2>(gelu_bwd_kernel<T, 2>, p, what, s);
-  return enqueue<1>(gelu_bwd_kernel<T, 1>, p, what, s);
+  constexpr int W = 16 / sizeof(T);
+  if (vec == W && p.features % kGroup == 0) return enqueue<W>(gelu_bwd_kernel<T, W, true>, p, what, s);
+  if constexpr (W == 8)
+    if (vec == 8) return enqueue<8>(gelu_bwd_kernel<T, 8, false>, p, what, s);
+  if (vec == 4) return enqueue<4>(gelu_bwd_kernel<T, 4, false>, p, what, s);
+  if (vec == 2) return enqueue<2>(gelu_bwd_kernel<T, 2, false>, p, what, s);
+  return enqueue<1>(gelu_bwd_kernel<T, 1, false>, p, what, s);
 }
 
 GeluParams params(const void* in, void* out, int8_t* codes, float* scales, int64_t rows, int64_t features) {

@@ -119,21 +119,27 @@ struct Share {
   }
 };
 
-// WARP: a warp for each row, 4 in a CTA; else a CTA for each row.
-template <typename T, int VEC, int NV, bool SCALED, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : kThreads<VEC>) quantize_i8_kernel(const QuantParams p) {
-  __shared__ uint32_t red[32];
+template <typename T, int VEC, int NV, bool SCALED>
+__global__ void __launch_bounds__(kThreads<VEC>) quantize_i8_kernel(const QuantParams p) {
+  __shared__ uint32_t red[2][32];
   grid_dependency_wait();  // x may come from the previous kernel of the stream
   grid_dependents_launch();
-  const int c0 = (WARP ? threadIdx.x & 31 : threadIdx.x) * VEC, step = (WARP ? 32 : blockDim.x) * VEC;
-  const int64_t first = WARP ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
-  const int64_t stride = WARP ? static_cast<int64_t>(gridDim.x) * 4 : gridDim.x;
-  for (int64_t row = first; row < p.rows; row += stride) {
-    Share<T, VEC, NV, SCALED> x;
-    x.load(p, row, c0, step);
-    const uint32_t top = WARP ? warp_max(x.top()) : block_max(x.top(), red);
+  const int c0 = threadIdx.x * VEC, step = blockDim.x * VEC, lane = threadIdx.x & 31;
+  int turn = 0;
+  Share<T, VEC, NV, SCALED> x, next;
+  next.load(p, blockIdx.x, c0, step);
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    x = next;
+    if (row + gridDim.x < p.rows) next.load(p, row + gridDim.x, c0, step);  // in flight while this row is worked on
+    uint32_t top = warp_max(x.top());
+    if (blockDim.x > 32) {
+      if (lane == 0) red[turn][threadIdx.x >> 5] = top;
+      __syncthreads();
+      top = warp_max(lane < (blockDim.x >> 5) ? red[turn][lane] : 0u);
+      turn ^= 1;
+    }
     x.store(p, row, c0, step, Quantized<T, SCALED>(top));
-    if (c0 == 0) p.scales[row] = scale8(top);
+    if (threadIdx.x == 0) p.scales[row] = scale8(top);
   }
 }
 
@@ -162,10 +168,12 @@ __global__ void __launch_bounds__(kThreads<VEC>) quantize_i8_long_kernel(const Q
   }
 }
 
-int enqueue(void (*kernel)(QuantParams), const QuantParams& p, int64_t rows_per_cta, int threads, cudaStream_t stream) {
-  const int64_t ctas = (p.rows + rows_per_cta - 1) / rows_per_cta;
+// As many CTAs as rows, up to about 1536 threads for each SM.
+int enqueue(void (*kernel)(QuantParams), const QuantParams& p, int threads, cudaStream_t stream) {
+  const int per_sm = threads > 768 ? 1 : threads < 64 ? 24 : 1536 / threads;
+  const int64_t most = static_cast<int64_t>(device_sm_count()) * per_sm;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas < (1LL << 30) ? ctas : (1LL << 30)), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(p.rows < most ? p.rows : most), 1, 1);
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -179,23 +187,17 @@ int enqueue(void (*kernel)(QuantParams), const QuantParams& p, int64_t rows_per_
 
 template <typename T, int VEC, bool SCALED>
 int launch_vec(const QuantParams& p, cudaStream_t stream) {
-  const int vectors = (p.features + VEC - 1) / VEC;
-  // Many rows of up to 16 vectors a lane (12 with column factors): a warp for
-  // each, which needs no barrier.  Few rows: a CTA for each.
-  if (VEC > 1 && p.rows >= 8LL * device_sm_count()) {
-    if (vectors <= 4 * 32) return enqueue(quantize_i8_kernel<T, VEC, 4, SCALED, true>, p, 4, 128, stream);
-    if (vectors <= 12 * 32) return enqueue(quantize_i8_kernel<T, VEC, 12, SCALED, true>, p, 4, 128, stream);
-  }
   // two vectors (four single elements) a thread, more where the CTA is full
   constexpr int kLeast = VEC == 1 ? 4 : 2;
+  const int vectors = (p.features + VEC - 1) / VEC;
   int nv = kLeast;
   while (nv < 4 * kLeast && vectors > nv * kThreads<VEC>) nv *= 2;
   const int64_t per = (vectors + nv - 1) / nv;
-  if (per > kThreads<VEC>) return enqueue(quantize_i8_long_kernel<T, VEC, SCALED>, p, 1, kThreads<VEC>, stream);
+  if (per > kThreads<VEC>) return enqueue(quantize_i8_long_kernel<T, VEC, SCALED>, p, kThreads<VEC>, stream);
   const int threads = static_cast<int>((per + 31) / 32 * 32);
-  if (nv == kLeast) return enqueue(quantize_i8_kernel<T, VEC, kLeast, SCALED, false>, p, 1, threads, stream);
-  if (nv == 2 * kLeast) return enqueue(quantize_i8_kernel<T, VEC, 2 * kLeast, SCALED, false>, p, 1, threads, stream);
-  return enqueue(quantize_i8_kernel<T, VEC, 4 * kLeast, SCALED, false>, p, 1, threads, stream);
+  if (nv == kLeast) return enqueue(quantize_i8_kernel<T, VEC, kLeast, SCALED>, p, threads, stream);
+  if (nv == 2 * kLeast) return enqueue(quantize_i8_kernel<T, VEC, 2 * kLeast, SCALED>, p, threads, stream);
+  return enqueue(quantize_i8_kernel<T, VEC, 4 * kLeast, SCALED>, p, threads, stream);
 }
 
 template <typename T>

@@ -11,10 +11,13 @@
 // each sample).  All arithmetic is float32; each output is rounded once.
 //
 // Memory-bound: forward reads and writes a row once; backward reads x and dy
-// and writes dx, once each.  A row stays in registers between its statistics
-// and its output.  In the backward pass a thread keeps the same columns for
-// all rows of its CTA, so the column sums stay in registers too; a second
-// small kernel adds up the CTAs' sums in a fixed order.
+// and writes dx, once each.  A thread keeps the same columns for all rows of
+// its CTA: a row stays in registers between its statistics and its output,
+// the weights are loaded once for a CTA, and the column sums of the backward
+// pass stay in registers too (a second small kernel adds up the CTAs' sums in
+// a fixed order).  What costs beside the memory is the exchange between the
+// threads of a row, so a thread has 24 values of a row (12 in float32) and a
+// CTA exchanges the sums of two rows at once.
 #include "rows.cuh"
 
 namespace convrot {
@@ -36,27 +39,52 @@ struct NormParams {
   float eps;
 };
 
-// Sums of N values over the rows' threads: a warp (WARP) or the CTA.  red
-// holds two sets of 32 warps' values, used in turn, so that one barrier for
-// each call is enough.
+// Adds up each of N values (1, 2 or 4) over a warp: while there are several,
+// lanes exchange halves of the set, so N values take about as many shuffles as
+// one.  Afterwards v[0] of lane l is the sum of value l / (32 / N).
+template <int N>
+__device__ __forceinline__ void warp_sums(float (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+  int o = 16;
+#pragma unroll
+  for (int n = N; n > 1; n /= 2, o /= 2) {
+    const bool high = lane & o;
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const float send = high ? v[i] : v[i + n / 2];
+      v[i] = (high ? v[i + n / 2] : v[i]) + __shfl_xor_sync(0xFFFFFFFFu, send, o);
+    }
+  }
+#pragma unroll
+  for (; o > 0; o /= 2) v[0] += __shfl_xor_sync(0xFFFFFFFFu, v[0], o);
+}
+
+// Sums of N values over the threads of a row, a warp (WARP) or the CTA, for
+// all of them.  red holds two sets of 16 warps' values, used in turn, so that
+// one barrier for each call is enough.
 template <bool WARP, int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[32][N], int& turn) {
+__device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[16][N], int& turn) {
+  warp_sums<N>(v);
+  const float mine = v[0];
+  if constexpr (WARP) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
-  if constexpr (!WARP) {
-    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0)
-#pragma unroll
-      for (int i = 0; i < N; ++i) red[turn][threadIdx.x >> 5][i] = v[i];
+    for (int i = 0; i < N; ++i) v[i] = __shfl_sync(0xFFFFFFFFu, mine, i * (32 / N));
+  } else {
+    const int lane = threadIdx.x & 31;
+    if (lane % (32 / N) == 0) red[turn][threadIdx.x >> 5][lane / (32 / N)] = mine;
     __syncthreads();
+    const int warps = blockDim.x >> 5;
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < warps ? red[turn][lane][i] : 0.0f);
+    for (int i = 0; i < N; ++i) v[i] = red[turn][0][i];
+    for (int w = 1; w < warps; ++w)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += red[turn][w][i];
     turn ^= 1;
   }
 }
 
-// A row's share of one thread: NV vectors of VEC elements, `threads` vectors
-// apart.  Columns past the end are never touched.
+// One thread's share of a row: NV vectors of VEC elements, `step` apart.
+// Columns past the end are never touched.
 template <typename T, int VEC, int NV>
 struct Share {
   Pack<T, VEC> v[NV];
@@ -65,22 +93,43 @@ struct Share {
     for (int j = 0; j < NV; ++j)
       if (c0 + j * step < features) v[j].load_nc(row + c0 + j * step);
   }
+  __device__ __forceinline__ void fill(float value) {
+    float f[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = value;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j].set(f);
+  }
 };
 
-template <typename TW, int VEC>
-__device__ __forceinline__ void weights(const NormParams& p, const TW* w, int c, float (&out)[VEC]) {
-  if (w) {
-    Pack<TW, VEC> pk;
-    pk.load_nc(w + c);
-    pk.get(out);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) out[i] = p.add_one ? 0.0f : 1.0f;
-  }
-  if (p.add_one)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) out[i] += 1.0f;
+// The vectors of a segment; an absent weight is 1 (0 with add_one), an absent
+// bias 0.
+template <typename TW, int VEC, int NV>
+__device__ __forceinline__ Share<TW, VEC, NV> vector_of(const TW* base, float absent, int c0, int step, int features) {
+  Share<TW, VEC, NV> s;
+  if (base) s.load(base, c0, step, features);
+  else s.fill(absent);
+  return s;
 }
+
+template <typename TW>
+__device__ __forceinline__ float weight_at(const NormParams& p, const TW* w, int c) {
+  const float v = w ? Elem<TW>::to_f(w[c]) : (p.add_one ? 0.0f : 1.0f);
+  return p.add_one ? 1.0f + v : v;
+}
+
+// The rows of a CTA: those of chunk blockIdx % chunks of its segment.
+struct Rows {
+  int64_t segment, begin, end;
+  __device__ __forceinline__ explicit Rows(const NormParams& p) {
+    segment = blockIdx.x / p.chunks;
+    const int64_t chunk = blockIdx.x % p.chunks, base = segment * p.rows_per_weight;
+    begin = base + p.rows_per_weight * chunk / p.chunks;
+    end = base + p.rows_per_weight * (chunk + 1) / p.chunks;
+  }
+};
+
+constexpr int kWarps = 4;  // of a CTA whose warps each have rows of their own
 
 template <typename TW>
 __device__ __forceinline__ const TW* at(const void* base, int64_t offset) {
@@ -90,68 +139,77 @@ __device__ __forceinline__ const TW* at(const void* base, int64_t offset) {
 // ---------------------------------------------------------------------------
 // forward
 
-template <typename T, typename TW, int VEC, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 512) norm_fwd_kernel(const NormParams p) {
-  __shared__ float red[2][32][1];
+// R rows at a time; WARP: each warp rows of its own, else the CTA together.
+template <typename T, typename TW, int VEC, int NV, int R, bool WARP>
+__global__ void __launch_bounds__(WARP ? 32 * kWarps : (R == 2 ? 256 : 512)) norm_fwd_kernel(const NormParams p) {
+  __shared__ float red[2][16][R];
   int turn = 0;
   grid_dependency_wait();
   grid_dependents_launch();
   const int F = p.features;
   const float inv = 1.0f / static_cast<float>(F);
   const int c0 = (WARP ? threadIdx.x & 31 : threadIdx.x) * VEC, step = (WARP ? 32 : blockDim.x) * VEC;
-  const int64_t first = WARP ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
-  const int64_t stride = WARP ? static_cast<int64_t>(gridDim.x) * 4 : gridDim.x;
-  for (int64_t row = first; row < p.rows; row += stride) {
-    Share<T, VEC, NV> x;
-    x.load(static_cast<const T*>(p.x) + row * F, c0, step, F);
-    float s[1] = {0.0f};
+  const Rows rows(p);
+  const auto weight = vector_of<TW, VEC, NV>(at<TW>(p.weight, rows.segment * p.weight_stride),
+                                             p.add_one ? 0.0f : 1.0f, c0, step, F);
+  const auto bias = vector_of<TW, VEC, NV>(at<TW>(p.bias, rows.segment * p.weight_stride), 0.0f, c0, step, F);
+  const float one = p.add_one ? 1.0f : 0.0f;
+  const int64_t first = rows.begin + (WARP ? (threadIdx.x >> 5) * R : 0);
+  for (int64_t row = first; row < rows.end; row += WARP ? kWarps * R : R) {
+    Share<T, VEC, NV> x[R];
+    float mean[R], s[R];
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (c0 + j * step < F) {
-        float v[VEC];
-        x.v[j].get(v);
+    for (int r = 0; r < R; ++r)
+      if (row + r < rows.end) x[r].load(static_cast<const T*>(p.x) + (row + r) * F, c0, step, F);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) s[0] += v[i];
-      }
-    row_sum<WARP>(s, red, turn);
-    const float mean = s[0] * inv;
-    s[0] = 0.0f;
+    for (int r = 0; r < R; ++r) {
+      s[r] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (c0 + j * step < F) {
-        float v[VEC];
-        x.v[j].get(v);
+      for (int j = 0; j < NV; ++j)
+        if (c0 + j * step < F) {
+          float v[VEC];
+          x[r].v[j].get(v);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) s[0] = fmaf(v[i] - mean, v[i] - mean, s[0]);
-      }
-    row_sum<WARP>(s, red, turn);
-    const float rstd = rsqrtf(s[0] * inv + p.eps);
-    if ((WARP ? threadIdx.x & 31 : threadIdx.x) == 0 && p.mean) {
-      p.mean[row] = mean;
-      p.rstd[row] = rstd;
-    }
-    const int64_t offset = p.rows == p.rows_per_weight ? 0 : row / p.rows_per_weight * p.weight_stride;
-    const TW* weight = at<TW>(p.weight, offset);
-    const TW* bias = at<TW>(p.bias, offset);
-    T* y = static_cast<T*>(p.y) + row * F;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = c0 + j * step;
-      if (c < F) {
-        float v[VEC], w[VEC], b[VEC];
-        x.v[j].get(v);
-        weights<TW, VEC>(p, weight, c, w);
-        if (bias) {
-          Pack<TW, VEC> pk;
-          pk.load_nc(bias + c);
-          pk.get(b);
+          for (int i = 0; i < VEC; ++i) s[r] += v[i];
         }
+    }
+    row_sums<WARP>(s, red, turn);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = fmaf((v[i] - mean) * rstd, w[i], bias ? b[i] : 0.0f);
-        Pack<T, VEC> out;
-        out.set(v);
-        out.store(y + c);
+    for (int r = 0; r < R; ++r) {
+      mean[r] = s[r] * inv;
+      s[r] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (c0 + j * step < F) {
+          float v[VEC];
+          x[r].v[j].get(v);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) s[r] = fmaf(v[i] - mean[r], v[i] - mean[r], s[r]);
+        }
+    }
+    row_sums<WARP>(s, red, turn);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (row + r >= rows.end) break;
+      const float rstd = rsqrtf(s[r] * inv + p.eps);
+      if (c0 == 0 && p.mean) {
+        p.mean[row + r] = mean[r];
+        p.rstd[row + r] = rstd;
       }
+      T* y = static_cast<T*>(p.y) + (row + r) * F;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (c0 + j * step < F) {
+          float v[VEC], w[VEC], b[VEC];
+          x[r].v[j].get(v);
+          weight.v[j].get(w);
+          bias.v[j].get(b);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[i] = fmaf((v[i] - mean[r]) * rstd, one + w[i], b[i]);
+          Pack<T, VEC> out;
+          out.set(v);
+          out.store(y + c0 + j * step);
+        }
     }
   }
 }
@@ -160,7 +218,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) norm_fwd_kernel(const NormPa
 // through L2.
 template <typename T, typename TW>
 __global__ void __launch_bounds__(512) norm_fwd_long_kernel(const NormParams p) {
-  __shared__ float red[2][32][1];
+  __shared__ float red[2][16][1];
   int turn = 0;
   grid_dependency_wait();
   grid_dependents_launch();
@@ -171,14 +229,14 @@ __global__ void __launch_bounds__(512) norm_fwd_long_kernel(const NormParams p) 
     T* y = static_cast<T*>(p.y) + row * F;
     float s[1] = {0.0f};
     for (int c = threadIdx.x; c < F; c += blockDim.x) s[0] += Elem<T>::to_f(x[c]);
-    row_sum<false>(s, red, turn);
+    row_sums<false>(s, red, turn);
     const float mean = s[0] * inv;
     s[0] = 0.0f;
     for (int c = threadIdx.x; c < F; c += blockDim.x) {
       const float d = Elem<T>::to_f(x[c]) - mean;
       s[0] = fmaf(d, d, s[0]);
     }
-    row_sum<false>(s, red, turn);
+    row_sums<false>(s, red, turn);
     const float rstd = rsqrtf(s[0] * inv + p.eps);
     if (threadIdx.x == 0 && p.mean) {
       p.mean[row] = mean;
@@ -188,10 +246,9 @@ __global__ void __launch_bounds__(512) norm_fwd_long_kernel(const NormParams p) 
     const TW* weight = at<TW>(p.weight, offset);
     const TW* bias = at<TW>(p.bias, offset);
     for (int c = threadIdx.x; c < F; c += blockDim.x) {
-      float w[1];
-      weights<TW, 1>(p, weight, c, w);
+      const float w = weight_at<TW>(p, weight, c);
       y[c] = Elem<T>::from_f(
-          fmaf((Elem<T>::to_f(x[c]) - mean) * rstd, w[0], bias ? Elem<TW>::to_f(bias[c]) : 0.0f));
+          fmaf((Elem<T>::to_f(x[c]) - mean) * rstd, w, bias ? Elem<TW>::to_f(bias[c]) : 0.0f));
     }
   }
 }
@@ -199,12 +256,11 @@ __global__ void __launch_bounds__(512) norm_fwd_long_kernel(const NormParams p) 
 // ---------------------------------------------------------------------------
 // backward
 
-// CTA (segment, chunk) walks the rows of its chunk.  WARP: each of 4 warps a
-// row of its own; else the CTA one row at a time.
-template <typename T, typename TW, int VEC, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 512) norm_bwd_kernel(const NormParams p) {
-  __shared__ float red[2][32][2];
-  extern __shared__ float sums[];  // WARP: (4, 2, features)
+// R rows at a time, as in the forward pass.
+template <typename T, typename TW, int VEC, int NV, int R, bool WARP>
+__global__ void __launch_bounds__(WARP ? 32 * kWarps : (R == 2 ? 256 : 512)) norm_bwd_kernel(const NormParams p) {
+  __shared__ float red[2][16][2 * R];
+  extern __shared__ float sums[];  // WARP: (kWarps, 2, features)
   int turn = 0;
   grid_dependency_wait();
   grid_dependents_launch();
@@ -212,79 +268,73 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) norm_bwd_kernel(const NormPa
   const float inv = 1.0f / static_cast<float>(F);
   const int warp = threadIdx.x >> 5;
   const int c0 = (WARP ? threadIdx.x & 31 : threadIdx.x) * VEC, step = (WARP ? 32 : blockDim.x) * VEC;
-  const int64_t seg = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks;
-  const int64_t base = seg * p.rows_per_weight;
-  const int64_t r0 = base + p.rows_per_weight * chunk / p.chunks;
-  const int64_t r1 = base + p.rows_per_weight * (chunk + 1) / p.chunks;
-  const TW* weight = at<TW>(p.weight, seg * p.weight_stride);
-  const T* xs = static_cast<const T*>(p.x);
-  const T* dys = static_cast<const T*>(p.dy);
-  T* dxs = static_cast<T*>(p.y);
+  const Rows rows(p);
+  const auto weight = vector_of<TW, VEC, NV>(at<TW>(p.weight, rows.segment * p.weight_stride),
+                                             p.add_one ? 0.0f : 1.0f, c0, step, F);
+  const float one = p.add_one ? 1.0f : 0.0f;
   float dw[NV][VEC], db[NV][VEC];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[j][i] = db[j][i] = 0.0f;
-  const int64_t first = WARP ? r0 + warp : r0, stride = WARP ? 4 : 1;
-  // the next row's loads are in flight while this row is worked on, where the
-  // registers hold both
-  constexpr bool kAhead = NV * Pack<T, VEC>::kWords <= 8;
-  Share<T, VEC, NV> x, dy, next_x, next_dy;
-  float mean, rstd, next_mean = 0.0f, next_rstd = 0.0f;
-  auto fetch = [&](int64_t row) {
-    if (row < r1) {
-      next_x.load(xs + row * F, c0, step, F);
-      next_dy.load(dys + row * F, c0, step, F);
-      next_mean = __ldg(p.mean + row);
-      next_rstd = __ldg(p.rstd + row);
-    }
-  };
-  if (kAhead) fetch(first);
-  for (int64_t row = first; row < r1; row += stride) {
-    if (!kAhead) fetch(row);
-    x = next_x;
-    dy = next_dy;
-    mean = next_mean;
-    rstd = next_rstd;
-    if (kAhead) fetch(row + stride);
-    float s[2] = {0.0f, 0.0f};
+  const int64_t first = rows.begin + (WARP ? warp * R : 0);
+  for (int64_t row = first; row < rows.end; row += WARP ? kWarps * R : R) {
+    Share<T, VEC, NV> x[R], dy[R];
+    float mean[R], rstd[R], s[2 * R];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = c0 + j * step;
-      if (c < F) {
-        float v[VEC], d[VEC], w[VEC];
-        x.v[j].get(v);
-        dy.v[j].get(d);
-        weights<TW, VEC>(p, weight, c, w);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float h = (v[i] - mean) * rstd, g = d[i] * w[i];
-          dw[j][i] = fmaf(d[i], h, dw[j][i]);
-          db[j][i] += d[i];
-          s[0] += g;
-          s[1] = fmaf(g, h, s[1]);
-        }
+    for (int r = 0; r < R; ++r) {
+      mean[r] = rstd[r] = 0.0f;
+      if (row + r < rows.end) {
+        x[r].load(static_cast<const T*>(p.x) + (row + r) * F, c0, step, F);
+        dy[r].load(static_cast<const T*>(p.dy) + (row + r) * F, c0, step, F);
+        mean[r] = __ldg(p.mean + row + r);
+        rstd[r] = __ldg(p.rstd + row + r);
       }
     }
-    row_sum<WARP>(s, red, turn);
-    const float mg = s[0] * inv, mgh = s[1] * inv;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = c0 + j * step;
-      if (c < F) {
-        float v[VEC], d[VEC], w[VEC];
-        x.v[j].get(v);
-        dy.v[j].get(d);
-        weights<TW, VEC>(p, weight, c, w);
+    for (int r = 0; r < R; ++r) {
+      s[2 * r] = s[2 * r + 1] = 0.0f;
+      if (row + r < rows.end) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float h = (v[i] - mean) * rstd, g = d[i] * w[i];
-          v[i] = rstd * (g - mg - h * mgh);
-        }
-        Pack<T, VEC> out;
-        out.set(v);
-        out.store(dxs + row * F + c);
+        for (int j = 0; j < NV; ++j)
+          if (c0 + j * step < F) {
+            float v[VEC], d[VEC], w[VEC];
+            x[r].v[j].get(v);
+            dy[r].v[j].get(d);
+            weight.v[j].get(w);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              const float h = (v[i] - mean[r]) * rstd[r], g = d[i] * (one + w[i]);
+              dw[j][i] = fmaf(d[i], h, dw[j][i]);
+              db[j][i] += d[i];
+              s[2 * r] += g;
+              s[2 * r + 1] = fmaf(g, h, s[2 * r + 1]);
+            }
+          }
       }
+    }
+    row_sums<WARP>(s, red, turn);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (row + r >= rows.end) break;
+      const float mg = s[2 * r] * inv, mgh = s[2 * r + 1] * inv;
+      T* dx = static_cast<T*>(p.y) + (row + r) * F;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (c0 + j * step < F) {
+          float v[VEC], d[VEC], w[VEC];
+          x[r].v[j].get(v);
+          dy[r].v[j].get(d);
+          weight.v[j].get(w);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float h = (v[i] - mean[r]) * rstd[r];
+            v[i] = rstd[r] * (fmaf(d[i], one + w[i], -mg) - h * mgh);
+          }
+          Pack<T, VEC> out;
+          out.set(v);
+          out.store(dx + c0 + j * step);
+        }
     }
   }
   if (!p.partial) return;
@@ -301,7 +351,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) norm_bwd_kernel(const NormPa
         }
       }
     __syncthreads();
-    for (int c = threadIdx.x; c < 2 * F; c += 128)
+    for (int c = threadIdx.x; c < 2 * F; c += 32 * kWarps)
       part[c] = (sums[c] + sums[2 * F + c]) + (sums[4 * F + c] + sums[6 * F + c]);
   } else {
 #pragma unroll
@@ -330,7 +380,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 512) norm_bwd_kernel(const NormPa
 // Rows too long for the registers: dx alone, in two passes over the row ...
 template <typename T, typename TW>
 __global__ void __launch_bounds__(512) norm_dx_long_kernel(const NormParams p) {
-  __shared__ float red[2][32][2];
+  __shared__ float red[2][16][2];
   int turn = 0;
   grid_dependency_wait();
   grid_dependents_launch();
@@ -344,18 +394,16 @@ __global__ void __launch_bounds__(512) norm_dx_long_kernel(const NormParams p) {
     const float mean = p.mean[row], rstd = p.rstd[row];
     float s[2] = {0.0f, 0.0f};
     for (int c = threadIdx.x; c < F; c += blockDim.x) {
-      float w[1];
-      weights<TW, 1>(p, weight, c, w);
-      const float g = Elem<T>::to_f(dy[c]) * w[0];
+      const float w = weight_at<TW>(p, weight, c);
+      const float g = Elem<T>::to_f(dy[c]) * w;
       s[0] += g;
       s[1] = fmaf(g, (Elem<T>::to_f(x[c]) - mean) * rstd, s[1]);
     }
-    row_sum<false>(s, red, turn);
+    row_sums<false>(s, red, turn);
     const float mg = s[0] * inv, mgh = s[1] * inv;
     for (int c = threadIdx.x; c < F; c += blockDim.x) {
-      float w[1];
-      weights<TW, 1>(p, weight, c, w);
-      const float g = Elem<T>::to_f(dy[c]) * w[0], h = (Elem<T>::to_f(x[c]) - mean) * rstd;
+      const float w = weight_at<TW>(p, weight, c);
+      const float g = Elem<T>::to_f(dy[c]) * w, h = (Elem<T>::to_f(x[c]) - mean) * rstd;
       dx[c] = Elem<T>::from_f(rstd * (g - mg - h * mgh));
     }
   }
@@ -397,7 +445,7 @@ __global__ void __launch_bounds__(512) norm_reduce_kernel(const NormParams p) {
   float dw = 0.0f, db = 0.0f;
   if (c < F) {
     const float* part = p.partial + seg * p.chunks * 2 * F;
-#pragma unroll 4
+#pragma unroll 8
     for (int chunk = y; chunk < p.chunks; chunk += 16) {
       dw += part[static_cast<int64_t>(chunk) * 2 * F + c];
       db += part[static_cast<int64_t>(chunk) * 2 * F + F + c];
@@ -423,11 +471,11 @@ __global__ void __launch_bounds__(512) norm_reduce_kernel(const NormParams p) {
 // ---------------------------------------------------------------------------
 // launches
 
-// CTAs that share a segment's rows, each with one partial sum: about two CTAs
-// for each SM in all.
+// Most CTAs that share a segment's rows, each with one partial sum: about four
+// for each SM in all, and at least 16 rows each.
 int chunks_of(int64_t rows_per_weight, int64_t segments) {
-  int64_t chunks = 2LL * device_sm_count() / segments;
-  if (chunks > rows_per_weight) chunks = rows_per_weight;
+  int64_t chunks = 4LL * device_sm_count() / segments;
+  if (chunks > rows_per_weight / 16) chunks = rows_per_weight / 16;
   return static_cast<int>(chunks < 1 ? 1 : chunks);
 }
 
@@ -446,24 +494,15 @@ int enqueue(void (*kernel)(NormParams), dim3 grid, int threads, size_t smem, con
   return check_launch("layer norm kernel");
 }
 
-// How a row is spread over threads: `wide` elements a vector where every row
-// and vector is aligned for it, else single elements.
-template <typename T>
-struct Plan {
-  static constexpr int kWide = 16 / sizeof(T);
-  bool wide;
-  int vectors;
-  Plan(const NormParams& p, bool weight_ok) {
-    wide = p.features % kWide == 0 && aligned_to(p.x, 16) && aligned_to(p.y, 16) && aligned_to(p.dy, 16) && weight_ok;
-    vectors = wide ? p.features / kWide : p.features;
-  }
-};
-
-template <typename TW>
-bool weight_aligned(const NormParams& p, int vec) {
-  const int64_t bytes = vec * static_cast<int64_t>(sizeof(TW)) < 16 ? vec * sizeof(TW) : 16;
-  return aligned_to(p.weight, bytes) && aligned_to(p.bias, bytes) &&
-         p.weight_stride * static_cast<int64_t>(sizeof(TW)) % bytes == 0;
+// Whether every vector of `vec` elements of the rows and of the weights is
+// aligned for its accesses.
+template <typename T, typename TW>
+bool aligned_for(const NormParams& p, int vec) {
+  const int64_t bytes = vec * sizeof(T) < 16 ? vec * sizeof(T) : 16;
+  const int64_t wbytes = vec * sizeof(TW) < 16 ? vec * sizeof(TW) : 16;
+  return p.features % vec == 0 && aligned_to(p.x, bytes) && aligned_to(p.y, bytes) && aligned_to(p.dy, bytes) &&
+         aligned_to(p.weight, wbytes) && aligned_to(p.bias, wbytes) &&
+         p.weight_stride * static_cast<int64_t>(sizeof(TW)) % wbytes == 0;
 }
 
 inline unsigned rows_grid(int64_t rows, int64_t per_cta, int64_t most) {
@@ -471,42 +510,55 @@ inline unsigned rows_grid(int64_t rows, int64_t per_cta, int64_t most) {
   return static_cast<unsigned>(ctas < most ? ctas : most);
 }
 
+// Threads that share a row of `vectors` vectors, NV each.
+constexpr int threads_of(int vectors, int nv) { return ((vectors + nv - 1) / nv + 31) / 32 * 32; }
+
+// NV counts in units of E vectors: 1 of 16 bytes, or 4 of one or two elements.
 template <typename T, typename TW, int VEC, int E>
-int forward_rows(const NormParams& p, int vectors, cudaStream_t s) {
-  // E: vectors that make 16 bytes' worth of elements (1 when wide)
-  const int64_t most = 64LL * device_sm_count();
-  if (vectors <= 32 * 4 * E) return enqueue(norm_fwd_kernel<T, TW, VEC, 4 * E, true>, rows_grid(p.rows, 4, most), 128, 0, p, s);
-  if (VEC > 1 && vectors <= 32 * 12 && p.rows >= 4LL * device_sm_count())
-    return enqueue(norm_fwd_kernel<T, TW, VEC, (VEC > 1 ? 12 : 4), true>, rows_grid(p.rows, 4, most), 128, 0, p, s);
-  const int per = vectors <= 512 * E ? E : 4 * E;
-  const int threads = (((vectors + per - 1) / per) + 31) / 32 * 32;
-  if (vectors <= 512 * E) return enqueue(norm_fwd_kernel<T, TW, VEC, E, false>, rows_grid(p.rows, 1, most), threads, 0, p, s);
-  if (vectors <= 512 * 4 * E)
-    return enqueue(norm_fwd_kernel<T, TW, VEC, 4 * E, false>, rows_grid(p.rows, 1, most), threads, 0, p, s);
-  return enqueue(norm_fwd_long_kernel<T, TW>, rows_grid(p.rows, 1, most), 512, 0, p, s);
+int forward_rows(NormParams p, int vectors, cudaStream_t s) {
+  const int64_t segments = p.rows / p.rows_per_weight;
+  // CTAs: for a few rows at a time each, many enough to fill the GPU
+  auto grid = [&](int64_t rows_at, int64_t most) {
+    int64_t chunks = (p.rows_per_weight + rows_at - 1) / rows_at, limit = (most * device_sm_count() + segments - 1) / segments;
+    p.chunks = static_cast<int>(chunks < limit ? chunks : limit);
+    return dim3(static_cast<unsigned>(segments * p.chunks));
+  };
+  if (vectors <= 32 * 4 * E) {
+    const dim3 g = grid(kWarps, 8);
+    return enqueue(norm_fwd_kernel<T, TW, VEC, 4 * E, 1, true>, g, 32 * kWarps, 0, p, s);
+  }
+  if (vectors <= 256 * 3 * E) {
+    const int threads = threads_of(vectors, 3 * E);
+    const dim3 g = grid(1, threads <= 128 ? 8 : 1024 / threads);
+    return enqueue(norm_fwd_kernel<T, TW, VEC, 3 * E, 2, false>, g, threads, 0, p, s);
+  }
+  if (vectors <= 512 * 4 * E) {
+    const dim3 g = grid(1, 2);
+    return enqueue(norm_fwd_kernel<T, TW, VEC, 4 * E, 1, false>, g, 512, 0, p, s);
+  }
+  return enqueue(norm_fwd_long_kernel<T, TW>, rows_grid(p.rows, 1, 8LL * device_sm_count()), 512, 0, p, s);
 }
 
 template <typename T, typename TW>
 int forward(const NormParams& p, cudaStream_t s) {
-  constexpr int W = Plan<T>::kWide;
-  const Plan<T> plan(p, weight_aligned<TW>(p, W));
-  if (plan.wide) return forward_rows<T, TW, W, 1>(p, plan.vectors, s);
-  return forward_rows<T, TW, 1, W>(p, plan.vectors, s);
+  constexpr int W = 16 / sizeof(T);
+  if (aligned_for<T, TW>(p, W)) return forward_rows<T, TW, W, 1>(p, p.features / W, s);
+  if constexpr (W == 8)
+    if (aligned_for<T, TW>(p, 2)) return forward_rows<T, TW, 2, 4>(p, p.features / 2, s);
+  return forward_rows<T, TW, 1, 4>(p, p.features, s);
 }
 
 template <typename T, typename TW, int VEC, int E>
 int backward_rows(const NormParams& p, int vectors, cudaStream_t s) {
   const unsigned ctas = static_cast<unsigned>(p.rows / p.rows_per_weight * p.chunks);
   if (vectors <= 32 * 4 * E)
-    return enqueue(norm_bwd_kernel<T, TW, VEC, 4 * E, true>, ctas, 128, 8 * sizeof(float) * p.features, p, s);
-  const int most = sizeof(T) == 2 ? 4 : 4;
-  const int per = vectors <= 512 * E ? 1 : vectors <= 1024 * E ? 2 : most;
-  const int threads = ((vectors + per * E - 1) / (per * E) + 31) / 32 * 32;
-  if (vectors <= 512 * E) return enqueue(norm_bwd_kernel<T, TW, VEC, E, false>, ctas, threads, 0, p, s);
-  if (vectors <= 1024 * E) return enqueue(norm_bwd_kernel<T, TW, VEC, 2 * E, false>, ctas, threads, 0, p, s);
-  if (vectors <= 2048 * E) return enqueue(norm_bwd_kernel<T, TW, VEC, 4 * E, false>, ctas, threads, 0, p, s);
-  const unsigned most_rows = rows_grid(p.rows, 1, 8LL * device_sm_count());
-  int rc = enqueue(norm_dx_long_kernel<T, TW>, most_rows, 512, 0, p, s);
+    return enqueue(norm_bwd_kernel<T, TW, VEC, 4 * E, 1, true>, ctas, 32 * kWarps, 2 * kWarps * sizeof(float) * p.features,
+                   p, s);
+  if (vectors <= 256 * 3 * E)
+    return enqueue(norm_bwd_kernel<T, TW, VEC, 3 * E, 2, false>, ctas, threads_of(vectors, 3 * E), 0, p, s);
+  if (vectors <= 512 * 4 * E)
+    return enqueue(norm_bwd_kernel<T, TW, VEC, 4 * E, 1, false>, ctas, threads_of(vectors, 4 * E), 0, p, s);
+  int rc = enqueue(norm_dx_long_kernel<T, TW>, rows_grid(p.rows, 1, 8LL * device_sm_count()), 512, 0, p, s);
   if (rc == CONVROT_OK && p.partial)
     rc = enqueue(norm_partial_long_kernel<T>, dim3((p.features + 255) / 256, ctas), 256, 0, p, s);
   return rc;
@@ -514,9 +566,11 @@ int backward_rows(const NormParams& p, int vectors, cudaStream_t s) {
 
 template <typename T, typename TW>
 int backward(const NormParams& p, cudaStream_t s) {
-  constexpr int W = Plan<T>::kWide;
-  const Plan<T> plan(p, weight_aligned<TW>(p, W));
-  const int rc = plan.wide ? backward_rows<T, TW, W, 1>(p, plan.vectors, s) : backward_rows<T, TW, 1, W>(p, plan.vectors, s);
+  constexpr int W = 16 / sizeof(T);
+  int rc;
+  if (aligned_for<T, TW>(p, W)) rc = backward_rows<T, TW, W, 1>(p, p.features / W, s);
+  else if (W == 8 && aligned_for<T, TW>(p, 2)) rc = backward_rows<T, TW, (W == 8 ? 2 : 1), 4>(p, p.features / 2, s);
+  else rc = backward_rows<T, TW, 1, 4>(p, p.features, s);
   if (rc != CONVROT_OK || !p.partial) return rc;
   const unsigned segments = static_cast<unsigned>(p.rows / p.rows_per_weight);
   return enqueue(norm_reduce_kernel<TW>, dim3((p.features + 31) / 32, segments), 512, 0, p, s);

@@ -119,17 +119,21 @@ __global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ 
     T* out = static_cast<T*>(t.out) + b * t.out_b + token * t.out_t + e0;
     // the next heads' values are in flight while these are turned
     Unit<T, VEC, WIDE> x[kUnroll], y[ADJACENT ? 1 : kUnroll], nx[kUnroll], ny[ADJACENT ? 1 : kUnroll];
+    const int begin = max(h0, lo);
+    const T* src = in + (begin - lo) * t.in_h;
+    T* dst = out + (begin - lo) * t.out_h;
+    const int64_t src_step = t.in_h, dst_step = t.out_h;
     auto fetch = [&](int h) {
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k)
+      for (int k = 0; k < kUnroll; ++k) {
         if (h + k < hi) {
-          const T* src = in + (h + k - lo) * t.in_h;
           nx[k].load(src, left);
           if constexpr (!ADJACENT)
             if (turns) ny[k].load(src + p.pairs, VEC);
         }
+        src += src_step;
+      }
     };
-    const int begin = max(h0, lo);
     fetch(begin);
 #pragma unroll 1
     for (int h = begin; h < hi; h += kUnroll) {
@@ -140,9 +144,8 @@ __global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ 
       }
       fetch(h + kUnroll);
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k)
+      for (int k = 0; k < kUnroll; ++k) {
         if (h + k < hi) {
-          T* dst = out + (h + k - lo) * t.out_h;
           if constexpr (ADJACENT) {
             // values past the pairs keep their bits
             float v[VEC];
@@ -171,6 +174,8 @@ __global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ 
           }
           x[k].store(dst, left);
         }
+        dst += dst_step;
+      }
     }
   }
 }
