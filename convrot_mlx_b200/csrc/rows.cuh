@@ -32,6 +32,49 @@ __device__ __forceinline__ __nv_bfloat162 pair_of<__nv_bfloat16>(float a, float 
 template <>
 __device__ __forceinline__ __half2 pair_of<__half>(float a, float b) { return __floats2half2_rn(a, b); }
 
+// Two float32 values in a register pair, for the paired instructions (one
+// issue slot for two operations), and the same operations on one float32.
+using P2 = unsigned long long;
+__device__ __forceinline__ P2 p2(float lo, float hi) {
+  P2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 p2_get(P2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ P2 add(P2 a, P2 b) {
+  P2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ P2 mul(P2 a, P2 b) {
+  P2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ P2 fma(P2 a, P2 b, P2 c) {
+  P2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+__device__ __forceinline__ float mul(float a, float b) { return a * b; }
+__device__ __forceinline__ float fma(float a, float b, float c) { return __fmaf_rn(a, b, c); }
+__device__ __forceinline__ float total(P2 a) { return p2_get(a).x + p2_get(a).y; }
+__device__ __forceinline__ float total(float a) { return a; }
+
+// What a vector of VEC values is calculated in: pairs, or one float32.
+template <int VEC> using Lane = typename std::conditional<VEC == 1, float, P2>::type;
+template <int VEC> constexpr int kLanes = (VEC + 1) / 2;
+template <int VEC>
+__device__ __forceinline__ Lane<VEC> splat(float v) {
+  if constexpr (VEC == 1) return v;
+  else return p2(v, v);
+}
+
 // VEC packed elements of T to float32.
 template <typename T, int VEC>
 __device__ __forceinline__ void unpack(const uint32_t* w, float (&v)[VEC]) {
@@ -39,6 +82,8 @@ __device__ __forceinline__ void unpack(const uint32_t* w, float (&v)[VEC]) {
   for (int i = 0; i < VEC; ++i) {
     if constexpr (sizeof(T) == 4) {
       v[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      v[i] = __uint_as_float(i % 2 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16);
     } else {
       const typename Elem<T>::Pair h = *reinterpret_cast<const typename Elem<T>::Pair*>(&w[i / 2]);
       v[i] = Elem<T>::to_f(i % 2 ? Elem<T>::hi(h) : Elem<T>::lo(h));
@@ -140,6 +185,30 @@ struct Pack {
     }
   }
   __device__ __forceinline__ void get(float (&v)[VEC]) const { unpack<T, VEC>(w, v); }
+  __device__ __forceinline__ void get_lanes(Lane<VEC> (&v)[kLanes<VEC>]) const {
+    float f[VEC];
+    unpack<T, VEC>(w, f);
+    if constexpr (VEC == 1) {
+      v[0] = f[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) v[i] = p2(f[2 * i], f[2 * i + 1]);
+    }
+  }
+  __device__ __forceinline__ void set_lanes(const Lane<VEC> (&v)[kLanes<VEC>]) {
+    if constexpr (VEC == 1) {
+      set(v);
+    } else {
+      float f[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        const float2 p = p2_get(v[i]);
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
+      }
+      set(f);
+    }
+  }
   __device__ __forceinline__ void set(const float (&v)[VEC]) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
