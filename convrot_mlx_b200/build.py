@@ -3,8 +3,10 @@
     python -m convrot_mlx_b200.build [--force] [--jobs N]
 
 Each ``csrc/*.cu`` is compiled to an object under ``_build/`` (in parallel),
-then linked into ``convrot_mlx_b200/libconvrot_b200.so``.  A source newer than
-the library (or a changed header) triggers a rebuild.
+then linked into ``convrot_mlx_b200/libconvrot_b200.so``; ``binding/ops.cpp``,
+the torch binding of the 8-bit and training operators, becomes
+``convrot_mlx_b200/_native_ops.so`` beside it.  A source newer than its product
+(or a changed header) triggers a rebuild.
 """
 
 from __future__ import annotations
@@ -14,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -22,6 +25,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = ROOT / "_build"
 LIB = PKG / "libconvrot_b200.so"
+OPS_SRC = PKG / "binding" / "ops.cpp"
+OPS_LIB = PKG / "_native_ops.so"
 HEADERS = [ROOT / "include" / "convrot_b200.h", *sorted(CSRC.glob("*.cuh"))]
 
 NVCC_FLAGS = [
@@ -44,6 +49,28 @@ def _stale(target: Path, deps) -> bool:
         return True
     t = target.stat().st_mtime
     return any(Path(d).stat().st_mtime > t for d in deps)
+
+
+def _build_ops(force: bool, verbose: bool) -> None:
+    """Compile the torch binding against the installed torch's headers."""
+
+    if not force and not _stale(OPS_LIB, [OPS_SRC, HEADERS[0]]):
+        return
+    import torch
+    from torch.utils import cpp_extension
+
+    includes = [ROOT / "include", *cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"]]
+    libs = cpp_extension.library_paths("cuda")
+    cmd = ["g++", "-shared", "-fPIC", "-O2", "-std=c++17", "-w", "-DTORCH_EXTENSION_NAME=_native_ops",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(f"-I{i}" for i in includes), str(OPS_SRC), "-o", str(OPS_LIB),
+           f"-L{PKG}", "-l:libconvrot_b200.so", "-Wl,-rpath,$ORIGIN", *(f"-L{d}" for d in libs),
+           "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {OPS_SRC.name}:\n{res.stdout}\n{res.stderr}")
 
 
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -> Path:
@@ -78,6 +105,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False) -
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    _build_ops(force, verbose)
     return LIB
 
 

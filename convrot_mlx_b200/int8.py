@@ -13,9 +13,8 @@ from __future__ import annotations
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
-from . import _lib
+from . import _lib, _native
 from .core import _dtype_code, _f32_vec, _require_cuda
 
 INT8_MAX = 127
@@ -115,43 +114,6 @@ def int8_matmul(codes, qweight, xscales, wscales, bias=None, *, output_dtype) ->
     return out
 
 
-def _product(x2, col_scale, qweight, layout, wscales, bias, n) -> torch.Tensor:
-    """The quantizer and the product in one call; x2 as ``_rows`` gives it."""
-
-    m, k = x2.shape
-    pitch = -(-k // _PITCH) * _PITCH
-    out = x2.new_empty((m, n))
-    # codes, then scales (16-byte aligned: the pitch is)
-    space = torch.empty((m * (pitch + 4),), dtype=torch.int8, device=x2.device)
-    codes, dtype = space.data_ptr(), _dtype_code(x2.dtype)
-    _lib.call("convrot_i8_linear", x2.get_device(), x2.data_ptr(), dtype, x2.stride(0),
-              None if col_scale is None else col_scale.data_ptr(), qweight.data_ptr(), qweight.stride(0), layout,
-              None if wscales is None else wscales.data_ptr(), None if bias is None else bias.data_ptr(),
-              out.data_ptr(), dtype, m, n, k, codes, pitch, codes + m * pitch)
-    return out
-
-
-def _forward(x, qweight, wscales, bias):
-    n = qweight.shape[0]
-    out = _product(_rows(x), None, qweight, _lib.LAYOUT_NK, wscales, bias, n)
-    return out if x.ndim == 2 else out.view(*x.shape[:-1], n)
-
-
-class _Int8Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, qweight, wscales, bias):
-        ctx.save_for_backward(qweight, wscales)
-        return _forward(x, qweight, wscales, bias)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        qweight, wscales = ctx.saved_tensors
-        k = qweight.shape[1]
-        dx = _product(_rows(dy), wscales, qweight, _lib.LAYOUT_KN, None, None, k)
-        return dx if dy.ndim == 2 else dx.view(*dy.shape[:-1], k), None, None, None
-
-
 def int8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor,
                 bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ (qweight * wscales[:, None]).T + bias`` with x quantized to 8 bits for each token.
@@ -162,18 +124,7 @@ def int8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor,
     dy * wscales is quantized for each token in turn and multiplied with the
     same weight.  The weight, its scales and the bias are frozen."""
 
-    if x.ndim == 0:
-        raise ValueError("int8 linear expects at least one dimension")
-    _validate(x.shape[-1], qweight, wscales, bias)
-    if wscales.requires_grad or (bias is not None and bias.requires_grad):
-        raise ValueError("the weight scales and the bias of an int8 linear are frozen: they may not require gradients")
-    _dtype_code(x.dtype)
-    _require_cuda(x, qweight, wscales, bias)
-    qweight, wscales = _padded_rows(qweight), _f32(wscales)
-    bias = None if bias is None else _f32(bias)
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _Int8Linear.apply(x, qweight, wscales, bias)
-    return _forward(x, qweight, wscales, bias)
+    return _native.ops().int8_linear(x, qweight, wscales, bias)
 
 
 class Int8Linear(nn.Module):
