@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(256) gelu_fwd_kernel(const GeluParams p) {
 #pragma unroll
     for (int j = 0; j < S::kVectors; ++j) {
       const int c = (lane + j * S::kLanes) * VEC;
-      if (FULL ? length[u] > 0 : c < length[u]) raw[u][j].load_nc(x + base[u] + c);
+      if (FULL ? length[u] > 0 : c < length[u]) raw[u][j].load_ahead(x + base[u] + c);
     }
   }
   if (p.codes) {
@@ -126,7 +126,8 @@ __global__ void __launch_bounds__(256) gelu_fwd_kernel(const GeluParams p) {
           float v[VEC];
           uint32_t code[VEC];
           raw[u][j].get(v);
-          quant.codes(v, code);
+          if (quant.tiny()) Quant8<float>(quant.bits).codes(v, code);
+          else quant.codes(v, code);
           store_codes<VEC>(p.codes + base[u] + c, code, quant.mask());
         }
       }
@@ -166,13 +167,13 @@ __global__ void __launch_bounds__(256) gelu_bwd_kernel(const GeluParams p) {
   for (int u = 0; u < kUnroll; ++u) {
     const uint32_t group = first + u * S::kSets;
     locate<FULL>(p, group, base[u], length[u]);
-    scale[u] = length[u] > 0 ? __ldg(p.scales + group) : 0.0f;
+    scale[u] = length[u] > 0 ? ld_f32(p.scales + group) : 0.0f;
 #pragma unroll
     for (int j = 0; j < S::kVectors; ++j) {
       const int c = (lane + j * S::kLanes) * VEC;
       if (FULL ? length[u] > 0 : c < length[u]) {
-        raw[u][j].load_nc(dy + base[u] + c);
-        codes[u][j].load_nc(reinterpret_cast<const uint8_t*>(p.codes) + base[u] + c);
+        raw[u][j].load_ahead(dy + base[u] + c);
+        codes[u][j].load_ahead(reinterpret_cast<const uint8_t*>(p.codes) + base[u] + c);
       }
     }
   }

@@ -7,15 +7,18 @@
 // product of the input's gradient.  Integer sums are exact, so neither the
 // tiling nor the split of K changes a bit.
 //
-// Two kernels on tcgen05 kind::i8, operands by TMA in 128-byte-swizzled
-// tiles, accumulators in TMEM:
+// Up to 8 tokens of the forward product: gemv_kernel, weights from memory into
+// mma.sync fragments, bound by reading them once and by latency.  Else two
+// kernels on tcgen05 kind::i8, operands by TMA in 128-byte-swizzled tiles,
+// accumulators in TMEM:
 // * pair_kernel: CTA pairs (cta_group::2), 256 tokens x 256 channels a tile,
 //   persistent, for products that fill the GPU with such tiles.  Bound by the
 //   tensor cores.
 // * swap_kernel: 128 channels on the MMA's M side and 16 to 128 tokens on its
-//   N side, K split over a cluster, for few tokens or few tiles.  Bound by
-//   reading the weights once.
+//   N side, K split over a cluster, for few tokens or few tiles.
 #include <cudaTypedefs.h>
+
+#include <algorithm>
 
 #include "rows.cuh"
 
@@ -109,6 +112,7 @@ __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorM
 namespace pair {
 
 constexpr int kTile = 256;
+constexpr int kBand = 8;
 constexpr int kStages = 6;
 constexpr int kOpBytes = 128 * kBK;  // one operand's half tile of a stage
 constexpr int kWarpA = 0, kWarpMma = 1, kWarpB = 2, kWarpE0 = 4, kEWarps = 8;
@@ -149,6 +153,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int m_tiles = (p.m + kTile - 1) / kTile, n_tiles = (p.n + kTile - 1) / kTile;
   const int num_tiles = m_tiles * n_tiles;
   const int k_stages = (p.k + kBK - 1) / kBK;
+  // Tiles in bands of kBand token tiles, within a band all of these for one
+  // channel tile, then the next: the tiles in work at one time then share
+  // about as many rows of either operand in L2.
+  auto place = [&](int tile, int& m_blk, int& n_blk) {
+    const int band = tile / (kBand * n_tiles), first = band * kBand;
+    const int rows = min(kBand, m_tiles - first), at = tile - first * n_tiles;
+    n_blk = at / rows;
+    m_blk = first + at - n_blk * rows;
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -182,8 +195,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       int g = 0;
       bool ok = true;
       for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs) {
-        const int row = (tile % m_tiles) * kTile + 128 * rank;
-        const int col = (tile / m_tiles) * kTile + 128 * rank;
+        int m_blk, n_blk;
+        place(tile, m_blk, n_blk);
+        const int row = m_blk * kTile + 128 * rank, col = n_blk * kTile + 128 * rank;
         for (int ks = 0; ks < k_stages; ++ks, ++g) {
           if (g % kStages != lane) continue;
           if (!wait(&bars->empty[lane], ((g / kStages) & 1) ^ 1, &bars->err, 61)) { ok = false; break; }
@@ -242,14 +256,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     int local = 0;
     for (int tile = pair_id; tile < num_tiles; tile += num_pairs, ++local) {
       const int buf = local & 1;
-      const int row0 = (tile % m_tiles) * kTile + 128 * rank + quarter * 32;
-      const int col0 = (tile / m_tiles) * kTile + 128 * half;
-      const float xs = row0 + lane < p.m ? __ldg(p.xscales + row0 + lane) : 0.0f;
+      int m_blk, n_blk;
+      place(tile, m_blk, n_blk);
+      const int row0 = m_blk * kTile + 128 * rank + quarter * 32, col0 = n_blk * kTile + 128 * half;
+      const float xs = row0 + lane < p.m ? ld_f32(p.xscales + row0 + lane) : 0.0f;
       __syncwarp();  // the previous tile's reads of the vectors are done
       for (int j = lane; j < 128; j += 32) {
         const bool in = col0 + j < p.n;
-        sws[j] = in ? (p.wscales ? __ldg(p.wscales + col0 + j) : 1.0f) : 0.0f;
-        sbias[j] = in && p.bias ? __ldg(p.bias + col0 + j) : 0.0f;
+        sws[j] = in ? (p.wscales ? ld_f32(p.wscales + col0 + j) : 1.0f) : 0.0f;
+        sbias[j] = in && p.bias ? ld_f32(p.bias + col0 + j) : 0.0f;
       }
       __syncwarp();
       if (!wait(&bars->acc_full[buf], (local >> 1) & 1, &bars->err, 65)) break;
@@ -303,16 +318,25 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           } else {
-            // rows off the 16-byte grid: one element a lane, consecutive lanes on consecutive columns
+            // rows off the 16-byte grid: one element a lane, consecutive
+            // lanes on consecutive columns, eight rows' reads at a time
             constexpr int kRowsAt = 32 / kCols;
-            const int cc = lane % kCols;
-            if (col + cc < p.n) {
-              for (int rr = lane / kCols; rr < 32; rr += kRowsAt) {
-                if (row0 + rr >= p.m) break;
-                const int q = cc / (kCols / 4), e = cc % (kCols / 4);
-                const uint8_t* src = stage_out + ew * kChunkBytes + rr * 64 + (((q + (rr >> 1)) & 3) << 4);
-                out[static_cast<int64_t>(row0 + rr) * p.n + col + cc] = reinterpret_cast<const TOut*>(src)[e];
+            const int cc = lane % kCols, q = cc / (kCols / 4), e = cc % (kCols / 4);
+            TOut* dst = out + static_cast<int64_t>(row0 + lane / kCols) * p.n + col + cc;
+            const int64_t step = static_cast<int64_t>(kRowsAt) * p.n;
+            const bool col_ok = col + cc < p.n;
+#pragma unroll
+            for (int r0 = 0; r0 < 32; r0 += 8 * kRowsAt) {
+              TOut v8[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int rr = r0 + i * kRowsAt + lane / kCols;
+                v8[i] = reinterpret_cast<const TOut*>(stage_out + ew * kChunkBytes + rr * 64 +
+                                                      (((q + (rr >> 1)) & 3) << 4))[e];
               }
+#pragma unroll
+              for (int i = 0; i < 8; ++i, dst += step)
+                if (col_ok && row0 + r0 + i * kRowsAt + lane / kCols < p.m) *dst = v8[i];
             }
           }
         }
@@ -363,10 +387,12 @@ struct alignas(8) Bars {
   int err;
 };
 
-template <int BT> constexpr int kStages = BT <= 32 ? 8 : (BT == 64 ? 8 : 6);
+// two CTAs for each SM
+template <int BT> constexpr int kStages = BT <= 32 ? 5 : (BT == 64 ? 4 : 3);
 template <int BT> constexpr int kXBytes = BT * kBK;
-template <int BT> constexpr size_t kSmem = 1024 + kStages<BT> * (kWBytes + kXBytes<BT>) + sizeof(Bars);
-static_assert(kSmem<128> <= 232448 && kSmem<64> <= 232448, "shared memory budget");
+template <int BT>
+constexpr size_t kSmem = 1024 + kStages<BT> * (kWBytes + kXBytes<BT>) + (BT + 4) * 4 + sizeof(Bars);
+static_assert(kSmem<128> <= 113 * 1024 && kSmem<64> <= 113 * 1024 && kSmem<32> <= 113 * 1024, "shared memory budget");
 
 __device__ __forceinline__ uint32_t dsmem_ld(uint32_t cluster_addr) {
   uint32_t v;
@@ -375,14 +401,15 @@ __device__ __forceinline__ uint32_t dsmem_ld(uint32_t cluster_addr) {
 }
 
 template <int LAYOUT, typename TOut, int BT>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
     swap_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const Params p) {
   constexpr int S = kStages<BT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sW = smem;
   uint8_t* sX = sW + S * kWBytes;
-  Bars* bars = reinterpret_cast<Bars*>(sX + S * kXBytes<BT>);
+  float* xs = reinterpret_cast<float*>(sX + S * kXBytes<BT>);  // the tokens' scales
+  Bars* bars = reinterpret_cast<Bars*>(xs + BT + 4);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int ranks = gridDim.x, rank = blockIdx.x;  // the cluster spans the grid's x
@@ -413,6 +440,7 @@ __global__ void __launch_bounds__(kThreads)
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
   if (!(warp == 0 && p.early_weights)) grid_dependency_wait();
+  grid_dependents_launch();
 
   if (warp == 0 || warp == 2) {
     if (lane < S) {
@@ -454,35 +482,50 @@ __global__ void __launch_bounds__(kThreads)
     mma_commit(&bars->mma_done);
   }
   __syncwarp();
-  grid_dependency_wait();  // warp 0 may not have waited yet; the epilogue reads the token scales
-  grid_dependents_launch();
+  if (warp == 3) {  // has waited for the previous kernel
+    for (int c = lane; c < BT + 4; c += 32) xs[c] = m0 + c < p.m ? ld_f32(p.xscales + m0 + c) : 0.0f;
+  }
+  __syncthreads();
   const bool done = wait(&bars->mma_done, 0, &bars->err, 74);
   tc_fence_after();
 
   const int n = n0 + warp * 32 + lane;
   const bool n_ok = n < p.n;
-  const float ws = n_ok && p.wscales ? __ldg(p.wscales + n) : 1.0f;
-  const float b = n_ok && p.bias ? __ldg(p.bias + n) : 0.0f;
+  const float ws = n_ok && p.wscales ? ld_f32(p.wscales + n) : 1.0f;
+  const float b = n_ok && p.bias ? ld_f32(p.bias + n) : 0.0f;
   TOut* out = static_cast<TOut*>(p.out);
   const uint32_t t_row = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
-  auto emit = [&](int m, int32_t dot) {
-    const float v = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(dot), __ldg(p.xscales + m)), ws), b);
-    if (n_ok) out[static_cast<int64_t>(m) * p.n + n] = cvt_out<TOut>(v);
+  const int rows = p.m - m0 < BT ? p.m - m0 : BT;
+  // N tokens from c on, of which the first `count` exist: all values first,
+  // then all stores, since one warp a scheduler has only itself to overlap
+  auto emit = [&](auto& dots, int c, int count) {
+    constexpr int N = sizeof(dots) / sizeof(dots[0]);
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(static_cast<int32_t>(dots[i])), xs[c + i]), ws), b);
+    TOut* dst = out + static_cast<int64_t>(m0 + c) * p.n + n;
+    if (count >= N && n_ok) {
+#pragma unroll
+      for (int i = 0; i < N; ++i, dst += p.n) *dst = cvt_out<TOut>(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i, dst += p.n)
+        if (i < count && n_ok) *dst = cvt_out<TOut>(v[i]);
+    }
   };
   if (ranks == 1) {
-    for (int c = 0; c < BT && m0 + c < p.m && done; c += 16) {
+    for (int c = 0; c < rows && done; c += 16) {
       uint32_t r[16];
       __syncwarp();
       tmem_ld_32x32b_x16(t_row + c, r);
       tmem_ld_wait();
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (m0 + c + i < p.m) emit(m0 + c + i, static_cast<int32_t>(r[i]));
+      emit(r, c, rows - c);
     }
   } else {
     // int32 sums (token, channel) over the ring, whose copies have all been consumed
     uint32_t* part = reinterpret_cast<uint32_t*>(smem);
-    for (int c = 0; c < BT && m0 + c < p.m && done; c += 16) {
+    for (int c = 0; c < rows && done; c += 16) {
       uint32_t r[16];
       __syncwarp();
       tmem_ld_32x32b_x16(t_row + c, r);
@@ -495,15 +538,18 @@ __global__ void __launch_bounds__(kThreads)
     uint32_t peer[kMaxCluster];
 #pragma unroll
     for (int r = 0; r < kMaxCluster; ++r) peer[r] = r < ranks ? mapa_shared(part + warp * 32 + lane, r) : 0u;
-    const int rows = p.m - m0 < BT ? p.m - m0 : BT;
-    for (int c = rank; c < rows && done; c += ranks) {
-      uint32_t v[kMaxCluster];
+    // this CTA's share of the tokens, four at a time so that their reads
+    // overlap (tokens past its share are read, in bounds, and not written)
+    const int c_lo = rows * rank / ranks, c_hi = done ? rows * (rank + 1) / ranks : 0;
+    for (int c = c_lo; c < c_hi; c += 4) {
+      uint32_t sum[4] = {};
 #pragma unroll
-      for (int r = 0; r < kMaxCluster; ++r) v[r] = r < ranks ? dsmem_ld(peer[r] + c * 512) : 0u;
-      uint32_t sum = 0;
+      for (int r = 0; r < kMaxCluster; ++r)
+        if (r < ranks) {
 #pragma unroll
-      for (int r = 0; r < kMaxCluster; ++r) sum += v[r];
-      emit(m0 + c, static_cast<int32_t>(sum));
+          for (int i = 0; i < 4; ++i) sum[i] += dsmem_ld(peer[r] + min(c + i, BT - 1) * 512);
+        }
+      emit(sum, c, c_hi - c);
     }
     __syncwarp();
     cluster_sync();  // no CTA leaves while another may still read its sums
@@ -519,6 +565,209 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 }  // namespace swap
+
+// ===========================================================================
+// GEMV kernel, up to 8 tokens.  A CTA has 16 channels; its 8 warps share out
+// K in units of 64.  Thread (g, t) of a warp reads 16 bytes of channels g and
+// g + 8 at k = 16 t of a unit: the four words of both are the A fragments of
+// two MMAs (m16n8k32), with word 2 i as the fragment's first half of k and
+// word 2 i + 1 as the second.  Which k a fragment index stands for only has to
+// agree with the B fragment, which are the same four words of token g's codes.
+// So weights go from memory to the MMA with no rearrangement, 64 contiguous
+// bytes of a channel for each quad of lanes; two sets of four units are in
+// flight in registers, also from one block of channels to the next (two CTAs
+// for each SM walk the blocks).  The codes of all tokens are in shared memory, copied,
+// or (FUSED, one or two tokens) formed there from x by every CTA itself, which
+// costs less than a kernel of its own before this one.
+// ===========================================================================
+namespace gemv {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kChannels = 16;
+constexpr int kUnit = 64;
+constexpr int kAhead = 4;  // units of a register set
+constexpr int kMaxTokens = 8;
+constexpr int kMaxFused = 2;
+constexpr int kFusedVectors = 2;  // 16-byte vectors of a token a thread holds
+constexpr int kMaxCodes = 96 * 1024;  // bytes of codes in shared memory
+
+struct GemvParams {
+  Params p;
+  const void* x;  // FUSED: the activation, x_stride elements a row
+  const int8_t* act;
+  const int8_t* weight;
+  int64_t x_stride, act_stride, weight_stride;
+};
+
+// Pitch of a token's codes: whole units, 64 bytes off a multiple of 128, so
+// that two tokens' quads fall on different banks.
+__host__ __device__ constexpr int pitch_of(int k) { return (k + kUnit - 1) / kUnit / 2 * 2 * kUnit + kUnit; }
+
+__device__ __forceinline__ void mma_s8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 bytes of a row at k0 (a multiple of 16), of which the row has `count`;
+// beyond the row's end the bytes of its padding are not read.
+__device__ __forceinline__ uint4 load16(const int8_t* row, int k0, int count) {
+  if (count >= 16) return ld_128(row + k0);
+  uint32_t w[4] = {};
+  for (int i = 0; i < count; ++i) w[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k0 + i])) << (8 * (i & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename TOut, bool FUSED>
+__global__ void __launch_bounds__(kThreads, 2) gemv_kernel(const GemvParams q) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __shared__ int32_t part[2][kWarps][kMaxTokens][kChannels + 1];
+  __shared__ float xs[kMaxTokens];
+  __shared__ uint32_t red[kMaxFused][kWarps];
+  const Params& p = q.p;
+  int8_t* codes = reinterpret_cast<int8_t*>(smem_raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int pitch = pitch_of(p.k), units = (p.k + kUnit - 1) / kUnit;
+  const int u_lo = units * warp / kWarps, u_hi = units * (warp + 1) / kWarps;
+  const int blocks = (p.n + kChannels - 1) / kChannels;
+
+  if (!p.early_weights) grid_dependency_wait();
+  uint4 wa[2][kAhead], wb[2][kAhead];
+  // The sets of this warp in its order: units from `at_u` on of channel block
+  // `at_n`; past a block's last unit comes the next block.
+  int at_n = blockIdx.x, at_u = u_lo;
+  auto fetch = [&](uint4 (&w)[2][kAhead]) {
+    const int n0 = at_n * kChannels;
+    // channels past the last are read as the last, and not written
+    const int8_t* row0 = q.weight + static_cast<int64_t>(min(n0 + g, p.n - 1)) * q.weight_stride;
+    const int8_t* row1 = q.weight + static_cast<int64_t>(min(n0 + g + 8, p.n - 1)) * q.weight_stride;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int k0 = (at_u + i) * kUnit + 16 * t;
+      const bool in = at_n < blocks && at_u + i < u_hi && k0 < p.k;
+      w[0][i] = in ? load16(row0, k0, p.k - k0) : make_uint4(0, 0, 0, 0);
+      w[1][i] = in ? load16(row1, k0, p.k - k0) : make_uint4(0, 0, 0, 0);
+    }
+    at_u += kAhead;
+  };
+  auto fetch_two = [&] {  // a block's sets come in pairs, the second perhaps empty
+    fetch(wa);
+    fetch(wb);
+  };
+  fetch_two();
+  if (p.early_weights) grid_dependency_wait();
+  grid_dependents_launch();
+
+  if constexpr (FUSED) {
+    // every CTA quantizes the tokens for itself
+    constexpr int W = 16 / sizeof(TOut);
+    Pack<TOut, W> x[kMaxFused][kFusedVectors];
+#pragma unroll
+    for (int m = 0; m < kMaxFused; ++m)
+#pragma unroll
+      for (int j = 0; j < kFusedVectors; ++j) {
+        const int c = (threadIdx.x + j * kThreads) * W;
+        x[m][j].clear();
+        if (m < p.m && c < p.k) {
+          const TOut* src = static_cast<const TOut*>(q.x) + m * q.x_stride + c;
+          if (c + W <= p.k) x[m][j].load_ahead(src);
+          else x[m][j].load_part(src, p.k - c);
+        }
+      }
+#pragma unroll
+    for (int m = 0; m < kMaxFused; ++m) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < kFusedVectors; ++j) top = max(top, x[m][j].top());
+      top = warp_max(top);
+      if (lane == 0) red[m][warp] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < kMaxFused; ++m) {
+      if (m >= p.m) break;
+      const uint32_t top = warp_max(lane < kWarps ? red[m][lane] : 0u);
+      const Quant8<float> quant(top);
+      if (threadIdx.x == 0) xs[m] = scale8(top);
+#pragma unroll
+      for (int j = 0; j < kFusedVectors; ++j) {
+        const int c = (threadIdx.x + j * kThreads) * W;
+        if (c < units * kUnit) {
+          float v[W];
+          uint32_t code[W];
+          x[m][j].get(v);
+          quant.codes(v, code);
+          store_codes<W>(codes + m * pitch + c, code, quant.mask());
+        }
+      }
+    }
+  } else {
+    const int chunks = units * (kUnit / 16);
+    for (int i = threadIdx.x; i < chunks; i += kThreads) {  // one place of all tokens at a time
+      const int k0 = i * 16;
+#pragma unroll 1
+      for (int m0 = 0; m0 < p.m; m0 += 4) {
+        uint4 v[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          v[m] = m0 + m < p.m && k0 < p.k ? load16(q.act + (m0 + m) * q.act_stride, k0, p.k - k0)
+                                          : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          if (m0 + m < p.m) *reinterpret_cast<uint4*>(codes + (m0 + m) * pitch + k0) = v[m];
+      }
+    }
+    if (threadIdx.x < p.m) xs[threadIdx.x] = ld_f32(p.xscales + threadIdx.x);
+  }
+  __syncthreads();
+
+  auto use = [&](const uint4 (&w)[2][kAhead], int u, int32_t (&acc)[4]) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (u + i >= u_hi) break;  // uniform across the warp
+      uint4 b = make_uint4(0, 0, 0, 0);
+      if (g < p.m) b = *reinterpret_cast<const uint4*>(codes + g * pitch + (u + i) * kUnit + 16 * t);
+      mma_s8(acc, w[0][i].x, w[1][i].x, w[0][i].y, w[1][i].y, b.x, b.y);
+      mma_s8(acc, w[0][i].z, w[1][i].z, w[0][i].w, w[1][i].w, b.z, b.w);
+    }
+  };
+  int turn = 0;
+  for (int block = blockIdx.x; block < blocks; block += gridDim.x, turn ^= 1) {
+    int32_t acc[4] = {};
+    int u = u_lo;
+    do {  // each pair of sets is followed by the next pair's loads
+      const bool last = u + 2 * kAhead >= u_hi;
+      if (last) {
+        at_n = block + gridDim.x;
+        at_u = u_lo;
+      }
+      use(wa, u, acc);
+      fetch(wa);
+      use(wb, u + kAhead, acc);
+      fetch(wb);
+      u += 2 * kAhead;
+    } while (u < u_hi);
+    // fragment C: rows g and g + 8 (channels), columns 2 t and 2 t + 1 (tokens)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[turn][warp][2 * t + (i & 1)][g + 8 * (i >> 1)] = acc[i];
+    __syncthreads();
+    const int m = threadIdx.x / kChannels, n = block * kChannels + threadIdx.x % kChannels;
+    if (m < p.m && n < p.n) {
+      int32_t dot = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) dot += part[turn][w][m][threadIdx.x % kChannels];
+      float v = __fmul_rn(__int2float_rn(dot), xs[m]);
+      if (p.wscales) v = __fmul_rn(v, ld_f32(p.wscales + n));
+      if (p.bias) v = __fadd_rn(v, ld_f32(p.bias + n));
+      static_cast<TOut*>(p.out)[static_cast<int64_t>(m) * p.n + n] = cvt_out<TOut>(v);
+    }
+  }
+}
+
+}  // namespace gemv
 
 // ---------------------------------------------------------------------------
 // host side
@@ -600,18 +849,85 @@ int launch_swap(const Operands& o, const Params& p, int ranks, cudaStream_t stre
   return check_launch("8-bit swap gemm");
 }
 
+template <typename TOut, bool FUSED>
+int launch_gemv(const gemv::GemvParams& q, cudaStream_t stream) {
+  auto kernel = gemv::gemv_kernel<TOut, FUSED>;
+  const int smem = q.p.m * gemv::pitch_of(q.p.k);
+  CONVROT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gemv::kMaxCodes));
+  cudaLaunchConfig_t cfg = {};
+  const int blocks = (q.p.n + gemv::kChannels - 1) / gemv::kChannels, most = 2 * device_sm_count();
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks < most ? blocks : most), 1, 1);
+  cfg.blockDim = dim3(gemv::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CONVROT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, q));
+  return check_launch("8-bit gemv");
+}
+
+bool gemv_takes(int layout, int64_t m, int64_t k) {
+  return layout == CONVROT_LAYOUT_NK && m <= gemv::kMaxTokens && m * gemv::pitch_of(static_cast<int>(k)) <= gemv::kMaxCodes;
+}
+
+// x quantized inside the product.
+template <typename T>
+int launch_fused(const void* x, int64_t x_stride, const Operands& o, Params p, cudaStream_t s) {
+  p.early_weights = 0;  // the previous kernel of the stream may have written them
+  return launch_gemv<T, true>({p, x, nullptr, o.weight, x_stride, 0, o.weight_stride}, s);
+}
+
+// Expected times of the two tile kernels in microseconds, fitted to sweeps of
+// 16 to 1024 tokens, 512 to 12288 channels and K from 128 to 12288 (times of a
+// call in a graph, within 15% of the fit).  A stage of 128 K takes a pair 0.36
+// us while its data comes from L2 alone, 0.45 with every pair at work.  A swap
+// CTA takes 0.46 us for a stage (the latency of its ring), more where two CTAs
+// of an SM share 94 bytes a nanosecond; its epilogue takes 12 ns a token, and
+// the exchange of a split K 1 us and 16 ns a token.  Measured on either side:
+// 64 x 4096 x 4096 (tokens, K, channels) swap 9.6, pair 16.7; 512 x 4096 x
+// 4096 swap 16.8, pair 17.4; 1024 x 1024 x 1024 swap 10.2, pair 8.8;
+// 512 x 4096 x 12288 swap 41, pair 30.
+double pair_time(const Params& p, int sms) {
+  const int64_t tiles = static_cast<int64_t>((p.m + 255) / 256) * ((p.n + 255) / 256), pairs = sms / 2;
+  const int64_t waves = (tiles + pairs - 1) / pairs, stages = (p.k + kBK - 1) / kBK;
+  return 5.0 + static_cast<double>(waves * stages) * (waves > 1 ? 0.45 : 0.36);
+}
+
+// The best split of K over 1, 2, 4 or 8 CTAs (others pack badly into the GPU's
+// clusters of SMs: 64 x 4096 x 12288 takes 14.0 in two, 26 in three), and its
+// time.
+double swap_time(const Params& p, int bt, int sms, int* ranks) {
+  const int64_t tiles = static_cast<int64_t>((p.n + 127) / 128) * ((p.m + bt - 1) / bt);
+  const int64_t stages = (p.k + kBK - 1) / kBK;
+  double best = 1e30;
+  for (int r = 1; r <= swap::kMaxCluster && r <= stages; r *= 2) {
+    const int64_t ctas = tiles * r, waves = (ctas + 2 * sms - 1) / (2 * sms);
+    const bool shared = ctas > sms;
+    const double stage = shared ? std::max(0.46, 2.0 * (swap::kWBytes + bt * kBK) / 94e3) : 0.46;
+    const double t = 2.8 + 0.012 * bt + static_cast<double>(waves * ((stages + r - 1) / r)) * stage +
+                     (r > 1 ? 1.0 + 0.016 * bt : 0.0) + (shared ? 1.0 : 0.0);
+    if (t < best) {
+      best = t;
+      *ranks = r;
+    }
+  }
+  return best;
+}
+
 template <int LAYOUT, typename TOut>
 int launch(const Operands& o, const Params& p, cudaStream_t s) {
   const int sms = device_sm_count();
-  const int64_t pair_tiles = static_cast<int64_t>((p.m + 255) / 256) * ((p.n + 255) / 256);
-  // Pair tiles need most of the GPU's pairs to be busy; otherwise smaller
-  // tiles, with K split until the CTAs fill the SMs.
-  if (p.m > 128 && 4 * pair_tiles >= sms) return launch_pair<LAYOUT, TOut>(o, p, s);
+  if (gemv_takes(LAYOUT, p.m, p.k)) {
+    const gemv::GemvParams q{p, nullptr, o.act, o.weight, 0, o.act_stride, o.weight_stride};
+    return launch_gemv<TOut, false>(q, s);
+  }
   const int bt = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
-  const int64_t tiles = static_cast<int64_t>((p.n + 127) / 128) * ((p.m + bt - 1) / bt);
-  const int k_stages = (p.k + kBK - 1) / kBK;
   int ranks = 1;
-  while (ranks < swap::kMaxCluster && 2 * ranks * tiles <= sms && 2 * ranks <= k_stages) ranks *= 2;
+  const double swap_us = swap_time(p, bt, sms, &ranks);
+  if (pair_time(p, sms) < swap_us) return launch_pair<LAYOUT, TOut>(o, p, s);
   switch (bt) {
     case 16: return launch_swap<LAYOUT, TOut, 16>(o, p, ranks, s);
     case 32: return launch_swap<LAYOUT, TOut, 32>(o, p, ranks, s);
@@ -683,6 +999,22 @@ int convrot_i8_linear(const void* x, int x_dtype, int64_t x_stride, const float*
   using namespace convrot;
   int rc = i8::check_args(codes, codes_stride, weight, weight_stride, layout, scales, out, out_dtype, m, n, k);
   if (rc != CONVROT_OK) return rc;
+  // One or two tokens: quantized inside the product, one kernel instead of two
+  // (1 x 4096 x 4096: 7.1 us, 7.4 as two, and less work for the host).
+  const int64_t x_size = valid_dtype(x_dtype) ? static_cast<int64_t>(dtype_size(x_dtype)) : 1;
+  if (m > 0 && m <= i8::gemv::kMaxFused && !col_scale && x_dtype == out_dtype && i8::gemv_takes(layout, m, k) &&
+      k * x_size <= i8::gemv::kFusedVectors * i8::gemv::kThreads * 16 && aligned_to(x, 16) && x_stride * x_size % 16 == 0) {
+    CONVROT_REQUIRE(x != nullptr && x_stride >= k, CONVROT_ERR_INVALID, "null pointer, or a row stride below k");
+    const i8::Operands o{codes, weight, codes_stride, weight_stride};
+    const i8::Params p{scales, wscales, bias, out, static_cast<int>(m), static_cast<int>(n), static_cast<int>(k),
+                       nullptr, 0};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (x_dtype) {
+      case CONVROT_BF16: return i8::launch_fused<__nv_bfloat16>(x, x_stride, o, p, s);
+      case CONVROT_F16: return i8::launch_fused<__half>(x, x_stride, o, p, s);
+      default: return i8::launch_fused<float>(x, x_stride, o, p, s);
+    }
+  }
   rc = convrot_quantize_i8(x, x_dtype, m, k, x_stride, col_scale, codes, codes_stride, scales, stream);
   if (rc != CONVROT_OK || m == 0) return rc;
   // The kernel before the product is the quantizer, which writes no weight

@@ -3,17 +3,16 @@
 // column (the gradient of the 8-bit linear folds the weight scales in).
 //
 // Memory-bound: a row is read once from HBM and its codes are written once.
-// One CTA for each row, which stays in registers between the maximum and the
-// codes; wide loads where address and pitch allow, else one element a lane
-// (consecutive lanes on consecutive elements).  Rows that do not fit the
-// registers are read a second time, through L2.
+// A row stays in the registers of a warp or a CTA between the maximum and the
+// codes, with the next row's loads in flight; accesses of 16 bytes, or of one
+// or two elements where addresses and pitch allow no more.  What limits beside
+// the memory is the number of instructions: a thread has up to 32 values of a
+// row, so that the exchange of the maximum and the division are little beside
+// them.  Rows that do not fit the registers are read twice, through L2.
 #include "rows.cuh"
 
 namespace convrot {
 namespace {
-
-// Most threads of a CTA: more for single elements, which are narrow loads.
-template <int VEC> constexpr int kThreads = VEC == 1 ? 1024 : 512;
 
 struct QuantParams {
   const void* x;
@@ -24,53 +23,50 @@ struct QuantParams {
   int features;
 };
 
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
+constexpr int kWarps = 4;  // of a CTA whose warps each have rows of their own
+
+// The maximum over the T threads of a row, for all of them.  red holds two
+// sets of a CTA's warps' values, used in turn, so that one barrier is enough.
+template <int T>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t (*red)[32], int& turn) {
   v = warp_max(v);
-  if (blockDim.x > 32) {
-    __syncthreads();  // red may still be read by the previous row
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  if constexpr (T > 32) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) red[turn][threadIdx.x >> 5] = v;
     __syncthreads();
-    v = (threadIdx.x & 31) < (blockDim.x >> 5) ? red[threadIdx.x & 31] : 0u;
-    v = warp_max(v);
+    v = warp_max(lane < T / 32 ? red[turn][lane] : 0u);
+    turn ^= 1;
   }
   return v;
 }
 
 // The type whose quantizer applies: that of x, or float32 after the product
 // with the column scales.
-template <typename T, bool SCALED>
-using Quantized = Quant8<typename std::conditional<SCALED, float, T>::type>;
+template <typename E, bool SCALED>
+using Quantized = Quant8<typename std::conditional<SCALED, float, E>::type>;
 
-// One thread's share of a row: NV vectors of VEC elements, `step` apart.
-template <typename T, int VEC, int NV, bool SCALED>
+// One thread's share of a row: NV vectors of VEC elements, T vectors apart,
+// from column c0 = VEC * (thread of the row) on; left: columns from there on.
+// Absent elements are 0.
+template <typename E, int VEC, int NV, int T, bool SCALED>
 struct Share {
-  Pack<T, VEC> raw[NV];
+  Pack<E, VEC> raw[NV];
   Pack<float, VEC> factor[SCALED ? NV : 1];
 
-  __device__ __forceinline__ void load(const QuantParams& p, int64_t row, int c0, int step) {
-    const T* src = static_cast<const T*>(p.x) + row * p.x_stride;
+  template <typename F>
+  static __device__ __forceinline__ void load_one(Pack<F, VEC>& pk, const F* src, int at, int left) {
+    pk.clear();
+    if (at + VEC <= left) pk.load_ahead(src + at);
+    else if (VEC > 1 && at < left) pk.load_part(src + at, left - at);
+  }
+  __device__ __forceinline__ void load(const E* row, int left) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = c0 + j * step;
-      raw[j].clear();
-      if (c + VEC <= p.features) {
-        raw[j].load_nc(src + c);
-      } else if (VEC > 1 && c < p.features) {
-        raw[j].load_part(src + c, p.features - c);
-      }
-    }
-    if constexpr (SCALED) {
+    for (int j = 0; j < NV; ++j) load_one(raw[j], row, j * T * VEC, left);
+  }
+  __device__ __forceinline__ void load_factors(const float* col_scale, int left) {
+    if constexpr (SCALED)
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int c = c0 + j * step;
-        factor[j].clear();
-        if (c + VEC <= p.features) {
-          factor[j].load_nc(p.col_scale + c);
-        } else if (VEC > 1 && c < p.features) {
-          factor[j].load_part(p.col_scale + c, p.features - c);
-        }
-      }
-    }
+      for (int j = 0; j < NV; ++j) load_one(factor[j], col_scale, j * T * VEC, left);
   }
   __device__ __forceinline__ void get(int j, float (&v)[VEC]) const {
     raw[j].get(v);
@@ -96,85 +92,94 @@ struct Share {
     }
     return m;
   }
-  __device__ __forceinline__ void store(const QuantParams& p, int64_t row, int c0, int step,
-                                        const Quantized<T, SCALED>& quant) const {
-    int8_t* dst = p.q + row * p.q_stride;
+  __device__ __forceinline__ void store(int8_t* dst, int left, const Quantized<E, SCALED>& quant) const {
+    if (quant.tiny()) store_as(dst, left, Quant8<float>(quant.bits));
+    else store_as(dst, left, quant);
+  }
+  template <typename Q>
+  __device__ __forceinline__ void store_as(int8_t* dst, int left, const Q& quant) const {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = c0 + j * step;
-      if (c < p.features) {
+      const int at = j * T * VEC;
+      if (at < left) {
         float v[VEC];
         uint32_t code[VEC];
         get(j, v);
         quant.codes(v, code);
-        if (c + VEC <= p.features) {
-          store_codes<VEC>(dst + c, code, quant.mask());
+        if (at + VEC <= left) {
+          store_codes<VEC>(dst + at, code, quant.mask());
         } else {
 #pragma unroll
           for (int i = 0; i < VEC; ++i)
-            if (c + i < p.features) dst[c + i] = static_cast<int8_t>(code[i] & quant.mask());
+            if (at + i < left) dst[at + i] = static_cast<int8_t>(code[i] & quant.mask());
         }
       }
     }
   }
 };
 
-template <typename T, int VEC, int NV, bool SCALED>
-__global__ void __launch_bounds__(kThreads<VEC>) quantize_i8_kernel(const QuantParams p) {
+// T threads share a row: 32 (each warp of the CTA rows of its own), or the CTA.
+template <typename E, int VEC, int NV, int T, bool SCALED>
+__global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, 1024 / (T == 32 ? 32 * kWarps : T))
+    quantize_i8_kernel(const QuantParams p) {
   __shared__ uint32_t red[2][32];
   grid_dependency_wait();  // x may come from the previous kernel of the stream
   grid_dependents_launch();
-  const int c0 = threadIdx.x * VEC, step = blockDim.x * VEC, lane = threadIdx.x & 31;
+  const int c0 = (T == 32 ? threadIdx.x & 31 : threadIdx.x) * VEC, left = p.features - c0;
+  const int64_t first = T == 32 ? static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5) : blockIdx.x;
+  const int64_t stride = T == 32 ? static_cast<int64_t>(gridDim.x) * kWarps : gridDim.x;
   int turn = 0;
-  Share<T, VEC, NV, SCALED> x, next;
-  next.load(p, blockIdx.x, c0, step);
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+  const E* src = static_cast<const E*>(p.x) + first * p.x_stride + c0;
+  int8_t* dst = p.q + first * p.q_stride + c0;
+  Share<E, VEC, NV, T, SCALED> x, next;
+  if (first < p.rows) next.load(src, left);
+  next.load_factors(p.col_scale + c0, left);
+  for (int64_t row = first; row < p.rows; row += stride) {
     x = next;
-    if (row + gridDim.x < p.rows) next.load(p, row + gridDim.x, c0, step);  // in flight while this row is worked on
-    uint32_t top = warp_max(x.top());
-    if (blockDim.x > 32) {
-      if (lane == 0) red[turn][threadIdx.x >> 5] = top;
-      __syncthreads();
-      top = warp_max(lane < (blockDim.x >> 5) ? red[turn][lane] : 0u);
-      turn ^= 1;
-    }
-    x.store(p, row, c0, step, Quantized<T, SCALED>(top));
-    if (threadIdx.x == 0) p.scales[row] = scale8(top);
+    src += stride * p.x_stride;
+    if (row + stride < p.rows) next.load(src, left);
+    const uint32_t top = row_max<T>(x.top(), red, turn);
+    x.store(dst, left, Quantized<E, SCALED>(top));
+    if (c0 == 0) p.scales[row] = scale8(top);
+    dst += stride * p.q_stride;
   }
 }
 
 // Rows too long for the registers: two passes, the second through L2.
-template <typename T, int VEC, bool SCALED>
-__global__ void __launch_bounds__(kThreads<VEC>) quantize_i8_long_kernel(const QuantParams p) {
-  __shared__ uint32_t red[32];
+template <typename E, int VEC, bool SCALED>
+__global__ void __launch_bounds__(512) quantize_i8_long_kernel(const QuantParams p) {
+  __shared__ uint32_t red[2][32];
   grid_dependency_wait();
   grid_dependents_launch();
-  const int step = blockDim.x * VEC;
+  int turn = 0;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const E* src = static_cast<const E*>(p.x) + row * p.x_stride;
+    Share<E, VEC, 4, 512, SCALED> x;
     uint32_t top = 0;
-    for (int c = threadIdx.x * VEC; c < p.features; c += 4 * step) {
-      Share<T, VEC, 4, SCALED> x;
-      x.load(p, row, c, step);
+    for (int c = threadIdx.x * VEC; c < p.features; c += 4 * 512 * VEC) {
+      x.load(src + c, p.features - c);
+      x.load_factors(p.col_scale + c, p.features - c);
       top = max(top, x.top());
     }
-    top = block_max(top, red);
-    const Quantized<T, SCALED> quant(top);
-    for (int c = threadIdx.x * VEC; c < p.features; c += 4 * step) {
-      Share<T, VEC, 4, SCALED> x;
-      x.load(p, row, c, step);
-      x.store(p, row, c, step, quant);
+    top = row_max<512>(top, red, turn);
+    const Quantized<E, SCALED> quant(top);
+    for (int c = threadIdx.x * VEC; c < p.features; c += 4 * 512 * VEC) {
+      x.load(src + c, p.features - c);
+      x.load_factors(p.col_scale + c, p.features - c);
+      x.store(p.q + row * p.q_stride + c, p.features - c, quant);
     }
     if (threadIdx.x == 0) p.scales[row] = scale8(top);
   }
 }
 
-// As many CTAs as rows, up to about 1536 threads for each SM.
+// As many CTAs as rows need, up to about 1024 threads for each SM.
 int enqueue(void (*kernel)(QuantParams), const QuantParams& p, int threads, cudaStream_t stream) {
-  const int per_sm = threads > 768 ? 1 : threads < 64 ? 24 : 1536 / threads;
-  const int64_t most = static_cast<int64_t>(device_sm_count()) * per_sm;
+  const int64_t at_once = threads == 32 ? kWarps : 1;
+  const int cta = threads == 32 ? 32 * kWarps : threads;
+  const int64_t want = (p.rows + at_once - 1) / at_once, most = static_cast<int64_t>(device_sm_count()) * (1024 / cta);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.rows < most ? p.rows : most), 1, 1);
-  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(want < most ? want : most), 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(cta), 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -185,28 +190,44 @@ int enqueue(void (*kernel)(QuantParams), const QuantParams& p, int threads, cuda
   return check_launch("convrot_quantize_i8");
 }
 
-template <typename T, int VEC, bool SCALED>
+// U vectors a thread: four of 16 bytes (two beside column scales, which take
+// registers too), or eight of one or two elements; one
+// or two for the shortest rows.
+template <typename E, int VEC, bool SCALED>
 int launch_vec(const QuantParams& p, cudaStream_t stream) {
-  // two vectors (four single elements) a thread, more where the CTA is full
-  constexpr int kLeast = VEC == 1 ? 4 : 2;
+  constexpr int U = VEC > 2 ? (SCALED ? 2 : 4) : 8;
+  constexpr int kShort = (U + 3) / 4;
   const int vectors = (p.features + VEC - 1) / VEC;
-  int nv = kLeast;
-  while (nv < 4 * kLeast && vectors > nv * kThreads<VEC>) nv *= 2;
-  const int64_t per = (vectors + nv - 1) / nv;
-  if (per > kThreads<VEC>) return enqueue(quantize_i8_long_kernel<T, VEC, SCALED>, p, kThreads<VEC>, stream);
-  const int threads = static_cast<int>((per + 31) / 32 * 32);
-  if (nv == kLeast) return enqueue(quantize_i8_kernel<T, VEC, kLeast, SCALED>, p, threads, stream);
-  if (nv == 2 * kLeast) return enqueue(quantize_i8_kernel<T, VEC, 2 * kLeast, SCALED>, p, threads, stream);
-  return enqueue(quantize_i8_kernel<T, VEC, 4 * kLeast, SCALED>, p, threads, stream);
+#define CONVROT_QUANT(NV, T) enqueue(quantize_i8_kernel<E, VEC, NV, T, SCALED>, p, T, stream)
+  if (vectors <= 32 * kShort) return CONVROT_QUANT(kShort, 32);
+  if (vectors <= 32 * U) return CONVROT_QUANT(U, 32);
+  if (vectors <= 64 * U) return CONVROT_QUANT(U, 64);
+  if (vectors <= 128 * U) return CONVROT_QUANT(U, 128);
+  if (vectors <= 256 * U) return CONVROT_QUANT(U, 256);
+  if (vectors <= 512 * U) return CONVROT_QUANT(U, 512);
+  if (vectors <= 1024 * U) return CONVROT_QUANT(U, 1024);
+  if constexpr (VEC == 1)
+    if (vectors <= 1024 * 2 * U) return CONVROT_QUANT(2 * U, 1024);
+#undef CONVROT_QUANT
+  return enqueue(quantize_i8_long_kernel<E, VEC, SCALED>, p, 512, stream);
 }
 
-template <typename T>
+template <typename E, bool SCALED>
+int launch_scaled(const QuantParams& p, cudaStream_t stream) {
+  constexpr int W = 16 / sizeof(E);
+  auto aligned_for = [&](int vec) {
+    const int64_t bytes = vec * static_cast<int64_t>(sizeof(E));
+    return aligned_to(p.x, bytes) && p.x_stride % vec == 0 && aligned_to(p.q, vec) && p.q_stride % vec == 0 &&
+           aligned_to(p.col_scale, vec * 4 < 16 ? vec * 4 : 16);
+  };
+  if (aligned_for(W)) return launch_vec<E, W, SCALED>(p, stream);
+  if (aligned_for(2)) return launch_vec<E, 2, SCALED>(p, stream);
+  return launch_vec<E, 1, SCALED>(p, stream);
+}
+
+template <typename E>
 int launch(const QuantParams& p, cudaStream_t stream) {
-  constexpr int kWide = 16 / sizeof(T);
-  const bool wide = aligned_to(p.x, 16) && p.x_stride * static_cast<int64_t>(sizeof(T)) % 16 == 0 &&
-                    aligned_to(p.q, 8) && p.q_stride % 8 == 0 && aligned_to(p.col_scale, 16);
-  if (p.col_scale) return wide ? launch_vec<T, kWide, true>(p, stream) : launch_vec<T, 1, true>(p, stream);
-  return wide ? launch_vec<T, kWide, false>(p, stream) : launch_vec<T, 1, false>(p, stream);
+  return p.col_scale ? launch_scaled<E, true>(p, stream) : launch_scaled<E, false>(p, stream);
 }
 
 }  // namespace

@@ -98,7 +98,7 @@ struct Share {
   __device__ __forceinline__ void load(const E* row, int left) {
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      if (j * T * VEC < left) v[j].load_nc(row + j * T * VEC);
+      if (j * T * VEC < left) v[j].load_ahead(row + j * T * VEC);
   }
 };
 
@@ -116,13 +116,13 @@ struct Vector {
     if (wide) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (j * T * VEC < left) raw[j].load_nc(static_cast<const float*>(base) + at + j * T * VEC);
+        if (j * T * VEC < left) raw[j].load_ahead(static_cast<const float*>(base) + at + j * T * VEC);
     } else {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (j * T * VEC < left) {
           Pack<E, VEC> pk;
-          pk.load_nc(static_cast<const E*>(base) + at + j * T * VEC);
+          pk.load_ahead(static_cast<const E*>(base) + at + j * T * VEC);
 #pragma unroll
           for (int i = 0; i < Pack<E, VEC>::kWords; ++i) raw[j].w[i] = pk.w[i];
         }
@@ -161,9 +161,9 @@ struct Rows {
 };
 
 template <typename E>
-__device__ __forceinline__ E ldg(const E* p) {
+__device__ __forceinline__ E ld(const E* p) {
   Pack<E, 1> pk;
-  pk.load_nc(p);
+  pk.load_ahead(p);
   if constexpr (sizeof(E) == 4) return __uint_as_float(pk.w[0]);
   else {
     const uint16_t h = static_cast<uint16_t>(pk.w[0]);
@@ -174,7 +174,7 @@ __device__ __forceinline__ E ldg(const E* p) {
 // One value of a segment's vectors.
 template <typename E>
 __device__ __forceinline__ float vector_at(const NormParams& p, const void* base, int64_t at) {
-  return p.wide_weight ? __ldg(static_cast<const float*>(base) + at) : Elem<E>::to_f(ldg(static_cast<const E*>(base) + at));
+  return p.wide_weight ? ld_f32(static_cast<const float*>(base) + at) : Elem<E>::to_f(ld(static_cast<const E*>(base) + at));
 }
 template <typename E>
 __device__ __forceinline__ float weight_at(const NormParams& p, int64_t at) {
@@ -278,13 +278,13 @@ __global__ void __launch_bounds__(512) norm_fwd_long_kernel(const NormParams p) 
     E* y = static_cast<E*>(p.y) + row * F;
     float s[1] = {0.0f};
 #pragma unroll 8
-    for (int c = threadIdx.x; c < F; c += 512) s[0] += Elem<E>::to_f(ldg(x + c));
+    for (int c = threadIdx.x; c < F; c += 512) s[0] += Elem<E>::to_f(ld(x + c));
     row_sums<512>(s, red, turn);
     const float mean = s[0] * inv;
     s[0] = 0.0f;
 #pragma unroll 8
     for (int c = threadIdx.x; c < F; c += 512) {
-      const float d = Elem<E>::to_f(ldg(x + c)) - mean;
+      const float d = Elem<E>::to_f(ld(x + c)) - mean;
       s[0] = fma(d, d, s[0]);
     }
     row_sums<512>(s, red, turn);
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(512) norm_fwd_long_kernel(const NormParams p) 
     const int64_t offset = row / p.rows_per_weight * p.weight_stride;
 #pragma unroll 4
     for (int c = threadIdx.x; c < F; c += 512)
-      y[c] = Elem<E>::from_f(fma((Elem<E>::to_f(ldg(x + c)) - mean) * rstd, weight_at<E>(p, offset + c),
+      y[c] = Elem<E>::from_f(fma((Elem<E>::to_f(ld(x + c)) - mean) * rstd, weight_at<E>(p, offset + c),
                                  bias_at<E>(p, offset + c)));
   }
 }
@@ -338,8 +338,8 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, T == 32 || T == 128
     if (row < rows.end) {
       next_x.load(static_cast<const E*>(p.x) + offset, left);
       next_dy.load(static_cast<const E*>(p.dy) + offset, left);
-      next_mean = __ldg(p.mean + row);
-      next_rstd = __ldg(p.rstd + row);
+      next_mean = ld_f32(p.mean + row);
+      next_rstd = ld_f32(p.rstd + row);
     }
   };
   if (kAhead) fetch(first, at);
@@ -436,16 +436,16 @@ __global__ void __launch_bounds__(512) norm_dx_long_kernel(const NormParams p) {
     float s[2] = {0.0f, 0.0f};
 #pragma unroll 4
     for (int c = threadIdx.x; c < F; c += 512) {
-      const float g = Elem<E>::to_f(ldg(dy + c)) * weight_at<E>(p, offset + c);
+      const float g = Elem<E>::to_f(ld(dy + c)) * weight_at<E>(p, offset + c);
       s[0] += g;
-      s[1] = fma(g, (Elem<E>::to_f(ldg(x + c)) - mean) * rstd, s[1]);
+      s[1] = fma(g, (Elem<E>::to_f(ld(x + c)) - mean) * rstd, s[1]);
     }
     row_sums<512>(s, red, turn);
     const float mg = s[0] * inv, mgh = s[1] * inv;
 #pragma unroll 4
     for (int c = threadIdx.x; c < F; c += 512) {
-      const float g = Elem<E>::to_f(ldg(dy + c)) * weight_at<E>(p, offset + c);
-      const float h = (Elem<E>::to_f(ldg(x + c)) - mean) * rstd;
+      const float g = Elem<E>::to_f(ld(dy + c)) * weight_at<E>(p, offset + c);
+      const float h = (Elem<E>::to_f(ld(x + c)) - mean) * rstd;
       dx[c] = Elem<E>::from_f(rstd * (g - mg - h * mgh));
     }
   }
@@ -467,8 +467,8 @@ __global__ void __launch_bounds__(256) norm_partial_long_kernel(const NormParams
   float dw = 0.0f, db = 0.0f;
 #pragma unroll 4
   for (int64_t row = r0; row < r1; ++row) {
-    const float d = Elem<E>::to_f(ldg(dy + row * F + c));
-    dw = fma(d, (Elem<E>::to_f(ldg(x + row * F + c)) - __ldg(p.mean + row)) * __ldg(p.rstd + row), dw);
+    const float d = Elem<E>::to_f(ld(dy + row * F + c));
+    dw = fma(d, (Elem<E>::to_f(ld(x + row * F + c)) - ld_f32(p.mean + row)) * ld_f32(p.rstd + row), dw);
     db += d;
   }
   p.partial[(part * 2) * F + c] = dw;

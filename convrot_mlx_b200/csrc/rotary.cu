@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ 
       cs[i] = 1.0f;
       sn[i] = 0.0f;
       if (j < p.pairs) {
-        const double turn = static_cast<double>(__ldg(pos + p.axis[j])) * p.turns[j];
+        const double turn = static_cast<double>(ld_f32(pos + p.axis[j])) * p.turns[j];
         sincospif(2.0f * static_cast<float>(turn - rint(turn)), &sn[i], &cs[i]);
         sn[i] *= p.sign;
       }

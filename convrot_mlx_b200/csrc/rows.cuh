@@ -91,6 +91,37 @@ __device__ __forceinline__ void unpack(const uint32_t* w, float (&v)[VEC]) {
   }
 }
 
+// Loads that keep their place among themselves and behind the wait for the
+// previous kernel (an invariant load, as __ldg is, could be moved above it),
+// but that ordinary stores do not hold back: for data that the kernel does not
+// write.
+__device__ __forceinline__ uint4 ld_128(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint2 ld_64(const void* p) {
+  uint2 r;
+  asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint32_t ld_32(const void* p) {
+  uint32_t r;
+  asm volatile("ld.global.u32 %0, [%1];" : "=r"(r) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint32_t ld_16(const void* p) {
+  uint16_t r;
+  asm volatile("ld.global.u16 %0, [%1];" : "=h"(r) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint32_t ld_8(const void* p) {
+  uint32_t r;
+  asm volatile("ld.global.u8 %0, [%1];" : "=r"(r) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ float ld_f32(const float* p) { return __uint_as_float(ld_32(p)); }
+
 // VEC consecutive elements as they lie in memory, moved in accesses of at
 // most 16 bytes (the address is a multiple of that, or of VEC elements where
 // those are fewer bytes).
@@ -117,24 +148,23 @@ struct Pack {
       w[0] = *reinterpret_cast<const uint8_t*>(src);
     }
   }
-  // The same through the read-only path, for data that the kernel does not
-  // write: such loads may be moved above stores.
-  __device__ __forceinline__ void load_nc(const T* src) {
+  // The same by ld_* below: not held back by the stores before it.
+  __device__ __forceinline__ void load_ahead(const T* src) {
     if constexpr (kBytes >= 16) {
 #pragma unroll
       for (int i = 0; i < kBytes / 16; ++i) {
-        const uint4 r = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        const uint4 r = ld_128(reinterpret_cast<const uint4*>(src) + i);
         w[4 * i] = r.x, w[4 * i + 1] = r.y, w[4 * i + 2] = r.z, w[4 * i + 3] = r.w;
       }
     } else if constexpr (kBytes == 8) {
-      const uint2 r = __ldg(reinterpret_cast<const uint2*>(src));
+      const uint2 r = ld_64(src);
       w[0] = r.x, w[1] = r.y;
     } else if constexpr (kBytes == 4) {
-      w[0] = __ldg(reinterpret_cast<const uint32_t*>(src));
+      w[0] = ld_32(src);
     } else if constexpr (kBytes == 2) {
-      w[0] = __ldg(reinterpret_cast<const uint16_t*>(src));
+      w[0] = ld_16(src);
     } else {
-      w[0] = __ldg(reinterpret_cast<const uint8_t*>(src));
+      w[0] = ld_8(src);
     }
   }
   // The first `count` < VEC elements, the rest 0.
@@ -263,7 +293,7 @@ __device__ __forceinline__ float signed_byte(uint32_t w, int i) {
 //   8 bits).  A half needs 254 x = (2 j + 1) top: since 127 is prime either
 //   2 j + 1 = 127, the tie 63.5, which rounding up sends to 64, the even one;
 //   or top's significand is 127, where f is a power of two and x f exact.
-//   (top below 2^-120, for which f overflows, goes the other way.)
+//   (top below 2^-120, for which f overflows, goes the other way: tiny().)
 // * other types: x and top are first scaled by the power of two that brings
 //   top near 1, so that nothing overflows; q = p r with p = 127 x misses p / top by at most two ulps, and
 //   one step of residual correction, q += (p - q top) r with the residual
@@ -305,20 +335,17 @@ struct Quant8 {
     return q;
   }
 
+  // Whether codes() has to be that of Quant8<float>(bits) instead.
+  __device__ __forceinline__ bool tiny() const { return kFast && bits < kLeastFast && bits != 0; }
+
   // The codes in two's complement in the words' low bytes.
   template <int VEC>
   __device__ __forceinline__ void codes(const float (&x)[VEC], uint32_t (&code)[VEC]) const {
-    if constexpr (kFast) {
-      if (bits < kLeastFast && bits != 0) {
-        const Quant8<float> wide(bits);
-        wide.codes(x, code);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      if constexpr (kFast) {
+        code[i] = __float_as_uint(__fmaf_rn(x[i], k, 12582912.0f));
       } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) code[i] = __float_as_uint(__fmaf_rn(x[i], k, 12582912.0f));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
         const float p = __fmul_rn(x[i], k);
         const float q = __fmul_rn(p, r);
         code[i] = __float_as_uint(__fadd_rn(__fmaf_rn(__fmaf_rn(-q, top, p), r, q), 12582912.0f));

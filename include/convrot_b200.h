@@ -314,11 +314,12 @@ int convrot_i8_gemm(const int8_t* act, int64_t act_stride, const int8_t* weight,
                     int64_t m, int64_t n, int64_t k, void* stream);
 
 /*
- * convrot_quantize_i8 of x into `codes` (m, k) and `scales` (m,), then
- * convrot_i8_gemm of them, in one call: the 8-bit linear (layout NK), or with
- * col_scale and layout KN the gradient of its input.  The product starts
- * reading the weight while the quantizer runs: `codes` and `scales` may not
- * overlap the weight.
+ * convrot_quantize_i8 of x, then convrot_i8_gemm of its codes, in one call:
+ * the 8-bit linear (layout NK), or with col_scale and layout KN the gradient
+ * of its input.  `codes` (m, k) and `scales` (m,) are workspace; what they hold
+ * afterwards is not specified (for one or two tokens the product forms the
+ * codes itself).  The product starts reading the weight while the quantizer
+ * runs: `codes` and `scales` may not overlap the weight.
  */
 int convrot_i8_linear(const void* x, int x_dtype, int64_t x_stride, const float* col_scale, const int8_t* weight,
                       int64_t weight_stride, int layout, const float* wscales, const float* bias, void* out,
