@@ -112,7 +112,7 @@ __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorM
 namespace pair {
 
 constexpr int kTile = 256;
-constexpr int kBand = 8;
+constexpr int kBand = 16;
 constexpr int kStages = 6;
 constexpr int kOpBytes = 128 * kBK;  // one operand's half tile of a stage
 constexpr int kWarpA = 0, kWarpMma = 1, kWarpB = 2, kWarpE0 = 4, kEWarps = 8;
