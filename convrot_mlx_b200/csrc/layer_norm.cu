@@ -11,31 +11,32 @@ namespace convrot {
 namespace norm {
 namespace {
 
-// dweight and dbias: the chunks' sums added up, 32 columns a CTA, 16 threads
-// for each column that take every 16th chunk, then a tree over the 16.
-template <typename TW>
+// dweight and dbias: the chunks' sums added up, COLS columns a CTA, 512 / COLS
+// threads for each column that take every so many-th chunk, then a tree.
+template <typename TW, int COLS>
 __global__ void __launch_bounds__(512) norm_reduce_kernel(const NormParams p) {
-  __shared__ float sw[16][33], sb[16][33];
+  constexpr int kWays = 512 / COLS;
+  __shared__ float sw[kWays][COLS + 1], sb[kWays][COLS + 1];
   grid_dependency_wait();
   grid_dependents_launch();
   const int F = p.features;
-  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + x;
+  const int x = threadIdx.x % COLS, y = threadIdx.x / COLS;
+  const int c = blockIdx.x * COLS + x;
   const int64_t seg = blockIdx.y;
   float dw = 0.0f, db = 0.0f;
   if (c < F) {
-    const float* part = p.partial + seg * p.chunks * 2 * F;
-#pragma unroll 8
-    for (int chunk = y; chunk < p.chunks; chunk += 16) {
-      dw += part[static_cast<int64_t>(chunk) * 2 * F + c];
-      db += part[static_cast<int64_t>(chunk) * 2 * F + F + c];
+    const float* part = p.partial + seg * p.chunks * 2 * F + c;
+#pragma unroll 4
+    for (int chunk = y; chunk < p.chunks; chunk += kWays) {
+      dw += ld_f32(part + static_cast<int64_t>(chunk) * 2 * F);
+      db += ld_f32(part + static_cast<int64_t>(chunk) * 2 * F + F);
     }
   }
   sw[y][x] = dw;
   sb[y][x] = db;
   __syncthreads();
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
+  for (int o = kWays / 2; o > 0; o >>= 1) {
     if (y < o) {
       sw[y][x] += sw[y + o][x];
       sb[y][x] += sb[y + o][x];
@@ -56,10 +57,13 @@ int chunks_of(int64_t rows_per_weight, int64_t segments) {
   return static_cast<int>(chunks < 1 ? 1 : chunks);
 }
 
+// Many chunks: few columns a CTA, so that there are CTAs and threads enough.
 template <typename TW>
 int reduce(const NormParams& p, cudaStream_t s) {
+  const bool many = p.chunks > 64;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((p.features + 31) / 32, static_cast<unsigned>(p.rows / p.rows_per_weight), 1);
+  cfg.gridDim = dim3((p.features + (many ? 7 : 31)) / (many ? 8 : 32),
+                     static_cast<unsigned>(p.rows / p.rows_per_weight), 1);
   cfg.blockDim = dim3(512, 1, 1);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -67,7 +71,7 @@ int reduce(const NormParams& p, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  CONVROT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, norm_reduce_kernel<TW>, p));
+  CONVROT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, many ? norm_reduce_kernel<TW, 8> : norm_reduce_kernel<TW, 32>, p));
   return check_launch("layer norm reduction");
 }
 

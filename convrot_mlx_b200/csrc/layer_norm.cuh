@@ -17,6 +17,8 @@
 // flight while a row is worked on.
 #pragma once
 
+#include <algorithm>
+
 #include "rows.cuh"
 
 namespace convrot {
@@ -104,6 +106,77 @@ struct Share {
 
 template <int VEC, int NV>
 using Lanes = Lane<VEC>[NV][kLanes<VEC>];
+
+// Rows ahead of the one in work: each thread copies its own columns of ARRAYS
+// arrays asynchronously into places of shared memory that only it reads, so
+// that no barrier is needed and no register is held.  kDepth places, of which
+// one is being read.
+template <typename E, int VEC, int NV, int T, int ARRAYS>
+struct Ahead {
+  static constexpr int kBytes = VEC * static_cast<int>(sizeof(E));
+  static constexpr bool kAsync = kBytes >= 4;  // the copies' least size
+  static constexpr int kDepth = 3;
+  static constexpr int kThreads = T == 32 ? 32 * kWarps : T;
+  static constexpr int kPlace = ARRAYS * NV * kThreads * kBytes;
+  static constexpr int kSmem = kAsync ? kDepth * kPlace : 0;
+
+  uint32_t base;
+  int write = 0, read = 0;
+  __device__ __forceinline__ explicit Ahead(const void* smem) : base(smem_u32(smem) + threadIdx.x * kBytes) {}
+
+  // A row of each array into the next place (`there`: whether the row exists).
+  template <typename... P>
+  __device__ __forceinline__ void issue(bool there, int left, const P*... rows) {
+    if (there) {
+      uint32_t dst = base + write * kPlace;
+      (copy(dst, rows, left), ...);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    write = write + 1 == kDepth ? 0 : write + 1;
+  }
+  __device__ __forceinline__ void copy(uint32_t& dst, const E* row, int left) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (j * T * VEC < left) {
+        const E* src = row + j * T * VEC;
+        if constexpr (kBytes == 16)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + j * kThreads * kBytes), "l"(src) : "memory");
+        else if constexpr (kBytes == 8)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst + j * kThreads * kBytes), "l"(src) : "memory");
+        else
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + j * kThreads * kBytes), "l"(src) : "memory");
+      }
+    }
+    dst += NV * kThreads * kBytes;
+  }
+  // The oldest row, once it has landed.
+  template <typename... S>
+  __device__ __forceinline__ void take(int left, S&... shares) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
+    uint32_t src = base + read * kPlace;
+    (fetch(src, shares, left), ...);
+    read = read + 1 == kDepth ? 0 : read + 1;
+  }
+  __device__ __forceinline__ void fetch(uint32_t& src, Share<E, VEC, NV, T>& share, int left) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (j * T * VEC < left) {
+        uint32_t(&w)[Pack<E, VEC>::kWords] = share.v[j].w;
+        const uint32_t at = src + j * kThreads * kBytes;
+        if constexpr (kBytes == 16)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(at)
+                       : "memory");
+        else if constexpr (kBytes == 8)
+          asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+        else
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
+      }
+    }
+    src += NV * kThreads * kBytes;
+  }
+};
 
 // A segment's vector: loaded as it lies in memory (of x's type or float32),
 // and turned into float32 plus a constant once everything else a thread needs
@@ -205,8 +278,17 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T) norm_fwd_kernel(con
   const int64_t first = rows.begin + (T == 32 ? threadIdx.x >> 5 : 0), stride = T == 32 ? kWarps : 1;
   const E* src = static_cast<const E*>(p.x) + first * F + c0;
   E* dst = static_cast<E*>(p.y) + first * F + c0;
+  const int64_t step = stride * F;
   Share<E, VEC, NV, T> x;
-  if (first < rows.end) x.load(src, left);
+  using Next = Ahead<E, VEC, NV, T, 1>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  Next next(smem);
+  if constexpr (Next::kAsync) {
+    next.issue(first < rows.end, left, src);
+    next.issue(first + stride < rows.end, left, src + step);
+  } else {
+    if (first < rows.end) x.load(src, left);
+  }
   Lanes<VEC, NV> weight, bias;
   {
     const int64_t offset = rows.segment * p.weight_stride + c0;
@@ -219,6 +301,10 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T) norm_fwd_kernel(con
   for (int64_t row = first; row < rows.end; row += stride) {
     Lanes<VEC, NV> v;
     A sum = splat<VEC>(0.0f);
+    if constexpr (Next::kAsync) {
+      next.take(left, x);
+      next.issue(row + 2 * stride < rows.end, left, src + 2 * step);
+    }
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (j * T * VEC < left) {
@@ -226,8 +312,8 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T) norm_fwd_kernel(con
 #pragma unroll
         for (int i = 0; i < L; ++i) sum = add(sum, v[j][i]);
       }
-    src += stride * F;
-    if (row + stride < rows.end) x.load(src, left);
+    src += step;
+    if (!Next::kAsync && row + stride < rows.end) x.load(src, left);
     float s[1] = {total(sum)};
     row_sums<T>(s, red, turn);
     const float mean = s[0] * inv;
@@ -259,7 +345,7 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T) norm_fwd_kernel(con
         out.set_lanes(v[j]);
         out.store(dst + j * T * VEC);
       }
-    dst += stride * F;
+    dst += step;
   }
 }
 
@@ -306,17 +392,20 @@ __global__ void __launch_bounds__(512) norm_fwd_long_kernel(const NormParams p) 
 
 // With h = x r - mean r and per row u = -r E[g h], v = -r E[g]:
 //   dx = (dy r) w + (h u + v).
-// With up to 24 values of a row a thread keeps h in float32 and has the next
-// row's loads in flight; with more it keeps the row as it lies in memory and
-// forms h twice.
+// With up to 24 values of a row a thread keeps h in float32; with more it
+// keeps the row as it lies in memory and forms h twice.
 template <typename E, int VEC, int NV, int T>
 __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, T == 32 || T == 128 ? 3 : (T == 64 ? 6 : 1))
     norm_bwd_kernel(const NormParams p) {
   constexpr int L = kLanes<VEC>;
   using A = Lane<VEC>;
-  constexpr bool kAhead = VEC * NV <= 24;
+  // h kept in float32 beside the row, and rows ahead: in shared memory, or in
+  // registers for elements that are too small to be copied
+  constexpr bool kKeep = VEC * NV <= 24;
+  using Next = Ahead<E, VEC, NV, T, 2>;
+  constexpr bool kRegs = !Next::kAsync && kKeep;
   __shared__ float red[2][16][2];
-  extern __shared__ float sums[];  // T = 32: (kWarps, 2, features)
+  extern __shared__ __align__(16) uint8_t smem[];  // rows ahead; then, T = 32, sums (kWarps, 2, features)
   int turn = 0;
   grid_dependency_wait();
   grid_dependents_launch();
@@ -332,36 +421,52 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, T == 32 || T == 128
     for (int i = 0; i < L; ++i) dw[j][i] = db[j][i] = splat<VEC>(0.0f);
   const int64_t first = rows.begin + (T == 32 ? warp : 0), stride = T == 32 ? kWarps : 1;
   int64_t at = first * F + c0;
+  const int64_t step = stride * F;
+  const E* xs = static_cast<const E*>(p.x);
+  const E* dys = static_cast<const E*>(p.dy);
   Share<E, VEC, NV, T> x, dy, next_x, next_dy;
+  Next next(smem);
   float mean = 0.0f, rstd = 0.0f, next_mean = 0.0f, next_rstd = 0.0f;
+  auto issue = [&](int64_t row, int64_t offset) { next.issue(row < rows.end, left, xs + offset, dys + offset); };
   auto fetch = [&](int64_t row, int64_t offset) {
     if (row < rows.end) {
-      next_x.load(static_cast<const E*>(p.x) + offset, left);
-      next_dy.load(static_cast<const E*>(p.dy) + offset, left);
+      if constexpr (!Next::kAsync) {
+        next_x.load(xs + offset, left);
+        next_dy.load(dys + offset, left);
+      }
       next_mean = ld_f32(p.mean + row);
       next_rstd = ld_f32(p.rstd + row);
     }
   };
-  if (kAhead) fetch(first, at);
+  if constexpr (Next::kAsync) {
+    issue(first, at);
+    issue(first + stride, at + step);
+  }
+  if (Next::kAsync || kRegs) fetch(first, at);
   {
     Vector<E, VEC, NV, T> w;
     w.load(p.weight, p.wide_weight, rows.segment * p.weight_stride + c0, left);
     w.get(p.weight, p.wide_weight, p.add_one ? 0.0f : 1.0f, p.add_one ? 1.0f : 0.0f, weight);
   }
   for (int64_t row = first; row < rows.end; row += stride) {
-    if (!kAhead) fetch(row, at);
-    x = next_x;
-    dy = next_dy;
+    if (!Next::kAsync && !kRegs) fetch(row, at);
     mean = next_mean;
     rstd = next_rstd;
-    if (kAhead) fetch(row + stride, at + stride * F);
+    if constexpr (Next::kAsync) {
+      next.take(left, x, dy);
+      issue(row + 2 * stride, at + 2 * step);
+    } else {
+      x = next_x;
+      dy = next_dy;
+    }
+    if (Next::kAsync || kRegs) fetch(row + stride, at + step);
     const A scale = splat<VEC>(rstd), minus = splat<VEC>(-mean * rstd);
-    A h[kAhead ? NV : 1][L], s0 = splat<VEC>(0.0f), s1 = s0;
+    A h[kKeep ? NV : 1][L], s0 = splat<VEC>(0.0f), s1 = s0;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (j * T * VEC < left) {
         A d[L];
-        A(&hj)[L] = h[kAhead ? j : 0];
+        A(&hj)[L] = h[kKeep ? j : 0];
         x.v[j].get_lanes(hj);
         dy.v[j].get_lanes(d);
 #pragma unroll
@@ -382,9 +487,9 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, T == 32 || T == 128
     for (int j = 0; j < NV; ++j)
       if (j * T * VEC < left) {
         A d[L];
-        A(&hj)[L] = h[kAhead ? j : 0];
+        A(&hj)[L] = h[kKeep ? j : 0];
         dy.v[j].get_lanes(d);
-        if constexpr (!kAhead) {
+        if constexpr (!kKeep) {
           x.v[j].get_lanes(hj);
 #pragma unroll
           for (int i = 0; i < L; ++i) hj[i] = fma(hj[i], scale, minus);
@@ -395,11 +500,13 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, T == 32 || T == 128
         out.set_lanes(d);
         out.store(dx + j * T * VEC);
       }
-    at += stride * F;
+    at += step;
   }
   if (!p.partial) return;
   float* part = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * F;
+  float* sums = reinterpret_cast<float*>(smem);
   float* to = T == 32 ? sums + warp * 2 * F : part;
+  if constexpr (T == 32) __syncthreads();  // every warp is done with its rows
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = c0 + j * T * VEC;
@@ -489,6 +596,8 @@ int enqueue(void (*kernel)(NormParams), dim3 grid, int threads, size_t smem, con
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (smem > 40 * 1024)
+    CONVROT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
   CONVROT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
   return check_launch("layer norm kernel");
 }
@@ -516,8 +625,7 @@ bool aligned_for(const NormParams& p, int vec) {
   if constexpr (U == 1)                               \
     if (vectors <= 64 * 3 * U) return RUN(3 * U, 64); \
   if (vectors <= 128 * 3 * U) return RUN(3 * U, 128); \
-  if constexpr (U == 1)                               \
-    if (vectors <= 256 * 3 * U) return RUN(3 * U, 256); \
+  if (vectors <= 256 * 3 * U) return RUN(3 * U, 256); \
   if (vectors <= 384 * 3 * U) return RUN(3 * U, 384); \
   if (vectors <= 512 * 4 * U) return RUN(4 * U, 512); \
   return LONG();
@@ -539,7 +647,7 @@ int forward_rows(NormParams p, int vectors, cudaStream_t s) {
     const int64_t most = 4LL * device_sm_count();
     return enqueue(norm_fwd_long_kernel<E>, dim3(static_cast<unsigned>(p.rows < most ? p.rows : most)), 512, 0, p, s);
   };
-#define CONVROT_RUN(NV, T) enqueue(norm_fwd_kernel<E, VEC, NV, T>, grid(T), T == 32 ? 32 * kWarps : T, 0, p, s)
+#define CONVROT_RUN(NV, T) enqueue(norm_fwd_kernel<E, VEC, NV, T>, grid(T), T == 32 ? 32 * kWarps : T, Ahead<E, VEC, NV, T, 1>::kSmem, p, s)
   CONVROT_NORM_SIZES(CONVROT_RUN, longest)
 #undef CONVROT_RUN
 }
@@ -554,9 +662,9 @@ int backward_rows(const NormParams& p, int vectors, cudaStream_t s) {
       rc = enqueue(norm_partial_long_kernel<E>, dim3((p.features + 255) / 256, ctas), 256, 0, p, s);
     return rc;
   };
-#define CONVROT_RUN(NV, T)                                                                \
-  enqueue(norm_bwd_kernel<E, VEC, NV, T>, ctas, T == 32 ? 32 * kWarps : T,                \
-          T == 32 ? 2 * kWarps * sizeof(float) * p.features : 0, p, s)
+#define CONVROT_RUN(NV, T)                                                 \
+  enqueue(norm_bwd_kernel<E, VEC, NV, T>, ctas, T == 32 ? 32 * kWarps : T, \
+          std::max<size_t>(Ahead<E, VEC, NV, T, 2>::kSmem, T == 32 ? 2 * kWarps * sizeof(float) * p.features : 0), p, s)
   CONVROT_NORM_SIZES(CONVROT_RUN, longest)
 #undef CONVROT_RUN
 }

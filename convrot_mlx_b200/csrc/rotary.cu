@@ -8,9 +8,10 @@
 // what follows the pairs is copied.  The rotation is orthogonal, so the
 // gradient of the input is the rotation by -t of the gradient of the output.
 //
-// The angle is formed in 64 bits as a number of turns and reduced to less
-// than half a turn there, so that large positions lose nothing; sine and
-// cosine are 32-bit.
+// The angle is formed as a number of turns, position times frequency, with the
+// frequency in two floats: the product with the first is exact in two floats
+// (its rounding error by one FMA), so that whole turns can be taken off
+// exactly and large positions lose nothing; sine and cosine are 32-bit.
 #include "rows.cuh"
 
 #include <cmath>
@@ -37,19 +38,24 @@ struct RotaryParams {
   int batch, dim, pairs, axes, adjacent;
   int units;       // threads that a head's values are spread over
   uint32_t slots;  // tokens of a CTA
+  uint32_t groups; // of heads in a CTA
   float sign;  // 1, or -1 for the gradient
-  double turns[kMaxPairs];  // frequency of each pair in turns a position
+  float2 turns[kMaxPairs];  // frequency of each pair in turns a position, high and low part
   uint8_t axis[kMaxPairs];
 };
 
-// One thread keeps the sines and cosines of its pairs of one token and applies
-// them to the same place of every head of its share of the heads, kHeads
-// heads (64 bytes) in flight and as many being turned.  Units of a head, adjacent pairs: unit u is the VEC values
-// from VEC u on (values past the pairs are copied).  Pairs half apart: unit u
-// is the VEC values from VEC u on and the VEC from pairs + VEC u on; further
-// units copy VEC values each.  WIDE: VEC values move in one access; else one
-// value an access.
-template <bool ADJACENT> constexpr int kHeads = ADJACENT ? 4 : 2;
+// A CTA has some tokens; its threads first form the sines and cosines of all
+// their pairs, once for all heads, in shared memory.  Then a thread has one
+// unit of a head's values, of one token and one group of the heads, keeps the
+// unit's sines and cosines in registers and turns its heads one after another,
+// kHeads of them at a time with as many more in flight.  Units of a head,
+// adjacent pairs: unit u is the VEC values from VEC u on (values past the
+// pairs are copied).  Pairs half apart: unit u is the VEC values from VEC u on
+// and the VEC from pairs + VEC u on; further units copy VEC values each.
+// WIDE: VEC values move in one access; else one value an access.
+template <bool ADJACENT> constexpr int kHeads = 4;
+template <bool ADJACENT> constexpr bool kAhead = ADJACENT;
+constexpr int kThreads = 256;
 
 template <typename T, int VEC, bool WIDE>
 struct Unit {
@@ -77,40 +83,64 @@ struct Unit {
 };
 
 template <typename T, int VEC, bool WIDE, bool ADJACENT>
-__global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kThreads, 3) rotary_kernel(const __grid_constant__ RotaryParams p) {
   constexpr int NP = ADJACENT ? VEC / 2 : VEC;  // pairs of a unit
   constexpr int kUnroll = kHeads<ADJACENT>;
+  // tokens x pairs: at most one unit of NP pairs for each thread
+  __shared__ float2 turned[kThreads * NP];
+  // the frequencies, since threads of a warp would read different ones from
+  // the parameters one after another
+  __shared__ float2 freq[kMaxPairs];
+  __shared__ uint8_t axis[kMaxPairs];
+  for (int j = threadIdx.x; j < p.pairs; j += kThreads) {
+    freq[j] = p.turns[j];
+    axis[j] = p.axis[j];
+  }
+  __syncthreads();
   grid_dependency_wait();
   grid_dependents_launch();
-  const uint32_t slot = threadIdx.x / static_cast<uint32_t>(p.units);  // token of the CTA
-  const int u = static_cast<int>(threadIdx.x - slot * p.units);
-  const uint32_t bt = blockIdx.x * p.slots + slot;
-  if (slot >= p.slots || bt >= p.batch * static_cast<uint32_t>(p.tokens)) return;
+  const uint32_t all = p.batch * static_cast<uint32_t>(p.tokens);
+  const uint32_t bt0 = blockIdx.x * p.slots;
+  for (uint32_t i = threadIdx.x; i < p.slots * p.pairs; i += kThreads) {
+    const uint32_t s = i / p.pairs, j = i - s * p.pairs, bt = bt0 + s;
+    if (bt < all) {
+      const uint32_t sample = bt / static_cast<uint32_t>(p.tokens);
+      const int64_t token = bt - sample * static_cast<uint32_t>(p.tokens);
+      const float pos = ld_f32(p.positions + sample * p.pos_b + token * p.axes + axis[j]);
+      const float whole = __fmul_rn(pos, freq[j].x);
+      const float rest = __fmaf_rn(pos, freq[j].y, __fmaf_rn(pos, freq[j].x, -whole));
+      float2 cs;
+      sincospif(2.0f * (__fsub_rn(whole, rintf(whole)) + rest), &cs.y, &cs.x);
+      cs.y *= p.sign;
+      turned[i] = cs;
+    }
+  }
+  __syncthreads();
+  // thread = (group of heads, token, unit)
+  const uint32_t per_group = p.slots * p.units;
+  const uint32_t group = threadIdx.x / per_group, at = threadIdx.x - group * per_group;
+  const uint32_t slot = at / static_cast<uint32_t>(p.units), bt = bt0 + slot;
+  const int u = static_cast<int>(at - slot * p.units);
+  if (group >= p.groups || bt >= all) return;
   const uint32_t sample = bt / static_cast<uint32_t>(p.tokens);
   const int64_t b = sample, token = bt - sample * static_cast<uint32_t>(p.tokens);
   const int turning = ADJACENT ? p.units : p.pairs / VEC;  // units that turn
   const bool turns = u < turning;
   const int e0 = ADJACENT || turns ? u * VEC : 2 * p.pairs + (u - turning) * VEC;  // first value of the unit
   const int left = p.dim - e0;
+  const int count = turns ? min(NP, max(0, p.pairs - u * NP)) : 0;  // pairs of the unit
 
   float cs[NP], sn[NP];
-  if (turns) {
-    const float* pos = p.positions + b * p.pos_b + token * p.axes;
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int j = u * NP + i;
-      cs[i] = 1.0f;
-      sn[i] = 0.0f;
-      if (j < p.pairs) {
-        const double turn = static_cast<double>(ld_f32(pos + p.axis[j])) * p.turns[j];
-        sincospif(2.0f * static_cast<float>(turn - rint(turn)), &sn[i], &cs[i]);
-        sn[i] *= p.sign;
-      }
-    }
+  for (int i = 0; i < NP; ++i) {
+    const float2 v = i < count ? turned[slot * p.pairs + u * NP + i] : make_float2(1.0f, 0.0f);
+    cs[i] = v.x;
+    sn[i] = v.y;
   }
   const int heads = p.t[0].heads + p.t[1].heads;
-  const int h0 = static_cast<int>(static_cast<int64_t>(heads) * blockIdx.y / gridDim.y);
-  const int h1 = static_cast<int>(static_cast<int64_t>(heads) * (blockIdx.y + 1) / gridDim.y);
+  const int share = static_cast<int>(blockIdx.y * p.groups + group), shares = static_cast<int>(gridDim.y * p.groups);
+  const int h0 = static_cast<int>(static_cast<int64_t>(heads) * share / shares);
+  const int h1 = static_cast<int>(static_cast<int64_t>(heads) * (share + 1) / shares);
 #pragma unroll 1
   for (int which = 0; which < 2; ++which) {
     const RotaryTensor& t = p.t[which];
@@ -134,30 +164,33 @@ __global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ 
         src += src_step;
       }
     };
-    fetch(begin);
+    if (kAhead<ADJACENT>) fetch(begin);
 #pragma unroll 1
     for (int h = begin; h < hi; h += kUnroll) {
+      if (!kAhead<ADJACENT>) fetch(h);
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) {
         x[k] = nx[k];
         if constexpr (!ADJACENT) y[k] = ny[k];
       }
-      fetch(h + kUnroll);
+      if (kAhead<ADJACENT>) fetch(h + kUnroll);
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) {
         if (h + k < hi) {
           if constexpr (ADJACENT) {
-            // values past the pairs keep their bits
-            float v[VEC];
-            x[k].raw.get(v);
+            if (count > 0) {  // values past the pairs keep their bits
+              float v[VEC];
+              x[k].raw.get(v);
+              const bool full = count == NP;
 #pragma unroll
-            for (int i = 0; i < NP; ++i)
-              if (u * NP + i < p.pairs) {
-                const float x0 = v[2 * i], x1 = v[2 * i + 1];
-                v[2 * i] = x0 * cs[i] - x1 * sn[i];
-                v[2 * i + 1] = x0 * sn[i] + x1 * cs[i];
-              }
-            x[k].raw.set(v);
+              for (int i = 0; i < NP; ++i)
+                if (full || i < count) {
+                  const float x0 = v[2 * i], x1 = v[2 * i + 1];
+                  v[2 * i] = x0 * cs[i] - x1 * sn[i];
+                  v[2 * i + 1] = x0 * sn[i] + x1 * cs[i];
+                }
+              x[k].raw.set(v);
+            }
           } else if (turns) {
             float v[VEC], w[VEC];
             x[k].raw.get(v);
@@ -183,17 +216,24 @@ __global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ 
 template <typename T, int VEC, bool WIDE, bool ADJACENT>
 int launch(RotaryParams& p, cudaStream_t stream) {
   p.units = ADJACENT ? (p.dim + VEC - 1) / VEC : p.pairs / VEC + (p.dim - 2 * p.pairs + VEC - 1) / VEC;
-  p.slots = 256 / p.units;
-  const int64_t blocks = (static_cast<int64_t>(p.batch) * p.tokens + p.slots - 1) / p.slots;
-  // The heads are shared out until there are about 16 CTAs for each SM (some
-  // waves, for an even end), each with kHeads heads at least.
+  // Several groups of heads in a CTA, so that the sines are formed by as many
+  // threads as use them, of eight heads at least (with three or four a thread
+  // only starts and ends: 17627 tokens of 24 heads took 70 us instead of 51).
   const int heads = p.t[0].heads + p.t[1].heads;
-  int64_t shares = (16LL * device_sm_count() + blocks - 1) / blocks;
   const int most = (heads + kHeads<ADJACENT> - 1) / kHeads<ADJACENT>;
-  if (shares > most) shares = most;
+  const int room = kThreads / (4 * p.units), wanted = heads / 8;
+  const int groups = room < wanted ? room : wanted;
+  p.groups = static_cast<uint32_t>(groups < 1 ? 1 : groups);
+  p.slots = kThreads / (p.units * p.groups);
+  const int64_t blocks = (static_cast<int64_t>(p.batch) * p.tokens + p.slots - 1) / p.slots;
+  // Few tokens: more CTAs for the same tokens, until there are about 4 for
+  // each SM.
+  int64_t shares = (4LL * device_sm_count() + blocks - 1) / blocks;
+  const int64_t limit = (most + p.groups - 1) / p.groups;
+  if (shares > limit) shares = limit;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(shares), 1);
-  cfg.blockDim = dim3(256, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -227,6 +267,8 @@ int launch_type(RotaryParams& p, cudaStream_t s) {
     return launch<T, 2, false, true>(p, s);
   }
   if (aligned_for<T>(p, W)) return launch<T, W, true, false>(p, s);
+  if constexpr (W == 8)
+    if (aligned_for<T>(p, 4)) return launch<T, 4, true, false>(p, s);
   if (aligned_for<T>(p, 2)) return launch<T, 2, true, false>(p, s);
   return launch<T, 1, false, false>(p, s);
 }
@@ -260,7 +302,8 @@ int convrot_axial_rotary(int dtype, int64_t batch, int64_t tokens, int64_t dim, 
     const double ratio = std::pow(theta, -2.0 / widths[a]);
     double turns = 0.15915494309189533577;  // 1 / (2 pi): pair 0 turns by one radian a position
     for (int j = 0; j < widths[a] / 2; ++j, ++pairs, turns *= ratio) {
-      p.turns[pairs] = turns;
+      const float high = static_cast<float>(turns);
+      p.turns[pairs] = make_float2(high, static_cast<float>(turns - high));
       p.axis[pairs] = static_cast<uint8_t>(a);
     }
   }
