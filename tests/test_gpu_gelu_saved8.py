@@ -58,7 +58,7 @@ def _check(x, y, dy, dx):
 
 
 SHAPES = [(1, 1), (3, 7), (2, 127), (2, 128), (5, 129), (4, 256), (1, 12288), (33, 4100), (500, 96), (17, 1000), (300, 513),
-          (9, 16384), (64, 2056)]
+          (9, 16384), (64, 2056), (5, 258), (40, 1030), (700, 384)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

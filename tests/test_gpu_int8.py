@@ -42,6 +42,29 @@ def test_codes(dtype, rows, features):
     assert codes.abs().amax(1).eq(127).all()
 
 
+# every row shape of the quantizer's kernels: widths on either side of each, in vectors of 16 bytes, of two elements
+# and of one; and rows enough that a CTA has several
+ROW_SHAPES = [(3, f) for f in (31, 32, 34, 62, 66, 250, 256, 258, 510, 513, 1000, 1026, 2040, 2050, 2056, 4094, 4100, 4104,
+                               8190, 8195, 8200, 16376, 16386, 16389, 16392, 32776)] + [(20000, 37), (20000, 64),
+                                                                                      (9000, 130), (5000, 1032),
+                                                                                      (3001, 2050)]
+
+
+@pytest.mark.parametrize("scaled", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,features", ROW_SHAPES)
+def test_codes_of_every_row_shape(dtype, rows, features, scaled):
+    x = randn((rows, features), dtype, rows + features)
+    factor = randn((features,), torch.float32, 5).abs() + 0.1 if scaled else None
+    pitch = -(-features // 16) * 16
+    codes = torch.full((rows, pitch), 99, dtype=torch.int8, device=dev())
+    scales = torch.empty(rows, device=dev())
+    _lib.call("convrot_quantize_i8", 0, x.data_ptr(), _lib.DTYPE_CODES[dtype], rows, features, features,
+              None if factor is None else factor.data_ptr(), codes.data_ptr(), pitch, scales.data_ptr())
+    assert codes[:, features:].eq(99).all()  # the padding is not touched
+    _check_codes(x, codes[:, :features], scales, (x.float() * factor).double() if scaled else None)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_codes_of_strided_and_unaligned_rows(dtype):
     base = randn((9, 700), dtype, 3)
@@ -89,7 +112,8 @@ SIZES = [(1, 1, 1), (1, 4096, 4096), (2, 33, 17), (5, 512, 640), (8, 1000, 264),
          (64, 3000, 200), (65, 160, 1211), (127, 128, 128), (128, 256, 256), (129, 144, 259), (333, 1997, 1211),
          (257, 4160, 520), (600, 96, 2050), (1100, 1536, 1024),
          (1300, 300, 2100), (1300, 2103, 333), (300, 1997, 5001), (300, 5008, 1040), (2500, 130, 1000), (2500, 1000, 129),
-         (4000, 1216, 1216)]
+         (4000, 1216, 1216), (5000, 128, 1100), (5000, 1100, 130), (40, 8192, 300), (100, 6000, 260), (16, 15000, 130),
+         (3, 8200, 70), (1, 8208, 40), (7, 130, 9000), (2, 4100, 5000), (200, 64, 6000)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -65,7 +65,8 @@ def _sums64(x, w, b, dy, over):
 
 
 SHAPES = [(1, 1), (3, 2), (4, 31), (8, 32), (5, 33), (8, 768), (300, 64), (7, 1153), (64, 3072), (33, 4100), (9, 8192),
-          (3, 12289), (2, 40000), (500, 96), (1, 16384)]
+          (3, 12289), (2, 40000), (500, 96), (1, 16384), (3000, 3072), (5000, 257), (2000, 130), (900, 1600), (700, 1602),
+          (400, 5000), (301, 5001), (200, 6146), (90, 9216), (90, 9218), (70, 4609), (2500, 512), (1500, 320)]
 
 
 def _inputs(rows, features, dtype, seed, offset=1.0):
