@@ -402,37 +402,53 @@ Tensor modulated_layer_norm(const Tensor& x, Tensor shift, Tensor scale, double 
 
 // --- GELU with its input saved in 8 bits -----------------------------------------
 
-Tensor gelu_forward(const Tensor& x, Tensor* codes, Tensor* scales) {
+// Codes, then from the next multiple of 16 bytes on the scales: one allocation.
+struct Saved {
+  int64_t rows, features, scales_at, bytes;
+  Saved(int64_t rows, int64_t features)
+      : rows(rows),
+        features(features),
+        scales_at((rows * features + 15) / 16 * 16),
+        bytes(scales_at + 4 * rows * ((features + kSavedGroup - 1) / kSavedGroup)) {}
+};
+
+Tensor gelu_forward(const Tensor& x, Tensor* saved) {
   const c10::cuda::OptionalCUDAGuard guard(x.device());
   const int64_t features = x.size(-1), rows = x.numel() / features;
   const Tensor y = at::empty_like(x);
-  if (codes) {
-    *codes = at::empty({rows, features}, x.options().dtype(at::kChar));
-    *scales = at::empty({rows, (features + kSavedGroup - 1) / kSavedGroup}, x.options().dtype(at::kFloat));
+  int8_t* codes = nullptr;
+  float* scales = nullptr;
+  if (saved && rows > 0) {
+    const Saved layout(rows, features);
+    *saved = at::empty({layout.bytes}, x.options().dtype(at::kChar));
+    codes = static_cast<int8_t*>(saved->data_ptr());
+    scales = reinterpret_cast<float*>(codes + layout.scales_at);
   }
-  check(convrot_gelu_saved8(x.data_ptr(), dtype_code(x.scalar_type()), rows, features, y.data_ptr(),
-                            codes ? static_cast<int8_t*>(codes->data_ptr()) : nullptr,
-                            codes ? static_cast<float*>(scales->data_ptr()) : nullptr, stream_of(x)),
+  check(convrot_gelu_saved8(x.data_ptr(), dtype_code(x.scalar_type()), rows, features, y.data_ptr(), codes, scales,
+                            stream_of(x)),
         "convrot_gelu_saved8");
   return y;
 }
 
 struct GeluSaved8 : torch::autograd::Function<GeluSaved8> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x) {
-    Tensor codes, scales;
-    const Tensor y = gelu_forward(x, &codes, &scales);
-    ctx->save_for_backward({codes, scales});
+    Tensor saved;
+    const Tensor y = gelu_forward(x, &saved);
+    ctx->save_for_backward({saved});
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("gelu_tanh_saved8");
-    const auto saved = ctx->get_saved_variables();
     const Tensor dy = grads[0].contiguous();
     const c10::cuda::OptionalCUDAGuard guard(dy.device());
     const Tensor dx = at::empty_like(dy);
-    check(convrot_gelu_saved8_backward(dy.data_ptr(), dtype_code(dy.scalar_type()), saved[0].size(0), saved[0].size(1),
-                                       static_cast<const int8_t*>(saved[0].data_ptr()),
-                                       static_cast<const float*>(saved[1].data_ptr()), dx.data_ptr(), stream_of(dy)),
+    const int64_t features = dy.size(-1), rows = dy.numel() / features;
+    if (rows == 0) return {dx};
+    const Tensor saved = ctx->get_saved_variables()[0];
+    const auto* codes = static_cast<const int8_t*>(saved.data_ptr());
+    const auto* scales = reinterpret_cast<const float*>(codes + Saved(rows, features).scales_at);
+    check(convrot_gelu_saved8_backward(dy.data_ptr(), dtype_code(dy.scalar_type()), rows, features, codes, scales,
+                                       dx.data_ptr(), stream_of(dy)),
           "convrot_gelu_saved8_backward");
     return {dx};
   }
@@ -444,7 +460,7 @@ Tensor gelu_tanh_saved8(Tensor x) {
   require_cuda(x);
   if (!x.is_contiguous()) x = x.contiguous();
   if (at::GradMode::is_enabled() && x.requires_grad()) return GeluSaved8::apply(x);
-  return gelu_forward(x, nullptr, nullptr);
+  return gelu_forward(x, nullptr);
 }
 
 }  // namespace

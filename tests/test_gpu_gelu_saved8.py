@@ -181,3 +181,12 @@ def test_refusals():
     assert lib.convrot_gelu_saved8(p, 7, 2, 4, p, p, p, None) == -1
     assert lib.convrot_gelu_saved8(p, 0, 2, 4, p, p, None, None) == -1
     assert lib.convrot_gelu_saved8_backward(p, 0, 2, 4, None, p, p, None) == -1
+
+
+def test_a_gradient_that_would_be_differentiated_again_is_refused():
+    x = randn((4, 8), torch.float32, 1).requires_grad_()
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(cr.gelu_tanh_saved8(x).sum(), x, create_graph=True)
+    w = torch.ones(8, device=dev())
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(cr.layer_norm(x, w).sum(), x, create_graph=True)
