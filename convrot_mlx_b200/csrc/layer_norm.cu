@@ -49,10 +49,12 @@ __global__ void __launch_bounds__(512) norm_reduce_kernel(const NormParams p) {
   }
 }
 
-// Most CTAs that share a segment's rows, each with one partial sum: about
-// three of 128 threads for each SM, and two rows each at least.
-int chunks_of(int64_t rows_per_weight, int64_t segments) {
-  int64_t chunks = 3LL * device_sm_count() / segments;
+// CTAs that share a segment's rows, each with one partial sum: as many as the
+// GPU holds at once (fewer for wide rows, whose CTAs and sums are large), and
+// two rows each at least.
+int chunks_of(int64_t rows_per_weight, int64_t segments, int64_t features) {
+  const int64_t per_sm = features <= 3072 ? 3 : features <= 8192 ? 2 : 1;
+  int64_t chunks = per_sm * device_sm_count() / segments;
   if (chunks > rows_per_weight / 2) chunks = rows_per_weight / 2;
   return static_cast<int>(chunks < 1 ? 1 : chunks);
 }
@@ -132,7 +134,7 @@ int64_t convrot_layer_norm_workspace(int64_t rows, int64_t features, int64_t row
   using namespace convrot::norm;
   if (rows <= 0 || features <= 0 || rows_per_weight <= 0) return 0;
   const int64_t segments = rows / rows_per_weight;
-  return segments * chunks_of(rows_per_weight, segments) * 2 * features * static_cast<int64_t>(sizeof(float));
+  return segments * chunks_of(rows_per_weight, segments, features) * 2 * features * static_cast<int64_t>(sizeof(float));
 }
 
 int convrot_layer_norm_backward(const void* x, const void* dy, int dtype, int64_t rows, int64_t features,
@@ -162,7 +164,7 @@ int convrot_layer_norm_backward(const void* x, const void* dy, int dtype, int64_
   p.rows_per_weight = rows_per_weight;
   p.weight_stride = weight_stride;
   p.features = static_cast<int>(features);
-  p.chunks = chunks_of(rows_per_weight, rows / rows_per_weight);
+  p.chunks = chunks_of(rows_per_weight, rows / rows_per_weight, features);
   p.add_one = add_one;
   p.wide_weight = dtype != CONVROT_F32 && weight_dtype == CONVROT_F32;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -50,6 +50,11 @@ namespace {
 
 constexpr int kWarps = 4;  // of a CTA whose warps each have rows of their own
 
+// CTAs of T threads that the registers of an SM are shared out to.
+constexpr int ctas_of(int threads) {
+  return threads == 64 ? 6 : threads == 32 || threads == 128 ? 3 : threads <= 256 ? 2 : 1;
+}
+
 // Adds up each of N values (1 or 2) over a warp: two are exchanged so that
 // each half of the lanes goes on with one.  Afterwards v[0] of lane l is the
 // sum of value l / (32 / N).
@@ -395,7 +400,7 @@ __global__ void __launch_bounds__(512) norm_fwd_long_kernel(const NormParams p) 
 // With up to 24 values of a row a thread keeps h in float32; with more it
 // keeps the row as it lies in memory and forms h twice.
 template <typename E, int VEC, int NV, int T>
-__global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, T == 32 || T == 128 ? 3 : (T == 64 ? 6 : 1))
+__global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, ctas_of(T))
     norm_bwd_kernel(const NormParams p) {
   constexpr int L = kLanes<VEC>;
   using A = Lane<VEC>;
@@ -602,6 +607,18 @@ int enqueue(void (*kernel)(NormParams), dim3 grid, int threads, size_t smem, con
   return check_launch("layer norm kernel");
 }
 
+// CTAs of a kernel that an SM holds at once.
+template <auto Kernel>
+int resident(int threads, int smem) {
+  static const int ctas = [&] {
+    int n = 0;
+    if (smem > 40 * 1024) cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, threads, smem) != cudaSuccess) cudaGetLastError();
+    return n < 1 ? 1 : n;
+  }();
+  return ctas;
+}
+
 // Whether every vector of `vec` elements of the rows and of the weights is
 // aligned for its accesses.
 template <typename E>
@@ -616,30 +633,28 @@ bool aligned_for(const NormParams& p, int vec) {
 // A pass over rows of `vectors` vectors: RUN(NV, T) launches with NV vectors
 // for each of T threads.  U: vectors of a unit, one of 16 bytes or four of one
 // or two elements.  Up to four units a lane a warp has a row to itself; then
-// CTAs whose threads have three units each, in the sizes that keep most of
-// them busy; then the largest, four units for each of 512 threads.
-#define CONVROT_NORM_SIZES(RUN, LONG)                 \
-  if (vectors <= 32 * U) return RUN(U, 32);           \
-  if (vectors <= 32 * 2 * U) return RUN(2 * U, 32);   \
-  if (vectors <= 32 * 4 * U) return RUN(4 * U, 32);   \
-  if constexpr (U == 1)                               \
-    if (vectors <= 64 * 3 * U) return RUN(3 * U, 64); \
-  if (vectors <= 128 * 3 * U) return RUN(3 * U, 128); \
-  if (vectors <= 256 * 3 * U) return RUN(3 * U, 256); \
-  if (vectors <= 384 * 3 * U) return RUN(3 * U, 384); \
-  if (vectors <= 512 * 4 * U) return RUN(4 * U, 512); \
+// CTAs of two or more for each SM, with three or four units a thread, in the
+// sizes that keep most of their threads busy; then the largest.
+#define CONVROT_NORM_SIZES(RUN, LONG)                   \
+  if (vectors <= 32 * U) return RUN(U, 32);             \
+  if (vectors <= 32 * 2 * U) return RUN(2 * U, 32);     \
+  if (vectors <= 32 * 4 * U) return RUN(4 * U, 32);     \
+  if (vectors <= 64 * 3 * U) return RUN(3 * U, 64);     \
+  if (vectors <= 128 * 3 * U) return RUN(3 * U, 128);   \
+  if (vectors <= 192 * 3 * U) return RUN(3 * U, 192);   \
+  if (vectors <= 384 * 3 * U) return RUN(3 * U, 384);   \
+  if (vectors <= 512 * 4 * U) return RUN(4 * U, 512);   \
   return LONG();
 
 template <typename E, int VEC, int U>
 int forward_rows(NormParams p, int vectors, cudaStream_t s) {
   const int64_t segments = p.rows / p.rows_per_weight;
-  // CTAs that share a segment's rows: a CTA for each row (4 rows), until there
-  // are about 512 threads for each SM
-  auto grid = [&](int threads) {
+  // CTAs that share a segment's rows: a CTA for each row (4 rows), until the
+  // SMs hold no more (12288 x 1024 bf16: 9.5 us, 13 with more CTAs than fit)
+  auto grid = [&](int threads, int64_t resident) {
     const int64_t rows_at = threads == 32 ? kWarps : 1;
-    const int64_t per_sm = threads == 32 ? 8 : threads < 512 ? 512 / threads : 1;
     const int64_t chunks = (p.rows_per_weight + rows_at - 1) / rows_at;
-    const int64_t limit = per_sm * device_sm_count() / segments;
+    const int64_t limit = resident * device_sm_count() / segments;
     p.chunks = static_cast<int>(chunks < limit ? chunks : (limit < 1 ? 1 : limit));
     return dim3(static_cast<unsigned>(segments * p.chunks));
   };
@@ -647,7 +662,10 @@ int forward_rows(NormParams p, int vectors, cudaStream_t s) {
     const int64_t most = 4LL * device_sm_count();
     return enqueue(norm_fwd_long_kernel<E>, dim3(static_cast<unsigned>(p.rows < most ? p.rows : most)), 512, 0, p, s);
   };
-#define CONVROT_RUN(NV, T) enqueue(norm_fwd_kernel<E, VEC, NV, T>, grid(T), T == 32 ? 32 * kWarps : T, Ahead<E, VEC, NV, T, 1>::kSmem, p, s)
+#define CONVROT_RUN(NV, T)                                                                                       \
+  enqueue(norm_fwd_kernel<E, VEC, NV, T>,                                                                        \
+          grid(T, resident<norm_fwd_kernel<E, VEC, NV, T>>(T == 32 ? 32 * kWarps : T, Ahead<E, VEC, NV, T, 1>::kSmem)), \
+          T == 32 ? 32 * kWarps : T, Ahead<E, VEC, NV, T, 1>::kSmem, p, s)
   CONVROT_NORM_SIZES(CONVROT_RUN, longest)
 #undef CONVROT_RUN
 }
