@@ -12,11 +12,17 @@
 // kernels on tcgen05 kind::i8, operands by TMA in 128-byte-swizzled tiles,
 // accumulators in TMEM:
 // * pair_kernel: CTA pairs (cta_group::2), 256 tokens x 256 channels a tile,
-//   persistent, for products that fill the GPU with such tiles.  Bound by the
-//   tensor cores and what L2 delivers to them: 8192^3 in 372 us (2950 TOPS),
-//   4096 x 3072 x 12288 (tokens, K, channels) in 117 us (2630), of which 6% are
-//   the last wave's idle pairs; 1536 x 3072 x 3072, one wave, in 16 us, of
-//   which 5 fill and drain the pipeline.
+//   persistent, for products that fill the GPU with such tiles.  Bound by
+//   shared memory, which the copies write and the tensor cores read: a stage
+//   of 128 K takes the MMAs alone 0.27 us, the copies alone 0.28, both 0.36 in
+//   one wave and 0.42 over many.  8192^3 in 372 us (2950 TOPS); 4096 x 3072 x
+//   12288 (tokens, K, channels) in 117 us (2630), 6% of it for the last wave's
+//   idle pairs; 1536 x 3072 x 3072, one wave, in 16 us, of which 7 are launch,
+//   first copies and the last tile's epilogue.  Tiles of 192 channels take as
+//   long a stage as 256 (0.36; 136 us instead of 117 for 12288 channels), so
+//   they gain only where both give one wave: 13.3 us instead of 14.8 for 2000 x
+//   1000 x 3000, too little for a second set of kernels.  Rings of 4 stages
+//   125 us, copies in halves 117.
 // * swap_kernel: 128 channels on the MMA's M side and 16 to 128 tokens on its
 //   N side, K split over a cluster, for few tokens or few tiles.
 #include <cudaTypedefs.h>
