@@ -91,6 +91,40 @@ def test_views_of_a_projection(dtype, interleaved, d, axes):
     assert_no_device_error()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d,axes", [(8, (2,)), (8, (6,)), (16, (14,)), (64, (10, 20, 20)), (64, (2, 4)), (88, (30, 30, 26)),
+                                    (96, (42, 42)), (128, (20, 42, 42)), (128, (126,)), (132, (44, 42, 42)),
+                                    (136, (40, 42, 42)), (248, (2,)), (256, (42, 84, 84)), (256, (86, 84, 86))])
+@pytest.mark.parametrize("t,h,kv", [(1, 1, 1), (3, 40, 8), (37, 5, 2), (260, 13, 25)])
+def test_halves_that_begin_anywhere(dtype, d, axes, t, h, kv):
+    b = 2
+    q, k = randn((b, h, t, d), dtype, 41).requires_grad_(), randn((b, kv, t, d), dtype, 42).requires_grad_()
+    pos = _positions(t, axes, 43)
+    yq, yk = cr.axial_rotary(q, k, pos, axes, interleaved=False)
+    for x, y in ((q, yq), (k, yk)):
+        assert_within(y.detach(), *_rotate64(x.detach(), pos, axes, 10000.0, False))
+    dq, dk = randn(q.shape, dtype, 44), randn(k.shape, dtype, 45)
+    gq, gk = torch.autograd.grad((yq, yk), (q, k), (dq, dk))
+    for x, y in ((dq, gq), (dk, gk)):
+        assert_within(y, *_rotate64(x, pos, axes, 10000.0, False, -1.0))
+    assert_no_device_error()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("d,axes", [(64, (10, 20, 20)), (128, (32, 40, 40)), (37, (6, 10, 14))])
+def test_values_past_the_pairs_are_copied(dtype, interleaved, d, axes):
+    turned = sum(axes)
+    q = randn((1, 3, 20, d), dtype, 51)
+    q[..., turned:] = torch.tensor([-0.0, float("inf"), float("-inf"), 1e-7], dtype=dtype, device=dev()).repeat(d)[: d - turned]
+    q[0, 0, 0, 0] = float("inf")  # one pair of one token: its two values and no others
+    y, _ = cr.axial_rotary(q, None, _positions(20, axes, 52, top=7) + 1, axes, interleaved=interleaved)
+    bits = torch.int32 if dtype == torch.float32 else torch.int16
+    assert torch.equal(y[..., turned:].contiguous().view(bits), q[..., turned:].contiguous().view(bits))
+    finite = torch.isfinite(y[..., :turned])
+    assert int((~finite).sum()) == 2 and not finite[0, 0, 0, 0] and not finite[0, 0, 0, 1 if interleaved else turned // 2]
+
+
 def test_positions_of_each_sample_types_and_size():
     axes, t = (16, 24, 24), 21
     q, k = randn((3, 4, t, 64), torch.float32, 11), randn((3, 2, t, 64), torch.float32, 12)
