@@ -8,6 +8,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <initializer_list>
 #include <string>
 #include <vector>
 
@@ -61,10 +62,16 @@ int dtype_code(at::ScalarType t) {
   }
 }
 
-void require_cuda(const Tensor& t) {
-  if (t.defined() && !t.is_cuda())
-    refuse("convrot_mlx_b200 runs on CUDA (sm_100a) only; got a tensor on ", t.device().str(),
-           " (there is no CPU fallback)");
+// All tensors of a call (undefined ones aside) on the device of the first.
+void require_cuda(std::initializer_list<const Tensor*> tensors) {
+  const c10::Device home = (*tensors.begin())->device();
+  for (const Tensor* t : tensors) {
+    if (!t->defined()) continue;
+    if (!t->is_cuda())
+      refuse("convrot_mlx_b200 runs on CUDA (sm_100a) only; got a tensor on ", t->device().str(),
+             " (there is no CPU fallback)");
+    if (t->device() != home) refuse("expected all tensors on ", home.str(), ", got one on ", t->device().str());
+  }
 }
 
 void once(const char* what) {
@@ -155,7 +162,7 @@ Tensor int8_linear(const Tensor& x, const Tensor& qweight, const Tensor& wscales
   if (wants_grad(wscales) || wants_grad(b))
     refuse("the weight scales and the bias of an int8 linear are frozen: they may not require gradients");
   dtype_code(x.scalar_type());
-  for (const Tensor* t : {&x, &qweight, &wscales, &b}) require_cuda(*t);
+  require_cuda({&x, &qweight, &wscales, &b});
   const Tensor w = padded_rows(qweight), ws = f32_vector(wscales), fb = f32_vector(b);
   if (at::GradMode::is_enabled() && x.requires_grad())
     return Int8Linear::apply(x, w, ws, fb.defined() ? std::optional<Tensor>(fb) : std::nullopt);
@@ -254,7 +261,7 @@ std::pair<Tensor, std::optional<Tensor>> axial_rotary(const Tensor& q, const std
   if (!whole && !each)
     refuse("positions must be (", t, ", ", n, ") or (", b, ", ", t, ", ", n, "), got ", shape_of(positions));
   dtype_code(q.scalar_type());
-  for (const Tensor* x : {&q, &k, &positions}) require_cuda(*x);
+  require_cuda({&q, &k, &positions});
   Tensor pos = positions.requires_grad() ? positions.detach() : positions;
   if (pos.scalar_type() != at::kFloat || !pos.is_contiguous()) pos = pos.to(at::kFloat).contiguous();
   if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k))) {
@@ -346,7 +353,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor run_norm(Tensor x, Tensor weight, Tensor bias, const NormHow& how) {
   if (!(how.eps >= 0)) refuse("eps must be non-negative, got ", how.eps);
   dtype_code(x.scalar_type());
-  for (const Tensor* t : {&x, &weight, &bias}) require_cuda(*t);
+  require_cuda({&x, &weight, &bias});
   // both vectors of x's dtype, or both float32
   for (const Tensor* t : {&weight, &bias}) {
     const Tensor& other = t == &weight ? bias : weight;
@@ -457,7 +464,7 @@ struct GeluSaved8 : torch::autograd::Function<GeluSaved8> {
 Tensor gelu_tanh_saved8(Tensor x) {
   if (x.dim() == 0 || x.size(-1) == 0) refuse("gelu expects features in the last dimension, got ", shape_of(x));
   dtype_code(x.scalar_type());
-  require_cuda(x);
+  require_cuda({&x});
   if (!x.is_contiguous()) x = x.contiguous();
   if (at::GradMode::is_enabled() && x.requires_grad()) return GeluSaved8::apply(x);
   return gelu_forward(x, nullptr);

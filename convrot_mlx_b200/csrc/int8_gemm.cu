@@ -587,9 +587,10 @@ __global__ void __launch_bounds__(kThreads, 2)
 // flight in registers, also from one block of channels to the next (two CTAs
 // for each SM walk the blocks).  The codes of all tokens are in shared memory, copied,
 // or (FUSED, one or two tokens) formed there from x by every CTA itself, which
-// costs less than a kernel of its own before this one.  1 x 4096 x 4096 in 6.5
-// us, 8 x 4096 x 4096 in 7.2, 8 x 4096 x 12288 in 14.2 (3.6 TB/s of weights; a
-// launch, a trip to memory and the join of the warps' sums are about 4 of each).
+// costs less than a kernel of its own before this one.  Weights from HBM: 1 x
+// 4096 x 4096 in 6.8 us (5.9 from L2), 8 x 4096 x 4096 in 7.6, 8 x 4096 x 12288
+// in 14.1 (3.6 TB/s; a launch, a trip to memory and the join of the warps' sums
+// are about 4 of each).
 // ===========================================================================
 namespace gemv {
 

@@ -104,6 +104,9 @@ def int8_matmul(codes, qweight, xscales, wscales, bias=None, *, output_dtype) ->
         raise ValueError(f"int8 activation scales must have shape {(codes.shape[0],)}, got {tuple(xscales.shape)}")
     _dtype_code(output_dtype)
     _require_cuda(codes, qweight, xscales, wscales, bias)
+    for t in (qweight, xscales, wscales, bias):
+        if t is not None and t.device != codes.device:
+            raise ValueError(f"expected all tensors on {codes.device}, got one on {t.device}")
     codes, qweight, xscales, wscales = _padded_rows(codes), _padded_rows(qweight), _f32(xscales), _f32(wscales)
     bias = None if bias is None else _f32(bias)
     m, k = codes.shape
