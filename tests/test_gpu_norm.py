@@ -99,6 +99,17 @@ def test_affine(dtype, rows, features, wide):
     assert_no_device_error()
 
 
+# each number of threads of a row, at its ends, for vectors of one, two and sixteen bytes' worth of elements
+ROW_SIZES = [255, 511, 512, 513, 514, 767, 768, 769, 1022, 1023, 1024, 1026, 1028, 1032, 1534, 1535, 1536, 1537, 1538, 1544, 2303,
+             2304, 2305, 2306, 3070, 3071, 3073, 3074, 3080, 4606, 4607, 4608, 4610, 4616, 6144, 8191, 8192, 8193, 9214, 9224, 16382]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("features", ROW_SIZES)
+def test_ends_of_the_row_shapes(dtype, features):
+    test_affine(dtype, 37, features, False)
+
+
 MOD_SHAPES = [(1, 1, 64), (3, 5, 257), (2, 700, 512), (8, 40, 3072), (5, 1, 33), (2, 3, 20000), (70, 9, 128), (300, 2, 40)]
 
 
