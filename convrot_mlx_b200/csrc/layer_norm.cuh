@@ -47,6 +47,7 @@ struct NormParams {
   int64_t rows, rows_per_weight, weight_stride;
   int features, chunks, add_one;
   int wide_weight;  // the vectors are float32 beside a 16-bit x
+  int keep;         // long rows: shared memory holds them between the passes
   float eps;
 };
 
@@ -247,30 +248,26 @@ struct Rows {
   }
 };
 
-template <typename E>
-__device__ __forceinline__ E ld(const E* p) {
-  Pack<E, 1> pk;
-  pk.load_ahead(p);
-  if constexpr (sizeof(E) == 4) return __uint_as_float(pk.w[0]);
-  else {
-    const uint16_t h = static_cast<uint16_t>(pk.w[0]);
-    return *reinterpret_cast<const E*>(&h);
+// VEC values of a segment's vector plus a constant, or `absent` ones.
+template <typename E, int VEC>
+__device__ __forceinline__ void vector_at(const NormParams& p, const void* base, int64_t at, float absent, float plus,
+                                          float (&v)[VEC]) {
+  if (base == nullptr) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = absent;
+    return;
   }
-}
-
-// One value of a segment's vectors.
-template <typename E>
-__device__ __forceinline__ float vector_at(const NormParams& p, const void* base, int64_t at) {
-  return p.wide_weight ? ld_f32(static_cast<const float*>(base) + at) : Elem<E>::to_f(ld(static_cast<const E*>(base) + at));
-}
-template <typename E>
-__device__ __forceinline__ float weight_at(const NormParams& p, int64_t at) {
-  const float one = p.add_one ? 1.0f : 0.0f;
-  return p.weight ? one + vector_at<E>(p, p.weight, at) : 1.0f;
-}
-template <typename E>
-__device__ __forceinline__ float bias_at(const NormParams& p, int64_t at) {
-  return p.bias ? vector_at<E>(p, p.bias, at) : 0.0f;
+  if (p.wide_weight) {
+    Pack<float, VEC> pk;
+    pk.load_ahead(static_cast<const float*>(base) + at);
+    pk.get(v);
+  } else {
+    Pack<E, VEC> pk;
+    pk.load_ahead(static_cast<const E*>(base) + at);
+    pk.get(v);
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] += plus;
 }
 
 // ---------------------------------------------------------------------------
@@ -363,31 +360,112 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T) norm_fwd_kernel(con
   }
 }
 
-// Rows too long for the registers: three passes over the row, the later ones
-// through L2.
-template <typename E>
-__global__ void __launch_bounds__(512) norm_fwd_long_kernel(const NormParams p) {
+// Rows too long for the registers: three passes over the row in shared memory
+// (in L2 where even that is too small).  The threads copy the 16-byte pieces
+// of memory that a row lies in, wherever it starts, and with room for two rows
+// the next one is on its way while a row is worked on.  2048 x 12288 float32:
+// forward 44 us (55 with the later passes through L2), dx 65 (106); rows that
+// start at any element, 2048 x 16383 bf16: 73 and 95 (80 and 177).
+constexpr int kLong = 512;              // threads of a long row
+constexpr int kLongSmem = 208 * 1024;  // most bytes of rows that are kept
+
+// ARRAYS rows in shared memory, p.keep (1 or 2) times.
+template <typename E, int ARRAYS>
+struct Kept {
+  uint32_t pitch;  // bytes of a row's place
+  int bytes, places;
+  const uint8_t* smem;
+  __host__ __device__ static int64_t pitch_of(int features) {
+    return (static_cast<int64_t>(features) * sizeof(E) + 15) / 16 * 16 + 16;
+  }
+  // Sets of rows: two where two CTAs for each SM have room for them, else one
+  // (2048 x 12288 float32, dx: 65 us, 88 with two sets and one CTA).
+  static int fitting(int features) {
+    const int64_t bytes = ARRAYS * pitch_of(features);
+    return 2 * bytes <= kLongSmem / 2 ? 2 : bytes <= kLongSmem ? 1 : 0;
+  }
+  __device__ __forceinline__ Kept(const NormParams& p, const uint8_t* smem)
+      : pitch(static_cast<uint32_t>(pitch_of(p.features))), bytes(p.features * static_cast<int>(sizeof(E))),
+        places(p.keep), smem(smem) {}
+  // Copies row `row` of array `a` into place `place`, asynchronously.
+  __device__ __forceinline__ void issue(const E* array, int64_t row, int a, int place) const {
+    const uint64_t start = reinterpret_cast<uint64_t>(array) + static_cast<uint64_t>(row) * bytes;
+    const int shift = static_cast<int>(start & 15), end = shift + bytes;
+    const uint32_t dst = smem_u32(smem) + (place * ARRAYS + a) * pitch;
+    for (int i = threadIdx.x * 16; i < end; i += kLong * 16) {
+      // a row's last piece ends with the row; its first may begin in the rows
+      // before, but not before the first row of all
+      if (i == 0 && shift > row * bytes) {
+        for (int e = shift; e < (end < 16 ? end : 16); e += sizeof(E)) {
+          const void* src = reinterpret_cast<const void*>(start - shift + e);
+          if constexpr (sizeof(E) == 4)
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + e), "r"(ld_32(src)) : "memory");
+          else
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + e), "h"(static_cast<uint16_t>(ld_16(src))) : "memory");
+        }
+      } else {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i), "l"(start - shift + i),
+                     "r"(end - i < 16 ? end - i : 16)
+                     : "memory");
+      }
+    }
+  }
+  __device__ __forceinline__ const E* at(const E* array, int64_t row, int a, int place) const {
+    const uint64_t start = reinterpret_cast<uint64_t>(array) + static_cast<uint64_t>(row) * bytes;
+    return reinterpret_cast<const E*>(smem + (place * ARRAYS + a) * pitch + (start & 15));
+  }
+};
+
+// Brings row `row` to its place; fetch starts a row's copies.
+template <typename F>
+__device__ __forceinline__ void bring(const NormParams& p, int64_t row, int64_t next, int place, F&& fetch) {
+  if (p.keep == 1) {
+    __syncthreads();  // the last row has been read
+    fetch(row, 0);
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();  // with two places this also says that the other one has been read
+  if (p.keep == 2 && next < p.rows) fetch(next, place ^ 1);
+}
+
+template <typename E, int VEC, bool KEPT>
+__global__ void __launch_bounds__(kLong, 2) norm_fwd_long_kernel(const NormParams p) {
   __shared__ float red[2][16][1];
-  int turn = 0;
+  extern __shared__ __align__(16) uint8_t smem[];
+  int turn = 0, place = 0;
   grid_dependency_wait();
   grid_dependents_launch();
-  const int F = p.features;
+  const int F = p.features, c0 = threadIdx.x * VEC;
+  constexpr int kStep = kLong * VEC;
   const float inv = 1.0f / static_cast<float>(F);
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const E* x = static_cast<const E*>(p.x) + row * F;
+  const Kept<E, 1> kept(p, smem);
+  const E* xs = static_cast<const E*>(p.x);
+  auto fetch = [&](int64_t row, int to) { kept.issue(xs, row, 0, to); };
+  if (KEPT && p.keep == 2 && blockIdx.x < p.rows) fetch(blockIdx.x, 0);
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, place ^= 1) {
+    if constexpr (KEPT) bring(p, row, row + gridDim.x, place, fetch);
+    const E* x = KEPT ? kept.at(xs, row, 0, p.keep == 2 ? place : 0) : xs + row * F;
     E* y = static_cast<E*>(p.y) + row * F;
-    float s[1] = {0.0f};
-#pragma unroll 8
-    for (int c = threadIdx.x; c < F; c += 512) s[0] += Elem<E>::to_f(ld(x + c));
-    row_sums<512>(s, red, turn);
+    float s[1] = {0.0f}, v[VEC];
+    Pack<E, VEC> pk;
+#pragma unroll 4
+    for (int c = c0; c < F; c += kStep) {
+      pk.load(x + c);
+      pk.get(v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[0] += v[e];
+    }
+    row_sums<kLong>(s, red, turn);
     const float mean = s[0] * inv;
     s[0] = 0.0f;
-#pragma unroll 8
-    for (int c = threadIdx.x; c < F; c += 512) {
-      const float d = Elem<E>::to_f(ld(x + c)) - mean;
-      s[0] = fma(d, d, s[0]);
+#pragma unroll 4
+    for (int c = c0; c < F; c += kStep) {
+      pk.load(x + c);
+      pk.get(v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[0] = fma(v[e] - mean, v[e] - mean, s[0]);
     }
-    row_sums<512>(s, red, turn);
+    row_sums<kLong>(s, red, turn);
     const float rstd = rsqrtf(s[0] * inv + p.eps);
     if (threadIdx.x == 0 && p.mean) {
       p.mean[row] = mean;
@@ -395,9 +473,17 @@ __global__ void __launch_bounds__(512) norm_fwd_long_kernel(const NormParams p) 
     }
     const int64_t offset = row / p.rows_per_weight * p.weight_stride;
 #pragma unroll 4
-    for (int c = threadIdx.x; c < F; c += 512)
-      y[c] = Elem<E>::from_f(fma((Elem<E>::to_f(ld(x + c)) - mean) * rstd, weight_at<E>(p, offset + c),
-                                 bias_at<E>(p, offset + c)));
+    for (int c = c0; c < F; c += kStep) {
+      float w[VEC], b[VEC];
+      vector_at<E, VEC>(p, p.weight, offset + c, 1.0f, p.add_one ? 1.0f : 0.0f, w);
+      vector_at<E, VEC>(p, p.bias, offset + c, 0.0f, 0.0f, b);
+      pk.load(x + c);
+      pk.get(v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = fma((v[e] - mean) * rstd, w[e], b[e]);
+      pk.set(v);
+      pk.store(y + c);
+    }
   }
 }
 
@@ -539,61 +625,111 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, ctas_of(T))
   }
 }
 
-// Rows too long for the registers: dx alone, in two passes over the row ...
-template <typename E>
-__global__ void __launch_bounds__(512) norm_dx_long_kernel(const NormParams p) {
+// Rows too long for the registers: dx alone, in two passes over the row in
+// shared memory or L2 ...
+template <typename E, int VEC, bool KEPT>
+__global__ void __launch_bounds__(kLong, 2) norm_dx_long_kernel(const NormParams p) {
   __shared__ float red[2][16][2];
-  int turn = 0;
+  extern __shared__ __align__(16) uint8_t smem[];
+  int turn = 0, place = 0;
   grid_dependency_wait();
   grid_dependents_launch();
-  const int F = p.features;
-  const float inv = 1.0f / static_cast<float>(F);
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const E* x = static_cast<const E*>(p.x) + row * F;
-    const E* dy = static_cast<const E*>(p.dy) + row * F;
+  const int F = p.features, c0 = threadIdx.x * VEC;
+  constexpr int kStep = kLong * VEC;
+  const float inv = 1.0f / static_cast<float>(F), plus = p.add_one ? 1.0f : 0.0f;
+  const Kept<E, 2> kept(p, smem);
+  const E* xs = static_cast<const E*>(p.x);
+  const E* dys = static_cast<const E*>(p.dy);
+  auto fetch = [&](int64_t row, int to) {
+    kept.issue(xs, row, 0, to);
+    kept.issue(dys, row, 1, to);
+  };
+  if (KEPT && p.keep == 2 && blockIdx.x < p.rows) fetch(blockIdx.x, 0);
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, place ^= 1) {
+    const float mean = ld_f32(p.mean + row), rstd = ld_f32(p.rstd + row);
+    if constexpr (KEPT) bring(p, row, row + gridDim.x, place, fetch);
+    const E* x = KEPT ? kept.at(xs, row, 0, p.keep == 2 ? place : 0) : xs + row * F;
+    const E* dy = KEPT ? kept.at(dys, row, 1, p.keep == 2 ? place : 0) : dys + row * F;
     E* dx = static_cast<E*>(p.y) + row * F;
     const int64_t offset = row / p.rows_per_weight * p.weight_stride;
-    const float mean = p.mean[row], rstd = p.rstd[row];
-    float s[2] = {0.0f, 0.0f};
+    float s[2] = {0.0f, 0.0f}, h[VEC], g[VEC], w[VEC];
+    Pack<E, VEC> px, pd;
 #pragma unroll 4
-    for (int c = threadIdx.x; c < F; c += 512) {
-      const float g = Elem<E>::to_f(ld(dy + c)) * weight_at<E>(p, offset + c);
-      s[0] += g;
-      s[1] = fma(g, (Elem<E>::to_f(ld(x + c)) - mean) * rstd, s[1]);
+    for (int c = c0; c < F; c += kStep) {
+      vector_at<E, VEC>(p, p.weight, offset + c, 1.0f, plus, w);
+      px.load(x + c);
+      pd.load(dy + c);
+      px.get(h);
+      pd.get(g);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        g[e] *= w[e];
+        s[0] += g[e];
+        s[1] = fma(g[e], (h[e] - mean) * rstd, s[1]);
+      }
     }
-    row_sums<512>(s, red, turn);
+    row_sums<kLong>(s, red, turn);
     const float mg = s[0] * inv, mgh = s[1] * inv;
 #pragma unroll 4
-    for (int c = threadIdx.x; c < F; c += 512) {
-      const float g = Elem<E>::to_f(ld(dy + c)) * weight_at<E>(p, offset + c);
-      const float h = (Elem<E>::to_f(ld(x + c)) - mean) * rstd;
-      dx[c] = Elem<E>::from_f(rstd * (g - mg - h * mgh));
+    for (int c = c0; c < F; c += kStep) {
+      vector_at<E, VEC>(p, p.weight, offset + c, 1.0f, plus, w);
+      px.load(x + c);
+      pd.load(dy + c);
+      px.get(h);
+      pd.get(g);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) g[e] = rstd * (g[e] * w[e] - mg - (h[e] - mean) * rstd * mgh);
+      pd.set(g);
+      pd.store(dx + c);
     }
   }
 }
 
-// ... and the sums of a chunk of rows, one thread for a column.
-template <typename E>
+// ... and the sums of a chunk of rows, one thread for VEC columns.
+template <typename E, int VEC>
 __global__ void __launch_bounds__(256) norm_partial_long_kernel(const NormParams p) {
   const int F = p.features;
-  const int c = blockIdx.x * 256 + threadIdx.x;
+  const int c = (blockIdx.x * 256 + threadIdx.x) * VEC;
   grid_dependency_wait();
   grid_dependents_launch();
   if (c >= F) return;
   const int64_t part = blockIdx.y, seg = part / p.chunks, chunk = part % p.chunks;
   const int64_t r0 = seg * p.rows_per_weight + p.rows_per_weight * chunk / p.chunks;
   const int64_t r1 = seg * p.rows_per_weight + p.rows_per_weight * (chunk + 1) / p.chunks;
-  const E* x = static_cast<const E*>(p.x);
-  const E* dy = static_cast<const E*>(p.dy);
-  float dw = 0.0f, db = 0.0f;
-#pragma unroll 4
-  for (int64_t row = r0; row < r1; ++row) {
-    const float d = Elem<E>::to_f(ld(dy + row * F + c));
-    dw = fma(d, (Elem<E>::to_f(ld(x + row * F + c)) - ld_f32(p.mean + row)) * ld_f32(p.rstd + row), dw);
-    db += d;
+  const E* x = static_cast<const E*>(p.x) + c;
+  const E* dy = static_cast<const E*>(p.dy) + c;
+  float dw[VEC] = {}, db[VEC] = {};
+  constexpr int kRows = VEC > 2 ? 2 : 4;  // rows loaded at a time
+  for (int64_t row = r0; row < r1; row += kRows) {
+    Pack<E, VEC> px[kRows], pd[kRows];
+    float mean[kRows], rstd[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (row + i < r1) {
+        px[i].load_ahead(x + (row + i) * F);
+        pd[i].load_ahead(dy + (row + i) * F);
+        mean[i] = ld_f32(p.mean + row + i);
+        rstd[i] = ld_f32(p.rstd + row + i);
+      }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (row + i < r1) {
+        float h[VEC], d[VEC];
+        px[i].get(h);
+        pd[i].get(d);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          dw[e] = fma(d[e], (h[e] - mean[i]) * rstd[i], dw[e]);
+          db[e] += d[e];
+        }
+      }
   }
-  p.partial[(part * 2) * F + c] = dw;
-  p.partial[(part * 2 + 1) * F + c] = db;
+  // F is a multiple of VEC, but the sums' rows may start at any float
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    p.partial[(part * 2) * F + c + e] = dw[e];
+    p.partial[(part * 2 + 1) * F + c + e] = db[e];
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -626,6 +762,17 @@ int resident(int threads, int smem) {
     return n < 1 ? 1 : n;
   }();
   return ctas;
+}
+
+// A CTA for each long row, as many as the GPU holds at once.
+template <auto Kernel>
+int longest_rows(const NormParams& p, int64_t smem, cudaStream_t s) {
+  int n = 0;
+  if (smem > 40 * 1024)
+    CONVROT_CUDA_CHECK(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  CONVROT_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, kLong, static_cast<size_t>(smem)));
+  const int64_t most = static_cast<int64_t>(n < 1 ? 1 : n) * device_sm_count();
+  return enqueue(Kernel, dim3(static_cast<unsigned>(p.rows < most ? p.rows : most)), kLong, static_cast<size_t>(smem), p, s);
 }
 
 // Whether every vector of `vec` elements of the rows and of the weights is
@@ -668,8 +815,10 @@ int forward_rows(NormParams p, int vectors, cudaStream_t s) {
     return dim3(static_cast<unsigned>(segments * p.chunks));
   };
   auto longest = [&] {
-    const int64_t most = 4LL * device_sm_count();
-    return enqueue(norm_fwd_long_kernel<E>, dim3(static_cast<unsigned>(p.rows < most ? p.rows : most)), 512, 0, p, s);
+    p.keep = Kept<E, 1>::fitting(p.features);
+    const int64_t bytes = p.keep * Kept<E, 1>::pitch_of(p.features);
+    return p.keep ? longest_rows<norm_fwd_long_kernel<E, VEC, true>>(p, bytes, s)
+                  : longest_rows<norm_fwd_long_kernel<E, VEC, false>>(p, 0, s);
   };
 #define CONVROT_RUN(NV, T)                                                                                       \
   enqueue(norm_fwd_kernel<E, VEC, NV, T>,                                                                        \
@@ -680,13 +829,15 @@ int forward_rows(NormParams p, int vectors, cudaStream_t s) {
 }
 
 template <typename E, int VEC, int U>
-int backward_rows(const NormParams& p, int vectors, cudaStream_t s) {
+int backward_rows(NormParams p, int vectors, cudaStream_t s) {
   const unsigned ctas = static_cast<unsigned>(p.rows / p.rows_per_weight * p.chunks);
   auto longest = [&] {
-    const int64_t most = 4LL * device_sm_count();
-    int rc = enqueue(norm_dx_long_kernel<E>, dim3(static_cast<unsigned>(p.rows < most ? p.rows : most)), 512, 0, p, s);
+    p.keep = Kept<E, 2>::fitting(p.features);
+    const int64_t bytes = 2 * p.keep * Kept<E, 2>::pitch_of(p.features);
+    int rc = p.keep ? longest_rows<norm_dx_long_kernel<E, VEC, true>>(p, bytes, s)
+                    : longest_rows<norm_dx_long_kernel<E, VEC, false>>(p, 0, s);
     if (rc == CONVROT_OK && p.partial)
-      rc = enqueue(norm_partial_long_kernel<E>, dim3((p.features + 255) / 256, ctas), 256, 0, p, s);
+      rc = enqueue(norm_partial_long_kernel<E, VEC>, dim3((p.features + 256 * VEC - 1) / (256 * VEC), ctas), 256, 0, p, s);
     return rc;
   };
 #define CONVROT_RUN(NV, T)                                                 \

@@ -110,6 +110,28 @@ def test_ends_of_the_row_shapes(dtype, features):
     test_affine(dtype, 37, features, False)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offset", [1, 2, 5])
+@pytest.mark.parametrize("rows,features", [(5, 64), (300, 1030), (3, 9001), (700, 9002), (2, 20001), (3, 30008), (2, 52000), (2, 110001)])
+def test_tensors_that_start_anywhere(dtype, offset, rows, features):
+    def at(t):
+        return torch.cat([t.new_zeros(offset), t.flatten()])[offset:].view(t.shape)
+
+    x = at(_inputs(rows, features, dtype, 61)).requires_grad_()
+    w, b = at((1 + randn((features,), dtype, 62, 0.3)).to(dtype)).requires_grad_(), at(randn((features,), dtype, 63)).requires_grad_()
+    dy = at(randn((rows, features), dtype, 64))
+    y = cr.layer_norm(x, w, b, EPS)
+    x0, w0, b0 = x.detach(), w.detach(), b.detach()
+    y64, slack, *_ = _norm64(x0, w0, b0)
+    assert_within(y.detach(), y64, slack, "y")
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    assert_within(dx, *_dx64(x0, w0, b0, dy), "dx")
+    dw64, sw, db64, sb = _sums64(x0, w0, b0, dy, (0,))
+    assert_within(dw, dw64, sw, "dw")
+    assert_within(db, db64, sb, "db")
+    assert_no_device_error()
+
+
 MOD_SHAPES = [(1, 1, 64), (3, 5, 257), (2, 700, 512), (8, 40, 3072), (5, 1, 33), (2, 3, 20000), (70, 9, 128), (300, 2, 40)]
 
 
