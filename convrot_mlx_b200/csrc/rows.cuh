@@ -18,12 +18,6 @@ constexpr uint32_t kInfBits = 0x7F800000u;
 
 __device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xFFFFFFFFu, v); }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  return v;
-}
-
 // Two float32 values rounded to a pair of a 16-bit type, in one conversion.
 template <typename T>
 __device__ __forceinline__ typename Elem<T>::Pair pair_of(float a, float b);
