@@ -400,13 +400,42 @@ struct alignas(8) Bars {
 template <int BT> constexpr int kStages = BT <= 32 ? 5 : (BT == 64 ? 4 : 3);
 template <int BT> constexpr int kXBytes = BT * kBK;
 template <int BT>
-constexpr size_t kSmem = 1024 + kStages<BT> * (kWBytes + kXBytes<BT>) + (BT + 4) * 4 + sizeof(Bars);
+constexpr size_t kSmem = 1024 + kStages<BT> * (kWBytes + kXBytes<BT>) + BT * 4 + sizeof(Bars);
 static_assert(kSmem<128> <= 113 * 1024 && kSmem<64> <= 113 * 1024 && kSmem<32> <= 113 * 1024, "shared memory budget");
 
-__device__ __forceinline__ uint32_t dsmem_ld(uint32_t cluster_addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+__device__ __forceinline__ uint4 dsmem_ld128(uint32_t cluster_addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(cluster_addr)
+               : "memory");
   return v;
+}
+
+// The sums of R ranks (token, 128 channels) for tokens c_lo to c_hi, every
+// fourth of them a warp's, a lane with four channels; tokens past the last are
+// read, in bounds, and not handed on.  16 reads of a thread are in flight: the
+// latency between SMs is what this takes.
+template <int R, int BT, typename Emit>
+__device__ __forceinline__ void join(const uint32_t* part, int c_lo, int c_hi, Emit&& emit) {
+  constexpr int kTokens = 16 / R;
+  uint32_t peer[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) peer[r] = mapa_shared(part + (threadIdx.x & 31) * 4, r);
+  for (int c = c_lo + (threadIdx.x >> 5); c < c_hi; c += 4 * kTokens) {
+    uint4 v[kTokens][R];
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t)
+#pragma unroll
+      for (int r = 0; r < R; ++r) v[t][r] = dsmem_ld128(peer[r] + min(c + 4 * t, BT - 1) * 512);
+#pragma unroll
+    for (int t = 0; t < kTokens; ++t) {
+      uint4 sum = v[t][0];
+#pragma unroll
+      for (int r = 1; r < R; ++r) sum.x += v[t][r].x, sum.y += v[t][r].y, sum.z += v[t][r].z, sum.w += v[t][r].w;
+      if (c + 4 * t < c_hi) emit(sum, c + 4 * t);
+    }
+  }
 }
 
 template <int LAYOUT, typename TOut, int BT>
@@ -418,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint8_t* sW = smem;
   uint8_t* sX = sW + S * kWBytes;
   float* xs = reinterpret_cast<float*>(sX + S * kXBytes<BT>);  // the tokens' scales
-  Bars* bars = reinterpret_cast<Bars*>(xs + BT + 4);
+  Bars* bars = reinterpret_cast<Bars*>(xs + BT);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int ranks = gridDim.x, rank = blockIdx.x;  // the cluster spans the grid's x
@@ -492,46 +521,50 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   __syncwarp();
   if (warp == 3) {  // has waited for the previous kernel
-    for (int c = lane; c < BT + 4; c += 32) xs[c] = m0 + c < p.m ? ld_f32(p.xscales + m0 + c) : 0.0f;
+    for (int c = lane; c < BT; c += 32) xs[c] = m0 + c < p.m ? ld_f32(p.xscales + m0 + c) : 0.0f;
   }
   __syncthreads();
   const bool done = wait(&bars->mma_done, 0, &bars->err, 74);
   tc_fence_after();
 
-  const int n = n0 + warp * 32 + lane;
-  const bool n_ok = n < p.n;
-  const float ws = n_ok && p.wscales ? ld_f32(p.wscales + n) : 1.0f;
-  const float b = n_ok && p.bias ? ld_f32(p.bias + n) : 0.0f;
   TOut* out = static_cast<TOut*>(p.out);
   const uint32_t t_row = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
   const int rows = p.m - m0 < BT ? p.m - m0 : BT;
-  // N tokens from c on, of which the first `count` exist: all values first,
-  // then all stores, since one warp a scheduler has only itself to overlap
-  auto emit = [&](auto& dots, int c, int count) {
-    constexpr int N = sizeof(dots) / sizeof(dots[0]);
-    float v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      v[i] = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(static_cast<int32_t>(dots[i])), xs[c + i]), ws), b);
-    TOut* dst = out + static_cast<int64_t>(m0 + c) * p.n + n;
-    if (count >= N && n_ok) {
-#pragma unroll
-      for (int i = 0; i < N; ++i, dst += p.n) *dst = cvt_out<TOut>(v[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i, dst += p.n)
-        if (i < count && n_ok) *dst = cvt_out<TOut>(v[i]);
-    }
-  };
   if (ranks == 1) {
+    const int n = n0 + warp * 32 + lane;
+    const bool n_ok = n < p.n;
+    const float ws = n_ok && p.wscales ? ld_f32(p.wscales + n) : 1.0f;
+    const float b = n_ok && p.bias ? ld_f32(p.bias + n) : 0.0f;
     for (int c = 0; c < rows && done; c += 16) {
       uint32_t r[16];
       __syncwarp();
       tmem_ld_32x32b_x16(t_row + c, r);
       tmem_ld_wait();
-      emit(r, c, rows - c);
+      // all values first, then all stores, since one warp a scheduler has only
+      // itself to overlap
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        v[i] = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(static_cast<int32_t>(r[i])), xs[c + i]), ws), b);
+      TOut* dst = out + static_cast<int64_t>(m0 + c) * p.n + n;
+      if (rows - c >= 16 && n_ok) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i, dst += p.n) *dst = cvt_out<TOut>(v[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i, dst += p.n)
+          if (i < rows - c && n_ok) *dst = cvt_out<TOut>(v[i]);
+      }
     }
   } else {
+    const int n = n0 + 4 * lane;  // of four channels
+    float ws[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ws[i] = n + i < p.n && p.wscales ? ld_f32(p.wscales + n + i) : 1.0f;
+      b[i] = n + i < p.n && p.bias ? ld_f32(p.bias + n + i) : 0.0f;
+    }
+    const bool whole = p.n % 4 == 0;  // four channels in one store
     // int32 sums (token, channel) over the ring, whose copies have all been consumed
     uint32_t* part = reinterpret_cast<uint32_t*>(smem);
     for (int c = 0; c < rows && done; c += 16) {
@@ -544,22 +577,27 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     __syncwarp();
     cluster_sync();
-    uint32_t peer[kMaxCluster];
+    const int c_lo = rows * rank / ranks, c_hi = done ? rows * (rank + 1) / ranks : 0;  // this CTA's share of the tokens
+    auto emit = [&](const uint4& dots, int c) {
+      const uint32_t dot[4] = {dots.x, dots.y, dots.z, dots.w};
+      float v[4];
 #pragma unroll
-    for (int r = 0; r < kMaxCluster; ++r) peer[r] = r < ranks ? mapa_shared(part + warp * 32 + lane, r) : 0u;
-    // this CTA's share of the tokens, four at a time so that their reads
-    // overlap (tokens past its share are read, in bounds, and not written)
-    const int c_lo = rows * rank / ranks, c_hi = done ? rows * (rank + 1) / ranks : 0;
-    for (int c = c_lo; c < c_hi; c += 4) {
-      uint32_t sum[4] = {};
+      for (int i = 0; i < 4; ++i)
+        v[i] = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(static_cast<int32_t>(dot[i])), xs[c]), ws[i]), b[i]);
+      TOut* dst = out + static_cast<int64_t>(m0 + c) * p.n + n;
+      if (whole) {
+        Pack<TOut, 4> pk;
+        pk.set(v);
+        if (n < p.n) pk.store(dst);
+      } else {
 #pragma unroll
-      for (int r = 0; r < kMaxCluster; ++r)
-        if (r < ranks) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum[i] += dsmem_ld(peer[r] + min(c + i, BT - 1) * 512);
-        }
-      emit(sum, c, c_hi - c);
-    }
+        for (int i = 0; i < 4; ++i)
+          if (n + i < p.n) dst[i] = cvt_out<TOut>(v[i]);
+      }
+    };
+    if (ranks == 2) join<2, BT>(part, c_lo, c_hi, emit);
+    else if (ranks == 4) join<4, BT>(part, c_lo, c_hi, emit);
+    else join<8, BT>(part, c_lo, c_hi, emit);
     __syncwarp();
     cluster_sync();  // no CTA leaves while another may still read its sums
   }
@@ -894,33 +932,38 @@ int launch_fused(const void* x, int64_t x_stride, const Operands& o, Params p, c
 
 // Expected times of the two tile kernels in microseconds, fitted to sweeps of
 // 16 to 1024 tokens, 512 to 12288 channels and K from 128 to 12288 (times of a
-// call in a graph, within 15% of the fit).  A stage of 128 K takes a pair 0.36
-// us while its data comes from L2 alone, 0.45 with every pair at work.  A swap
-// CTA takes 0.46 us for a stage (the latency of its ring), more where two CTAs
-// of an SM share 94 bytes a nanosecond; its epilogue takes 12 ns a token, and
-// the exchange of a split K 1 us and 16 ns a token.  Measured on either side:
-// 64 x 4096 x 4096 (tokens, K, channels) swap 9.6, pair 16.7; 512 x 4096 x
-// 4096 swap 16.8, pair 17.4; 1024 x 1024 x 1024 swap 10.2, pair 8.8;
-// 512 x 4096 x 12288 swap 41, pair 30.
+// call in a graph).  A stage of 128 K takes a pair 0.36 us in one wave, 0.45
+// over several.  A swap CTA takes 0.46 us for a stage (the latency of its
+// ring), more where two CTAs of an SM share 125 bytes a nanosecond; its
+// epilogue takes 12 ns a token and the exchange of a split K the more, the more
+// tokens and CTAs take part; a second wave of CTAs costs all of that again.
+// Over 72 sizes of 12 to 1000 tokens the choices take 1% longer than the best
+// of all splits and both kernels.  Measured on either side (tokens, K,
+// channels; weights from HBM): 64 x 4096 x 4096 swap 10.2, pair 17.3; 512 x 4096
+// x 4096 swap 16.5, pair 18.0; 200 x 4096 x 12288 swap 22.8, pair 19.6; 1000 x
+// 3072 x 3072 swap 17.8, pair 15.8.
 double pair_time(const Params& p, int sms) {
   const int64_t tiles = static_cast<int64_t>((p.m + 255) / 256) * ((p.n + 255) / 256), pairs = sms / 2;
   const int64_t waves = (tiles + pairs - 1) / pairs, stages = (p.k + kBK - 1) / kBK;
-  return 5.0 + static_cast<double>(waves * stages) * (waves > 1 ? 0.45 : 0.36);
+  return 6.0 + static_cast<double>(waves * stages) * (waves > 1 ? 0.45 : 0.36);
 }
 
-// The best split of K over 1, 2, 4 or 8 CTAs (others pack badly into the GPU's
-// clusters of SMs: 64 x 4096 x 12288 takes 14.0 in two, 26 in three), and its
-// time.
+// The best split of K over 1, 2, 4 or 8 CTAs, and its time: 64 x 4096 x 12288
+// takes 15.9 in two and 28 in eight, whose CTAs are three waves; 64 x 12288 x
+// 3072 28 and 14.3.  (Splits in three pack badly into the GPU's clusters of SMs;
+// clusters of four or eight do not fill it either: 72 of four are two waves.)
 double swap_time(const Params& p, int bt, int sms, int* ranks) {
   const int64_t tiles = static_cast<int64_t>((p.n + 127) / 128) * ((p.m + bt - 1) / bt);
   const int64_t stages = (p.k + kBK - 1) / kBK;
   double best = 1e30;
   for (int r = 1; r <= swap::kMaxCluster && r <= stages; r *= 2) {
-    const int64_t ctas = tiles * r, waves = (ctas + 2 * sms - 1) / (2 * sms);
+    const int64_t ctas = tiles * r, at_once = r < 4 ? 2 * sms : 2 * sms / 8 * 7;
+    const int64_t waves = (ctas + at_once - 1) / at_once;
     const bool shared = ctas > sms;
-    const double stage = shared ? std::max(0.46, 2.0 * (swap::kWBytes + bt * kBK) / 94e3) : 0.46;
-    const double t = 2.8 + 0.012 * bt + static_cast<double>(waves * ((stages + r - 1) / r)) * stage +
-                     (r > 1 ? 1.0 + 0.016 * bt : 0.0) + (shared ? 1.0 : 0.0);
+    const double stage = shared ? std::max(0.46, 2.0 * (swap::kWBytes + bt * kBK) / 125e3) : 0.46;
+    const double exchange = r > 1 ? 0.9 + 0.08 * r + bt * (0.006 + 0.001 * r) : 0.0;
+    const double t = static_cast<double>(waves) * (2.8 + 0.012 * bt + static_cast<double>((stages + r - 1) / r) * stage +
+                                                   exchange + (shared ? 0.4 + 0.007 * bt : 0.0));
     if (t < best) {
       best = t;
       *ranks = r;
