@@ -275,7 +275,7 @@ std::pair<Tensor, std::optional<Tensor>> axial_rotary(const Tensor& q, const std
 // --- layer norm ---------------------------------------------------------------
 
 // weight and bias: vectors that follow one another at the same stride, one for
-// each segment of the rows (either may be undefined).
+// each segment of the rows (either may be undefined; run_norm sees to it).
 struct NormHow {
   int64_t segments;
   bool add_one;
@@ -364,6 +364,15 @@ Tensor run_norm(Tensor x, Tensor weight, Tensor bias, const NormHow& how) {
       break;
     }
   }
+  // After the conversion, which packs the one vector that it touches: unit
+  // stride, and segments at one stride that covers the features.
+  auto inner = [](const Tensor& t) { return !t.defined() || t.stride(-1) == 1; };
+  const bool split = how.segments > 1 && weight.defined() && bias.defined() &&
+                     (weight.stride(0) != bias.stride(0) || weight.stride(0) < x.size(-1));
+  if (!inner(weight) || !inner(bias) || split) {
+    weight = weight.defined() ? weight.contiguous() : weight;
+    bias = bias.defined() ? bias.contiguous() : bias;
+  }
   if (!x.is_contiguous()) x = x.contiguous();
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(bias)))
     return LayerNorm::apply(x, weight.defined() ? std::optional<Tensor>(weight) : std::nullopt,
@@ -380,7 +389,6 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
     if (!v[i].defined()) continue;
     if (v[i].dim() != 1 || v[i].size(0) != features)
       refuse("layer norm ", i ? "bias" : "weight", " must have shape (", features, ",), got ", shape_of(v[i]));
-    if (v[i].stride(0) != 1) v[i] = v[i].contiguous();
   }
   return run_norm(x, v[0], v[1], {1, false, eps});
 }
@@ -398,11 +406,6 @@ Tensor modulated_layer_norm(const Tensor& x, Tensor shift, Tensor scale, double 
   if (shift.size(0) != scale.size(0)) {  // the shared one is repeated, its gradient summed over the samples
     shift = shift.reshape({-1, features}).expand({batch, features});
     scale = scale.reshape({-1, features}).expand({batch, features});
-  }
-  if (shift.stride(-1) != 1 || scale.stride(-1) != 1 ||
-      (scale.size(0) > 1 && (shift.stride(0) != scale.stride(0) || scale.stride(0) < features))) {
-    shift = shift.contiguous();
-    scale = scale.contiguous();
   }
   return run_norm(x, scale, shift, {std::max<int64_t>(1, scale.size(0)), true, eps});
 }
