@@ -5,6 +5,15 @@
 //   g  = dy w
 //   dx = r (g - E[g] - h E[g h])
 //   dweight = sum dy h,  dbias = sum dy  (over the rows that share a weight)
+// A row far from zero would lose its values to the rounding of the mean: that of
+// 1664 times 30000, by sum * (1 / F) in float32, is off by 0.002, which eps =
+// 1e-6 makes 0.9 of h.  So where the mean is beyond twice the deviation the
+// centred values d are summed once more, and h = (d - E[d]) r with variance
+// E[d^2] - E[d]^2 (E[d] is a rounding error, so nothing cancels).  Other rows'
+// h is off by at most 2 + max|h| of a row sum's relative error, and they pay
+// one comparison: d summed for every row took 10 to 14% longer where one CTA
+// fills an SM (2048 x 16384 bf16 28.7 us instead of 26.2).  The backward pass
+// subtracts the mean before it multiplies, as the forward pass does.
 // Memory-bound: forward reads and writes a row once; backward reads x and dy
 // and writes dx, once each.  A thread keeps the same columns for all rows of
 // its CTA: a row stays in registers between its statistics and its output,
@@ -18,10 +27,10 @@
 // flight while a row is worked on.
 // us (fraction of a copy's bandwidth), bf16, backward with all three gradients:
 //   rows x features   65536 x 512  12288 x 1024  12288 x 3072  8192 x 4096  4096 x 8192  2048 x 16384
-//   forward           22 (0.93)    9.4 (0.82)    26 (0.89)     27 (0.77)    30 (0.68)    26 (0.79)
-//   backward          39 (0.79)    17 (0.67)     44 (0.79)     39 (0.78)    50 (0.62)    75 (0.41)
+//   forward           22 (0.93)    9.4 (0.82)    25 (0.89)     27 (0.77)    30 (0.68)    27 (0.75)
+//   backward          39 (0.79)    17 (0.67)     44 (0.79)     40 (0.77)    51 (0.60)    75 (0.41)
 // Rows of odd length, whose elements are moved one by one: 5003 x 1153 float32
-// 10.8 and 18.5 us (1152: 7.5 and 14.8).  16-byte pieces copied to shared
+// 12.0 and 18.6 us (1152: 8.1 and 14.9).  16-byte pieces copied to shared
 // memory across the rows' ends and read back by element took longer, for the
 // barrier that each row then needs: 12.9 and 18.6.
 #pragma once
@@ -104,6 +113,11 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*red)[16][N], int
     turn ^= 1;
   }
 }
+
+// Whether a row's first mean has to be corrected, from its variance about it
+// (false for NaN); and the variance less the square of the correction.
+__device__ __forceinline__ bool far_from_zero(float mean, float var, float eps) { return mean * mean > 4.0f * (var + eps); }
+__device__ __forceinline__ float corrected(float var, float off) { return fmaxf(fma(-off, off, var), 0.0f); }
 
 // One thread's share of a row: NV vectors of VEC elements, T vectors apart,
 // from column c0 = VEC * (thread of the row) on.  Columns past the end are
@@ -273,9 +287,19 @@ __device__ __forceinline__ void vector_at(const NormParams& p, const void* base,
 // ---------------------------------------------------------------------------
 // forward
 
+// Least CTAs of an SM that the registers are shared out to; 0: the compiler's
+// choice.  With 1 it spends more registers on loads ahead: 4096 x 6142 bf16 37 us
+// instead of 47, but 4096 x 3072 float32 23.6 instead of 18.7.  Two vectors of
+// eight values for each lane of a warp would lose the sixth CTA by it (65536 x
+// 512 bf16 22.7 us instead of 21.6).
+constexpr int fwd_ctas(int size, int vec, int nv, int threads) {
+  return size == 4 ? 0 : vec == 8 && nv == 2 && threads == 32 ? 6 : 1;
+}
+
 // T threads share a row: 32 (each warp of the CTA rows of its own), or the CTA.
 template <typename E, int VEC, int NV, int T>
-__global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T) norm_fwd_kernel(const NormParams p) {
+__global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, fwd_ctas(sizeof(E), VEC, NV, T))
+    norm_fwd_kernel(const NormParams p) {
   constexpr int L = kLanes<VEC>;
   using A = Lane<VEC>;
   __shared__ float red[2][16][1];
@@ -341,17 +365,31 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T) norm_fwd_kernel(con
       }
     s[0] = total(sum);
     row_sums<T>(s, red, turn);
-    const float rstd = rsqrtf(s[0] * inv + p.eps);
-    const A scale = splat<VEC>(rstd);
+    float var = s[0] * inv, off = 0.0f;
+    if (far_from_zero(mean, var, p.eps)) {  // the same for all threads of the row
+      sum = splat<VEC>(0.0f);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (j * T * VEC < left) {
+#pragma unroll
+          for (int i = 0; i < L; ++i) sum = add(sum, v[j][i]);
+        }
+      s[0] = total(sum);
+      row_sums<T>(s, red, turn);
+      off = s[0] * inv;
+      var = corrected(var, off);
+    }
+    const float rstd = rsqrtf(var + p.eps);
+    const A scale = splat<VEC>(rstd), rest = splat<VEC>(-off * rstd);
     if (c0 == 0 && p.mean) {
-      p.mean[row] = mean;
+      p.mean[row] = mean + off;
       p.rstd[row] = rstd;
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (j * T * VEC < left) {
 #pragma unroll
-        for (int i = 0; i < L; ++i) v[j][i] = fma(mul(v[j][i], scale), weight[j][i], bias[j][i]);
+        for (int i = 0; i < L; ++i) v[j][i] = fma(fma(v[j][i], scale, rest), weight[j][i], bias[j][i]);
         Pack<E, VEC> out;
         out.set_lanes(v[j]);
         out.store(dst + j * T * VEC);
@@ -466,9 +504,23 @@ __global__ void __launch_bounds__(kLong, 2) norm_fwd_long_kernel(const NormParam
       for (int e = 0; e < VEC; ++e) s[0] = fma(v[e] - mean, v[e] - mean, s[0]);
     }
     row_sums<kLong>(s, red, turn);
-    const float rstd = rsqrtf(s[0] * inv + p.eps);
+    float var = s[0] * inv, off = 0.0f;
+    if (far_from_zero(mean, var, p.eps)) {  // the same for all threads
+      s[0] = 0.0f;
+#pragma unroll 4
+      for (int c = c0; c < F; c += kStep) {
+        pk.load(x + c);
+        pk.get(v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[0] += v[e] - mean;
+      }
+      row_sums<kLong>(s, red, turn);
+      off = s[0] * inv;
+      var = corrected(var, off);
+    }
+    const float rstd = rsqrtf(var + p.eps), rest = -off * rstd;
     if (threadIdx.x == 0 && p.mean) {
-      p.mean[row] = mean;
+      p.mean[row] = mean + off;
       p.rstd[row] = rstd;
     }
     const int64_t offset = row / p.rows_per_weight * p.weight_stride;
@@ -480,7 +532,7 @@ __global__ void __launch_bounds__(kLong, 2) norm_fwd_long_kernel(const NormParam
       pk.load(x + c);
       pk.get(v);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = fma((v[e] - mean) * rstd, w[e], b[e]);
+      for (int e = 0; e < VEC; ++e) v[e] = fma(fma(v[e] - mean, rstd, rest), w[e], b[e]);
       pk.set(v);
       pk.store(y + c);
     }
@@ -490,16 +542,16 @@ __global__ void __launch_bounds__(kLong, 2) norm_fwd_long_kernel(const NormParam
 // ---------------------------------------------------------------------------
 // backward
 
-// With h = x r - mean r and per row u = -r E[g h], v = -r E[g]:
-//   dx = (dy r) w + (h u + v).
-// With up to 24 values of a row a thread keeps h in float32; with more it
-// keeps the row as it lies in memory and forms h twice.
+// With c = x - mean, t = dy c and per row u = -r^2 E[g h], v = -r E[g]:
+//   dw += t r,  E[g h] = r E[t w],  dx = (dy r) w + (c u + v).
+// With up to 24 values of a row a thread keeps c in float32; with more it
+// keeps the row as it lies in memory and forms c twice.
 template <typename E, int VEC, int NV, int T>
 __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, ctas_of(T))
     norm_bwd_kernel(const NormParams p) {
   constexpr int L = kLanes<VEC>;
   using A = Lane<VEC>;
-  // h kept in float32 beside the row, and rows ahead: in shared memory, or in
+  // c kept in float32 beside the row, and rows ahead: in shared memory, or in
   // registers for elements that are too small to be copied
   constexpr bool kKeep = VEC * NV <= 24;
   using Next = Ahead<E, VEC, NV, T, 2>;
@@ -560,20 +612,20 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, ctas_of(T))
       dy = next_dy;
     }
     if (Next::kAsync || kRegs) fetch(row + stride, at + step);
-    const A scale = splat<VEC>(rstd), minus = splat<VEC>(-mean * rstd);
-    A h[kKeep ? NV : 1][L], s0 = splat<VEC>(0.0f), s1 = s0;
+    const A scale = splat<VEC>(rstd), minus = splat<VEC>(-mean);
+    A centred[kKeep ? NV : 1][L], s0 = splat<VEC>(0.0f), s1 = s0;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (j * T * VEC < left) {
         A d[L];
-        A(&hj)[L] = h[kKeep ? j : 0];
-        x.v[j].get_lanes(hj);
+        A(&c)[L] = centred[kKeep ? j : 0];
+        x.v[j].get_lanes(c);
         dy.v[j].get_lanes(d);
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-          hj[i] = fma(hj[i], scale, minus);
-          const A t = mul(d[i], hj[i]);
-          dw[j][i] = add(dw[j][i], t);
+          c[i] = add(c[i], minus);
+          const A t = mul(d[i], c[i]);
+          dw[j][i] = fma(t, scale, dw[j][i]);
           db[j][i] = add(db[j][i], d[i]);
           s0 = fma(d[i], weight[j][i], s0);
           s1 = fma(t, weight[j][i], s1);
@@ -581,21 +633,22 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, ctas_of(T))
       }
     float s[2] = {total(s0), total(s1)};
     row_sums<T>(s, red, turn);
-    const A v = splat<VEC>(-s[0] * inv * rstd), u = splat<VEC>(-s[1] * inv * rstd);
+    const float gh = s[1] * inv * rstd;  // E[g h]
+    const A v = splat<VEC>(-s[0] * inv * rstd), u = splat<VEC>(-gh * rstd * rstd);
     E* dx = static_cast<E*>(p.y) + at;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (j * T * VEC < left) {
         A d[L];
-        A(&hj)[L] = h[kKeep ? j : 0];
+        A(&c)[L] = centred[kKeep ? j : 0];
         dy.v[j].get_lanes(d);
         if constexpr (!kKeep) {
-          x.v[j].get_lanes(hj);
+          x.v[j].get_lanes(c);
 #pragma unroll
-          for (int i = 0; i < L; ++i) hj[i] = fma(hj[i], scale, minus);
+          for (int i = 0; i < L; ++i) c[i] = add(c[i], minus);
         }
 #pragma unroll
-        for (int i = 0; i < L; ++i) d[i] = fma(mul(d[i], scale), weight[j][i], fma(hj[i], u, v));
+        for (int i = 0; i < L; ++i) d[i] = fma(mul(d[i], scale), weight[j][i], fma(c[i], u, v));
         Pack<E, VEC> out;
         out.set_lanes(d);
         out.store(dx + j * T * VEC);
