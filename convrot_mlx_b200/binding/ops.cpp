@@ -8,6 +8,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <string>
 #include <vector>
@@ -21,6 +22,7 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 constexpr int64_t kPitch = 16;        // rows of codes start on multiples of 16 bytes
+constexpr int64_t kMaxDot = 131072;   // products that one int32 dot can sum
 constexpr int64_t kSavedGroup = 128;  // features of a row that share one scale of a saved GELU input
 
 // --- errors -------------------------------------------------------------
@@ -134,6 +136,33 @@ Tensor i8_product(const Tensor& x, const Tensor& col_scale, const Tensor& qweigh
   return out;
 }
 
+// The gradient of the input over more channels k than one int32 dot can sum:
+// the codes are formed once for the whole token, each range of kMaxDot channels
+// is an exact dot, and the ranges' products are added in float32, in order.
+Tensor i8_gradient_in_ranges(const Tensor& dy, const Tensor& wscales, const Tensor& qweight) {
+  const c10::cuda::OptionalCUDAGuard guard(dy.device());
+  const Tensor r = rows_of(dy);
+  const int64_t m = r.size(0), k = r.size(1), n = qweight.size(1), pitch = (k + kPitch - 1) / kPitch * kPitch;
+  std::vector<int64_t> shape(dy.sizes().begin(), dy.sizes().end());
+  shape.back() = n;
+  const Tensor codes = at::empty({m, pitch}, qweight.options()), scales = at::empty({m}, wscales.options());
+  check(convrot_quantize_i8(r.data_ptr(), dtype_code(r.scalar_type()), m, k, r.stride(0),
+                            static_cast<const float*>(wscales.data_ptr()), static_cast<int8_t*>(codes.data_ptr()), pitch,
+                            static_cast<float*>(scales.data_ptr()), stream_of(dy)),
+        "convrot_quantize_i8");
+  Tensor sum;
+  for (int64_t at = 0; at < k; at += kMaxDot) {
+    const Tensor part = at::empty(shape, scales.options());
+    check(convrot_i8_gemm(static_cast<const int8_t*>(codes.data_ptr()) + at, pitch,
+                          static_cast<const int8_t*>(qweight.data_ptr()) + at * qweight.stride(0), qweight.stride(0),
+                          CONVROT_LAYOUT_KN, static_cast<const float*>(scales.data_ptr()), nullptr, nullptr,
+                          part.data_ptr(), CONVROT_F32, m, n, std::min(kMaxDot, k - at), stream_of(dy)),
+          "convrot_i8_gemm");
+    sum = sum.defined() ? sum.add_(part) : part;
+  }
+  return sum.to(dy.scalar_type());
+}
+
 struct Int8Linear : torch::autograd::Function<Int8Linear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& qweight, const Tensor& wscales,
                         const std::optional<Tensor>& bias) {
@@ -143,7 +172,9 @@ struct Int8Linear : torch::autograd::Function<Int8Linear> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("int8_linear");
     const auto saved = ctx->get_saved_variables();
-    return {i8_product(grads[0], saved[1], saved[0], CONVROT_LAYOUT_KN, {}, {}, saved[0].size(1)), {}, {}, {}};
+    const Tensor &qweight = saved[0], &wscales = saved[1];
+    if (qweight.size(0) > kMaxDot) return {i8_gradient_in_ranges(grads[0], wscales, qweight), {}, {}, {}};
+    return {i8_product(grads[0], wscales, qweight, CONVROT_LAYOUT_KN, {}, {}, qweight.size(1)), {}, {}, {}};
   }
 };
 

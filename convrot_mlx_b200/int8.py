@@ -125,7 +125,10 @@ def int8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor,
     rows padded to 16 bytes as ``quantize_int8_weight`` returns it (else every
     call copies it); wscales, bias: (n,).  Differentiable in x: the gradient
     dy * wscales is quantized for each token in turn and multiplied with the
-    same weight.  The weight, its scales and the bias are frozen."""
+    same weight.  The weight, its scales and the bias are frozen.
+
+    k is at most 131072, what an exact int32 dot can sum; of more than 131072
+    channels n the gradient adds the exact dots of ranges in float32."""
 
     return _native.ops().int8_linear(x, qweight, wscales, bias)
 
