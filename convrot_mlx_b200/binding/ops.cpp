@@ -4,6 +4,7 @@
 // interpreter and a backward pass needs no interpreter at all.  The Python
 // modules int8, rotary, norm and activation hold the public functions and
 // their documentation; everything they refuse is refused here.
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -79,6 +80,18 @@ void require_cuda(std::initializer_list<const Tensor*> tensors) {
 void once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "the gradient of ", what,
               " cannot itself be differentiated (create_graph is not supported)");
+}
+
+// Forward-mode derivatives are not formed: a tangent would be dropped, and the
+// output read as constant.
+void no_tangents(const char* what, std::initializer_list<const Tensor*> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : tensors) {
+    if (!t->defined() || !t->_fw_grad(/*level=*/0).defined()) continue;
+    PyErr_SetString(PyExc_NotImplementedError,
+                    c10::str("the forward-mode derivative of ", what, " is not supported").c_str());
+    throw py::error_already_set();
+  }
 }
 
 // --- small helpers --------------------------------------------------------
@@ -193,6 +206,7 @@ Tensor int8_linear(const Tensor& x, const Tensor& qweight, const Tensor& wscales
   if (wants_grad(wscales) || wants_grad(b))
     refuse("the weight scales and the bias of an int8 linear are frozen: they may not require gradients");
   dtype_code(x.scalar_type());
+  no_tangents("int8_linear", {&x, &wscales, &b});
   require_cuda({&x, &qweight, &wscales, &b});
   const Tensor w = padded_rows(qweight), ws = f32_vector(wscales), fb = f32_vector(b);
   if (at::GradMode::is_enabled() && x.requires_grad())
@@ -292,6 +306,7 @@ std::pair<Tensor, std::optional<Tensor>> axial_rotary(const Tensor& q, const std
   if (!whole && !each)
     refuse("positions must be (", t, ", ", n, ") or (", b, ", ", t, ", ", n, "), got ", shape_of(positions));
   dtype_code(q.scalar_type());
+  no_tangents("axial_rotary", {&q, &k, &positions});
   require_cuda({&q, &k, &positions});
   Tensor pos = positions.requires_grad() ? positions.detach() : positions;
   if (pos.scalar_type() != at::kFloat || !pos.is_contiguous()) pos = pos.to(at::kFloat).contiguous();
@@ -384,6 +399,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor run_norm(Tensor x, Tensor weight, Tensor bias, const NormHow& how) {
   if (!(how.eps >= 0)) refuse("eps must be non-negative, got ", how.eps);
   dtype_code(x.scalar_type());
+  no_tangents(how.add_one ? "modulated_layer_norm" : "layer_norm", {&x, &weight, &bias});
   require_cuda({&x, &weight, &bias});
   // both vectors of x's dtype, or both float32
   for (const Tensor* t : {&weight, &bias}) {
@@ -498,6 +514,7 @@ struct GeluSaved8 : torch::autograd::Function<GeluSaved8> {
 Tensor gelu_tanh_saved8(Tensor x) {
   if (x.dim() == 0 || x.size(-1) == 0) refuse("gelu expects features in the last dimension, got ", shape_of(x));
   dtype_code(x.scalar_type());
+  no_tangents("gelu_tanh_saved8", {&x});
   require_cuda({&x});
   if (!x.is_contiguous()) x = x.contiguous();
   if (at::GradMode::is_enabled() && x.requires_grad()) return GeluSaved8::apply(x);
