@@ -135,7 +135,7 @@ def int8_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor,
 
 class Int8Linear(nn.Module):
     """A frozen linear layer held in 8 bits (``int8_linear``).  ``qweight`` keeps the codes on rows padded to 16
-    bytes; ``scales`` and ``bias`` are float32 buffers."""
+    bytes; ``scales`` and ``bias`` are float32 buffers, and stay so when the module is cast to another type."""
 
     def __init__(self, in_features: int, out_features: int, *, bias: bool = True, device=None):
         super().__init__()
@@ -160,6 +160,16 @@ class Int8Linear(nn.Module):
         if linear.bias is not None:
             layer.bias = linear.bias.detach().float().clone()
         return layer
+
+    def _apply(self, fn, *args, **kwargs):
+        # a cast would round each channel's scale (by up to 2^-9 in bfloat16): only the device follows it
+        held = {name: self._buffers[name] for name in ("scales", "bias") if self._buffers[name] is not None}
+        super()._apply(fn, *args, **kwargs)
+        for name, value in held.items():
+            cast = self._buffers[name]
+            if cast.dtype != torch.float32:
+                self._buffers[name] = value.to(device=cast.device, dtype=torch.float32)
+        return self
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.shape[-1] != self.in_features:
