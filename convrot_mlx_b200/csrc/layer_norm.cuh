@@ -551,11 +551,12 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, ctas_of(T))
     norm_bwd_kernel(const NormParams p) {
   constexpr int L = kLanes<VEC>;
   using A = Lane<VEC>;
-  // c kept in float32 beside the row, and rows ahead: in shared memory, or in
-  // registers for elements that are too small to be copied
+  // c kept in float32 beside the row, and rows ahead: in shared memory, or, for
+  // elements that are too small to be copied (of which there are few), in
+  // registers
   constexpr bool kKeep = VEC * NV <= 24;
   using Next = Ahead<E, VEC, NV, T, 2>;
-  constexpr bool kRegs = !Next::kAsync && kKeep;
+  static_assert(Next::kAsync || kKeep, "room in the registers for the next row");
   __shared__ float red[2][16][2];
   extern __shared__ __align__(16) uint8_t smem[];  // rows ahead; then, T = 32, sums (kWarps, 2, features)
   int turn = 0;
@@ -594,14 +595,13 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, ctas_of(T))
     issue(first, at);
     issue(first + stride, at + step);
   }
-  if (Next::kAsync || kRegs) fetch(first, at);
+  fetch(first, at);
   {
     Vector<E, VEC, NV, T> w;
     w.load(p.weight, p.wide_weight, rows.segment * p.weight_stride + c0, left);
     w.get(p.weight, p.wide_weight, p.add_one ? 0.0f : 1.0f, p.add_one ? 1.0f : 0.0f, weight);
   }
   for (int64_t row = first; row < rows.end; row += stride) {
-    if (!Next::kAsync && !kRegs) fetch(row, at);
     mean = next_mean;
     rstd = next_rstd;
     if constexpr (Next::kAsync) {
@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarps : T, ctas_of(T))
       x = next_x;
       dy = next_dy;
     }
-    if (Next::kAsync || kRegs) fetch(row + stride, at + step);
+    fetch(row + stride, at + step);
     const A scale = splat<VEC>(rstd), minus = splat<VEC>(-mean);
     A centred[kKeep ? NV : 1][L], s0 = splat<VEC>(0.0f), s1 = s0;
 #pragma unroll
