@@ -68,9 +68,7 @@ def build(width: int, heads: int, device, dtype=torch.bfloat16, seed: int = 0) -
     block = Block(width, heads).to(device)
     keep = [name for name, m in block.named_modules() if isinstance(m, nn.Linear) and name not in FROZEN]
     replace_int8_linears(block, keep=keep)
-    for p in block.parameters():
-        p.data = p.data.to(dtype)
-    return block
+    return block.to(dtype)
 
 
 def grid_positions(frames: int, rows: int, cols: int, device) -> torch.Tensor:
