@@ -12,19 +12,26 @@
 // kernels on tcgen05 kind::i8, operands by TMA in 128-byte-swizzled tiles,
 // accumulators in TMEM:
 // * pair_kernel: CTA pairs (cta_group::2), 256 tokens x 256 channels a tile,
-//   persistent, for products that fill the GPU with such tiles.  Bound by
-//   shared memory, which the copies write and the tensor cores read: a stage
-//   of 128 K takes the MMAs alone 0.27 us, the copies alone 0.28, both 0.36 in
-//   one wave and 0.42 over many.  8192^3 in 372 us (2950 TOPS); 4096 x 3072 x
-//   12288 (tokens, K, channels) in 117 us (2630), 6% of it for the last wave's
-//   idle pairs; 1536 x 3072 x 3072, one wave, in 16 us, of which 7 are launch,
-//   first copies and the last tile's epilogue.  Tiles of 192 channels take as
+//   persistent, for products that fill the GPU with such tiles.  Bound by the
+//   copies and the MMAs holding up one another: a stage of 128 K takes the MMAs
+//   alone 0.27 us, the copies alone 0.28, both 0.37 in one wave and 0.39 to 0.42
+//   over many, while no unit is full (4096 x 3072 x 12288: tensor pipe active in
+//   58% of the cycles, its reads of shared memory 29% of their peak rate, copies
+//   into an SM 38 bytes a cycle, L2 37%).  8192^3 in 372 us (2950 TOPS); 4096 x
+//   3072 x 12288 (tokens, K, channels) in 117 us (2630), 6% of it for the last
+//   wave's idle pairs; 1536 x 3072 x 3072, one wave, in 16 us, of which 7 are
+//   launch, first copies and the last tile's epilogue.  A tile's whole K is one
+//   pair's work, so few tiles of a long K are far from either limit: 512 x 12288
+//   x 3072, 24 tiles for 74 pairs, 33 us, floor 12.  Tiles of 192 channels take as
 //   long a stage as 256 (0.36; 136 us instead of 117 for 12288 channels), so
 //   they gain only where both give one wave: 13.3 us instead of 14.8 for 2000 x
 //   1000 x 3000, too little for a second set of kernels.  Rings of 4 stages
 //   125 us, copies in halves 117.
 // * swap_kernel: 128 channels on the MMA's M side and 16 to 128 tokens on its
-//   N side, K split over a cluster, for few tokens or few tiles.
+//   N side, K split over a cluster, for few tokens or few tiles.  Its tiles
+//   read each operand twice as often as the pairs', and a stage takes a CTA 0.46
+//   us, the latency of its ring, or more where two share an SM: 100 x 12288 x 3072
+//   17 us (floor 6), 333 x 12288 x 3072 31 (8).
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -932,13 +939,14 @@ int launch_fused(const void* x, int64_t x_stride, const Operands& o, Params p, c
 
 // Expected times of the two tile kernels in microseconds, fitted to sweeps of
 // 16 to 1024 tokens, 512 to 12288 channels and K from 128 to 12288 (times of a
-// call in a graph).  A stage of 128 K takes a pair 0.36 us in one wave, 0.45
-// over several.  A swap CTA takes 0.46 us for a stage (the latency of its
+// call in a graph).  A stage of 128 K takes a pair 0.36 us in one wave; 0.45 over
+// several lies between the 0.39 of K = 4096 and the 0.6 of K = 1024, whose waves'
+// fill is no term of its own.  A swap CTA takes 0.46 us for a stage (the latency of its
 // ring), more where two CTAs of an SM share 125 bytes a nanosecond; its
 // epilogue takes 12 ns a token and the exchange of a split K the more, the more
 // tokens and CTAs take part; a second wave of CTAs costs all of that again.
-// Over 72 sizes of 12 to 1000 tokens the choices take 1% longer than the best
-// of all splits and both kernels.  Measured on either side (tokens, K,
+// Over the 72 sizes of 12 to 1000 tokens that it was fitted to the choices take
+// 1% longer than the best of all splits and both kernels.  Measured on either side (tokens, K,
 // channels; weights from HBM): 64 x 4096 x 4096 swap 10.2, pair 17.3; 512 x 4096
 // x 4096 swap 16.5, pair 18.0; 200 x 4096 x 12288 swap 22.8, pair 19.6; 1000 x
 // 3072 x 3072 swap 17.8, pair 15.8.

@@ -10,8 +10,11 @@
 // row, so that the exchange of the maximum and the division are little beside
 // them.  Rows that do not fit the registers are read twice, through L2.
 // bf16 rows from HBM: 4096 x 12288 in 27.6 us (0.84 of a copy's bandwidth),
-// 4096 x 3072 in 9.5 (0.61), 16 x 4096 in 1.6 (a launch); with column scales
-// 33.6 and 11.1; 4096 x 3071, whose rows start at any byte pair, 14 to 16.
+// 4096 x 3072 in 9.6 (0.61), 16 x 4096 in 1.6 (a launch); with column scales
+// 33.6 and 11.2, 1536 x 3072 5.1 (floor 2.2); 4096 x 3071, whose rows start at any
+// byte pair, 14 to 16.  At 4096 x 3072 64% of the issue slots are used by 45% of
+// the warps that an SM holds: the codes' instructions, and only one row ahead to
+// cover the memory's latency, rather than its bandwidth.
 #include "rows.cuh"
 
 namespace convrot {

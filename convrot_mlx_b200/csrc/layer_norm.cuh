@@ -12,7 +12,7 @@
 // E[d^2] - E[d]^2 (E[d] is a rounding error, so nothing cancels).  Other rows'
 // h is off by at most 2 + max|h| of a row sum's relative error, and they pay
 // one comparison: d summed for every row took 10 to 14% longer where one CTA
-// fills an SM (2048 x 16384 bf16 28.7 us instead of 26.2).  The backward pass
+// fills an SM (2048 x 16384 bf16 28.7 us instead of 27.3).  The backward pass
 // subtracts the mean before it multiplies, as the forward pass does.
 // Memory-bound: forward reads and writes a row once; backward reads x and dy
 // and writes dx, once each.  A thread keeps the same columns for all rows of
@@ -27,12 +27,16 @@
 // flight while a row is worked on.
 // us (fraction of a copy's bandwidth), bf16, backward with all three gradients:
 //   rows x features   65536 x 512  12288 x 1024  12288 x 3072  8192 x 4096  4096 x 8192  2048 x 16384
-//   forward           22 (0.93)    9.4 (0.82)    25 (0.89)     27 (0.77)    30 (0.68)    27 (0.75)
-//   backward          39 (0.79)    17 (0.67)     44 (0.79)     40 (0.77)    51 (0.60)    75 (0.41)
+//   forward           25 (0.82)    11 (0.71)     27 (0.86)     27 (0.76)    30 (0.69)    27 (0.75)
+//   backward          38 (0.80)    19 (0.61)     44 (0.79)     40 (0.77)    51 (0.60)    75 (0.41)
+// (inputs and outputs rotated beyond L2; with one output, which L2 holds,
+// forward 22, 9.1 and 25 for the first three).  Rows far from zero 12288 x 3072:
+// forward 27.0 instead of 25.5.
 // Rows of odd length, whose elements are moved one by one: 5003 x 1153 float32
-// 12.0 and 18.6 us (1152: 8.1 and 14.9).  16-byte pieces copied to shared
-// memory across the rows' ends and read back by element took longer, for the
-// barrier that each row then needs: 12.9 and 18.6.
+// 13.1 and 21.5 us (1152: 9.7 and 16.8), 4096 x 6143 bf16 42 and 83 (6142: 37 and
+// 56).  16-byte pieces copied to shared memory across the rows' ends and read
+// back by element took a fifth longer forward and as long backward, for the
+// barrier that each row then needs.
 #pragma once
 
 #include <algorithm>

@@ -16,7 +16,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     x: (..., features) float32, float16 or bfloat16; weight and bias:
     (features,) or None.  Differentiable in all three; the gradients of weight
     and bias are float32 sums over all rows, in an order that depends on the
-    shape alone."""
+    shape, the types, the tensors' alignment and the GPU's size, but not from
+    run to run."""
 
     return _native.ops().layer_norm(x, weight, bias, eps)
 
@@ -26,7 +27,9 @@ def modulated_layer_norm(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tens
 
     x: (batch, ..., features); shift and scale: (batch, 1, features) or
     (batch, features), columns of a wider modulation output included; a batch
-    of 1 is shared by all samples.  Differentiable in all three; the gradients
-    of scale and shift are float32 sums over their sample's rows."""
+    of 1 is shared by all samples.  At most 65535 samples may have a shift and
+    scale of their own.  Differentiable in all three; the gradients of scale and
+    shift are float32 sums over their sample's rows, ordered as in
+    ``layer_norm``."""
 
     return _native.ops().modulated_layer_norm(x, shift, scale, eps)

@@ -306,8 +306,9 @@ int convrot_quantize_i8(const void* x, int dtype, int64_t rows, int64_t features
  * i * act_stride bytes.  weight: int8, layout CONVROT_LAYOUT_NK = (n, k) rows
  * or CONVROT_LAYOUT_KN = (k, n) rows (the same matrix contracted over its
  * rows: the gradient of the input), row r at r * weight_stride bytes.
- * Strides are multiples of 16 and cover the rows.  wscales and bias may be
- * NULL (ones, zeros).  Codes are in [-127, 127].  No reference counterpart.
+ * Strides are multiples of 16 and cover the rows; m and n are below 2^22.
+ * wscales and bias may be NULL (ones, zeros).  Codes are in [-127, 127].  No
+ * reference counterpart.
  */
 int convrot_i8_gemm(const int8_t* act, int64_t act_stride, const int8_t* weight, int64_t weight_stride, int layout,
                     const float* xscales, const float* wscales, const float* bias, void* out, int out_dtype,
@@ -345,14 +346,15 @@ int convrot_axial_rotary(int dtype, int64_t batch, int64_t tokens, int64_t dim, 
                          double theta, int interleaved, int inverse, void* stream);
 
 /*
- * Layer norm of the rows of x (rows, features), packed:
+ * Layer norm of the rows of x (rows, features), packed, features <= 2^20:
  * y = (x - mean) * rsqrt(var + eps) * w + bias in float32, one rounding; w =
  * weight, or 1 + weight with add_one.  Rows r with the same r /
  * rows_per_weight share a weight and a bias vector, at weight_stride elements
  * from one another: all rows (affine norm), or those of a sample (modulated
- * norm).  weight_dtype: that of x, or CONVROT_F32.  weight and bias may be
- * NULL (w = 1, bias 0).  mean and rstd: (rows,) float32 for the backward
- * pass, or both NULL.  No reference counterpart.
+ * norm), of which there are at most 65535.  weight_dtype: that of x, or
+ * CONVROT_F32.  weight and bias may be NULL (w = 1, bias 0).  mean and rstd:
+ * (rows,) float32 for the backward pass, or both NULL.  No reference
+ * counterpart.
  */
 int convrot_layer_norm(const void* x, int dtype, int64_t rows, int64_t features, const void* weight,
                        const void* bias, int weight_dtype, int64_t rows_per_weight, int64_t weight_stride,
@@ -363,7 +365,8 @@ int convrot_layer_norm(const void* x, int dtype, int64_t rows, int64_t features,
  * sums over the rows that share a weight, dweight = sum dy h and dbias = sum
  * dy with h the normalized row, (rows / rows_per_weight, features) packed, of
  * weight_dtype, either NULL when not wanted.  Sums are float32, in an order
- * fixed by the shape.  mean, rstd: from the forward pass.  workspace:
+ * fixed by the shape, the types, the addresses' alignment and the number of
+ * SMs (no atomics).  mean, rstd: from the forward pass.  workspace:
  * convrot_layer_norm_workspace bytes, 16-byte aligned (not used when neither
  * sum is wanted).  With 0 rows nothing is written.
  */
