@@ -59,6 +59,11 @@ SIGNATURES: dict[str, tuple] = {
                                          _P]),
     "convrot_gelu_saved8": (_I, [_P, _I, _I64, _I64, _P, _P, _P, _P]),
     "convrot_gelu_saved8_backward": (_I, [_P, _I, _I64, _I64, _P, _P, _P, _P]),
+    "convrot_quantize_fp8": (_I, [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _I64, _P]),
+    "convrot_quantize_fp8_weight": (_I, [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _I64, _P]),
+    "convrot_fp8_gemm": (_I, [_P, _I64, _P, _I64, _P, _I64, _I, _P, _I64, _P, _P, _I, _I64, _I64, _I64, _P]),
+    "convrot_fp8_linear": (_I, [_P, _I, _I64, _P, _I64, _I, _P, _I64, _P, _P, _I, _I64, _I64, _I64, _P, _I64, _P, _I64,
+                                _P]),
     "convrot_set_gemm_route": (_I, [_I]),
     "convrot_take_device_error": (_I, [ctypes.POINTER(_I)]),
 }

@@ -214,6 +214,69 @@ Tensor int8_linear(const Tensor& x, const Tensor& qweight, const Tensor& wscales
   return i8_product(x, {}, w, CONVROT_LAYOUT_NK, ws, fb, n);
 }
 
+// --- 8-bit floating-point linear ------------------------------------------------
+
+constexpr int64_t kSpan = 128;  // values of a row, rows and columns of a weight, that share a scale
+
+// The quantizer and the product in one call; n columns out.
+Tensor fp8_product(const Tensor& x, const Tensor& qweight, int layout, const Tensor& wscales, const Tensor& bias,
+                   int64_t n) {
+  const c10::cuda::OptionalCUDAGuard guard(x.device());
+  const Tensor r = rows_of(x);
+  const int64_t m = r.size(0), k = r.size(1), pitch = (k + kPitch - 1) / kPitch * kPitch;
+  const int64_t scales_pitch = (k + 4 * kSpan - 1) / (4 * kSpan) * 4;
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = n;
+  const Tensor out = at::empty(shape, x.options());
+  const Tensor space = at::empty({m * (pitch + scales_pitch)}, x.options().dtype(at::kByte));  // codes, then scales
+  auto* codes = static_cast<uint8_t*>(space.data_ptr());
+  const int dtype = dtype_code(x.scalar_type());
+  check(convrot_fp8_linear(r.data_ptr(), dtype, r.stride(0), static_cast<const uint8_t*>(qweight.data_ptr()),
+                           qweight.stride(0), layout, static_cast<const uint8_t*>(wscales.data_ptr()), wscales.size(1),
+                           static_cast<const float*>(address(bias)), out.data_ptr(), dtype, m, n, k, codes, pitch,
+                           codes + m * pitch, scales_pitch, stream_of(x)),
+        "convrot_fp8_linear");
+  return out;
+}
+
+struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& qweight, const Tensor& wscales,
+                        const std::optional<Tensor>& bias) {
+    ctx->save_for_backward({qweight, wscales});
+    return fp8_product(x, qweight, CONVROT_LAYOUT_NK, wscales, or_undefined(bias), qweight.size(0));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    once("fp8_linear");
+    const auto saved = ctx->get_saved_variables();
+    return {fp8_product(grads[0], saved[0], CONVROT_LAYOUT_KN, saved[1], {}, saved[0].size(1)), {}, {}, {}};
+  }
+};
+
+Tensor fp8_linear(const Tensor& x, const Tensor& qweight, const Tensor& wscales, const std::optional<Tensor>& bias) {
+  if (x.dim() == 0) refuse("fp8 linear expects at least one dimension");
+  if (qweight.dim() != 2 || qweight.scalar_type() != at::kFloat8_e4m3fn)
+    refuse("fp8 weight must be a 2D float8_e4m3fn tensor, got ", shape_of(qweight), " ", qweight.scalar_type());
+  const int64_t n = qweight.size(0), k = x.size(-1);
+  if (qweight.size(1) != k || k == 0 || n == 0)
+    refuse("fp8 weight must be (N, K) rows; activation K=", k, ", weight=", shape_of(qweight));
+  const int64_t nb = (n + kSpan - 1) / kSpan, kb = (k + kSpan - 1) / kSpan;
+  if (wscales.dim() != 2 || wscales.size(0) != nb || wscales.size(1) != kb || wscales.scalar_type() != at::kFloat8_e8m0fnu)
+    refuse("fp8 weight scales must be (", nb, ", ", kb, ") float8_e8m0fnu, got ", shape_of(wscales), " ",
+           wscales.scalar_type());
+  const Tensor b = or_undefined(bias);
+  if (b.defined() && (b.dim() != 1 || b.size(0) != n))
+    refuse("fp8 bias must have shape (", n, ",), got ", shape_of(b));
+  if (wants_grad(qweight) || wants_grad(wscales) || wants_grad(b))
+    refuse("the weight, its scales and the bias of an fp8 linear are frozen: they may not require gradients");
+  dtype_code(x.scalar_type());
+  no_tangents("fp8_linear", {&x, &b});
+  require_cuda({&x, &qweight, &wscales, &b});
+  const Tensor w = padded_rows(qweight), ws = wscales.contiguous(), fb = f32_vector(b);
+  if (at::GradMode::is_enabled() && x.requires_grad())
+    return Fp8Linear::apply(x, w, ws, fb.defined() ? std::optional<Tensor>(fb) : std::nullopt);
+  return fp8_product(x, w, CONVROT_LAYOUT_NK, ws, fb, n);
+}
+
 // --- rotary -------------------------------------------------------------------
 
 struct RotaryHow {
@@ -525,6 +588,7 @@ Tensor gelu_tanh_saved8(Tensor x) {
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("int8_linear", &int8_linear);
+  m.def("fp8_linear", &fp8_linear);
   m.def("axial_rotary", &axial_rotary);
   m.def("layer_norm", &layer_norm);
   m.def("modulated_layer_norm", &modulated_layer_norm);

@@ -282,7 +282,11 @@ int convrot_set_gemm_route(int route);
  * 57 activation slot free); 61-65 8-bit pair GEMM (61 copy slot free, 62
  * accumulator buffer free, 63 stage landed, 64 final MMA drain, 65
  * accumulator ready); 71-74 8-bit swap GEMM (71 copy slot free, 72 weight
- * stage landed, 73 activation stage landed, 74 final MMA drain).
+ * stage landed, 73 activation stage landed, 74 final MMA drain); 81-86 8-bit
+ * float pair GEMM (81 copy slot free, 82 accumulator free, 83 stage landed, 84
+ * scales landed, 85 accumulator ready, 86 scale slot free); 91-96 8-bit float
+ * swap GEMM (91 copy slot free, 92 weight stage landed, 93 activation stage
+ * landed, 94 final MMA drain, 95 scale slot free, 96 scales landed).
  */
 int convrot_take_device_error(int* code);
 
@@ -388,6 +392,56 @@ int convrot_gelu_saved8(const void* x, int dtype, int64_t rows, int64_t features
                         float* scales, void* stream);
 int convrot_gelu_saved8_backward(const void* dy, int dtype, int64_t rows, int64_t features, const int8_t* codes,
                                  const float* scales, void* dx, void* stream);
+
+/*
+ * Quantizers of the 8-bit floating-point linear: e4m3 codes and one scale 2^e
+ * for each block of 128 consecutive values of a row (convrot_quantize_fp8), or
+ * for each block of 128 x 128 (convrot_quantize_fp8_weight), with e the least
+ * exponent, at least -127, for which max|x| <= 448 * 2^e, stored as the byte
+ * e + 127; code = e4m3(x * 2^-e), to nearest even.  A block of zeros has codes
+ * and byte 0; one that holds an infinity or a NaN has codes 0 and byte 255,
+ * which stands for NaN.  Blocks at the ends of rows (and of the rows) are of
+ * what is there.  Row r of x starts at r * x_stride elements, of the codes at
+ * r * codes_stride bytes (a multiple of 16; the bytes of a row past its
+ * features up to a multiple of 16 are overwritten), of the scales at r *
+ * scales_stride (or r / 128 times it).  No reference counterpart.
+ */
+int convrot_quantize_fp8(const void* x, int dtype, int64_t rows, int64_t features, int64_t x_stride, uint8_t* codes,
+                         int64_t codes_stride, uint8_t* scales, int64_t scales_stride, void* stream);
+int convrot_quantize_fp8_weight(const void* w, int dtype, int64_t rows, int64_t features, int64_t w_stride,
+                                uint8_t* codes, int64_t codes_stride, uint8_t* scales, int64_t scales_stride,
+                                void* stream);
+
+/*
+ * 8-bit floating-point linear: out[i, j] = T(sum over blocks b of 128 of k of
+ * xscale[i, b] * wscale[j / 128, b] * sum over k in b of act[i, k] w[j, k], +
+ * bias[j]), sums in float32 (tcgen05 kind::mxf8f6f4).  act: (m, k) e4m3 codes
+ * with scales (m, ceil(k / 128)), rows of scales at multiples of 4 bytes.
+ * weight: e4m3, layout CONVROT_LAYOUT_NK = (n, k) rows or CONVROT_LAYOUT_KN =
+ * (k, n) rows (the same matrix contracted over its rows: the gradient of the
+ * input); wscales: one byte for each 128 x 128 block of the matrix as it
+ * lies, rows of them at wscales_stride bytes.  Scales are the bytes of the
+ * quantizers above.  Row strides of codes are multiples of 16 and cover the
+ * rows; m, n and k are below 2^22.  bias may be NULL (zeros).  The order of
+ * the sums is fixed by the shape, the layout and the number of SMs.  No
+ * reference counterpart.
+ */
+int convrot_fp8_gemm(const uint8_t* act, int64_t act_stride, const uint8_t* xscales, int64_t xscales_stride,
+                     const uint8_t* weight, int64_t weight_stride, int layout, const uint8_t* wscales,
+                     int64_t wscales_stride, const float* bias, void* out, int out_dtype, int64_t m, int64_t n,
+                     int64_t k, void* stream);
+
+/*
+ * convrot_quantize_fp8 of x, then convrot_fp8_gemm of its codes, in one call.
+ * `codes` (m, k) and `scales` (m, ceil(k / 128), rows at multiples of 4 bytes)
+ * are workspace; what they hold afterwards is not specified.  The product
+ * starts reading the weight while the quantizer runs: the workspace may not
+ * overlap the weight.
+ */
+int convrot_fp8_linear(const void* x, int x_dtype, int64_t x_stride, const uint8_t* weight, int64_t weight_stride,
+                       int layout, const uint8_t* wscales, int64_t wscales_stride, const float* bias, void* out,
+                       int out_dtype, int64_t m, int64_t n, int64_t k, uint8_t* codes, int64_t codes_stride,
+                       uint8_t* scales, int64_t scales_stride, void* stream);
 
 #ifdef __cplusplus
 }
