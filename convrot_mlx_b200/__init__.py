@@ -47,6 +47,7 @@ from .activation import gelu_tanh_saved8
 from .fp8 import Fp8Linear, fp8_linear, fp8_matmul, quantize_fp8_blockwise, quantize_fp8_weight
 from .int8 import Int8Linear, int8_linear, int8_matmul, quantize_int8_weight, quantize_signed_int8_rowwise
 from .norm import layer_norm, modulated_layer_norm
+from .optim import AdamW, adamw_step, grad_norm
 from .rotary import axial_rotary
 
 __version__ = "0.1.0"

@@ -8,6 +8,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
+#include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
 #include <initializer_list>
@@ -584,11 +585,232 @@ Tensor gelu_tanh_saved8(Tensor x) {
   return gelu_forward(x, nullptr);
 }
 
+// --- AdamW and the gradient norm ---------------------------------------------------
+
+// The tensors of a Python sequence without a reference each (the caller holds
+// the sequence for the length of the call); nothing where it has None.
+class TensorList {
+ public:
+  TensorList(const py::object& o, const char* what) : what_(what) {
+    seq_ = py::reinterpret_steal<py::object>(PySequence_Fast(o.ptr(), "expected a sequence of tensors"));
+    if (!seq_) throw py::error_already_set();
+    items_ = PySequence_Fast_ITEMS(seq_.ptr());
+    size_ = PySequence_Fast_GET_SIZE(seq_.ptr());
+  }
+  int64_t size() const { return size_; }
+  const Tensor* at(int64_t i) const {
+    if (items_[i] == Py_None) return nullptr;
+    if (!THPVariable_Check(items_[i])) refuse(what_, " must be tensors, got ", Py_TYPE(items_[i])->tp_name);
+    return &THPVariable_Unpack(items_[i]);
+  }
+
+ private:
+  py::object seq_;
+  PyObject** items_;
+  int64_t size_;
+  const char* what_;
+};
+
+int dtype_slot(const Tensor& t) { return dtype_code(t.scalar_type()); }  // 0, 1 or 2
+
+// t where its values are dense in memory in some order, else packed.
+Tensor dense(const Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_and_dense() ? t : t.contiguous(); }
+
+// Partial sums of the squares of gradients of any of the three types, all on
+// one device, in one tensor; None is passed over.
+Tensor square_sums_of(const std::vector<const Tensor*>& grads) {
+  std::vector<convrot_grad_tensor> by_type[3];
+  std::vector<Tensor> held;
+  const Tensor& first = *grads.front();
+  require_cuda({&first});
+  const c10::Device home = first.device();
+  for (const Tensor* g : grads) {
+    if (g->layout() != at::kStrided) refuse("gradients must be dense tensors");
+    if (g->device() != home) refuse("expected all tensors on ", home.str(), ", got one on ", g->device().str());
+    const int slot = dtype_slot(*g);
+    if (g->is_contiguous()) {
+      by_type[slot].push_back({g->data_ptr(), g->numel()});
+    } else {
+      held.push_back(dense(*g));
+      by_type[slot].push_back({held.back().data_ptr(), g->numel()});
+    }
+  }
+  const c10::cuda::OptionalCUDAGuard guard(home);
+  int64_t counts[3] = {}, total = 0;
+  for (int i = 0; i < 3; ++i)
+    if (!by_type[i].empty())
+      total += counts[i] = convrot_square_sums_count(static_cast<int64_t>(by_type[i].size()), by_type[i].data());
+  const Tensor sums = at::empty({total}, first.options().dtype(at::kDouble).requires_grad(false));
+  auto* at = static_cast<double*>(sums.data_ptr());
+  for (int i = 0; i < 3; ++i) {
+    if (!counts[i]) continue;
+    check(convrot_square_sums(static_cast<int64_t>(by_type[i].size()), by_type[i].data(), i, at, counts[i],
+                              stream_of(first)),
+          "convrot_square_sums");
+    at += counts[i];
+  }
+  return sums;
+}
+
+std::vector<const Tensor*> present(const TensorList& list) {
+  std::vector<const Tensor*> out;
+  out.reserve(list.size());
+  for (int64_t i = 0; i < list.size(); ++i)
+    if (const Tensor* t = list.at(i)) out.push_back(t);
+  if (out.empty()) refuse("expected at least one gradient");
+  return out;
+}
+
+Tensor square_sums(const py::object& grads) {
+  const TensorList list(grads, "gradients");
+  return square_sums_of(present(list));
+}
+
+Tensor grad_norm(const py::object& grads) {
+  const TensorList list(grads, "gradients");
+  const std::vector<const Tensor*> tensors = present(list);
+  const Tensor sums = square_sums_of(tensors);
+  const c10::cuda::OptionalCUDAGuard guard(sums.device());
+  const Tensor norm = at::empty({}, sums.options().dtype(at::kFloat));
+  check(convrot_norm_of_sums(static_cast<const double*>(sums.data_ptr()), sums.numel(),
+                             static_cast<float*>(norm.data_ptr()), stream_of(sums)),
+        "convrot_norm_of_sums");
+  return norm;
+}
+
+// A scalar that is a number, or one float32 on the device.
+const float* device_scalar(const py::object& o, const char* what, const c10::Device& home, double* number) {
+  if (!THPVariable_Check(o.ptr())) {
+    *number = o.cast<double>();
+    return nullptr;
+  }
+  const Tensor& t = THPVariable_Unpack(o.ptr());
+  if (t.numel() != 1 || t.scalar_type() != at::kFloat || t.device() != home)
+    refuse("a ", what, " on the device must be one float32 on ", home.str());
+  return static_cast<const float*>(t.data_ptr());
+}
+
+// Whether no address occurs twice (0 aside).
+bool distinct(const std::vector<const void*>& addresses) {
+  size_t size = 64;
+  while (size < 2 * addresses.size()) size *= 2;
+  std::vector<const void*> table(size, nullptr);
+  for (const void* a : addresses) {
+    size_t i = (reinterpret_cast<uintptr_t>(a) >> 2) * 0x9E3779B97F4A7C15ull >> 20 & (size - 1);
+    for (; table[i]; i = (i + 1) & (size - 1))
+      if (table[i] == a) return false;
+    table[i] = a;
+  }
+  return true;
+}
+
+// The step; with max_norm the gradients' norm, else nothing.  sums: of
+// square_sums, where the norm is over more gradients than these.
+std::optional<Tensor> adamw_step(const py::object& params, const py::object& grads, const py::object& exp_avgs,
+                                 const py::object& exp_avg_sqs, const py::object& scales, const py::object& step,
+                                 const py::object& lr, double beta1, double beta2, double eps, double weight_decay,
+                                 std::optional<double> max_norm, const std::optional<Tensor>& sums_in) {
+  const TensorList p(params, "parameters"), g(grads, "gradients"), m(exp_avgs, "moments"), v(exp_avg_sqs, "moments");
+  const bool eight = !scales.is_none();
+  const TensorList s(eight ? scales : exp_avgs, "scales");
+  const int64_t count = p.size();
+  if (g.size() != count || m.size() != count || v.size() != count || s.size() != count)
+    refuse("parameters, gradients, moments and scales must be equally many, got ", count, ", ", g.size(), ", ", m.size(),
+           ", ", v.size(), " and ", s.size());
+  if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1)) refuse("betas must be in [0, 1), got ", beta1, " and ", beta2);
+  if (!(eps >= 0) || !(weight_decay >= 0)) refuse("eps and weight decay must be non-negative");
+  if (max_norm && !(*max_norm >= 0)) refuse("the largest norm must be non-negative, got ", *max_norm);
+  const at::ScalarType moment = eight ? at::kFloat8_e4m3fn : at::kFloat;
+  std::vector<convrot_adamw_tensor> by_type[3];
+  std::vector<const void*> addresses;
+  std::vector<const Tensor*> used, written;
+  std::vector<Tensor> held;
+  addresses.reserve(count);
+  used.reserve(count);
+  written.reserve(count);
+  c10::Device home(c10::DeviceType::CPU);
+  for (int64_t i = 0; i < count; ++i) {
+    const Tensor* gi = g.at(i);
+    if (!gi) continue;
+    const Tensor *pi = p.at(i), *mi = m.at(i), *vi = v.at(i), *si = eight ? s.at(i) : mi;
+    if (!pi || !mi || !vi || !si) refuse("parameter ", i, " has a gradient, but a parameter, moment or scale is missing");
+    if (used.empty()) home = pi->device();
+    for (const Tensor* t : {pi, gi, mi, vi, si}) {
+      if (!t->is_cuda() || t->device() != home) require_cuda({used.empty() ? pi : written.front(), t});
+      if (t->layout() != at::kStrided) refuse("the AdamW step takes dense tensors");
+    }
+    if (gi->scalar_type() != pi->scalar_type() || gi->sizes() != pi->sizes())
+      refuse("gradient ", i, " is ", shape_of(*gi), " ", gi->scalar_type(), ", its parameter ", shape_of(*pi), " ",
+             pi->scalar_type());
+    for (const Tensor* t : {mi, vi})
+      if (t->scalar_type() != moment || t->sizes() != pi->sizes())
+        refuse("moments of parameter ", i, " must be ", shape_of(*pi), " ", moment, ", got ", shape_of(*t), " ",
+               t->scalar_type());
+    const int64_t n = pi->numel(), blocks = (n + 255) / 256;
+    if (eight && (si->scalar_type() != at::kFloat || si->dim() != 2 || si->size(0) != blocks || si->size(1) != 2 ||
+                  !si->is_contiguous()))
+      refuse("scales of parameter ", i, " must be (", blocks, ", 2) float32 and contiguous, got ", shape_of(*si), " ",
+             si->scalar_type());
+    const Tensor* grad = gi;
+    if (!pi->is_contiguous() || !mi->is_contiguous() || !vi->is_contiguous() || !gi->is_contiguous()) {
+      // values are taken in memory order: one order for all four
+      if (!pi->is_non_overlapping_and_dense() || mi->strides() != pi->strides() || vi->strides() != pi->strides())
+        refuse("parameter ", i, " must be dense in memory, and its moments laid out as it is");
+      if (gi->strides() != pi->strides()) {
+        held.push_back(at::empty_strided(pi->sizes(), pi->strides(), gi->options()).copy_(gi->detach()));
+        grad = &held.back();
+      }
+    }
+    if (n == 0) continue;
+    by_type[dtype_slot(*pi)].push_back({pi->data_ptr(), grad->data_ptr(), mi->data_ptr(), vi->data_ptr(),
+                                        eight ? static_cast<float*>(si->data_ptr()) : nullptr, n});
+    addresses.push_back(pi->data_ptr());
+    used.push_back(gi);
+    written.push_back(pi);
+  }
+  if (!distinct(addresses)) refuse("a parameter occurs twice in one AdamW step");
+  convrot_adamw_options o = {};
+  if (used.empty()) {
+    if (max_norm) refuse("clipping needs at least one gradient");
+    return std::nullopt;
+  }
+  o.step_device = device_scalar(step, "step", home, &o.step);
+  o.lr_device = device_scalar(lr, "learning rate", home, &o.lr);
+  if (!o.step_device && !(o.step >= 1)) refuse("the step counts from 1, got ", o.step);
+  if (!o.lr_device && !(o.lr >= 0)) refuse("the learning rate must be non-negative, got ", o.lr);
+  o.beta1 = beta1, o.beta2 = beta2, o.eps = eps, o.weight_decay = weight_decay;
+  const c10::cuda::OptionalCUDAGuard guard(home);
+  std::optional<Tensor> norm;
+  Tensor sums;
+  if (max_norm) {
+    sums = sums_in.has_value() ? *sums_in : square_sums_of(used);
+    if (sums.scalar_type() != at::kDouble || sums.device() != home || !sums.is_contiguous() || sums.numel() == 0)
+      refuse("sums of squares must be float64 on ", home.str());
+    norm = at::empty({}, sums.options().dtype(at::kFloat));
+    o.sums = static_cast<const double*>(sums.data_ptr());
+    o.sums_count = sums.numel();
+    o.max_norm = *max_norm;
+    o.norm = static_cast<float*>(norm->data_ptr());
+  }
+  for (int i = 0; i < 3; ++i) {
+    if (by_type[i].empty()) continue;
+    check(convrot_adamw(static_cast<int64_t>(by_type[i].size()), by_type[i].data(), i, eight ? 8 : 32, &o,
+                        stream_of(*written.front())),
+          "convrot_adamw");
+  }
+  for (const Tensor* t : written)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("int8_linear", &int8_linear);
   m.def("fp8_linear", &fp8_linear);
+  m.def("square_sums", &square_sums);
+  m.def("grad_norm", &grad_norm);
+  m.def("adamw_step", &adamw_step);
   m.def("axial_rotary", &axial_rotary);
   m.def("layer_norm", &layer_norm);
   m.def("modulated_layer_norm", &modulated_layer_norm);

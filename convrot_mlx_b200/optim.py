@@ -1,0 +1,165 @@
+"""The AdamW step over many tensors at once, with its moments in 32 bits or in 8, and the gradient norm that clips it.
+
+What is trained around frozen quantized linears (modulations, norms, adapters)
+is many tensors, often small, and for a whole block its moments are the largest
+part of what training holds.  One launch updates up to 512 tensors; the norm
+stays on the device, and the step scales the gradients by it as it reads them.
+No counterpart in the reference (it does not train).
+
+Moments in 8 bits: m and sqrt(v) as float8_e4m3fn with a float32 scale each for
+256 consecutive values of a tensor (the largest becomes 448).  A block whose
+scales are not finite, as an infinite or NaN gradient makes them, stays NaN.
+"""
+
+from __future__ import annotations
+
+import itertools
+from typing import Iterable, Sequence
+
+import torch
+
+from . import _native
+
+MOMENT_BLOCK = 256  # values of a tensor whose 8-bit moments share their scales
+
+
+@torch.no_grad()
+def grad_norm(grads: Iterable[torch.Tensor | None]) -> torch.Tensor:
+    """The 2-norm of all values of ``grads`` (CUDA tensors of one device; None is passed over), float32 on the device.
+
+    Squares are summed in 64 bits, so neither large nor small values leave its
+    range before the norm itself does; the same bits on every call."""
+
+    return _native.ops().grad_norm(grads if isinstance(grads, (list, tuple)) else list(grads))
+
+
+@torch.no_grad()
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | None], exp_avgs: Sequence[torch.Tensor],
+               exp_avg_sqs: Sequence[torch.Tensor], scales: Sequence[torch.Tensor] | None, step, *, lr, betas=(0.9, 0.999),
+               eps: float = 1e-8, weight_decay: float = 1e-2, max_norm: float | None = None) -> torch.Tensor | None:
+    """One AdamW step in place: parameters float32, float16 or bfloat16 with gradients of their type (None: left as it is).
+
+        m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
+        p = p (1 - lr weight_decay) - lr / (1 - b1^step) m / (sqrt(v / (1 - b2^step)) + eps)
+
+    ``scales`` None: ``exp_avgs`` and ``exp_avg_sqs`` hold m and v in float32.
+    Else they hold float8_e4m3fn codes of m and of sqrt(v), and ``scales`` for
+    each parameter (ceil(n / 256), 2) float32, the scales of both for each 256
+    values; zeros are the start of either.  ``step`` counts from 1; ``step`` and ``lr``
+    may each be one float32 on the device, which a captured step reads when
+    it is replayed.  ``max_norm``: gradients are scaled by
+    min(1, max_norm / (norm + 1e-6)) as they are read, with the norm of them all, which
+    is returned.  Gradients are not changed.  A parameter that is not contiguous has to be dense, with
+    its moments laid out as it is."""
+
+    return _native.ops().adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales, step, lr, betas[0], betas[1], eps,
+                                    weight_decay, max_norm, None)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW by ``adamw_step``: all parameters of a group in one launch.
+
+    ``state_bits`` 8 keeps the moments in 8 bits (2.03 bytes a parameter), 32 in
+    float32 (8 bytes) whatever the parameter's type, under the names of
+    ``torch.optim.AdamW``, whose state dict can be loaded.  ``max_norm`` clips by
+    the norm of all gradients of all groups; ``last_norm`` is that of the last step, on
+    the device.  ``capturable``: the step count of a group is on the device
+    (``group["step"]``), so that a graph that captured ``step`` counts on as it
+    is replayed; all its parameters share it.  ``lr`` may be one float32 on the
+    device.  All parameters lie on one CUDA device."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
+                 state_bits: int = 32, max_norm: float | None = None, capturable: bool = False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"moments are kept in 8 or 32 bits, not {state_bits}")
+        if not torch.is_tensor(lr) and not lr >= 0:
+            raise ValueError(f"the learning rate must be non-negative, got {lr}")
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError(f"betas must be in [0, 1), got {betas}")
+        if not eps >= 0 or not weight_decay >= 0:
+            raise ValueError("eps and weight decay must be non-negative")
+        if max_norm is not None and not max_norm >= 0:
+            raise ValueError(f"the largest norm must be non-negative, got {max_norm}")
+        self.state_bits = state_bits
+        self.max_norm = max_norm
+        self.last_norm: torch.Tensor | None = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, capturable=capturable))
+
+    def _start(self, p: torch.Tensor) -> dict:
+        state = self.state[p]
+        if not state:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW starts its moments in its first step: take one before the capture")
+            keep = torch.preserve_format
+            kind = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
+            state["step"] = 0
+            state["exp_avg"] = torch.zeros_like(p, dtype=kind, memory_format=keep)
+            state["exp_avg_sq"] = torch.zeros_like(p, dtype=kind, memory_format=keep)
+            if self.state_bits == 8:
+                state["scales"] = torch.zeros((-(-p.numel() // MOMENT_BLOCK), 2), dtype=torch.float32, device=p.device)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step; returns the closure's loss, if there is one."""
+
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        ops, sums, norm = _native.ops(), None, None
+        if not all(group["capturable"] for group in self.param_groups) and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a captured AdamW step needs capturable=True: its step count has to be on the device")
+        if self.max_norm is not None:
+            grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
+            if not grads:
+                return loss
+            sums = ops.square_sums(grads)
+        for group in self.param_groups:
+            runs: dict = {}  # the parameters by their step, nearly always one
+            for p in group["params"]:
+                if p.grad is not None:
+                    state = self._start(p)
+                    state["step"] += 1
+                    runs.setdefault(0 if group["capturable"] else state["step"], []).append((p, state))
+            if runs and group["capturable"]:
+                if "step" not in group:
+                    first = next(iter(runs.values()))[0]
+                    group["step"] = torch.full((), float(first[1]["step"] - 1), device=first[0].device)
+                group["step"].add_(1.0)
+            for step, run in runs.items():
+                states = [state for _, state in run]
+                norm = ops.adamw_step([p for p, _ in run], [p.grad for p, _ in run], [s["exp_avg"] for s in states],
+                                      [s["exp_avg_sq"] for s in states],
+                                      [s["scales"] for s in states] if self.state_bits == 8 else None,
+                                      group["step"] if group["capturable"] else step, group["lr"], *group["betas"],
+                                      group["eps"], group["weight_decay"], self.max_norm, sums)
+        self.last_norm = norm
+        return loss
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        """Load a state of this class, or with ``state_bits`` 32 of ``torch.optim.AdamW``; moments keep their types."""
+
+        super().load_state_dict(state_dict)
+        ids = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
+        for key, p in zip(ids, params):
+            saved = state_dict["state"].get(key)
+            if not saved:
+                continue
+            if ("scales" in saved) != (self.state_bits == 8):
+                raise ValueError(f"the state's moments are not kept in {self.state_bits} bits")
+            if self.state_bits == 8 and saved["exp_avg"].stride() != p.stride():
+                raise ValueError("8-bit moments were kept for a parameter of another memory layout")
+            state = {"step": int(saved["step"])}
+            for name in ("exp_avg", "exp_avg_sq"):
+                # the parameter's own layout, whatever that of the saved tensor was
+                kind = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
+                state[name] = torch.empty_like(p, dtype=kind, memory_format=torch.preserve_format).copy_(saved[name])
+            if self.state_bits == 8:
+                state["scales"] = saved["scales"].to(p.device, torch.float32, copy=True).contiguous()
+            self.state[p] = state
+        for group in self.param_groups:
+            group.setdefault("capturable", False)
+            if torch.is_tensor(group.get("step")):
+                group["step"] = group["step"].to(group["params"][0].device, torch.float32, copy=True)

@@ -443,6 +443,57 @@ int convrot_fp8_linear(const void* x, int x_dtype, int64_t x_stride, const uint8
                        int out_dtype, int64_t m, int64_t n, int64_t k, uint8_t* codes, int64_t codes_stride,
                        uint8_t* scales, int64_t scales_stride, void* stream);
 
+/*
+ * Sums of squares of many tensors of one dtype, for their norm.  `tensors` is
+ * a host array.  Writes `sums_count` partial sums (float64) that add up to the
+ * total; convrot_square_sums_count gives a good number of them for these
+ * tensors.  Which values a sum holds depends on the sizes and sums_count alone.
+ * convrot_norm_of_sums: sqrt of the total of sums (of several dtypes, one
+ * after another in memory) as float32.  No reference counterpart.
+ */
+typedef struct {
+  const void* grad;
+  int64_t numel;
+} convrot_grad_tensor;
+int64_t convrot_square_sums_count(int64_t count, const convrot_grad_tensor* tensors);
+int convrot_square_sums(int64_t count, const convrot_grad_tensor* tensors, int dtype, double* sums,
+                        int64_t sums_count, void* stream);
+int convrot_norm_of_sums(const double* sums, int64_t sums_count, float* norm, void* stream);
+
+/*
+ * One AdamW step (decoupled weight decay) over many tensors of one dtype, in
+ * one launch for each 512 of them; `tensors` is a host array.  state_bits 32:
+ * exp_avg and exp_avg_sq are float32 (m and v).  state_bits 8: they are e4m3
+ * codes of m and of sqrt(v), and scales holds {scale of m, scale of sqrt(v)}
+ * for each 256 values of the tensor, float32; a block that is not finite gets
+ * scales NaN.  Values are taken in memory order, so a tensor and its moments
+ * have to be laid out alike.  step counts from 1; step_device and lr_device, where not NULL, are
+ * one float32 each on the device and take the place of step and lr (for a
+ * captured step).  With sums (of convrot_square_sums) gradients are scaled by
+ * min(1, max_norm / (norm + 1e-6)) as they are read, and the norm is written
+ * to `norm` if that is not NULL.  Gradients are not written.  No tensor may overlap
+ * another.  No reference counterpart.
+ */
+typedef struct {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* scales;
+  int64_t numel;
+} convrot_adamw_tensor;
+typedef struct {
+  double step, lr, beta1, beta2, eps, weight_decay;
+  const float* step_device;
+  const float* lr_device;
+  const double* sums;
+  int64_t sums_count;
+  double max_norm;
+  float* norm;
+} convrot_adamw_options;
+int convrot_adamw(int64_t count, const convrot_adamw_tensor* tensors, int dtype, int state_bits,
+                  const convrot_adamw_options* options, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

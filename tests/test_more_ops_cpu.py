@@ -95,3 +95,71 @@ def test_fp8_python_refusals():
     assert layer.qweight.dtype == layer.scales.dtype == torch.uint8 and layer.bias.dtype == torch.float32
     with pytest.raises(ValueError, match="expected K=300"):
         layer(x[:, :200])
+
+
+# --- AdamW and the gradient norm ----------------------------------------------
+
+
+class _AdamWTensor(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "scales")] + [("numel", ctypes.c_int64)]
+
+
+class _AdamWOptions(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_double) for n in ("step", "lr", "beta1", "beta2", "eps", "weight_decay")] + [
+        ("step_device", ctypes.c_void_p), ("lr_device", ctypes.c_void_p), ("sums", ctypes.c_void_p),
+        ("sums_count", ctypes.c_int64), ("max_norm", ctypes.c_double), ("norm", ctypes.c_void_p)]
+
+
+class _GradTensor(ctypes.Structure):
+    _fields_ = [("grad", ctypes.c_void_p), ("numel", ctypes.c_int64)]
+
+
+def test_adamw_arguments(lib):
+    def run(count=1, dtype=0, bits=8, tensor=None, options=None, how=True):
+        t = dict(param=4096, grad=4096, exp_avg=4096, exp_avg_sq=4096, scales=4096, numel=0)
+        o = dict(step=1.0, lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.0)
+        tensors = (_AdamWTensor * 1)(_AdamWTensor(**{**t, **(tensor or {})}))
+        return lib.convrot_adamw(count, tensors, dtype, bits, ctypes.byref(_AdamWOptions(**{**o, **(options or {})})) if how else None,
+                                 None)
+
+    assert run() == 0 and run(count=0) == 0  # no values: nothing to do
+    assert run(dtype=4) == -1 and run(bits=16) == -1 and "8 or 32" in _err(lib)
+    assert run(count=-1) == -1 and run(how=False) == -1
+    assert lib.convrot_adamw(1, None, 0, 8, ctypes.byref(_AdamWOptions(step=1.0)), None) == -1
+    for bad in (dict(beta1=1.0), dict(beta2=-0.1), dict(eps=-1.0), dict(weight_decay=-1.0), dict(step=0.0), dict(lr=-1.0),
+                dict(lr=float("nan")), dict(sums=4096), dict(sums=4096, sums_count=4, max_norm=-1.0)):
+        assert run(options=bad) == -1
+    for bad in (dict(numel=-1), dict(numel=4, param=None), dict(numel=4, grad=4098), dict(numel=4, exp_avg=None),
+                dict(numel=4, scales=None), dict(numel=4, scales=4097)):
+        assert run(tensor=bad) == -1
+    assert run(bits=32, tensor=dict(numel=4, exp_avg_sq=4098)) == -1 and "misaligned" in _err(lib)
+
+
+def test_norm_arguments(lib):
+    one = (_GradTensor * 1)(_GradTensor(4096, 10))
+    assert lib.convrot_square_sums(1, one, 3, FAKE, 1, None) == -1
+    assert lib.convrot_square_sums(1, one, 0, None, 1, None) == -1 and lib.convrot_square_sums(1, one, 0, FAKE, 0, None) == -1
+    assert lib.convrot_square_sums(1, (_GradTensor * 1)(_GradTensor(None, 10)), 0, FAKE, 1, None) == -1
+    assert lib.convrot_square_sums(1, (_GradTensor * 1)(_GradTensor(4097, 10)), 0, FAKE, 1, None) == -1
+    assert lib.convrot_norm_of_sums(FAKE, 0, FAKE, None) == -1 and lib.convrot_norm_of_sums(None, 1, FAKE, None) == -1
+    assert lib.convrot_square_sums_count(0, None) == 1
+    assert lib.convrot_square_sums_count(1, (_GradTensor * 1)(_GradTensor(None, 256 * 8 * 3 + 1))) == 4
+
+
+def test_optimizer_refusals():
+    p = [torch.nn.Parameter(torch.zeros(10))]
+    for bad in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0), dict(weight_decay=-1.0),
+                dict(max_norm=-1.0)):
+        with pytest.raises(ValueError):
+            cr.AdamW(p, **bad)
+    with pytest.raises(ValueError, match="CUDA"):
+        cr.adamw_step([p[0]], [torch.zeros(10)], [torch.zeros(10)], [torch.zeros(10)], None, 1, lr=1e-3)
+    with pytest.raises(ValueError, match="CUDA"):
+        cr.grad_norm([torch.zeros(3)])
+    with pytest.raises(ValueError, match="at least one"):
+        cr.grad_norm([])
+    with pytest.raises(TypeError):
+        cr.adamw_step(3, [], [], [], None, 1, lr=1e-3)
+    assert cr.adamw_step([], [], [], [], None, 1, lr=1e-3) is None
+    optimizer = cr.AdamW(p)
+    assert optimizer.step() is None and not optimizer.state  # no gradients: nothing happens
