@@ -88,7 +88,7 @@ class AdamW(torch.optim.Optimizer):
     def _start(self, p: torch.Tensor) -> dict:
         state = self.state[p]
         if not state:
-            if torch.cuda.is_current_stream_capturing():
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW starts its moments in its first step: take one before the capture")
             keep = torch.preserve_format
             kind = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
@@ -108,8 +108,6 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         ops, sums, norm = _native.ops(), None, None
-        if not all(group["capturable"] for group in self.param_groups) and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a captured AdamW step needs capturable=True: its step count has to be on the device")
         if self.max_norm is not None:
             grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
             if not grads:
@@ -119,6 +117,8 @@ class AdamW(torch.optim.Optimizer):
             runs: dict = {}  # the parameters by their step, nearly always one
             for p in group["params"]:
                 if p.grad is not None:
+                    if p.is_cuda and not group["capturable"] and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("a captured AdamW step needs capturable=True: its count has to be on the device")
                     state = self._start(p)
                     state["step"] += 1
                     runs.setdefault(0 if group["capturable"] else state["step"], []).append((p, state))
