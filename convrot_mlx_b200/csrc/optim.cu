@@ -13,7 +13,9 @@
 // Memory-bound.  The tensors' addresses and sizes are kernel parameters, so a
 // step needs no table on the device and can be captured.  A warp has 256
 // values at a time, 8 a lane, so the maximum over a block of 8-bit moments is one
-// exchange in the warp.  CTAs take contiguous shares of all tensors' blocks.
+// exchange in the warp.  A CTA's 2048 values are of one tensor, so that all that
+// depends on the tensor is the same in its threads and costs no instruction of
+// theirs.  CTAs take contiguous shares of all tensors' chunks.
 #include "rows.cuh"
 
 namespace convrot {
@@ -23,6 +25,7 @@ constexpr int kBlock = 256;  // values of a warp's turn; of a scale
 constexpr int kLane = kBlock / 32;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kChunk = kThreads * kLane;  // values of a CTA's turn
 constexpr float kTop = 448.0f;         // the largest e4m3 value
 constexpr float kLeast = 0.001953125f;  // the smallest above 0, 2^-9
 
@@ -33,13 +36,13 @@ struct Entry {
   void* v;
   float* scales;
   int64_t n;
-  uint32_t first;    // of the blocks of all tensors, in the order of the table
+  uint32_t first;    // of the chunks of all tensors, in the order of the table
   uint32_t aligned;  // vector accesses may be used
 };
 
 struct Scalars {
   int count;
-  int64_t blocks;
+  uint32_t chunks;
   float decay, beta1, beta2, rest1, rest2, eps, step_size, root;  // root: 1 / sqrt(1 - b2^t)
   // the step and the learning rate where they are on the device
   const float* step;
@@ -61,85 +64,180 @@ struct Table {
   Entry e[CAP];
 };
 
+// ---------------------------------------------------------------------------
+// A thread's 8 values: groups of GROUP consecutive ones, 32 lanes' groups one
+// after another, in the 256 of its warp.  Groups of 4 where something is
+// float32 (16 bytes), else one of 8.
+
+template <typename T, int BITS> constexpr int kGroup = sizeof(T) == 4 || BITS == 32 ? 4 : 8;
+
+template <int GROUP>
+__device__ __forceinline__ int place(int group) {  // the first value of a group in the chunk
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  return warp * kBlock + group * 32 * GROUP + lane * GROUP;
+}
+
+// WHOLE: the chunk is all in the tensor and vector accesses may be used.
+template <typename T, int GROUP, bool WHOLE>
+__device__ __forceinline__ void fetch_values(const T* src, int count, uint32_t (&w)[kLane * sizeof(T) / 4]) {
+  constexpr int kWords = GROUP * sizeof(T) / 4;
+#pragma unroll
+  for (int j = 0; j < kLane / GROUP; ++j) {
+    const int at = place<GROUP>(j);
+    Pack<T, GROUP> g;
+    if constexpr (WHOLE) {
+      g.load_ahead(src + at);
+    } else {
+      g.clear();
+#pragma unroll
+      for (int i = 0; i < GROUP; ++i)
+        if (at + i < count) reinterpret_cast<T*>(g.w)[i] = src[at + i];
+    }
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[j * kWords + i] = g.w[i];
+  }
+}
 template <typename T>
-__device__ __forceinline__ void load(const T* src, int count, bool vec, float (&v)[kLane]) {
-  if (vec) {
-    Pack<T, kLane> p;
-    p.load_ahead(src);
-    p.get(v);
-  } else {
+__device__ __forceinline__ void pairs_of(const uint32_t (&w)[kLane * sizeof(T) / 4], P2 (&v)[kLane / 2]) {
+  float f[kLane];
+  unpack<T, kLane>(w, f);
 #pragma unroll
-    for (int i = 0; i < kLane; ++i) v[i] = i < count ? Elem<T>::to_f(src[i]) : 0.0f;
+  for (int i = 0; i < kLane / 2; ++i) v[i] = p2(f[2 * i], f[2 * i + 1]);
+}
+template <typename T, int GROUP, bool WHOLE>
+__device__ __forceinline__ void store_values(T* dst, int count, const uint32_t (&w)[kLane * sizeof(T) / 4]) {
+  constexpr int kWords = GROUP * sizeof(T) / 4;
+#pragma unroll
+  for (int j = 0; j < kLane / GROUP; ++j) {
+    const int at = place<GROUP>(j);
+    Pack<T, GROUP> g;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) g.w[i] = w[j * kWords + i];
+    if constexpr (WHOLE) {
+      g.store(dst + at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < GROUP; ++i)
+        if (at + i < count) dst[at + i] = reinterpret_cast<const T*>(g.w)[i];
+    }
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store(T* dst, int count, bool vec, const float (&v)[kLane]) {
-  if (vec) {
-    Pack<T, kLane> p;
-    p.set(v);
-    p.store(dst);
-  } else {
+constexpr int kPairs = kLane / 2;
+
+__device__ __forceinline__ void decode(const uint32_t (&w)[2], P2 (&v)[kPairs]) {
 #pragma unroll
-    for (int i = 0; i < kLane; ++i)
-      if (i < count) dst[i] = cvt_out<T>(v[i]);
+  for (int i = 0; i < 2; ++i) {
+    uint32_t lo, hi;
+    asm("{\n\t.reg .b16 a, b;\n\t"
+        "mov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w[i]));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    v[2 * i] = p2(a.x, a.y), v[2 * i + 1] = p2(b.x, b.y);
   }
 }
 
-__device__ __forceinline__ uint2 load_codes(const uint8_t* src, int count, bool vec) {
-  if (vec) return ld_64(src);
-  uint32_t w[2] = {};
+__device__ __forceinline__ void encode(const P2 (&v)[kPairs], uint32_t (&w)[2]) {
 #pragma unroll
-  for (int i = 0; i < kLane; ++i)
-    if (i < count) w[i / 4] |= static_cast<uint32_t>(src[i]) << (8 * (i & 3));
-  return make_uint2(w[0], w[1]);
-}
-
-__device__ __forceinline__ void store_codes8(uint8_t* dst, int count, bool vec, uint2 w) {
-  if (vec) {
-    *reinterpret_cast<uint2*>(dst) = w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < kLane; ++i)
-      if (i < count) dst[i] = static_cast<uint8_t>((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
+  for (int i = 0; i < 2; ++i) {
+    const float2 lo = p2_get(v[2 * i]), hi = p2_get(v[2 * i + 1]);
+    asm("{\n\t.reg .b16 a, b;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\n\t"
+        "mov.b32 %0, {a, b};\n\t}"
+        : "=r"(w[i])
+        : "f"(lo.x), "f"(lo.y), "f"(hi.x), "f"(hi.y));
   }
 }
 
-__device__ __forceinline__ void decode(uint2 w, float (&v)[kLane]) {
-#pragma unroll
-  for (int i = 0; i < kLane / 2; ++i) {
-    const uint16_t pair = static_cast<uint16_t>((i < 2 ? w.x : w.y) >> (16 * (i & 1)));
-    uint32_t h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(pair));
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
+// One instruction each, good to 22 bits; subnormal numbers count as 0.
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rsqrt_approx(float x) {
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
-__device__ __forceinline__ uint2 encode(const float (&v)[kLane]) {
-  uint32_t w[2] = {};
-#pragma unroll
-  for (int i = 0; i < kLane / 2; ++i) {
-    uint16_t pair;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pair) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-    w[i / 2] |= static_cast<uint32_t>(pair) << (16 * (i & 1));
-  }
-  return make_uint2(w[0], w[1]);
+// Square roots: s = v y with y = 1 / sqrt(v) is what divides: 0 has 0 and an
+// infinite v an infinite s, no update.  (v below 2^-126 has too small a root,
+// but eps is what divides there.)
+__device__ __forceinline__ P2 root_of(P2 v, P2& y) {
+  constexpr float kLow = 0x1p-126f, kHigh = 0x1.fffffep127f;
+  const float2 f = p2_get(v);
+  y = p2(rsqrt_approx(fminf(fmaxf(f.x, kLow), kHigh)), rsqrt_approx(fminf(fmaxf(f.y, kLow), kHigh)));
+  return mul(v, y);
+}
+// What is kept in 8 bits is s after one step of Newton's iteration on s * s = v,
+// the residual in one FMA: rounded as a root is but for a last bit (an infinite
+// one becomes NaN).
+__device__ __forceinline__ P2 refined_root(P2 v, P2 y, P2 s) {
+  const P2 half_residual = mul(fma(mul(s, p2(-1.0f, -1.0f)), s, v), p2(0.5f, 0.5f));
+  return fma(half_residual, y, s);
 }
 
 // Codes of the block's values, whose largest magnitude has the bits `top`, and
-// their scale: 0 for a block of zeros, NaN (codes 0) for one that is not finite.
+// their scale: 0 for a block of zeros (and of values below 2^-117, whose scale
+// is no normal number), NaN for one that is not finite, both with codes 0.
+// The quotient by the scale is a product with its reciprocal and one residual
+// correction: rounded as a division is.
 template <bool ROOT>
-__device__ __forceinline__ uint2 quantize(float (&v)[kLane], uint32_t top, float& scale) {
-  scale = top < kInfBits ? __fdiv_rn(__uint_as_float(top), kTop) : __uint_as_float(0x7FC00000u);
-  const bool live = scale > 0.0f;
-#pragma unroll
-  for (int i = 0; i < kLane; ++i) {
-    const float q = live ? __fdiv_rn(v[i], scale) : 0.0f;
-    v[i] = ROOT && live && v[i] > 0.0f ? fmaxf(q, kLeast) : q;
+__device__ __forceinline__ float quantize(const P2 (&v)[kPairs], uint32_t top, uint32_t (&w)[2]) {
+  const float scale = top < kInfBits ? __fmul_rn(__uint_as_float(top), 1.0f / kTop) : __uint_as_float(0x7FC00000u);
+  if (!(scale >= 0x1p-126f)) {
+    w[0] = w[1] = 0;
+    return scale < 0x1p-126f ? 0.0f : scale;
   }
-  return encode(v);
+  const float inv = rcp_approx(scale);
+  const P2 inv2 = p2(inv, inv), by2 = p2(-scale, -scale);
+  P2 q[kPairs];
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    const P2 a = mul(v[i], inv2);
+    q[i] = fma(fma(a, by2, v[i]), inv2, a);
+  }
+  if constexpr (ROOT) {
+    // the least quotient above 0, by its bits less one: seldom one that would become 0
+    uint32_t least = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const float2 f = p2_get(q[i]);
+      least = min(least, min(__float_as_uint(f.x) - 1u, __float_as_uint(f.y) - 1u));
+    }
+    if (least < __float_as_uint(kLeast)) {
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        const float2 f = p2_get(q[i]);
+        q[i] = p2(f.x > 0.0f ? fmaxf(f.x, kLeast) : 0.0f, f.y > 0.0f ? fmaxf(f.y, kLeast) : 0.0f);
+      }
+    }
+  }
+  encode(q, w);
+  return scale;
+}
+
+// The bits of the largest magnitude of the warp's values: those of a NaN, if
+// there is one.
+__device__ __forceinline__ float larger(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t top_of(const P2 (&v)[kPairs]) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    const float2 f = p2_get(v[i]);
+    top = larger(top, f.x, f.y);
+  }
+  return warp_max(abs_bits(top));
 }
 
 // The sum of `count` values in an order that depends on count alone, for all
@@ -157,27 +255,96 @@ __device__ __forceinline__ double sum_all(const double* sums, int count, double*
   return v;
 }
 
-// The last tensor whose first block is not behind `block`; one with no values
-// is never it, since the next begins at the same block.
-template <int CAP>
-__device__ __forceinline__ int find(const Table<CAP>& t, int64_t block) {
-  int lo = 0, hi = t.s.count - 1;
+// The last tensor whose first chunk is not behind `chunk`; one with no values
+// is never it, since the next begins at the same chunk.
+template <typename TABLE>
+__device__ __forceinline__ int find(const TABLE& t, int count, uint32_t chunk) {
+  int lo = 0, hi = count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
-    if (t.e[mid].first <= block) lo = mid;
+    if (t.e[mid].first <= chunk) lo = mid;
     else hi = mid - 1;
   }
   return lo;
 }
 
+template <int BITS> using Moment = typename std::conditional<BITS == 32, float, uint8_t>::type;
+
+// A thread's values of a chunk as they lie in memory.
+template <typename T, int BITS>
+struct Words {
+  uint32_t g[kLane * sizeof(T) / 4], p[kLane * sizeof(T) / 4];
+  uint32_t m[kLane * sizeof(Moment<BITS>) / 4], v[kLane * sizeof(Moment<BITS>) / 4];
+  float2 scales;
+};
+
+// CTAs that an SM holds: 80 or 64 registers a thread, as the words of the chunk ahead ask for.
+template <typename T, int BITS> constexpr int kCtas = sizeof(T) == 4 || BITS == 32 ? 3 : 4;
+
+template <typename T, int BITS, bool WHOLE>
+__device__ __forceinline__ void fetch(const Entry& e, uint32_t in, int count, Words<T, BITS>& w) {
+  using M = Moment<BITS>;
+  constexpr int G = kGroup<T, BITS>;
+  const int64_t base = static_cast<int64_t>(in) * kChunk;
+  fetch_values<T, G, WHOLE>(static_cast<const T*>(e.g) + base, count, w.g);
+  fetch_values<T, G, WHOLE>(static_cast<const T*>(e.p) + base, count, w.p);
+  fetch_values<M, G, WHOLE>(static_cast<const M*>(e.m) + base, count, w.m);
+  fetch_values<M, G, WHOLE>(static_cast<const M*>(e.v) + base, count, w.v);
+  if constexpr (BITS == 8) {
+    // the scales of a warp's block; it may be behind the tensor's end, where all codes are 0
+    const int block = threadIdx.x / 32;
+    uint2 scales = make_uint2(0u, 0u);
+    if (WHOLE || block * kBlock < count) scales = ld_64(e.scales + 2 * (base / kBlock + block));
+    w.scales = make_float2(__uint_as_float(scales.x), __uint_as_float(scales.y));
+  }
+}
+
+template <typename T, int BITS, bool WHOLE>
+__device__ __forceinline__ void leave(const Entry& e, uint32_t in, int count, const uint32_t (&p)[kLane * sizeof(T) / 4],
+                                      const uint32_t (&m)[kLane * sizeof(Moment<BITS>) / 4],
+                                      const uint32_t (&v)[kLane * sizeof(Moment<BITS>) / 4], float2 scales) {
+  using M = Moment<BITS>;
+  constexpr int G = kGroup<T, BITS>;
+  const int64_t base = static_cast<int64_t>(in) * kChunk;
+  store_values<T, G, WHOLE>(static_cast<T*>(e.p) + base, count, p);
+  store_values<M, G, WHOLE>(static_cast<M*>(e.m) + base, count, m);
+  store_values<M, G, WHOLE>(static_cast<M*>(e.v) + base, count, v);
+  if constexpr (BITS == 8) {
+    const int block = threadIdx.x / 32;
+    if (threadIdx.x % 32 == 0 && (WHOLE || block * kBlock < count))
+      *reinterpret_cast<float2*>(e.scales + 2 * (base / kBlock + block)) = scales;
+  }
+}
+
+// Values of the chunk that the tensor has.
+__device__ __forceinline__ int count_of(int64_t n, uint32_t in) {
+  const int64_t left = n - static_cast<int64_t>(in) * kChunk;
+  return left < kChunk ? static_cast<int>(left) : kChunk;
+}
+
 template <typename T, int BITS, int CAP>
-__global__ void __launch_bounds__(kThreads, 3) adamw_kernel(const __grid_constant__ Table<CAP> t) {
+__global__ void __launch_bounds__(kThreads, kCtas<T, BITS>) adamw_kernel(const __grid_constant__ Table<CAP> t) {
   __shared__ double red[kWarps];
   __shared__ float how[3];
+  using M = Moment<BITS>;
   const Scalars& s = t.s;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_wait();
   grid_dependents_launch();
+  const uint32_t per = (s.chunks + gridDim.x - 1) / gridDim.x;
+  uint32_t chunk = per * blockIdx.x;
+  const uint32_t end = min(chunk + per, s.chunks);
+  int at = chunk < end ? find(t, s.count, chunk) : 0, ahead_at = at;
+  Words<T, BITS> next;
+  auto fetch_ahead = [&](uint32_t ahead) {
+    if (ahead >= end) return;
+    while (ahead_at + 1 < s.count && t.e[ahead_at + 1].first <= ahead) ++ahead_at;
+    const Entry& e = t.e[ahead_at];
+    const uint32_t in = ahead - e.first;
+    const int count = count_of(e.n, in);
+    if (e.aligned && count == kChunk) fetch<T, BITS, true>(e, in, count, next);
+    else fetch<T, BITS, false>(e, in, count, next);
+  };
+  fetch_ahead(chunk);
   float step_size = s.step_size, root = s.root, decay = s.decay, coef = 1.0f;
   if (s.step || s.lr) {
     if (threadIdx.x == 0) {
@@ -195,69 +362,65 @@ __global__ void __launch_bounds__(kThreads, 3) adamw_kernel(const __grid_constan
     coef = c >= 1.0f ? 1.0f : c;  // NaN stays
     if (s.norm && blockIdx.x == 0 && threadIdx.x == 0) *s.norm = norm;
   }
-  const int64_t per = (s.blocks + gridDim.x - 1) / gridDim.x;
-  const int64_t begin = per * blockIdx.x, end = begin + per < s.blocks ? begin + per : s.blocks;
-  int64_t block = begin + warp;
-  if (block >= end) return;
-  int at = find(t, block);
-  for (; block < end; block += kWarps) {
-    while (at + 1 < s.count && t.e[at + 1].first <= block) ++at;
+  const P2 coef2 = p2(coef, coef), beta1 = p2(s.beta1, s.beta1), beta2 = p2(s.beta2, s.beta2), rest1 = p2(s.rest1, s.rest1),
+           rest2 = p2(s.rest2, s.rest2), root2 = p2(root, root), eps = p2(s.eps, s.eps), decay2 = p2(decay, decay),
+           minus_step = p2(-step_size, -step_size);
+  for (; chunk < end; ++chunk, at = ahead_at) {
+    P2 p[kPairs], g[kPairs], m[kPairs], v[kPairs], r[kPairs];
+    pairs_of<T>(next.p, p);
+    pairs_of<T>(next.g, g);
+    if constexpr (BITS == 32) {
+      pairs_of<float>(next.m, m);
+      pairs_of<float>(next.v, v);
+    } else {
+      decode(next.m, m);
+      decode(next.v, r);
+    }
+    float2 scales = next.scales;
     const Entry& e = t.e[at];
-    const int64_t i0 = (block - e.first) * kBlock + lane * kLane, left = e.n - i0;
-    const int count = left >= kLane ? kLane : (left > 0 ? static_cast<int>(left) : 0);
-    const bool vec = e.aligned && count == kLane;
-    T* p_at = static_cast<T*>(e.p) + i0;
-    float p[kLane], g[kLane], m[kLane], v[kLane];
-    load(static_cast<const T*>(e.g) + i0, count, vec, g);
-    load(p_at, count, vec, p);
+    fetch_ahead(chunk + 1);
+    if constexpr (BITS == 8) {
+      const P2 ms = p2(scales.x, scales.x), rs = p2(scales.y, scales.y);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        m[i] = mul(m[i], ms);
+        r[i] = mul(r[i], rs);
+        v[i] = mul(r[i], r[i]);
+      }
+    }
+    if (s.sums) {
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) g[i] = mul(g[i], coef2);
+    }
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      m[i] = add(mul(m[i], beta1), mul(g[i], rest1));
+      v[i] = add(mul(v[i], beta2), mul(mul(g[i], g[i]), rest2));
+      P2 y;
+      r[i] = root_of(v[i], y);
+      const float2 den = p2_get(fma(r[i], root2, eps));
+      if constexpr (BITS == 8) r[i] = refined_root(v[i], y, r[i]);
+      p[i] = fma(mul(m[i], minus_step), p2(rcp_approx(den.x), rcp_approx(den.y)), mul(p[i], decay2));
+    }
+    Pack<T, kLane> out;
+    out.set_lanes(p);
+    uint32_t m_words[kLane * sizeof(M) / 4], v_words[kLane * sizeof(M) / 4];
     if constexpr (BITS == 32) {
-      load(static_cast<const float*>(e.m) + i0, count, vec, m);
-      load(static_cast<const float*>(e.v) + i0, count, vec, v);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        const float2 a = p2_get(m[i]), b = p2_get(v[i]);
+        m_words[2 * i] = __float_as_uint(a.x), m_words[2 * i + 1] = __float_as_uint(a.y);
+        v_words[2 * i] = __float_as_uint(b.x), v_words[2 * i + 1] = __float_as_uint(b.y);
+      }
     } else {
-      const uint2 mc = load_codes(static_cast<const uint8_t*>(e.m) + i0, count, vec);
-      const uint2 rc = load_codes(static_cast<const uint8_t*>(e.v) + i0, count, vec);
-      const float* scales = e.scales + 2 * (block - e.first);
-      const float ms = ld_f32(scales), rs = ld_f32(scales + 1);
-      decode(mc, m);
-      decode(rc, v);
-#pragma unroll
-      for (int i = 0; i < kLane; ++i) {
-        m[i] = __fmul_rn(m[i], ms);
-        const float r = __fmul_rn(v[i], rs);
-        v[i] = __fmul_rn(r, r);
-      }
+      // values behind the tensor's end have moments of 0
+      scales.x = quantize<false>(m, top_of(m), m_words);
+      scales.y = quantize<true>(r, top_of(r), v_words);
     }
-    float r[kLane];
-#pragma unroll
-    for (int i = 0; i < kLane; ++i) {
-      if (s.sums) g[i] = __fmul_rn(g[i], coef);
-      m[i] = __fadd_rn(__fmul_rn(m[i], s.beta1), __fmul_rn(g[i], s.rest1));
-      v[i] = __fadd_rn(__fmul_rn(v[i], s.beta2), __fmul_rn(__fmul_rn(g[i], g[i]), s.rest2));
-      r[i] = __fsqrt_rn(v[i]);
-      p[i] = __fsub_rn(__fmul_rn(p[i], decay),
-                       __fdividef(__fmul_rn(step_size, m[i]), __fadd_rn(__fmul_rn(r[i], root), s.eps)));
-    }
-    store(p_at, count, vec, p);
-    if constexpr (BITS == 32) {
-      store(static_cast<float*>(e.m) + i0, count, vec, m);
-      store(static_cast<float*>(e.v) + i0, count, vec, v);
-    } else {
-      uint32_t m_top = 0, r_top = 0;
-#pragma unroll
-      for (int i = 0; i < kLane; ++i) {
-        m_top = max(m_top, i < count ? abs_bits(m[i]) : 0u);
-        r_top = max(r_top, i < count ? abs_bits(r[i]) : 0u);
-      }
-      float ms, rs;
-      const uint2 mc = quantize<false>(m, warp_max(m_top), ms), rc = quantize<true>(r, warp_max(r_top), rs);
-      store_codes8(static_cast<uint8_t*>(e.m) + i0, count, vec, mc);
-      store_codes8(static_cast<uint8_t*>(e.v) + i0, count, vec, rc);
-      if (lane == 0) {
-        float* scales = e.scales + 2 * (block - e.first);
-        scales[0] = ms;
-        scales[1] = rs;
-      }
-    }
+    const uint32_t in = chunk - e.first;
+    const int count = count_of(e.n, in);
+    if (e.aligned && count == kChunk) leave<T, BITS, true>(e, in, count, out.w, m_words, v_words, scales);
+    else leave<T, BITS, false>(e, in, count, out.w, m_words, v_words, scales);
   }
 }
 
@@ -277,10 +440,12 @@ struct NormEntry {
 template <int CAP>
 struct NormTable {
   int count, add;  // add: to what an earlier launch has left
-  int64_t blocks;
+  uint32_t chunks;
   double* sums;
   NormEntry e[CAP];
 };
+
+constexpr int kAhead = 4;  // chunks in flight
 
 template <typename T, int CAP>
 __global__ void __launch_bounds__(kThreads) square_sums(const __grid_constant__ NormTable<CAP> t) {
@@ -288,34 +453,55 @@ __global__ void __launch_bounds__(kThreads) square_sums(const __grid_constant__ 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_dependency_wait();
   grid_dependents_launch();
-  const int64_t per = (t.blocks + gridDim.x - 1) / gridDim.x;
-  const int64_t begin = per * blockIdx.x, end = begin + per < t.blocks ? begin + per : t.blocks;
-  int64_t block = begin + warp;
+  const uint32_t per = (t.chunks + gridDim.x - 1) / gridDim.x;
+  uint32_t chunk = min(per * blockIdx.x, t.chunks);
+  const uint32_t end = min(chunk + per, t.chunks);
   double acc = 0.0;
-  if (block < end) {
-    int at = 0, hi = t.count - 1;
-    while (at < hi) {
-      const int mid = (at + hi + 1) / 2;
-      if (t.e[mid].first <= block) at = mid;
-      else hi = mid - 1;
-    }
-    for (; block < end; block += kWarps) {
-      while (at + 1 < t.count && t.e[at + 1].first <= block) ++at;
-      const NormEntry& e = t.e[at];
-      const int64_t i0 = (block - e.first) * kBlock + lane * kLane, left = e.n - i0;
-      const int count = left >= kLane ? kLane : (left > 0 ? static_cast<int>(left) : 0);
-      float g[kLane];
-      load(static_cast<const T*>(e.g) + i0, count, e.aligned && count == kLane, g);
-      float sum = 0.0f;
+  if (chunk < end) {
+    int at = find(t, t.count, chunk);
+    for (; chunk < end; chunk += kAhead) {
+      constexpr int G = sizeof(T) == 4 ? 4 : 8;
+      Pack<T, G> w[kAhead][kLane / G];
 #pragma unroll
-      for (int i = 0; i < kLane; ++i) sum = __fmaf_rn(g[i], g[i], sum);
-      double part = sum;
-      if (!(sum < 0x1p120f && sum > 0x1p-90f)) {
-        part = 0.0;
+      for (int j = 0; j < kAhead; ++j) {
 #pragma unroll
-        for (int i = 0; i < kLane; ++i) part += static_cast<double>(g[i]) * static_cast<double>(g[i]);
+        for (int i = 0; i < kLane / G; ++i) w[j][i].clear();
+        if (chunk + j >= end) continue;
+        while (at + 1 < t.count && t.e[at + 1].first <= chunk + j) ++at;
+        const NormEntry& e = t.e[at];
+        const uint32_t in = chunk + j - e.first;
+        const T* src = static_cast<const T*>(e.g) + static_cast<int64_t>(in) * kChunk;
+        const int count = count_of(e.n, in);
+        if (e.aligned && count == kChunk) {
+#pragma unroll
+          for (int i = 0; i < kLane / G; ++i) w[j][i].load_ahead(src + place<G>(i));
+        } else {
+#pragma unroll
+          for (int i = 0; i < kLane / G; ++i) w[j][i].load_part(src + place<G>(i), count - place<G>(i));
+        }
       }
-      acc += part;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kLane / G; ++i) {
+          float g[G];
+          w[j][i].get(g);
+#pragma unroll
+          for (int k = 0; k < G; ++k) sum = __fmaf_rn(g[k], g[k], sum);
+        }
+        if (sum < 0x1p120f && sum > 0x1p-90f) {
+          acc += static_cast<double>(sum);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kLane / G; ++i) {
+            float g[G];
+            w[j][i].get(g);
+#pragma unroll
+            for (int k = 0; k < G; ++k) acc += static_cast<double>(g[k]) * static_cast<double>(g[k]);
+          }
+        }
+      }
     }
   }
 #pragma unroll
@@ -361,14 +547,14 @@ int launch(K kernel, int64_t ctas, const A& args, cudaStream_t s, const char* wh
   return check_launch(what);
 }
 
-int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
+int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
 
 template <typename T, int BITS, int CAP>
 int adamw_part(const Scalars& s, const convrot_adamw_tensor* tensors, int count, cudaStream_t stream) {
   Table<CAP> t;
   t.s = s;
   t.s.count = count;
-  int64_t blocks = 0;
+  int64_t chunks = 0;
   for (int i = 0; i < count; ++i) {
     const convrot_adamw_tensor& c = tensors[i];
     const uintptr_t moments = BITS == 8 ? 8 : 16;
@@ -376,13 +562,13 @@ int adamw_part(const Scalars& s, const convrot_adamw_tensor* tensors, int count,
                          aligned_to(c.exp_avg_sq, moments);
     Entry& e = t.e[i];
     e.p = c.param, e.g = c.grad, e.m = c.exp_avg, e.v = c.exp_avg_sq, e.scales = c.scales, e.n = c.numel;
-    e.first = static_cast<uint32_t>(blocks), e.aligned = aligned;
-    blocks += blocks_of(c.numel);
+    e.first = static_cast<uint32_t>(chunks), e.aligned = aligned;
+    chunks += chunks_of(c.numel);
   }
-  if (blocks == 0) return CONVROT_OK;
-  CONVROT_REQUIRE(blocks < (1LL << 32), CONVROT_ERR_UNSUPPORTED, "tensors too large");
-  t.s.blocks = blocks;
-  const int64_t ctas = (blocks + kWarps - 1) / kWarps, most = 3 * static_cast<int64_t>(device_sm_count());
+  if (chunks == 0) return CONVROT_OK;
+  CONVROT_REQUIRE(chunks < (1LL << 31), CONVROT_ERR_UNSUPPORTED, "tensors too large");
+  t.s.chunks = static_cast<uint32_t>(chunks);
+  const int64_t ctas = chunks, most = kCtas<T, BITS> * static_cast<int64_t>(device_sm_count());
   return launch(adamw_kernel<T, BITS, CAP>, ctas < most ? ctas : most, t, stream, "adamw step");
 }
 
@@ -406,14 +592,14 @@ template <typename T, int CAP>
 int sums_part(const convrot_grad_tensor* tensors, int count, int64_t ctas, double* sums, bool add, cudaStream_t stream) {
   NormTable<CAP> t;
   t.count = count, t.add = add, t.sums = sums;
-  int64_t blocks = 0;
+  int64_t chunks = 0;
   for (int i = 0; i < count; ++i) {
     t.e[i].g = tensors[i].grad, t.e[i].n = tensors[i].numel;
-    t.e[i].first = static_cast<uint32_t>(blocks), t.e[i].aligned = aligned_to(tensors[i].grad, 16);
-    blocks += blocks_of(tensors[i].numel);
+    t.e[i].first = static_cast<uint32_t>(chunks), t.e[i].aligned = aligned_to(tensors[i].grad, 16);
+    chunks += chunks_of(tensors[i].numel);
   }
-  CONVROT_REQUIRE(blocks < (1LL << 32), CONVROT_ERR_UNSUPPORTED, "tensors too large");
-  t.blocks = blocks;
+  CONVROT_REQUIRE(chunks < (1LL << 31), CONVROT_ERR_UNSUPPORTED, "tensors too large");
+  t.chunks = static_cast<uint32_t>(chunks);
   return launch(square_sums<T, CAP>, ctas, t, stream, "sums of squares");
 }
 
@@ -437,9 +623,9 @@ extern "C" {
 int64_t convrot_square_sums_count(int64_t count, const convrot_grad_tensor* tensors) {
   using namespace convrot;
   if (count < 0 || (count > 0 && !tensors)) return 1;
-  int64_t blocks = 0;
-  for (int64_t i = 0; i < count; ++i) blocks += tensors[i].numel > 0 ? optim::blocks_of(tensors[i].numel) : 0;
-  const int64_t ctas = (blocks + optim::kWarps - 1) / optim::kWarps, most = 4 * static_cast<int64_t>(device_sm_count());
+  int64_t chunks = 0;
+  for (int64_t i = 0; i < count; ++i) chunks += tensors[i].numel > 0 ? optim::chunks_of(tensors[i].numel) : 0;
+  const int64_t ctas = chunks, most = 4 * static_cast<int64_t>(device_sm_count());
   return ctas < 1 ? 1 : (ctas < most ? ctas : most);
 }
 
@@ -498,7 +684,7 @@ int convrot_adamw(int64_t count, const convrot_adamw_tensor* tensors, int dtype,
                                                       aligned_to(t.grad, e) && aligned_to(t.exp_avg, moment) &&
                                                       aligned_to(t.exp_avg_sq, moment))),
                     CONVROT_ERR_INVALID, "tensor %lld: null or misaligned pointer, or negative size", static_cast<long long>(i));
-    CONVROT_REQUIRE(state_bits == 32 || t.numel == 0 || (t.scales && aligned_to(t.scales, 4)), CONVROT_ERR_INVALID,
+    CONVROT_REQUIRE(state_bits == 32 || t.numel == 0 || (t.scales && aligned_to(t.scales, 8)), CONVROT_ERR_INVALID,
                     "tensor %lld: 8-bit moments need their scales", static_cast<long long>(i));
   }
   const double c1 = 1.0 - pow(o->beta1, o->step), c2 = 1.0 - pow(o->beta2, o->step);
