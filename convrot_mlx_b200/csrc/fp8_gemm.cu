@@ -60,10 +60,26 @@ __device__ __forceinline__ void mma_mx(uint32_t d_tmem, uint64_t a_desc, uint64_
       : "memory");
 }
 
+__device__ __forceinline__ void mma_mx_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t a_scale, uint32_t b_scale, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scale), "r"(b_scale), "r"(accumulate)
+      : "memory");
+}
+
 // 512 bytes of scales (32 rows of 16, contiguous) to 4 columns of tensor
 // memory, the same for each quarter of its lanes.
 __device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t saddr) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc(saddr, 16, 128, 0))
+               : "memory");
+}
+
+// The same in both CTAs of a pair, each from its own shared memory.
+__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint32_t saddr) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc(saddr, 16, 128, 0))
                : "memory");
 }
 
@@ -78,16 +94,302 @@ __device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int b0, int b
   return __funnelshift_r(lo, hi, 8 * (b0 & 3));
 }
 
-// The scales of output block `nb` of the weight for K blocks b0 to b0 + 3 as a
-// word, in every lane of the warp.
-__device__ __forceinline__ uint32_t weight_word(const Params& p, int nb, int b0, int blocks) {
-  const int lane = threadIdx.x & 31, b = b0 + (lane & 3);
-  const uint32_t v = b < blocks ? ld_8(p.wscales + nb * p.ws_n + b * p.ws_k) : 0x7Fu;
+// The scales of output block `nb` of the weight for K blocks b0 to b0 + 3: a
+// byte in each of four lanes, and from these the word in every lane of the warp.
+__device__ __forceinline__ uint32_t weight_byte(const Params& p, int nb, int b0, int blocks) {
+  const int b = b0 + (threadIdx.x & 3);
+  return b < blocks && nb * 128 < p.n ? ld_8(p.wscales + nb * p.ws_n + b * p.ws_k) : 0x7Fu;
+}
+__device__ __forceinline__ uint32_t word_of(uint32_t byte) {
   uint32_t word = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) word |= __shfl_sync(0xFFFFFFFFu, v, i) << (8 * i);
+  for (int i = 0; i < 4; ++i) word |= __shfl_sync(0xFFFFFFFFu, byte, i) << (8 * i);
   return word;
 }
+
+// ===========================================================================
+// Pair kernel.  CTA pairs (cta_group::2), 256 tokens x 256 channels a tile,
+// persistent.  Each CTA holds 128 tokens and 128 channels of a tile:
+//   warp 0   activation producer, warp 2 weight producer: lane s issues the
+//            16 KB box of ring slot s (copies of one thread are served one
+//            after another), completing on the leader's full[s]
+//   warp 1   leader: MMA issuer (M = 256, N = 256); both: TMEM owner
+//   warp 3   scales of this CTA's 128 tokens and of the tile's 256 channels,
+//            which both CTAs need
+//   warps 4-11  epilogue of this CTA's 128 rows: warp w reads TMEM lanes
+//            32 (w % 4) .. + 31, columns 128 ((w - 4) / 4) .. + 127
+// Tensor memory has 512 columns: two accumulators of 256 that share 32, and
+// two sets of scales of 12 (4 for the tokens, 8 for the channels).  The epilogue
+// reads the shared columns first, and with them free the next tile may begin.
+// ===========================================================================
+namespace pair {
+
+constexpr int kTile = 256;
+constexpr int kBand = 16;
+constexpr int kStages = 6;
+constexpr int kOpBytes = 128 * kBK;  // one operand's half tile of a stage
+constexpr int kWarpA = 0, kWarpMma = 1, kWarpB = 2, kWarpS = 3, kWarpE0 = 4, kEWarps = 8;
+constexpr int kThreads = (kWarpE0 + kEWarps) * 32;
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kSecond = 224;    // column of the second accumulator
+constexpr uint32_t kScaleCol = 480;  // 16 columns for each of two sets of scales
+constexpr int kSetBytes = 3 * kScaleBytes;
+constexpr int kVecBytes = kEWarps * 128 * 4;  // bias of a warp's 128 columns
+
+struct alignas(8) Bars {
+  uint64_t full[kStages];
+  uint64_t empty[kStages];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint64_t shared_empty;
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  int err;
+};
+
+constexpr size_t kSmem = 1024 + kStages * 2 * kOpBytes + 2 * kSetBytes + kEWarps * kChunkBytes + kVecBytes + sizeof(Bars);
+static_assert(kSmem <= 232448, "shared memory budget");
+
+template <int LAYOUT, typename TOut>
+__global__ void __launch_bounds__(kThreads, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + kStages * kOpBytes;
+  uint8_t* sS = sB + kStages * kOpBytes;  // each set: tokens, channels 0-127, channels 128-255
+  uint8_t* stage_out = sS + 2 * kSetBytes;
+  float* vecs = reinterpret_cast<float*>(stage_out + kEWarps * kChunkBytes);
+  Bars* bars = reinterpret_cast<Bars*>(reinterpret_cast<uint8_t*>(vecs) + kVecBytes);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();  // 0 = leader
+  const int pair_id = blockIdx.x >> 1;
+  const int num_pairs = gridDim.x >> 1;
+  const int m_tiles = (p.m + kTile - 1) / kTile, n_tiles = (p.n + kTile - 1) / kTile;
+  const int num_tiles = m_tiles * n_tiles;
+  const int k_stages = (p.k + kBK - 1) / kBK;
+  // Tiles in bands of kBand token tiles, within a band all of these for one
+  // channel tile, then the next: the tiles in work at one time then share
+  // about as many rows of either operand in L2.
+  auto place = [&](int tile, int& m_blk, int& n_blk) {
+    const int band = tile / (kBand * n_tiles), first = band * kBand;
+    const int rows = min(kBand, m_tiles - first), at = tile - first * n_tiles;
+    n_blk = at / rows;
+    m_blk = first + at - n_blk * rows;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&bars->full[s], 3);  // the copies, and the scales of either CTA
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars->acc_full[b], 1);
+      mbar_init(&bars->acc_empty[b], 2 * kEWarps);
+    }
+    mbar_init(&bars->shared_empty, kEWarps);  // four warps of each CTA
+    mbar_init(&bars->mma_done, 1);
+    bars->err = 0;
+    fence_mbar_init();
+    prefetch_tensormap(&tmap_a);
+    prefetch_tensormap(&tmap_b);
+  }
+  if (warp == kWarpMma) {
+    tmem_alloc_pair(&bars->tmem_base, kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();  // barriers of both CTAs exist before any signal crosses
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+  grid_dependency_wait();
+  grid_dependents_launch();
+
+  if (warp == kWarpA || warp == kWarpB) {
+    if (lane < kStages) {
+      const uint32_t lead_full = mapa_shared(&bars->full[lane], 0);
+      int g = 0;
+      bool ok = true;
+      for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs) {
+        int m_blk, n_blk;
+        place(tile, m_blk, n_blk);
+        const int row = m_blk * kTile + 128 * rank, col = n_blk * kTile + 128 * rank;
+        for (int ks = 0; ks < k_stages; ++ks, ++g) {
+          if (g % kStages != lane) continue;
+          if (!wait(&bars->empty[lane], ((g / kStages) & 1) ^ 1, &bars->err, 81)) { ok = false; break; }
+          if (warp == kWarpA) {
+            if (rank == 0) mbar_arrive_expect_tx(&bars->full[lane], 4 * kOpBytes);
+            tma_load_2d_pair(sA + lane * kOpBytes, &tmap_a, lead_full, ks * kBK, row);
+          } else if (LAYOUT == CONVROT_LAYOUT_NK) {
+            tma_load_2d_pair(sB + lane * kOpBytes, &tmap_b, lead_full, ks * kBK, col);
+          } else {
+            tma_load_2d_pair(sB + lane * kOpBytes, &tmap_b, lead_full, col, ks * kBK);
+          }
+        }
+      }
+      if (!ok) settle();
+    }
+  } else if (warp == kWarpS) {
+    // Each group's words are on their way while the group before is written: a
+    // trip to memory takes as long as the MMAs of two to three stages.  A
+    // stage is full only with this warp's arrival too, so that the MMA thread
+    // has nothing more to wait for or to commit than without scales.
+    const uint32_t lead_full0 = mapa_shared(&bars->full[0], 0);
+    struct {
+      uint32_t x[4], w0, w1;
+    } now, next = {};
+    int ahead = pair_id, b0 = 0;
+    auto load_next = [&] {  // of group b0 of tile `ahead`, and on to the one after
+      if (ahead >= num_tiles) return;
+      int m_blk, n_blk;
+      place(ahead, m_blk, n_blk);
+      const int row = m_blk * kTile + 128 * rank + lane;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        next.x[j] = row + 32 * j < p.m ? scale_word(p.xscales + (row + 32 * j) * p.xs_stride, b0, k_stages) : kOneWord;
+      next.w0 = weight_byte(p, 2 * n_blk, b0, k_stages);
+      next.w1 = weight_byte(p, 2 * n_blk + 1, b0, k_stages);
+      b0 += kGroup;
+      if (b0 >= k_stages) {
+        b0 = 0;
+        ahead += num_pairs;
+      }
+    };
+    auto wait_empty = [&](int stage) {  // whose MMAs are complete
+      const bool ok = wait(&bars->empty[stage % kStages], (stage / kStages) & 1, &bars->err, 86);
+      return !__any_sync(0xFFFFFFFFu, !ok);
+    };
+    load_next();
+    int g = 0, group = 0, before = 0;  // stages of the group before
+    bool ok = true;
+    for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs) {
+      for (int ks = 0; ks < k_stages; ++ks, ++g) {
+        if (g >= kStages && !wait_empty(g - kStages)) { ok = false; break; }
+        if (ks % kGroup == 0) {
+          now = next;
+          load_next();
+          // the set's last group is the one two before
+          if (group >= 2 && !wait_empty(g - before - 1)) { ok = false; break; }
+          const uint32_t w0 = word_of(now.w0), w1 = word_of(now.w1);
+          const uint32_t at = smem_u32(sS) + (group & 1) * kSetBytes + lane * 16;
+          sts128(at, now.x[0], now.x[1], now.x[2], now.x[3]);
+          sts128(at + kScaleBytes, w0, w0, w0, w0);
+          sts128(at + 2 * kScaleBytes, w1, w1, w1, w1);
+          fence_proxy_async_smem();
+          __syncwarp();
+          ++group;
+          before = min(kGroup, k_stages - ks);
+        }
+        // a release of all memory at cluster scope would take a microsecond: only shared memory is published
+        if (lane == 0) mbar_arrive_cluster_publish_smem(lead_full0 + (g % kStages) * 8);
+      }
+    }
+  } else if (warp == kWarpMma) {
+    if (rank == 0 && lane == 0) {
+      constexpr uint32_t idesc = idesc_mx(kTile, kTile, false, LAYOUT == CONVROT_LAYOUT_KN);
+      const uint32_t a_base = smem_u32(sA), b_base = smem_u32(sB), s_base = smem_u32(sS);
+      int g = 0, local = 0, group = 0;
+      bool ok = true;
+      for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs, ++local) {
+        const int buf = local & 1;
+        if (!wait(&bars->acc_empty[buf], ((local >> 1) & 1) ^ 1, &bars->err, 82)) break;
+        if (local > 0 && !wait(&bars->shared_empty, (local - 1) & 1, &bars->err, 82)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + (buf ? kSecond : 0);
+        for (int ks = 0; ks < k_stages; ++ks, ++g) {
+          const int slot = g % kStages;
+          const uint32_t a_scale = tmem_base + kScaleCol + (group & 1) * 16, b_scale = a_scale + 4;
+          if (!wait(&bars->full[slot], (g / kStages) & 1, &bars->err, 83)) { ok = false; break; }
+          tc_fence_after();
+          if (ks % kGroup == 0) {
+            const uint32_t from = s_base + (group & 1) * kSetBytes;
+            copy_scales_pair(a_scale, from);
+            copy_scales_pair(b_scale, from + kScaleBytes);
+            copy_scales_pair(b_scale + 4, from + 2 * kScaleBytes);
+          }
+          const uint32_t a_addr = a_base + slot * kOpBytes, b_addr = b_base + slot * kOpBytes;
+          const uint32_t id = idesc_byte(idesc, ks % kGroup);
+#pragma unroll
+          for (int j = 0; j < kBK / 32; ++j) {  // K beyond the end is zero in both operands
+            const uint64_t adesc = smem_desc(a_addr + j * 32, 16, 1024, 2);
+            const uint64_t bdesc = LAYOUT == CONVROT_LAYOUT_NK ? smem_desc(b_addr + j * 32, 16, 1024, 2)
+                                                               : smem_desc(b_addr + j * 4096, kOpBytes, 1024, 2);
+            mma_mx_pair(d_tmem, adesc, bdesc, id, a_scale, b_scale, (ks | j) != 0 ? 1u : 0u);
+          }
+          mma_commit_pair_multicast(&bars->empty[slot], 0x3);
+          if (ks % kGroup == kGroup - 1 || ks == k_stages - 1) ++group;
+        }
+        if (!ok) break;
+        mma_commit_pair_multicast(&bars->acc_full[buf], 0x3);
+      }
+      // every MMA issued above finishes before the pair's TMEM is released
+      mma_commit_pair_multicast(&bars->mma_done, 0x1);
+      wait(&bars->mma_done, 0, &bars->err, 87);
+    }
+  } else if (warp >= kWarpE0) {
+    const int ew = warp - kWarpE0, quarter = warp & 3, half = ew >> 2;
+    float* sbias = vecs + ew * 128;
+    const uint32_t lead_empty0 = mapa_shared(&bars->acc_empty[0], 0), lead_shared = mapa_shared(&bars->shared_empty, 0);
+    int local = 0;
+    for (int tile = pair_id; tile < num_tiles; tile += num_pairs, ++local) {
+      const int buf = local & 1;
+      int m_blk, n_blk;
+      place(tile, m_blk, n_blk);
+      const int row0 = m_blk * kTile + 128 * rank + quarter * 32, col0 = n_blk * kTile + 128 * half;
+      __syncwarp();  // the previous tile's reads of the bias are done
+      for (int j = lane; j < 128; j += 32) sbias[j] = col0 + j < p.n && p.bias ? ld_f32(p.bias + col0 + j) : 0.0f;
+      __syncwarp();
+      if (!wait(&bars->acc_full[buf], (local >> 1) & 1, &bars->err, 85)) break;
+      tc_fence_after();
+      const uint32_t t_row =
+          tmem_base + ((static_cast<uint32_t>(quarter) * 32u) << 16) + (buf ? kSecond : 0) + 128 * half;
+      // the columns that both accumulators have: the last 32 of the first, the first 32 of the second
+      const bool shared = half != buf;
+      for (int i = 0; i < 4; ++i) {
+        const int c = shared && !buf ? (i + 3) & 3 : i;
+        const bool in = col0 + 32 * c < p.n;  // uniform across the warp
+        uint32_t r[32];
+        if (in) {
+          __syncwarp();
+          tmem_ld_32x32b_x32(t_row + c * 32, r);
+          tmem_ld_wait();
+        }
+        if (shared && i == 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_publish_smem(lead_shared);
+        }
+        if (!in) continue;
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 b4 = *reinterpret_cast<const float4*>(sbias + c * 32 + j);
+          const float bv[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+          for (int u = 0; u < 4; ++u) v[j + u] = __fadd_rn(__uint_as_float(r[j + u]), bv[u]);
+        }
+        store_rows(v, stage_out + ew * kChunkBytes, static_cast<TOut*>(p.out), row0, col0 + c * 32, p.m, p.n);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(lead_empty0 + buf * 8);
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();  // no CTA leaves while its partner may still touch its shared memory or TMEM
+  tc_fence_after();
+  if (warp == kWarpMma) {
+    __syncwarp();
+    tmem_dealloc_pair(tmem_base, kTmemCols);
+  }
+  if (threadIdx.x == 0 && bars->err) atomicCAS(p.err_word, 0, bars->err);
+}
+
+}  // namespace pair
 
 // ===========================================================================
 // Swap kernel.  One tile of 128 channels (the MMA's M side) x BT tokens and one
@@ -224,17 +526,26 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else if (warp == 3) {
     constexpr int kRows = (BT + 31) / 32;  // of a lane
-    for (int b0 = k_lo, i = 0; b0 < k_hi; b0 += kGroup, ++i) {
-      const uint32_t w = weight_word(p, n0 / 128, b0, k_stages);
-      uint32_t x[4] = {kOneWord, kOneWord, kOneWord, kOneWord};
+    struct {
+      uint32_t x[4], w;
+    } now, next = {{kOneWord, kOneWord, kOneWord, kOneWord}, 0};
+    auto load_next = [&](int b0) {  // while the group before is written
+      if (b0 >= k_hi) return;
 #pragma unroll
       for (int j = 0; j < kRows; ++j)
-        if (m0 + lane + 32 * j < p.m) x[j] = scale_word(p.xscales + (m0 + lane + 32 * j) * p.xs_stride, b0, k_stages);
+        if (m0 + lane + 32 * j < p.m) next.x[j] = scale_word(p.xscales + (m0 + lane + 32 * j) * p.xs_stride, b0, k_stages);
+      next.w = weight_byte(p, n0 / 128, b0, k_stages);
+    };
+    load_next(k_lo);
+    for (int b0 = k_lo, i = 0; b0 < k_hi; b0 += kGroup, ++i) {
+      now = next;
+      load_next(b0 + kGroup);
       const bool ok = wait(&bars->sf_empty[i & 1], ((i >> 1) & 1) ^ 1, &bars->err, 95);
       if (__any_sync(0xFFFFFFFFu, !ok)) break;
       const uint32_t at = smem_u32(sS) + (i & 1) * 2 * kScaleBytes + lane * 16;
+      const uint32_t w = word_of(now.w);
       sts128(at, w, w, w, w);
-      sts128(at + kScaleBytes, x[0], x[1], x[2], x[3]);
+      sts128(at + kScaleBytes, now.x[0], now.x[1], now.x[2], now.x[3]);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->sf_full[i & 1]);
@@ -374,6 +685,35 @@ int weight_map(CUtensorMap* map, const Operands& o, int layout, const Params& p)
                                      : tile_map(map, o.weight, p.n, p.k, o.weight_stride, 128);
 }
 
+template <int LAYOUT, typename TOut>
+int launch_pair(const Operands& o, const Params& p, cudaStream_t stream) {
+  CUtensorMap map_a, map_b;
+  int rc = tile_map(&map_a, o.act, p.k, p.m, o.act_stride, 128);
+  if (rc == CONVROT_OK) rc = weight_map(&map_b, o, LAYOUT, p);
+  if (rc != CONVROT_OK) return rc;
+  auto kernel = pair::pair_kernel<LAYOUT, TOut>;
+  CONVROT_CUDA_CHECK(
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(pair::kSmem)));
+  const int64_t tiles = static_cast<int64_t>((p.m + 255) / 256) * ((p.n + 255) / 256);
+  const int most = device_sm_count() / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * static_cast<unsigned>(tiles < most ? tiles : most), 1, 1);
+  cfg.blockDim = dim3(pair::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = pair::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see grid_dependency_wait
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  CONVROT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, map_a, map_b, p));
+  return check_launch("8-bit float pair gemm");
+}
+
 template <int LAYOUT, typename TOut, int BT>
 int launch_swap(const Operands& o, const Params& p, int ranks, cudaStream_t stream) {
   CUtensorMap map_x, map_w;
@@ -402,10 +742,41 @@ int launch_swap(const Operands& o, const Params& p, int ranks, cudaStream_t stre
   return check_launch("8-bit float swap gemm");
 }
 
+// Expected times of the two tile kernels in microseconds.
+double pair_time(const Params& p, int sms) {
+  const int64_t tiles = static_cast<int64_t>((p.m + 255) / 256) * ((p.n + 255) / 256), pairs = sms / 2;
+  const int64_t waves = (tiles + pairs - 1) / pairs, stages = (p.k + kBK - 1) / kBK;
+  return 6.0 + static_cast<double>(waves * stages) * (waves > 1 ? 0.45 : 0.36);
+}
+
+// The best split of K over 1, 2, 4 or 8 CTAs, and its time.
+double swap_time(const Params& p, int bt, int sms, int* ranks) {
+  const int64_t tiles = static_cast<int64_t>((p.n + 127) / 128) * ((p.m + bt - 1) / bt);
+  const int64_t stages = (p.k + kBK - 1) / kBK;
+  double best = 1e30;
+  for (int r = 1; r <= swap::kMaxCluster && r <= stages; r *= 2) {
+    const int64_t ctas = tiles * r, at_once = r < 4 ? 2 * sms : 2 * sms / 8 * 7;
+    const int64_t waves = (ctas + at_once - 1) / at_once;
+    const bool shared = ctas > sms;
+    const double stage = shared ? std::max(0.46, 2.0 * (swap::kWBytes + bt * kBK) / 125e3) : 0.46;
+    const double exchange = r > 1 ? 0.9 + 0.08 * r + bt * (0.006 + 0.001 * r) : 0.0;
+    const double t = static_cast<double>(waves) * (2.8 + 0.012 * bt + static_cast<double>((stages + r - 1) / r) * stage +
+                                                   exchange + (shared ? 0.4 + 0.007 * bt : 0.0));
+    if (t < best) {
+      best = t;
+      *ranks = r;
+    }
+  }
+  return best;
+}
+
 template <int LAYOUT, typename TOut>
 int launch(const Operands& o, const Params& p, cudaStream_t s) {
+  const int sms = device_sm_count();
   const int bt = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
   int ranks = 1;
+  const double swap_us = swap_time(p, bt, sms, &ranks);
+  if (pair_time(p, sms) < swap_us) return launch_pair<LAYOUT, TOut>(o, p, s);
   switch (bt) {
     case 16: return launch_swap<LAYOUT, TOut, 16>(o, p, ranks, s);
     case 32: return launch_swap<LAYOUT, TOut, 32>(o, p, ranks, s);

@@ -282,9 +282,10 @@ int convrot_set_gemm_route(int route);
  * 57 activation slot free); 61-65 8-bit pair GEMM (61 copy slot free, 62
  * accumulator buffer free, 63 stage landed, 64 final MMA drain, 65
  * accumulator ready); 71-74 8-bit swap GEMM (71 copy slot free, 72 weight
- * stage landed, 73 activation stage landed, 74 final MMA drain); 81-86 8-bit
- * float pair GEMM (81 copy slot free, 82 accumulator free, 83 stage landed, 84
- * scales landed, 85 accumulator ready, 86 scale slot free); 91-96 8-bit float
+ * stage landed, 73 activation stage landed, 74 final MMA drain); 81-87 8-bit
+ * float pair GEMM (81 copy slot free, 82 accumulator free, 83 stage with its
+ * scales landed, 85 accumulator ready, 86 scale slot free, 87 final MMA drain);
+ * 91-96 8-bit float
  * swap GEMM (91 copy slot free, 92 weight stage landed, 93 activation stage
  * landed, 94 final MMA drain, 95 scale slot free, 96 scales landed).
  */
