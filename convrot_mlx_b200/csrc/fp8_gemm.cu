@@ -15,6 +15,7 @@
 // columns of tensor memory, for 4 stages of K.
 #include <algorithm>
 
+#include "fp8.cuh"
 #include "tile8.cuh"
 
 namespace convrot {
@@ -665,6 +666,189 @@ __global__ void __launch_bounds__(kThreads, 2)
 
 }  // namespace swap
 
+// ===========================================================================
+// GEMV kernel, up to 8 tokens of the forward product.  A CTA has 16 channels;
+// its 8 warps share out the blocks of 128 of K.  Thread (g, t) of a warp reads
+// 16 bytes of channels g and g + 8 at k = 16 t of each half of a block: the
+// four words of both are the A fragments of two MMAs (m16n8k32), with word 2 i
+// as the fragment's first half of k and word 2 i + 1 as the second.  Which k a
+// fragment index stands for only has to agree with the B fragment, which are
+// the same four words of token g's codes.  So weights go from memory to the MMA
+// with no rearrangement; two sets of two blocks are in flight in registers, also
+// from one set of channels to the next.  A block's products are summed from 0
+// and added to the total with its two scales.  The codes of all tokens are in
+// shared memory, copied, or (FUSED, one or two tokens) formed there from x by
+// every CTA itself, which costs less than a kernel of its own before this one.
+// ===========================================================================
+namespace gemv {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kChannels = 16;
+constexpr int kAhead = 2;  // blocks of a register set
+constexpr int kMaxTokens = 8;
+constexpr int kMaxFused = 2;
+constexpr int kMaxCodes = 96 * 1024;  // bytes of codes and scales in shared memory
+
+struct GemvParams {
+  Params p;
+  const void* x;  // FUSED: the activation, x_stride elements a row
+  const int8_t* act;
+  const int8_t* weight;
+  int64_t x_stride, act_stride, weight_stride;
+};
+
+__host__ __device__ constexpr int blocks_of(int k) { return (k + kBK - 1) / kBK; }
+// Pitch of a token's codes: 64 bytes off a multiple of 128, so that two tokens'
+// quads fall on different banks.  Then come the scales, a float32 a block and token.
+__host__ __device__ constexpr int pitch_of(int k) { return blocks_of(k) * kBK + 64; }
+__host__ __device__ constexpr int smem_of(int m, int k) { return m * (pitch_of(k) + 4 * blocks_of(k)); }
+
+__device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The value of a scale's byte: 2^(byte - 127), NaN for 255.
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+  return __uint_as_float(byte == 255u ? 0x7FC00000u : byte == 0u ? 0x00400000u : byte << 23);
+}
+
+template <typename TOut, bool FUSED>
+__global__ void __launch_bounds__(kThreads, 2) gemv_kernel(const GemvParams q) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  __shared__ float part[2][kWarps][kMaxTokens][kChannels + 1];
+  const Params& p = q.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int pitch = pitch_of(p.k), k_blocks = blocks_of(p.k);
+  uint8_t* codes = smem_raw;
+  float* xs = reinterpret_cast<float*>(smem_raw + p.m * pitch);  // of token m and block b at m * k_blocks + b
+  const int b_lo = k_blocks * warp / kWarps, b_hi = k_blocks * (warp + 1) / kWarps;
+  const int sets = (p.n + kChannels - 1) / kChannels;  // of channels
+
+  if (!p.early_weights) grid_dependency_wait();
+  struct Set {
+    uint4 w[2][2][kAhead];  // half of the block, channel g or g + 8
+    uint32_t scale[kAhead];
+  } wa, wb;
+  // The sets of this warp in its order: blocks from `at_b` on of channel set
+  // `at_n`; past a channel set's last block comes the next channel set.
+  int at_n = blockIdx.x, at_b = b_lo;
+  auto fetch = [&](Set& s) {
+    const int n0 = at_n * kChannels;
+    // channels past the last are read as the last, and not written
+    const int8_t* row0 = q.weight + static_cast<int64_t>(min(n0 + g, p.n - 1)) * q.weight_stride;
+    const int8_t* row1 = q.weight + static_cast<int64_t>(min(n0 + g + 8, p.n - 1)) * q.weight_stride;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const bool live = at_n < sets && at_b + i < b_hi;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k0 = (at_b + i) * kBK + 64 * h + 16 * t;
+        const bool in = live && k0 < p.k;
+        s.w[h][0][i] = in ? load16(row0, k0, p.k - k0) : make_uint4(0, 0, 0, 0);
+        s.w[h][1][i] = in ? load16(row1, k0, p.k - k0) : make_uint4(0, 0, 0, 0);
+      }
+      s.scale[i] = live ? ld_8(p.wscales + n0 / 128 * p.ws_n + (at_b + i) * p.ws_k) : 0u;
+    }
+    at_b += kAhead;
+  };
+  fetch(wa);
+  fetch(wb);
+  if (p.early_weights) grid_dependency_wait();
+  grid_dependents_launch();
+
+  if constexpr (FUSED) {
+    // every CTA quantizes the tokens for itself
+    const int chunks = k_blocks * kSpanThreads, all = p.m * chunks;
+    for (int i0 = 0; i0 < all; i0 += kThreads) {
+      const int i = i0 + threadIdx.x, m = i / chunks, c = (i - m * chunks) * kChunk;
+      float v[kChunk] = {};
+      if (i < all) load_chunk<TOut, true>(static_cast<const TOut*>(q.x) + m * q.x_stride, c, p.k, v);
+      const uint32_t byte = scale_byte(span_max(top_of(v)));
+      if (i < all) {
+        *reinterpret_cast<uint4*>(codes + m * pitch + c) = codes_of(v, byte);
+        if (c % kSpan == 0) xs[m * k_blocks + c / kSpan] = scale_of(byte);
+      }
+    }
+  } else {
+    const int chunks = k_blocks * (kBK / 16);
+    for (int i = threadIdx.x; i < chunks; i += kThreads) {  // one place of all tokens at a time
+      const int k0 = i * 16;
+#pragma unroll 1
+      for (int m0 = 0; m0 < p.m; m0 += 4) {
+        uint4 v[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          v[m] = m0 + m < p.m && k0 < p.k ? load16(q.act + (m0 + m) * q.act_stride, k0, p.k - k0)
+                                          : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          if (m0 + m < p.m) *reinterpret_cast<uint4*>(codes + (m0 + m) * pitch + k0) = v[m];
+      }
+    }
+    for (int i = threadIdx.x; i < p.m * k_blocks; i += kThreads) {
+      const int m = i / k_blocks;
+      xs[i] = scale_of(ld_8(p.xscales + m * p.xs_stride + (i - m * k_blocks)));
+    }
+  }
+  __syncthreads();
+
+  auto use = [&](const Set& s, int b, float (&acc)[4]) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (b + i >= b_hi) break;  // uniform across the warp
+      float sum[4] = {};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (g < p.m) x = *reinterpret_cast<const uint4*>(codes + g * pitch + (b + i) * kBK + 64 * h + 16 * t);
+        mma_e4m3(sum, s.w[h][0][i].x, s.w[h][1][i].x, s.w[h][0][i].y, s.w[h][1][i].y, x.x, x.y);
+        mma_e4m3(sum, s.w[h][0][i].z, s.w[h][1][i].z, s.w[h][0][i].w, s.w[h][1][i].w, x.z, x.w);
+      }
+      // fragment C: rows g and g + 8 (channels), columns 2 t and 2 t + 1 (tokens)
+      const float ws = scale_of(s.scale[i]);
+      const float x0 = 2 * t < p.m ? xs[2 * t * k_blocks + b + i] : 0.0f;
+      const float x1 = 2 * t + 1 < p.m ? xs[(2 * t + 1) * k_blocks + b + i] : 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = __fmaf_rn(__fmul_rn(sum[j], ws), j & 1 ? x1 : x0, acc[j]);
+    }
+  };
+  int turn = 0;
+  for (int set = blockIdx.x; set < sets; set += gridDim.x, turn ^= 1) {
+    float acc[4] = {};
+    int b = b_lo;
+    do {  // each pair of register sets is followed by the next pair's loads
+      const bool last = b + 2 * kAhead >= b_hi;
+      if (last) {
+        at_n = set + gridDim.x;
+        at_b = b_lo;
+      }
+      use(wa, b, acc);
+      fetch(wa);
+      use(wb, b + kAhead, acc);
+      fetch(wb);
+      b += 2 * kAhead;
+    } while (b < b_hi);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[turn][warp][2 * t + (i & 1)][g + 8 * (i >> 1)] = acc[i];
+    __syncthreads();
+    const int m = threadIdx.x / kChannels, n = set * kChannels + threadIdx.x % kChannels;
+    if (m < p.m && n < p.n) {
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) v = __fadd_rn(v, part[turn][w][m][threadIdx.x % kChannels]);
+      if (p.bias) v = __fadd_rn(v, ld_f32(p.bias + n));
+      static_cast<TOut*>(p.out)[static_cast<int64_t>(m) * p.n + n] = cvt_out<TOut>(v);
+    }
+  }
+}
+
+}  // namespace gemv
+
 // ---------------------------------------------------------------------------
 // host side
 
@@ -742,6 +926,38 @@ int launch_swap(const Operands& o, const Params& p, int ranks, cudaStream_t stre
   return check_launch("8-bit float swap gemm");
 }
 
+template <typename TOut, bool FUSED>
+int launch_gemv(const gemv::GemvParams& q, cudaStream_t stream) {
+  auto kernel = gemv::gemv_kernel<TOut, FUSED>;
+  CONVROT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gemv::kMaxCodes));
+  cudaLaunchConfig_t cfg = {};
+  const int sets = (q.p.n + gemv::kChannels - 1) / gemv::kChannels, most = 2 * device_sm_count();
+  cfg.gridDim = dim3(static_cast<unsigned>(sets < most ? sets : most), 1, 1);
+  cfg.blockDim = dim3(gemv::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(gemv::smem_of(q.p.m, q.p.k));
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CONVROT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, q));
+  return check_launch("8-bit float gemv");
+}
+
+bool gemv_takes(int layout, int64_t m, int64_t k) {
+  return layout == CONVROT_LAYOUT_NK && m <= gemv::kMaxTokens &&
+         m * (k + 256) + 4 * m * (k / kBK + 1) <= gemv::kMaxCodes;  // no less than smem_of
+}
+
+// x quantized inside the product.
+template <typename T>
+int launch_fused(const void* x, int64_t x_stride, const Operands& o, Params p, cudaStream_t s) {
+  p.early_weights = 0;  // the previous kernel of the stream may have written them
+  return launch_gemv<T, true>(
+      {p, x, nullptr, reinterpret_cast<const int8_t*>(o.weight), x_stride, 0, o.weight_stride}, s);
+}
+
 // Expected times of the two tile kernels in microseconds.
 double pair_time(const Params& p, int sms) {
   const int64_t tiles = static_cast<int64_t>((p.m + 255) / 256) * ((p.n + 255) / 256), pairs = sms / 2;
@@ -773,6 +989,11 @@ double swap_time(const Params& p, int bt, int sms, int* ranks) {
 template <int LAYOUT, typename TOut>
 int launch(const Operands& o, const Params& p, cudaStream_t s) {
   const int sms = device_sm_count();
+  if (gemv_takes(LAYOUT, p.m, p.k)) {
+    const gemv::GemvParams q{p, nullptr, reinterpret_cast<const int8_t*>(o.act), reinterpret_cast<const int8_t*>(o.weight),
+                             0, o.act_stride, o.weight_stride};
+    return launch_gemv<TOut, false>(q, s);
+  }
   const int bt = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
   int ranks = 1;
   const double swap_us = swap_time(p, bt, sms, &ranks);
@@ -828,11 +1049,14 @@ int by_layout(const Call& c, const Params& p, cudaStream_t s) {
                                        : launch<CONVROT_LAYOUT_KN, TOut>(c.o, p, s);
 }
 
-int run(const Call& c, bool early_weights, cudaStream_t s) {
+Params params_of(const Call& c, int* err_word, bool early_weights) {
   const bool nk = c.layout == CONVROT_LAYOUT_NK;
-  const Params p{c.xscales, c.wscales, c.xs_stride, nk ? c.ws_stride : 1, nk ? 1 : c.ws_stride, c.bias, c.out,
-                 static_cast<int>(c.m), static_cast<int>(c.n), static_cast<int>(c.k), device_error_word(),
-                 early_weights ? 1 : 0};
+  return {c.xscales, c.wscales, c.xs_stride, nk ? c.ws_stride : 1, nk ? 1 : c.ws_stride, c.bias, c.out,
+          static_cast<int>(c.m), static_cast<int>(c.n), static_cast<int>(c.k), err_word, early_weights ? 1 : 0};
+}
+
+int run(const Call& c, bool early_weights, cudaStream_t s) {
+  const Params p = params_of(c, device_error_word(), early_weights);
   CONVROT_REQUIRE(p.err_word != nullptr, CONVROT_ERR_CUDA, "device error word unavailable");
   switch (c.out_dtype) {
     case CONVROT_BF16: return by_layout<__nv_bfloat16>(c, p, s);
@@ -868,6 +1092,19 @@ int convrot_fp8_linear(const void* x, int x_dtype, int64_t x_stride, const uint8
                     bias, out, out_dtype, m, n, k};
   int rc = fp8::check_call(c);
   if (rc != CONVROT_OK) return rc;
+  // One or two tokens: quantized inside the product, one kernel instead of two.
+  const int64_t x_size = valid_dtype(x_dtype) ? static_cast<int64_t>(dtype_size(x_dtype)) : 1;
+  if (m > 0 && m <= fp8::gemv::kMaxFused && x_dtype == out_dtype && fp8::gemv_takes(layout, m, k) && aligned_to(x, 16) &&
+      x_stride * x_size % 16 == 0) {
+    CONVROT_REQUIRE(x != nullptr && x_stride >= k, CONVROT_ERR_INVALID, "null pointer, or a row stride below k");
+    const fp8::Params p = fp8::params_of(c, nullptr, false);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (x_dtype) {
+      case CONVROT_BF16: return fp8::launch_fused<__nv_bfloat16>(x, x_stride, c.o, p, s);
+      case CONVROT_F16: return fp8::launch_fused<__half>(x, x_stride, c.o, p, s);
+      default: return fp8::launch_fused<float>(x, x_stride, c.o, p, s);
+    }
+  }
   rc = convrot_quantize_fp8(x, x_dtype, m, k, x_stride, codes, codes_stride, scales, scales_stride, stream);
   if (rc != CONVROT_OK || m == 0) return rc;
   // The kernel before the product is the quantizer, which writes no weight

@@ -10,15 +10,12 @@
 // Activations: blocks of 128 consecutive values of a row.  Eight threads a
 // block, 16 values a thread: 16 codes are one 16-byte store, and the maximum
 // is three exchanges.  Weights: blocks of 128 x 128, a CTA each.
-#include "rows.cuh"
+#include "fp8.cuh"
 
 namespace convrot {
 namespace fp8 {
 
-constexpr int kSpan = 128;   // values that share a scale
-constexpr int kChunk = 16;   // values of a thread
 constexpr int kThreads = 256;
-constexpr int kBlockThreads = kSpan / kChunk;
 
 struct QuantParams {
   const void* x;
@@ -28,90 +25,33 @@ struct QuantParams {
   int features, spans;
 };
 
-// The biased exponent of the scale for magnitudes up to the value of `top`.
-__device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
-  if (top >= kInfBits) return 255u;
-  // top = 1.f * 2^E with biased exponent E + 127: e = E - 8, one more where 1.f > 1.75
-  const int e = static_cast<int>(top >> 23) - 8 + ((top & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-  return static_cast<uint32_t>(max(e, 0));
-}
-
-// 2^-e for the scale byte e + 127; 0 where the block is not finite.  (Bytes
-// are at most 247: 448 * 2^120 is above every float32.)
-__device__ __forceinline__ float inverse_of(uint32_t byte) {
-  return byte == 255u ? 0.0f : __uint_as_float((254u - byte) << 23);
-}
-
-// Two codes, a in the low byte.  The product is exact, at most 448.
-__device__ __forceinline__ uint32_t code_pair(float a, float b) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
-  return r;
-}
-
-__device__ __forceinline__ uint4 codes_of(const float (&v)[kChunk], uint32_t byte) {
-  const float f = inverse_of(byte);
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float s[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = byte == 255u ? 0.0f : __fmul_rn(v[4 * i + j], f);  // inf * 0 is no 0
-    w[i] = code_pair(s[0], s[1]) | code_pair(s[2], s[3]) << 16;
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// 16 values of a row of `features` values from c on; 0 past its end.
-template <typename T, bool WHOLE>
-__device__ __forceinline__ void load_chunk(const T* row, int c, int features, float (&v)[kChunk]) {
-  if (WHOLE && c + kChunk <= features) {
-    Pack<T, kChunk> p;
-    p.load_ahead(row + c);
-    p.get(v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) v[i] = c + i < features ? Elem<T>::to_f(row[c + i]) : 0.0f;
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t top_of(const float (&v)[kChunk]) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < kChunk; ++i) top = max(top, abs_bits(v[i]));
-  return top;
-}
-
 // WHOLE: rows start on multiples of 16 bytes.
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) quantize_rows(const QuantParams p) {
   grid_dependency_wait();
   grid_dependents_launch();
-  const uint32_t unit = blockIdx.x * (kThreads / kBlockThreads) + threadIdx.x / kBlockThreads;
+  const uint32_t unit = blockIdx.x * (kThreads / kSpanThreads) + threadIdx.x / kSpanThreads;
   const uint32_t row = unit / static_cast<uint32_t>(p.spans), span = unit - row * p.spans;
   const bool live = row < p.rows;
-  const int c = static_cast<int>(span) * kSpan + static_cast<int>(threadIdx.x % kBlockThreads) * kChunk;
+  const int c = static_cast<int>(span) * kSpan + static_cast<int>(threadIdx.x % kSpanThreads) * kChunk;
   float v[kChunk] = {};
   if (live) load_chunk<T, WHOLE>(static_cast<const T*>(p.x) + static_cast<int64_t>(row) * p.x_stride, c, p.features, v);
-  uint32_t top = top_of<T>(v);
-#pragma unroll
-  for (int d = 1; d < kBlockThreads; d *= 2) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+  const uint32_t top = span_max(top_of(v));
   if (!live) return;
   const uint32_t byte = scale_byte(top);
   // rows of codes are on a pitch of a multiple of 16 bytes: a chunk that begins inside a row ends inside its pitch
   if (c < p.features)
     *reinterpret_cast<uint4*>(p.codes + static_cast<int64_t>(row) * p.codes_stride + c) = codes_of(v, byte);
-  if (threadIdx.x % kBlockThreads == 0)
+  if (threadIdx.x % kSpanThreads == 0)
     p.scales[static_cast<int64_t>(row) * p.scales_stride + span] = static_cast<uint8_t>(byte);
 }
 
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) quantize_blocks(const QuantParams p) {
-  constexpr int kRowsAt = kThreads / kBlockThreads, kTurns = kSpan / kRowsAt;
+  constexpr int kRowsAt = kThreads / kSpanThreads, kTurns = kSpan / kRowsAt;
   __shared__ uint32_t red[kThreads / 32];
-  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kSpan + threadIdx.x / kBlockThreads;
-  const int c = blockIdx.x * kSpan + static_cast<int>(threadIdx.x % kBlockThreads) * kChunk;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kSpan + threadIdx.x / kSpanThreads;
+  const int c = blockIdx.x * kSpan + static_cast<int>(threadIdx.x % kSpanThreads) * kChunk;
   float v[kTurns][kChunk] = {};
   uint32_t top = 0;
 #pragma unroll
@@ -120,7 +60,7 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks(const QuantParams p)
     if (row < p.rows) load_chunk<T, WHOLE>(static_cast<const T*>(p.x) + row * p.x_stride, c, p.features, v[i]);
   }
 #pragma unroll
-  for (int i = 0; i < kTurns; ++i) top = max(top, top_of<T>(v[i]));
+  for (int i = 0; i < kTurns; ++i) top = max(top, top_of(v[i]));
   top = warp_max(top);
   if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = top;
   __syncthreads();
@@ -161,7 +101,7 @@ bool whole(const QuantParams& p) {
 
 template <typename T>
 int launch_rows(const QuantParams& p, cudaStream_t s) {
-  const int64_t units = p.rows * p.spans, per = kThreads / kBlockThreads;
+  const int64_t units = p.rows * p.spans, per = kThreads / kSpanThreads;
   auto kernel = whole<T>(p) ? quantize_rows<T, true> : quantize_rows<T, false>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((units + per - 1) / per), 1, 1);
