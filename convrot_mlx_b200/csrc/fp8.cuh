@@ -59,6 +59,23 @@ __device__ __forceinline__ void load_chunk(const T* row, int c, int features, fl
   }
 }
 
+// The same of rows that start on multiples of 16 bytes, by whole 16 bytes
+// wherever a row ends.
+template <typename T>
+__device__ __forceinline__ void load_pieces(const T* row, int c, int features, float (&v)[kChunk]) {
+  constexpr int W = 16 / sizeof(T);
+#pragma unroll
+  for (int j = 0; j < kChunk / W; ++j) {
+    Pack<T, W> w;
+    w.clear();
+    if (c + j * W < features) w.load_ahead(row + c + j * W);
+    float f[W];
+    w.get(f);
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[j * W + i] = c + j * W + i < features ? f[i] : 0.0f;
+  }
+}
+
 __device__ __forceinline__ uint32_t top_of(const float (&v)[kChunk]) {
   uint32_t top = 0;
 #pragma unroll

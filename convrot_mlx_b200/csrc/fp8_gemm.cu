@@ -669,16 +669,18 @@ __global__ void __launch_bounds__(kThreads, 2)
 // ===========================================================================
 // GEMV kernel, up to 8 tokens of the forward product.  A CTA has 16 channels;
 // its 8 warps share out the blocks of 128 of K.  Thread (g, t) of a warp reads
-// 16 bytes of channels g and g + 8 at k = 16 t of each half of a block: the
-// four words of both are the A fragments of two MMAs (m16n8k32), with word 2 i
-// as the fragment's first half of k and word 2 i + 1 as the second.  Which k a
-// fragment index stands for only has to agree with the B fragment, which are
-// the same four words of token g's codes.  So weights go from memory to the MMA
-// with no rearrangement; two sets of two blocks are in flight in registers, also
-// from one set of channels to the next.  A block's products are summed from 0
-// and added to the total with its two scales.  The codes of all tokens are in
-// shared memory, copied, or (FUSED, one or two tokens) formed there from x by
-// every CTA itself, which costs less than a kernel of its own before this one.
+// 16 bytes of channels g and g + 8 at k = 16 t of each half of a block; as f16
+// pairs (a conversion each, exact) pairs 2 j and 2 j + 1 of both are the A
+// fragment of MMA j (m16n8k16).  Which k a fragment index stands for only has to
+// agree with the B fragment, which are the same pairs of token g's codes.  So
+// weights go from memory to the MMA with no rearrangement; two sets of two
+// blocks are in flight in registers, also from one set of channels to the next.
+// A block's products are summed from 0 and added to the total with its two
+// scales.  The tokens are in shared memory as f16, converted from their codes
+// or (FUSED, one or two tokens) quantized there by every CTA itself, which costs
+// less than a kernel of its own before this one.  A launch of a few microseconds
+// waits for its instructions as much as for its data: the loop has each piece
+// of code once.
 // ===========================================================================
 namespace gemv {
 
@@ -688,28 +690,59 @@ constexpr int kChannels = 16;
 constexpr int kAhead = 2;  // blocks of a register set
 constexpr int kMaxTokens = 8;
 constexpr int kMaxFused = 2;
-constexpr int kMaxCodes = 96 * 1024;  // bytes of codes and scales in shared memory
+constexpr int kMaxBytes = 96 * 1024;  // of shared memory for the tokens and their scales
 
 struct GemvParams {
   Params p;
   const void* x;  // FUSED: the activation, x_stride elements a row
-  const int8_t* act;
-  const int8_t* weight;
+  const uint8_t* act;
+  const uint8_t* weight;
   int64_t x_stride, act_stride, weight_stride;
 };
 
 __host__ __device__ constexpr int blocks_of(int k) { return (k + kBK - 1) / kBK; }
-// Pitch of a token's codes: 64 bytes off a multiple of 128, so that two tokens'
-// quads fall on different banks.  Then come the scales, a float32 a block and token.
-__host__ __device__ constexpr int pitch_of(int k) { return blocks_of(k) * kBK + 64; }
+// Bytes of a token: 16 off a multiple of 128, so that the 32 bytes of eight
+// tokens' quads fall on different banks.  Then come the scales, a float32 a
+// token and block.
+__host__ __device__ constexpr int pitch_of(int k) { return 2 * blocks_of(k) * kBK + 16; }
 __host__ __device__ constexpr int smem_of(int m, int k) { return m * (pitch_of(k) + 4 * blocks_of(k)); }
 
-__device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+__device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Four codes as two pairs of f16.
+__device__ __forceinline__ uint2 halves_of(uint32_t w) {
+  uint2 r;
+  asm("{\n\t.reg .b16 a, b;\n\t"
+      "mov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(r.x), "=r"(r.y)
+      : "r"(w));
+  return r;
+}
+
+// 16 bytes of a row of codes with those past `count` cleared (a pitch is of
+// whole 16 bytes, so that they can be read).
+__device__ __forceinline__ uint4 only(uint4 v, int count) {
+  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int keep = min(max(count - 4 * i, 0), 4);
+    w[i] &= static_cast<uint32_t>((1ull << (8 * keep)) - 1);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ void store_halves(uint8_t* to, uint4 codes) {
+  const uint2 a = halves_of(codes.x), b = halves_of(codes.y), c = halves_of(codes.z), d = halves_of(codes.w);
+  reinterpret_cast<uint4*>(to)[0] = make_uint4(a.x, a.y, b.x, b.y);
+  reinterpret_cast<uint4*>(to)[1] = make_uint4(c.x, c.y, d.x, d.y);
 }
 
 // The value of a scale's byte: 2^(byte - 127), NaN for 255.
@@ -724,7 +757,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_kernel(const GemvParams q) {
   const Params& p = q.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int pitch = pitch_of(p.k), k_blocks = blocks_of(p.k);
-  uint8_t* codes = smem_raw;
+  uint8_t* tokens = smem_raw;
   float* xs = reinterpret_cast<float*>(smem_raw + p.m * pitch);  // of token m and block b at m * k_blocks + b
   const int b_lo = k_blocks * warp / kWarps, b_hi = k_blocks * (warp + 1) / kWarps;
   const int sets = (p.n + kChannels - 1) / kChannels;  // of channels
@@ -733,106 +766,113 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_kernel(const GemvParams q) {
   struct Set {
     uint4 w[2][2][kAhead];  // half of the block, channel g or g + 8
     uint32_t scale[kAhead];
-  } wa, wb;
-  // The sets of this warp in its order: blocks from `at_b` on of channel set
-  // `at_n`; past a channel set's last block comes the next channel set.
+  } ring[2];
+  // The blocks of this warp in its order, two register sets of kAhead a round:
+  // from `at_b` on of channel set `at_n`; past its last block comes the next
+  // channel set.
   int at_n = blockIdx.x, at_b = b_lo;
-  auto fetch = [&](Set& s) {
-    const int n0 = at_n * kChannels;
-    // channels past the last are read as the last, and not written
-    const int8_t* row0 = q.weight + static_cast<int64_t>(min(n0 + g, p.n - 1)) * q.weight_stride;
-    const int8_t* row1 = q.weight + static_cast<int64_t>(min(n0 + g + 8, p.n - 1)) * q.weight_stride;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const bool live = at_n < sets && at_b + i < b_hi;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k0 = (at_b + i) * kBK + 64 * h + 16 * t;
-        const bool in = live && k0 < p.k;
-        s.w[h][0][i] = in ? load16(row0, k0, p.k - k0) : make_uint4(0, 0, 0, 0);
-        s.w[h][1][i] = in ? load16(row1, k0, p.k - k0) : make_uint4(0, 0, 0, 0);
-      }
-      s.scale[i] = live ? ld_8(p.wscales + n0 / 128 * p.ws_n + (at_b + i) * p.ws_k) : 0u;
-    }
-    at_b += kAhead;
-  };
-  fetch(wa);
-  fetch(wb);
-  if (p.early_weights) grid_dependency_wait();
-  grid_dependents_launch();
-
-  if constexpr (FUSED) {
-    // every CTA quantizes the tokens for itself
-    const int chunks = k_blocks * kSpanThreads, all = p.m * chunks;
-    for (int i0 = 0; i0 < all; i0 += kThreads) {
-      const int i = i0 + threadIdx.x, m = i / chunks, c = (i - m * chunks) * kChunk;
-      float v[kChunk] = {};
-      if (i < all) load_chunk<TOut, true>(static_cast<const TOut*>(q.x) + m * q.x_stride, c, p.k, v);
-      const uint32_t byte = scale_byte(span_max(top_of(v)));
-      if (i < all) {
-        *reinterpret_cast<uint4*>(codes + m * pitch + c) = codes_of(v, byte);
-        if (c % kSpan == 0) xs[m * k_blocks + c / kSpan] = scale_of(byte);
-      }
-    }
-  } else {
-    const int chunks = k_blocks * (kBK / 16);
-    for (int i = threadIdx.x; i < chunks; i += kThreads) {  // one place of all tokens at a time
-      const int k0 = i * 16;
+  float acc[4];
+  bool first = true;  // nothing has been fetched yet
+  int turn = 0, set = blockIdx.x;
 #pragma unroll 1
-      for (int m0 = 0; m0 < p.m; m0 += 4) {
-        uint4 v[4];
+  while (set < sets) {
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
-          v[m] = m0 + m < p.m && k0 < p.k ? load16(q.act + (m0 + m) * q.act_stride, k0, p.k - k0)
-                                          : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-          if (m0 + m < p.m) *reinterpret_cast<uint4*>(codes + (m0 + m) * pitch + k0) = v[m];
-      }
-    }
-    for (int i = threadIdx.x; i < p.m * k_blocks; i += kThreads) {
-      const int m = i / k_blocks;
-      xs[i] = scale_of(ld_8(p.xscales + m * p.xs_stride + (i - m * k_blocks)));
-    }
-  }
-  __syncthreads();
-
-  auto use = [&](const Set& s, int b, float (&acc)[4]) {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (b + i >= b_hi) break;  // uniform across the warp
-      float sum[4] = {};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (g < p.m) x = *reinterpret_cast<const uint4*>(codes + g * pitch + (b + i) * kBK + 64 * h + 16 * t);
-        mma_e4m3(sum, s.w[h][0][i].x, s.w[h][1][i].x, s.w[h][0][i].y, s.w[h][1][i].y, x.x, x.y);
-        mma_e4m3(sum, s.w[h][0][i].z, s.w[h][1][i].z, s.w[h][0][i].w, s.w[h][1][i].w, x.z, x.w);
-      }
-      // fragment C: rows g and g + 8 (channels), columns 2 t and 2 t + 1 (tokens)
-      const float ws = scale_of(s.scale[i]);
-      const float x0 = 2 * t < p.m ? xs[2 * t * k_blocks + b + i] : 0.0f;
-      const float x1 = 2 * t + 1 < p.m ? xs[(2 * t + 1) * k_blocks + b + i] : 0.0f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = __fmaf_rn(__fmul_rn(sum[j], ws), j & 1 ? x1 : x0, acc[j]);
-    }
-  };
-  int turn = 0;
-  for (int set = blockIdx.x; set < sets; set += gridDim.x, turn ^= 1) {
-    float acc[4] = {};
+    for (int i = 0; i < 4; ++i) acc[i] = 0.0f;
     int b = b_lo;
-    do {  // each pair of register sets is followed by the next pair's loads
-      const bool last = b + 2 * kAhead >= b_hi;
-      if (last) {
-        at_n = set + gridDim.x;
-        at_b = b_lo;
+#pragma unroll 1
+    do {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        Set& s = ring[r];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int block = b + r * kAhead + i;
+          if (first || block >= b_hi) break;  // uniform across the warp
+          float sum[4] = {};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int k0 = block * kBK + 64 * h + 16 * t;
+            uint4 w0 = s.w[h][0][i], w1 = s.w[h][1][i];
+            if (k0 + 16 > p.k) w0 = only(w0, p.k - k0), w1 = only(w1, p.k - k0);
+            uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
+            if (g < p.m) {
+              const uint4* x = reinterpret_cast<const uint4*>(tokens + g * pitch + 2 * k0);
+              x0 = x[0], x1 = x[1];
+            }
+            const uint32_t wa[4] = {w0.x, w0.y, w0.z, w0.w}, wb[4] = {w1.x, w1.y, w1.z, w1.w};
+            const uint32_t xw[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint2 c = halves_of(wa[j]), d = halves_of(wb[j]);
+              mma_f16_16816(sum, c.x, d.x, c.y, d.y, xw[2 * j], xw[2 * j + 1]);
+            }
+          }
+          // fragment C: rows g and g + 8 (channels), columns 2 t and 2 t + 1 (tokens)
+          const float ws = scale_of(s.scale[i]);
+          const float x0 = 2 * t < p.m ? xs[2 * t * k_blocks + block] : 0.0f;
+          const float x1 = 2 * t + 1 < p.m ? xs[(2 * t + 1) * k_blocks + block] : 0.0f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j] = __fmaf_rn(__fmul_rn(sum[j], ws), j & 1 ? x1 : x0, acc[j]);
+        }
+        const int n0 = at_n * kChannels;
+        // channels past the last are read as the last, and not written
+        const uint8_t* row0 = q.weight + min(n0 + g, p.n - 1) * q.weight_stride + 16 * t;
+        const uint8_t* row1 = q.weight + min(n0 + g + 8, p.n - 1) * q.weight_stride + 16 * t;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int block = at_b + r * kAhead + i;
+          const bool live = at_n < sets && block < b_hi;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int k0 = block * kBK + 64 * h;
+            const bool in = live && k0 + 16 * t < p.k;
+            s.w[h][0][i] = in ? ld_128(row0 + k0) : make_uint4(0, 0, 0, 0);
+            s.w[h][1][i] = in ? ld_128(row1 + k0) : make_uint4(0, 0, 0, 0);
+          }
+          s.scale[i] = live ? ld_8(p.wscales + n0 / 128 * p.ws_n + block * p.ws_k) : 0u;
+        }
       }
-      use(wa, b, acc);
-      fetch(wa);
-      use(wb, b + kAhead, acc);
-      fetch(wb);
       b += 2 * kAhead;
-    } while (b < b_hi);
+      at_b += 2 * kAhead;
+      if (at_b >= b_hi) {
+        at_b = b_lo;
+        at_n += gridDim.x;
+      }
+    } while (!first && b < b_hi);
+    if (first) {
+      first = false;
+      if (p.early_weights) grid_dependency_wait();
+      grid_dependents_launch();
+      if constexpr (FUSED) {
+        // every CTA quantizes the tokens for itself
+        const int chunks = k_blocks * kSpanThreads, all = p.m * chunks;
+#pragma unroll 1
+        for (int i0 = 0; i0 < all; i0 += kThreads) {
+          const int i = i0 + threadIdx.x, m = i / chunks, c = (i - m * chunks) * kChunk;
+          float v[kChunk];
+          load_pieces(static_cast<const TOut*>(q.x) + m * q.x_stride, c, i < all ? p.k : 0, v);
+          const uint32_t byte = scale_byte(span_max(top_of(v)));
+          if (i < all) {
+            store_halves(tokens + m * pitch + 2 * c, codes_of(v, byte));
+            if (c % kSpan == 0) xs[m * k_blocks + c / kSpan] = scale_of(byte);
+          }
+        }
+      } else {
+        const int chunks = k_blocks * (kBK / 16), all = p.m * chunks;
+        for (int i = threadIdx.x; i < all; i += kThreads) {
+          const int m = i / chunks, k0 = (i - m * chunks) * 16;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (k0 < p.k) v = ld_128(q.act + m * q.act_stride + k0);
+          store_halves(tokens + m * pitch + 2 * k0, k0 + 16 > p.k ? only(v, p.k - k0) : v);
+        }
+        for (int i = threadIdx.x; i < p.m * k_blocks; i += kThreads) {
+          const int m = i / k_blocks;
+          xs[i] = scale_of(ld_8(p.xscales + m * p.xs_stride + (i - m * k_blocks)));
+        }
+      }
+      __syncthreads();
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[turn][warp][2 * t + (i & 1)][g + 8 * (i >> 1)] = acc[i];
     __syncthreads();
@@ -844,6 +884,8 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_kernel(const GemvParams q) {
       if (p.bias) v = __fadd_rn(v, ld_f32(p.bias + n));
       static_cast<TOut*>(p.out)[static_cast<int64_t>(m) * p.n + n] = cvt_out<TOut>(v);
     }
+    set += gridDim.x;
+    turn ^= 1;
   }
 }
 
@@ -929,7 +971,7 @@ int launch_swap(const Operands& o, const Params& p, int ranks, cudaStream_t stre
 template <typename TOut, bool FUSED>
 int launch_gemv(const gemv::GemvParams& q, cudaStream_t stream) {
   auto kernel = gemv::gemv_kernel<TOut, FUSED>;
-  CONVROT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gemv::kMaxCodes));
+  CONVROT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, gemv::kMaxBytes));
   cudaLaunchConfig_t cfg = {};
   const int sets = (q.p.n + gemv::kChannels - 1) / gemv::kChannels, most = 2 * device_sm_count();
   cfg.gridDim = dim3(static_cast<unsigned>(sets < most ? sets : most), 1, 1);
@@ -947,15 +989,14 @@ int launch_gemv(const gemv::GemvParams& q, cudaStream_t stream) {
 
 bool gemv_takes(int layout, int64_t m, int64_t k) {
   return layout == CONVROT_LAYOUT_NK && m <= gemv::kMaxTokens &&
-         m * (k + 256) + 4 * m * (k / kBK + 1) <= gemv::kMaxCodes;  // no less than smem_of
+         m * (2 * k + 2 * kBK + 16 + 4 * (k / kBK + 1)) <= gemv::kMaxBytes;  // no less than smem_of
 }
 
 // x quantized inside the product.
 template <typename T>
 int launch_fused(const void* x, int64_t x_stride, const Operands& o, Params p, cudaStream_t s) {
   p.early_weights = 0;  // the previous kernel of the stream may have written them
-  return launch_gemv<T, true>(
-      {p, x, nullptr, reinterpret_cast<const int8_t*>(o.weight), x_stride, 0, o.weight_stride}, s);
+  return launch_gemv<T, true>({p, x, nullptr, o.weight, x_stride, 0, o.weight_stride}, s);
 }
 
 // Expected times of the two tile kernels in microseconds.
@@ -990,8 +1031,7 @@ template <int LAYOUT, typename TOut>
 int launch(const Operands& o, const Params& p, cudaStream_t s) {
   const int sms = device_sm_count();
   if (gemv_takes(LAYOUT, p.m, p.k)) {
-    const gemv::GemvParams q{p, nullptr, reinterpret_cast<const int8_t*>(o.act), reinterpret_cast<const int8_t*>(o.weight),
-                             0, o.act_stride, o.weight_stride};
+    const gemv::GemvParams q{p, nullptr, o.act, o.weight, 0, o.act_stride, o.weight_stride};
     return launch_gemv<TOut, false>(q, s);
   }
   const int bt = p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
