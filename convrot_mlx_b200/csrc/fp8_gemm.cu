@@ -108,6 +108,11 @@ __device__ __forceinline__ uint32_t word_of(uint32_t byte) {
   return word;
 }
 
+// An arrival that publishes nothing of its own.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
+
 // ===========================================================================
 // Pair kernel.  CTA pairs (cta_group::2), 256 tokens x 256 channels a tile,
 // persistent.  Each CTA holds 128 tokens and 128 channels of a tile:
@@ -270,7 +275,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (g >= kStages && !wait_empty(g - kStages)) { ok = false; break; }
         if (ks % kGroup == 0) {
           now = next;
-          load_next();
           // the set's last group is the one two before
           if (group >= 2 && !wait_empty(g - before - 1)) { ok = false; break; }
           const uint32_t w0 = word_of(now.w0), w1 = word_of(now.w1);
@@ -283,8 +287,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++group;
           before = min(kGroup, k_stages - ks);
         }
-        // a release of all memory at cluster scope would take a microsecond: only shared memory is published
-        if (lane == 0) mbar_arrive_cluster_publish_smem(lead_full0 + (g % kStages) * 8);
+        // A release of all memory at cluster scope would take a microsecond: only shared memory is published, and
+        // before the next loads are issued, which it would wait for.
+        if (lane == 0) {
+          if (ks % kGroup == 0) mbar_arrive_cluster_publish_smem(lead_full0 + (g % kStages) * 8);
+          else mbar_arrive_cluster_relaxed(lead_full0 + (g % kStages) * 8);
+        }
+        if (ks % kGroup == 0) load_next();
       }
     }
   } else if (warp == kWarpMma) {
@@ -530,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     struct {
       uint32_t x[4], w;
     } now, next = {{kOneWord, kOneWord, kOneWord, kOneWord}, 0};
-    auto load_next = [&](int b0) {  // while the group before is written
+    auto load_next = [&](int b0) {
       if (b0 >= k_hi) return;
 #pragma unroll
       for (int j = 0; j < kRows; ++j)
@@ -540,7 +549,6 @@ __global__ void __launch_bounds__(kThreads, 2)
     load_next(k_lo);
     for (int b0 = k_lo, i = 0; b0 < k_hi; b0 += kGroup, ++i) {
       now = next;
-      load_next(b0 + kGroup);
       const bool ok = wait(&bars->sf_empty[i & 1], ((i >> 1) & 1) ^ 1, &bars->err, 95);
       if (__any_sync(0xFFFFFFFFu, !ok)) break;
       const uint32_t at = smem_u32(sS) + (i & 1) * 2 * kScaleBytes + lane * 16;
@@ -550,6 +558,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->sf_full[i & 1]);
+      load_next(b0 + kGroup);  // behind the fence, which would wait for it
     }
   } else if (warp == 1 && lane == 0) {
     constexpr uint32_t idesc = idesc_mx(128, BT, LAYOUT == CONVROT_LAYOUT_KN, false);

@@ -183,6 +183,14 @@ __device__ __forceinline__ P2 refined_root(P2 v, P2 y, P2 s) {
   return fma(half_residual, y, s);
 }
 
+// A paired product and a paired sum may be compiled to one operation with one
+// rounding.  The moments are defined with two, so that 8-bit codes are the same
+// however a step is computed; sums of the halves stay sums.
+__device__ __forceinline__ P2 sum_of(P2 a, P2 b) {
+  const float2 x = p2_get(a), y = p2_get(b);
+  return p2(__fadd_rn(x.x, y.x), __fadd_rn(x.y, y.y));
+}
+
 // Codes of the block's values, whose largest magnitude has the bits `top`, and
 // their scale: 0 for a block of zeros (and of values below 2^-117, whose scale
 // is no normal number), NaN for one that is not finite, both with codes 0.
@@ -394,8 +402,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<T, BITS>) adamw_kernel(const _
     }
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
-      m[i] = add(mul(m[i], beta1), mul(g[i], rest1));
-      v[i] = add(mul(v[i], beta2), mul(mul(g[i], g[i]), rest2));
+      m[i] = sum_of(mul(m[i], beta1), mul(g[i], rest1));
+      v[i] = sum_of(mul(v[i], beta2), mul(mul(g[i], g[i]), rest2));
       P2 y;
       r[i] = root_of(v[i], y);
       const float2 den = p2_get(fma(r[i], root2, eps));
