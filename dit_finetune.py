@@ -1,11 +1,13 @@
 """Fine-tuning around frozen 8-bit linears: a small diffusion-transformer block over video tokens whose projections are
-``Int8Linear`` (frozen, 8-bit weights), with the modulations, the norms of the queries and keys and a final head left
-trainable.  It runs the 8-bit and training operators of ``convrot_mlx_b200`` together as a training step uses them:
+``Int8Linear`` or ``Fp8Linear`` (frozen, 8-bit weights), with the modulations, the norms of the queries and keys and a
+final head left trainable.  It runs the 8-bit and training operators of ``convrot_mlx_b200`` together as a training step
+uses them:
 
   modulated_layer_norm -> int8 qkv -> layer_norm of q and k -> axial_rotary -> attention -> int8 projection
   modulated_layer_norm -> int8 -> gelu_tanh_saved8 -> int8
 
     python dit_finetune.py [--steps 20] [--width 768] [--frames 4 --rows 16 --cols 16] [--batch 2]
+                           [--linears int8|fp8] [--optimizer adam|adamw32|adamw8]
 
 prints the loss of each step.  Inputs and targets are synthetic; the block learns a fixed random target.
 """
@@ -19,7 +21,7 @@ import torch.nn.functional as F
 from torch import nn
 
 import convrot_mlx_b200 as cr
-from convrot_mlx_b200.adapter import replace_int8_linears
+from convrot_mlx_b200.adapter import replace_fp8_linears, replace_int8_linears
 
 
 class Norm(nn.Module):
@@ -59,15 +61,16 @@ class Block(nn.Module):
 
 
 FROZEN = ("qkv", "proj", "up", "down")
+LINEARS = {"int8": replace_int8_linears, "fp8": replace_fp8_linears}
 
 
-def build(width: int, heads: int, device, dtype=torch.bfloat16, seed: int = 0) -> Block:
+def build(width: int, heads: int, device, dtype=torch.bfloat16, seed: int = 0, linears: str = "int8") -> Block:
     """A block with its projections frozen in 8 bits; the rest trainable."""
 
     torch.manual_seed(seed)
     block = Block(width, heads).to(device)
     keep = [name for name, m in block.named_modules() if isinstance(m, nn.Linear) and name not in FROZEN]
-    replace_int8_linears(block, keep=keep)
+    LINEARS[linears](block, keep=keep)
     return block.to(dtype)
 
 
@@ -77,24 +80,32 @@ def grid_positions(frames: int, rows: int, cols: int, device) -> torch.Tensor:
     return torch.cartesian_prod(*(torch.arange(n, device=device) for n in (frames, rows, cols))).float()
 
 
-def train(steps: int, width: int, heads: int, batch: int, frames: int, rows: int, cols: int, device="cuda",
-          lr: float = 2e-3, seed: int = 0) -> list[float]:
-    """Adam steps on the trainable parameters; returns the losses."""
+def make_optimizer(kind: str, params, lr: float):
+    """torch's Adam, or AdamW with its moments in 32 or 8 bits and the gradients clipped at a norm of 1."""
 
-    block = build(width, heads, device, seed=seed)
+    if kind == "adam":
+        return torch.optim.Adam(params, lr=lr)
+    return cr.AdamW(params, lr=lr, weight_decay=0.0, state_bits={"adamw32": 32, "adamw8": 8}[kind], max_norm=1.0)
+
+
+def train(steps: int, width: int, heads: int, batch: int, frames: int, rows: int, cols: int, device="cuda",
+          lr: float = 2e-3, seed: int = 0, linears: str = "int8", optimizer: str = "adam") -> list[float]:
+    """Optimizer steps on the trainable parameters; returns the losses."""
+
+    block = build(width, heads, device, seed=seed, linears=linears)
     g = torch.Generator(device=device).manual_seed(seed + 1)
     positions = grid_positions(frames, rows, cols, device)
     shape = (batch, positions.shape[0], width)
     x = torch.randn(shape, generator=g, device=device).bfloat16()
     vec = torch.randn((batch, width), generator=g, device=device).bfloat16()
     target = x + 0.5 * torch.randn((batch, 1, width), generator=g, device=device).bfloat16()
-    optimizer = torch.optim.Adam(block.parameters(), lr=lr)
+    stepper = make_optimizer(optimizer, block.parameters(), lr)
     losses = []
     for _ in range(steps):
         loss = F.mse_loss(block(x, vec, positions).float(), target.float())
-        optimizer.zero_grad()
+        stepper.zero_grad()
         loss.backward()
-        optimizer.step()
+        stepper.step()
         losses.append(loss.detach())
     return [float(v) for v in losses]
 
@@ -108,8 +119,11 @@ def main() -> None:
     ap.add_argument("--frames", type=int, default=4)
     ap.add_argument("--rows", type=int, default=16)
     ap.add_argument("--cols", type=int, default=16)
+    ap.add_argument("--linears", choices=tuple(LINEARS), default="int8")
+    ap.add_argument("--optimizer", choices=("adam", "adamw32", "adamw8"), default="adam")
     a = ap.parse_args()
-    for i, loss in enumerate(train(a.steps, a.width, a.heads, a.batch, a.frames, a.rows, a.cols)):
+    losses = train(a.steps, a.width, a.heads, a.batch, a.frames, a.rows, a.cols, linears=a.linears, optimizer=a.optimizer)
+    for i, loss in enumerate(losses):
         print(f"step {i}: loss {loss:.5f}")
 
 
