@@ -685,11 +685,13 @@ std::vector<const Tensor*> present(const TensorList& list) {
 }
 
 Tensor square_sums(const py::object& grads) {
+  const at::NoGradGuard no_grad;
   const TensorList list(grads, "gradients");
   return square_sums_of(present(list));
 }
 
 Tensor grad_norm(const py::object& grads) {
+  const at::NoGradGuard no_grad;
   const TensorList list(grads, "gradients");
   const std::vector<const Tensor*> tensors = present(list);
   const Tensor sums = square_sums_of(tensors);
@@ -733,6 +735,7 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
                                  const py::object& exp_avg_sqs, const py::object& scales, const py::object& step,
                                  const py::object& lr, double beta1, double beta2, double eps, double weight_decay,
                                  std::optional<double> max_norm, const std::optional<Tensor>& sums_in) {
+  const at::NoGradGuard no_grad;
   const TensorList p(params, "parameters"), g(grads, "gradients"), m(exp_avgs, "moments"), v(exp_avg_sqs, "moments");
   const bool eight = !scales.is_none();
   const TensorList s(eight ? scales : exp_avgs, "scales");

@@ -433,10 +433,10 @@ __global__ void __launch_bounds__(kThreads, kCtas<T, BITS>) adamw_kernel(const _
 }
 
 // ---------------------------------------------------------------------------
-// Sums of squares.  Eight squares are added in float32 and their sum to a
-// 64-bit one; where eight squares leave the range of float32 (a sum that is not
-// finite, or so small that squares may have been lost) they are formed in 64
-// bits.  Each CTA writes one sum, of a share that depends on the sizes alone.
+// Sums of squares.  A thread adds 32 squares in float32, in four sums of eight
+// and these in pairs, and the total to a 64-bit one; where a sum of eight leaves
+// the range of float32 (not finite, or so small that squares may have been lost)
+// the squares are formed in 64 bits.  Each CTA writes one sum, of a share that depends on the sizes alone.
 
 struct NormEntry {
   const void* g;
@@ -454,6 +454,7 @@ struct NormTable {
 };
 
 constexpr int kAhead = 4;  // chunks in flight
+constexpr int kSumCtas = 4;  // of an SM
 
 template <typename T, int CAP>
 __global__ void __launch_bounds__(kThreads) square_sums(const __grid_constant__ NormTable<CAP> t) {
@@ -488,19 +489,26 @@ __global__ void __launch_bounds__(kThreads) square_sums(const __grid_constant__ 
           for (int i = 0; i < kLane / G; ++i) w[j][i].load_part(src + place<G>(i), count - place<G>(i));
         }
       }
+      float sums[kAhead];
+      bool fine = true;
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        float sum = 0.0f;
+        P2 square = p2(0.0f, 0.0f);
 #pragma unroll
         for (int i = 0; i < kLane / G; ++i) {
-          float g[G];
-          w[j][i].get(g);
+          P2 g[G / 2];
+          w[j][i].get_lanes(g);
 #pragma unroll
-          for (int k = 0; k < G; ++k) sum = __fmaf_rn(g[k], g[k], sum);
+          for (int k = 0; k < G / 2; ++k) square = fma(g[k], g[k], square);
         }
-        if (sum < 0x1p120f && sum > 0x1p-90f) {
-          acc += static_cast<double>(sum);
-        } else {
+        sums[j] = total(square);
+        fine = fine && ((sums[j] < 0x1p120f && sums[j] > 0x1p-90f) || chunk + j >= end);
+      }
+      if (fine) {
+        acc += static_cast<double>(__fadd_rn(__fadd_rn(sums[0], sums[1]), __fadd_rn(sums[2], sums[3])));
+      } else {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
 #pragma unroll
           for (int i = 0; i < kLane / G; ++i) {
             float g[G];
@@ -633,7 +641,7 @@ int64_t convrot_square_sums_count(int64_t count, const convrot_grad_tensor* tens
   if (count < 0 || (count > 0 && !tensors)) return 1;
   int64_t chunks = 0;
   for (int64_t i = 0; i < count; ++i) chunks += tensors[i].numel > 0 ? optim::chunks_of(tensors[i].numel) : 0;
-  const int64_t ctas = chunks, most = 4 * static_cast<int64_t>(device_sm_count());
+  const int64_t ctas = chunks, most = optim::kSumCtas * static_cast<int64_t>(device_sm_count());
   return ctas < 1 ? 1 : (ctas < most ? ctas : most);
 }
 

@@ -23,7 +23,6 @@ from . import _native
 MOMENT_BLOCK = 256  # values of a tensor whose 8-bit moments share their scales
 
 
-@torch.no_grad()
 def grad_norm(grads: Iterable[torch.Tensor | None]) -> torch.Tensor:
     """The 2-norm of all values of ``grads`` (CUDA tensors of one device; None is passed over), float32 on the device.
 
@@ -33,7 +32,6 @@ def grad_norm(grads: Iterable[torch.Tensor | None]) -> torch.Tensor:
     return _native.ops().grad_norm(grads if isinstance(grads, (list, tuple)) else list(grads))
 
 
-@torch.no_grad()
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | None], exp_avgs: Sequence[torch.Tensor],
                exp_avg_sqs: Sequence[torch.Tensor], scales: Sequence[torch.Tensor] | None, step, *, lr, betas=(0.9, 0.999),
                eps: float = 1e-8, weight_decay: float = 1e-2, max_norm: float | None = None) -> torch.Tensor | None:
