@@ -263,6 +263,17 @@ Tensor fp8_product(const Tensor& x, const Tensor& qweight, int layout, const Ten
   return out;
 }
 
+// padded_rows, and the last row too can be read in whole 16 bytes.
+Tensor whole_rows(const Tensor& codes) {
+  const Tensor t = padded_rows(codes);
+  const int64_t last = (t.size(0) - 1) * t.stride(0) + (t.size(1) + kPitch - 1) / kPitch * kPitch;
+  if (static_cast<int64_t>(t.storage().nbytes()) >= t.storage_offset() + last) return t;
+  const Tensor rows = at::empty({t.size(0), (t.size(1) + kPitch - 1) / kPitch * kPitch}, t.options());
+  const Tensor out = rows.narrow(1, 0, t.size(1));
+  out.copy_(t);
+  return out;
+}
+
 struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& qweight, const Tensor& wscales,
                         const std::optional<Tensor>& bias) {
@@ -295,7 +306,7 @@ Tensor fp8_linear(const Tensor& x, const Tensor& qweight, const Tensor& wscales,
   dtype_code(x.scalar_type());
   no_tangents("fp8_linear", {&x, &b});
   require_cuda({&x, &qweight, &wscales, &b});
-  const Tensor w = padded_rows(qweight), ws = wscales.contiguous(), fb = f32_vector(b);
+  const Tensor w = whole_rows(qweight), ws = wscales.contiguous(), fb = f32_vector(b);
   if (at::GradMode::is_enabled() && x.requires_grad())
     return Fp8Linear::apply(x, w, ws, fb.defined() ? std::optional<Tensor>(fb) : std::nullopt);
   return fp8_product(x, w, CONVROT_LAYOUT_NK, ws, fb, n);
@@ -703,6 +714,14 @@ Tensor grad_norm(const py::object& grads) {
   return norm;
 }
 
+// Whether the values of two tensors of one shape lie in memory in the same
+// order, both without gaps if one is.
+bool same_layout(const Tensor& a, const Tensor& b) {
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+  return true;
+}
+
 // A scalar that is a number, or one float32 on the device.
 const float* device_scalar(const py::object& o, const char* what, const c10::Device& home, double* number) {
   if (!THPVariable_Check(o.ptr())) {
@@ -751,7 +770,7 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
   std::vector<const void*> addresses;
   std::vector<const Tensor*> used, written;
   std::vector<Tensor> held;
-  addresses.reserve(count);
+  addresses.reserve(3 * count);
   used.reserve(count);
   written.reserve(count);
   c10::Device home(c10::DeviceType::CPU);
@@ -780,9 +799,9 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
     const Tensor* grad = gi;
     if (!pi->is_contiguous() || !mi->is_contiguous() || !vi->is_contiguous() || !gi->is_contiguous()) {
       // values are taken in memory order: one order for all four
-      if (!pi->is_non_overlapping_and_dense() || mi->strides() != pi->strides() || vi->strides() != pi->strides())
+      if (!pi->is_non_overlapping_and_dense() || !same_layout(*mi, *pi) || !same_layout(*vi, *pi))
         refuse("parameter ", i, " must be dense in memory, and its moments laid out as it is");
-      if (gi->strides() != pi->strides()) {
+      if (!same_layout(*gi, *pi)) {
         held.push_back(at::empty_strided(pi->sizes(), pi->strides(), gi->options()).copy_(gi->detach()));
         grad = &held.back();
       }
@@ -790,11 +809,11 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
     if (n == 0) continue;
     by_type[dtype_slot(*pi)].push_back({pi->data_ptr(), grad->data_ptr(), mi->data_ptr(), vi->data_ptr(),
                                         eight ? static_cast<float*>(si->data_ptr()) : nullptr, n});
-    addresses.push_back(pi->data_ptr());
+    for (const Tensor* t : {pi, mi, vi}) addresses.push_back(t->data_ptr());
     used.push_back(gi);
     written.push_back(pi);
   }
-  if (!distinct(addresses)) refuse("a parameter occurs twice in one AdamW step");
+  if (!distinct(addresses)) refuse("a parameter or a moment occurs twice in one AdamW step");
   convrot_adamw_options o = {};
   if (used.empty()) {
     if (max_norm) refuse("clipping needs at least one gradient");

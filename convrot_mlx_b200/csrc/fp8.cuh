@@ -59,8 +59,8 @@ __device__ __forceinline__ void load_chunk(const T* row, int c, int features, fl
   }
 }
 
-// The same of rows that start on multiples of 16 bytes, by whole 16 bytes
-// wherever a row ends.
+// The same of rows that start and end on multiples of 16 bytes, wherever in the
+// 16 values a row ends.
 template <typename T>
 __device__ __forceinline__ void load_pieces(const T* row, int c, int features, float (&v)[kChunk]) {
   constexpr int W = 16 / sizeof(T);

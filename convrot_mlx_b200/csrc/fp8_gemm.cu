@@ -736,8 +736,8 @@ __device__ __forceinline__ uint2 halves_of(uint32_t w) {
   return r;
 }
 
-// 16 bytes of a row of codes with those past `count` cleared (a pitch is of
-// whole 16 bytes, so that they can be read).
+// 16 bytes of a row of codes with those past `count` cleared (rows are on a
+// pitch of whole 16 bytes, and all of them can be read).
 __device__ __forceinline__ uint4 only(uint4 v, int count) {
   uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -1144,7 +1144,7 @@ int convrot_fp8_linear(const void* x, int x_dtype, int64_t x_stride, const uint8
   // One or two tokens: quantized inside the product, one kernel instead of two.
   const int64_t x_size = valid_dtype(x_dtype) ? static_cast<int64_t>(dtype_size(x_dtype)) : 1;
   if (m > 0 && m <= fp8::gemv::kMaxFused && x_dtype == out_dtype && fp8::gemv_takes(layout, m, k) && aligned_to(x, 16) &&
-      x_stride * x_size % 16 == 0) {
+      x_stride * x_size % 16 == 0 && k * x_size % 16 == 0) {
     CONVROT_REQUIRE(x != nullptr && x_stride >= k, CONVROT_ERR_INVALID, "null pointer, or a row stride below k");
     const fp8::Params p = fp8::params_of(c, nullptr, false);
     cudaStream_t s = static_cast<cudaStream_t>(stream);

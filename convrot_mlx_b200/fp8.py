@@ -31,12 +31,13 @@ def _spans(n: int) -> int:
 
 
 def _padded_codes(codes: torch.Tensor) -> torch.Tensor:
-    """Rows of codes on a pitch of a multiple of 16 bytes (a copy only when they are not)."""
+    """Rows of codes on a pitch of a multiple of 16 bytes, the last one's padding too (a copy only when they are not)."""
 
-    if codes.stride(1) == 1 and codes.stride(0) >= codes.shape[1] and codes.stride(0) % _PITCH == 0 \
-            and codes.data_ptr() % _PITCH == 0:
-        return codes
     rows, features = codes.shape
+    if codes.stride(1) == 1 and codes.stride(0) >= features and codes.stride(0) % _PITCH == 0 \
+            and codes.data_ptr() % _PITCH == 0 and codes.untyped_storage().nbytes() >= \
+            codes.storage_offset() + (rows - 1) * codes.stride(0) + -(-features // _PITCH) * _PITCH:
+        return codes
     out = torch.empty((rows, -(-features // _PITCH) * _PITCH), dtype=codes.dtype, device=codes.device)[:, :features]
     return out.copy_(codes)
 

@@ -138,6 +138,11 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict) -> None:
         """Load a state of this class, or with ``state_bits`` 32 of ``torch.optim.AdamW``; moments keep their types."""
 
+        for group in state_dict["param_groups"]:
+            if group.get("amsgrad") or group.get("maximize"):
+                raise ValueError("this AdamW has neither amsgrad nor maximize")
+            if group.get("decoupled_weight_decay") is False and group["weight_decay"] != 0:
+                raise ValueError("this AdamW's weight decay is decoupled, that of the state is not")
         super().load_state_dict(state_dict)
         ids = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)

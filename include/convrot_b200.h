@@ -423,7 +423,8 @@ int convrot_quantize_fp8_weight(const void* w, int dtype, int64_t rows, int64_t 
  * input); wscales: one byte for each 128 x 128 block of the matrix as it
  * lies, rows of them at wscales_stride bytes.  Scales are the bytes of the
  * quantizers above.  Row strides of codes are multiples of 16 and cover the
- * rows; m, n and k are below 2^22.  bias may be NULL (zeros).  The order of
+ * rows, and the rows are read in whole 16 bytes, the last one too (what is
+ * behind its end is not used); m, n and k are below 2^22.  bias may be NULL (zeros).  The order of
  * the sums is fixed by the shape, the layout and the number of SMs.  No
  * reference counterpart.
  */

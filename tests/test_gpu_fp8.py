@@ -117,6 +117,25 @@ def test_linear(dtype, m, k, n):
     assert_no_device_error()
 
 
+@pytest.mark.parametrize("m,k,n", [(30, 8192, 100), (30, 8193, 100), (300, 20000, 40), (4, 17000, 33)])
+def test_float32_outputs_over_long_sums(m, k, n):
+    # ranges of 8192 channels: each 256 steps, as product64 counts them, and the additions of the ranges
+    qweight, wscales = _weights(n, k, 15)
+    bias = randn((n,), torch.float32, 16)
+    x = _uneven((m, k), torch.float32, 17).requires_grad_()
+    y = cr.fp8_linear(x, qweight, wscales, bias)
+    a, w = values_of_rows(*cr.quantize_fp8_blockwise(x)), values_of_blocks(qweight, wscales)
+    want, _ = product64(a, w, bias)
+    slack = (256 + 32 + 4) * 2.0 ** -22 * (a.abs() @ w.abs().T) + 2.0 ** -22 * want.abs()
+    assert_within(y.detach(), want, slack)
+    dy = _uneven((k, m), torch.float32, 18).t()[:, :].contiguous()
+    back, bscales = cr.quantize_fp8_weight(w.T.float())  # a weight of k channels: the gradient sums over them
+    z = torch.zeros((m, n), device=dev(), requires_grad=True)
+    (dz,) = torch.autograd.grad(cr.fp8_linear(z, back, bscales), z, dy)
+    a, w = values_of_rows(*cr.quantize_fp8_blockwise(dy)), values_of_blocks(back, bscales)
+    assert_within(dz, a @ w, (256 + 32 + 4) * 2.0 ** -22 * (a.abs() @ w.abs()) + 2.0 ** -22 * (a @ w).abs())
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,k,n", SIZES)
 def test_input_gradient(dtype, m, k, n):
@@ -183,6 +202,25 @@ def test_matmul_copies_rows_off_the_pitch():
     for a, b, s in ((odd, w.contiguous(), scales), (codes.t().contiguous().t(), w, packed), (codes, w, packed)):
         assert torch.equal(cr.fp8_matmul(a, b, s.view(torch.float8_e8m0fnu), ws, output_dtype=torch.float32), want)
     assert cr.fp8_matmul(codes[:0], w, xs[:0], ws, output_dtype=torch.bfloat16).shape == (0, 50)
+
+
+@pytest.mark.parametrize("m", [1, 5, 40])
+def test_weights_whose_storage_ends_with_the_last_row(m):
+    # the padding of the rows holds NaN codes, that of the last row is not there
+    n, k = 70, 203
+    w, ws = _weights(n, k, 43)
+    x = randn((m, k), torch.bfloat16, 44)
+    want = cr.fp8_linear(x, w, ws)
+    short = torch.full(((n - 1) * 208 + k,), 127, dtype=torch.uint8, device=dev()).view(torch.float8_e4m3fn)
+    short = short.as_strided((n, k), (208, 1))
+    short.copy_(w)
+    assert torch.equal(cr.fp8_linear(x, short, ws), want)
+    padded = torch.full((n, 208), 255, dtype=torch.uint8, device=dev()).view(torch.float8_e4m3fn)[:, :k]
+    padded.copy_(w)
+    assert torch.equal(cr.fp8_linear(x, padded, ws), want)
+    codes, xs = cr.quantize_fp8_blockwise(x)
+    assert torch.equal(cr.fp8_matmul(codes, short, xs, ws, output_dtype=torch.bfloat16),
+                       cr.fp8_matmul(codes, w, xs, ws, output_dtype=torch.bfloat16))
 
 
 @pytest.mark.parametrize("m", [3, 12, 200, 3000])

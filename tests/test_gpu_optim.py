@@ -450,5 +450,21 @@ def test_refusals():
         cr.adamw_step([base[:, :5]], [base[:, 5:10]], [base[:, 10:15]], [base[:, 15:]], None, 1, **HOW)
     with pytest.raises(ValueError, match="one float32"):
         run(step=torch.tensor(1, device=dev()))
-    kept = params[0].clone()
-    assert torch.equal(kept, params[0])
+    with pytest.raises(ValueError, match="twice"):
+        run(m=[ms[0], ms[1]], v=[ms[0], vs[1]])
+    p = [torch.nn.Parameter(torch.zeros(4, device=dev()))]
+    for other in (torch.optim.AdamW(p, amsgrad=True), torch.optim.AdamW(p, maximize=True), torch.optim.Adam(p, weight_decay=0.1)):
+        p[0].grad = torch.ones(4, device=dev())
+        other.step()
+        with pytest.raises(ValueError, match="this AdamW"):
+            cr.AdamW(p).load_state_dict(other.state_dict())
+
+
+def test_dimensions_of_one_may_have_any_stride():
+    p, g, m, v = (randn((40,), torch.float32, i).as_strided((1, 40), (s, 1)) for i, s in enumerate((7, 1, 40, 3)))
+    v = v.square()
+    q = [t.clone().reshape(40) for t in (p, g, m, v)]
+    g2 = torch.stack((g[0], g[0]), 1)[:, 0].reshape(1, 40)  # not contiguous: copied
+    cr.adamw_step([p], [g2], [m], [v], None, 3, **HOW)
+    cr.adamw_step([q[0]], [q[1]], [q[2]], [q[3]], None, 3, **HOW)
+    assert torch.equal(p[0], q[0]) and torch.equal(m[0], q[2])
