@@ -7,6 +7,8 @@
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -274,17 +276,23 @@ Tensor whole_rows(const Tensor& codes) {
   return out;
 }
 
-struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& qweight, const Tensor& wscales,
-                        const std::optional<Tensor>& bias) {
-    ctx->save_for_backward({qweight, wscales});
-    return fp8_product(x, qweight, CONVROT_LAYOUT_NK, wscales, or_undefined(bias), qweight.size(0));
-  }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+// The gradient of the input; a node of its own, which costs a small call less
+// than torch::autograd::Function.
+struct Fp8LinearBackward : torch::autograd::Node {
+  torch::autograd::SavedVariable qweight, wscales;
+  variable_list apply(variable_list&& grads) override {
     once("fp8_linear");
-    const auto saved = ctx->get_saved_variables();
-    return {fp8_product(grads[0], saved[0], CONVROT_LAYOUT_KN, saved[1], {}, saved[0].size(1)), {}, {}, {}};
+    const std::lock_guard<std::mutex> lock(mutex_);
+    if (!grads[0].defined()) return {Tensor()};
+    const Tensor w = qweight.unpack(), ws = wscales.unpack();
+    return {fp8_product(grads[0], w, CONVROT_LAYOUT_KN, ws, {}, w.size(1))};
   }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    qweight.reset_data();
+    wscales.reset_data();
+  }
+  std::string name() const override { return "Fp8LinearBackward"; }
 };
 
 Tensor fp8_linear(const Tensor& x, const Tensor& qweight, const Tensor& wscales, const std::optional<Tensor>& bias) {
@@ -307,9 +315,18 @@ Tensor fp8_linear(const Tensor& x, const Tensor& qweight, const Tensor& wscales,
   no_tangents("fp8_linear", {&x, &b});
   require_cuda({&x, &qweight, &wscales, &b});
   const Tensor w = whole_rows(qweight), ws = wscales.contiguous(), fb = f32_vector(b);
-  if (at::GradMode::is_enabled() && x.requires_grad())
-    return Fp8Linear::apply(x, w, ws, fb.defined() ? std::optional<Tensor>(fb) : std::nullopt);
-  return fp8_product(x, w, CONVROT_LAYOUT_NK, ws, fb, n);
+  if (!at::GradMode::is_enabled() || !x.requires_grad()) return fp8_product(x, w, CONVROT_LAYOUT_NK, ws, fb, n);
+  const std::shared_ptr<Fp8LinearBackward> node(new Fp8LinearBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(x));
+  node->qweight = torch::autograd::SavedVariable(w, /*is_output=*/false);
+  node->wscales = torch::autograd::SavedVariable(ws, /*is_output=*/false);
+  Tensor y;
+  {
+    const at::NoGradGuard no_grad;
+    y = fp8_product(x, w, CONVROT_LAYOUT_NK, ws, fb, n);
+  }
+  torch::autograd::set_history(y, node);
+  return y;
 }
 
 // --- rotary -------------------------------------------------------------------

@@ -269,6 +269,26 @@ def test_leading_dimensions_empty_rows_and_expanded_gradients():
         torch.autograd.grad(cr.fp8_linear(xr, qweight, wscales).sum(), xr, create_graph=True)
 
 
+def test_graphs_kept_released_and_changed():
+    qweight, wscales = _weights(48, 80, 53)
+    x = randn((7, 80), torch.bfloat16, 54).requires_grad_()
+    y = cr.fp8_linear(x, qweight, wscales)
+    dy = torch.ones_like(y)
+    (a,) = torch.autograd.grad(y, x, dy, retain_graph=True)
+    (b,) = torch.autograd.grad(y, x, dy)
+    assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, x, dy)
+    y = cr.fp8_linear(x, qweight, wscales)
+    qweight.view(torch.uint8).zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, x, dy)
+    cr.fp8_linear(x, qweight, wscales).sum().backward()
+    assert x.grad.eq(0).all()
+    with torch.no_grad():
+        assert not cr.fp8_linear(x, qweight, wscales).requires_grad
+
+
 def test_strided_inputs_and_gradients():
     qweight, wscales = _weights(200, 300, 55)
     base = randn((64, 700), torch.float16, 56)
