@@ -20,67 +20,48 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
   return static_cast<uint32_t>(max(e, 0));
 }
 
-// 2^-e for the scale byte e + 127; 0 where the block is not finite.  (Bytes
-// are at most 247: 448 * 2^120 is above every float32.)
-__device__ __forceinline__ float inverse_of(uint32_t byte) {
-  return byte == 255u ? 0.0f : __uint_as_float((254u - byte) << 23);
-}
-
-// Two codes, a in the low byte.  The product is exact, at most 448.
-__device__ __forceinline__ uint32_t code_pair(float a, float b) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
-  return r;
-}
-
-__device__ __forceinline__ uint4 codes_of(const float (&v)[kChunk], uint32_t byte) {
-  const float f = inverse_of(byte);
+// The codes of 16 values: e4m3(v * 2^-e) for the scale byte e + 127, the first
+// in the lowest byte.  (Bytes are at most 247: 448 * 2^120 is above every
+// float32; the product is exact, at most 448.)  0 where the block is not finite.
+__device__ __forceinline__ uint4 codes_of(const P2 (&v)[kChunk / 2], uint32_t byte) {
+  if (byte == 255u) return make_uint4(0u, 0u, 0u, 0u);
+  const float inverse = __uint_as_float((254u - byte) << 23);
+  const P2 f = p2(inverse, inverse);
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float s[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = byte == 255u ? 0.0f : __fmul_rn(v[4 * i + j], f);  // inf * 0 is no 0
-    w[i] = code_pair(s[0], s[1]) | code_pair(s[2], s[3]) << 16;
+    const float2 a = p2_get(mul(v[2 * i], f)), b = p2_get(mul(v[2 * i + 1], f));
+    asm("{\n\t.reg .b16 lo, hi;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(w[i])
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// 16 values of a row of `features` values from c on; 0 past its end.
+// 16 values of a row of `features` values from c on; 0 past its end.  WHOLE:
+// rows start on multiples of 16 bytes.
 template <typename T, bool WHOLE>
-__device__ __forceinline__ void load_chunk(const T* row, int c, int features, float (&v)[kChunk]) {
-  if (WHOLE && c + kChunk <= features) {
-    Pack<T, kChunk> p;
-    p.load_ahead(row + c);
-    p.get(v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) v[i] = c + i < features ? Elem<T>::to_f(row[c + i]) : 0.0f;
-  }
+__device__ __forceinline__ void load_chunk(const T* row, int c, int features, Pack<T, kChunk>& w) {
+  if (WHOLE && c + kChunk <= features) w.load_ahead(row + c);
+  else w.load_part(row + c, features - c);
 }
 
 // The same of rows that start and end on multiples of 16 bytes, wherever in the
 // 16 values a row ends.
 template <typename T>
-__device__ __forceinline__ void load_pieces(const T* row, int c, int features, float (&v)[kChunk]) {
+__device__ __forceinline__ void load_pieces(const T* row, int c, int features, Pack<T, kChunk>& w) {
   constexpr int W = 16 / sizeof(T);
 #pragma unroll
   for (int j = 0; j < kChunk / W; ++j) {
-    Pack<T, W> w;
-    w.clear();
-    if (c + j * W < features) w.load_ahead(row + c + j * W);
-    float f[W];
-    w.get(f);
+    Pack<T, W> piece;
+    piece.clear();
+    if (c + j * W < features) piece.load_ahead(row + c + j * W);
 #pragma unroll
-    for (int i = 0; i < W; ++i) v[j * W + i] = c + j * W + i < features ? f[i] : 0.0f;
+    for (int i = 0; i < 4; ++i) w.w[4 * j + i] = piece.w[i];
   }
-}
-
-__device__ __forceinline__ uint32_t top_of(const float (&v)[kChunk]) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < kChunk; ++i) top = max(top, abs_bits(v[i]));
-  return top;
 }
 
 // The largest of the 8 threads that have a block, for all of them.

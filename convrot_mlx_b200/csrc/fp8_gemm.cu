@@ -858,10 +858,12 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_kernel(const GemvParams q) {
 #pragma unroll 1
         for (int i0 = 0; i0 < all; i0 += kThreads) {
           const int i = i0 + threadIdx.x, m = i / chunks, c = (i - m * chunks) * kChunk;
-          float v[kChunk];
-          load_pieces(static_cast<const TOut*>(q.x) + m * q.x_stride, c, i < all ? p.k : 0, v);
-          const uint32_t byte = scale_byte(span_max(top_of(v)));
+          Pack<TOut, kChunk> w;
+          load_pieces(static_cast<const TOut*>(q.x) + m * q.x_stride, c, i < all ? p.k : 0, w);
+          const uint32_t byte = scale_byte(span_max(w.top()));
           if (i < all) {
+            P2 v[kChunk / 2];
+            w.get_lanes(v);
             store_halves(tokens + m * pitch + 2 * c, codes_of(v, byte));
             if (c % kSpan == 0) xs[m * k_blocks + c / kSpan] = scale_of(byte);
           }

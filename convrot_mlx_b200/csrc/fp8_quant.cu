@@ -34,12 +34,15 @@ __global__ void __launch_bounds__(kThreads) quantize_rows(const QuantParams p) {
   const uint32_t row = unit / static_cast<uint32_t>(p.spans), span = unit - row * p.spans;
   const bool live = row < p.rows;
   const int c = static_cast<int>(span) * kSpan + static_cast<int>(threadIdx.x % kSpanThreads) * kChunk;
-  float v[kChunk] = {};
-  if (live) load_chunk<T, WHOLE>(static_cast<const T*>(p.x) + static_cast<int64_t>(row) * p.x_stride, c, p.features, v);
-  const uint32_t top = span_max(top_of(v));
+  Pack<T, kChunk> w;
+  w.clear();
+  if (live) load_chunk<T, WHOLE>(static_cast<const T*>(p.x) + static_cast<int64_t>(row) * p.x_stride, c, p.features, w);
+  const uint32_t top = span_max(w.top());
   if (!live) return;
   const uint32_t byte = scale_byte(top);
   // rows of codes are on a pitch of a multiple of 16 bytes: a chunk that begins inside a row ends inside its pitch
+  P2 v[kChunk / 2];
+  w.get_lanes(v);
   if (c < p.features)
     *reinterpret_cast<uint4*>(p.codes + static_cast<int64_t>(row) * p.codes_stride + c) = codes_of(v, byte);
   if (threadIdx.x % kSpanThreads == 0)
@@ -52,15 +55,16 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks(const QuantParams p)
   __shared__ uint32_t red[kThreads / 32];
   const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kSpan + threadIdx.x / kSpanThreads;
   const int c = blockIdx.x * kSpan + static_cast<int>(threadIdx.x % kSpanThreads) * kChunk;
-  float v[kTurns][kChunk] = {};
+  Pack<T, kChunk> w[kTurns];
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < kTurns; ++i) {
     const int64_t row = row0 + i * kRowsAt;
-    if (row < p.rows) load_chunk<T, WHOLE>(static_cast<const T*>(p.x) + row * p.x_stride, c, p.features, v[i]);
+    w[i].clear();
+    if (row < p.rows) load_chunk<T, WHOLE>(static_cast<const T*>(p.x) + row * p.x_stride, c, p.features, w[i]);
   }
 #pragma unroll
-  for (int i = 0; i < kTurns; ++i) top = max(top, top_of(v[i]));
+  for (int i = 0; i < kTurns; ++i) top = max(top, w[i].top());
   top = warp_max(top);
   if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = top;
   __syncthreads();
@@ -69,8 +73,10 @@ __global__ void __launch_bounds__(kThreads) quantize_blocks(const QuantParams p)
 #pragma unroll
   for (int i = 0; i < kTurns; ++i) {
     const int64_t row = row0 + i * kRowsAt;
+    P2 v[kChunk / 2];
+    w[i].get_lanes(v);
     if (row < p.rows && c < p.features)
-      *reinterpret_cast<uint4*>(p.codes + row * p.codes_stride + c) = codes_of(v[i], byte);
+      *reinterpret_cast<uint4*>(p.codes + row * p.codes_stride + c) = codes_of(v, byte);
   }
   if (threadIdx.x == 0) p.scales[blockIdx.y * p.scales_stride + blockIdx.x] = static_cast<uint8_t>(byte);
 }
