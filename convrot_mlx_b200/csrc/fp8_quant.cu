@@ -9,7 +9,11 @@
 //
 // Activations: blocks of 128 consecutive values of a row.  Eight threads a
 // block, 16 values a thread: 16 codes are one 16-byte store, and the maximum
-// is three exchanges.  Weights: blocks of 128 x 128, a CTA each.
+// is three exchanges.  Memory-bound: 7800 x 5120 bf16 in 18.6 us (6.4 TB/s, a
+// copy's 6.6; 23.9 with a select and a product for each value instead of paired
+// products), 1536 x 5120 in 3.9, 451 x 2203, whose rows start at any byte pair and
+// are read value by value, in 2.5.  Weights: blocks of 128 x 128, a CTA each, once
+// for a layer (13824 x 5120 in 52 us with cold caches).
 #include "fp8.cuh"
 
 namespace convrot {

@@ -3,19 +3,30 @@
 //
 //   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,
 //   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps),
-// all in float32, each operation rounded; p rounded once to its type.
+// all in float32.  The moments' products and sums are rounded one by one, so
+// that codes are what separate operations give; p is rounded once to its type,
+// its quotient good to 22 bits.
 // Moments in 32 bits are kept as they are.  In 8 bits m and r = sqrt(v) are
 // kept as e4m3 codes with a float32 scale for each 256 values of a tensor,
 // max|m| / 448 and max r / 448: a square would need twice the range, and a block
 // whose gradients grow or fade together follows its scale exactly, however small
-// a step changes it.  A root above 0 keeps a code above 0, since it divides.
+// a step changes it.  The update uses the moments before they are rounded; the
+// codes are rounded to nearest (2^-4 of a value at most), so a change of a value
+// against its block's largest is kept once it is more than half a step.  A root
+// above 0 keeps a code above 0, since it divides.
 //
 // Memory-bound.  The tensors' addresses and sizes are kernel parameters, so a
 // step needs no table on the device and can be captured.  A warp has 256
 // values at a time, 8 a lane, so the maximum over a block of 8-bit moments is one
 // exchange in the warp.  A CTA's 2048 values are of one tensor, so that all that
 // depends on the tensor is the same in its threads and costs no instruction of
-// theirs.
+// theirs.  Times of the step: 246M bf16 values with 8-bit moments 444 us (5.6
+// TB/s of a copy's 6.6), 62M float32 ones in 640 tensors with 8-bit moments 185
+// (5.5), 113M float32 with 32-bit moments 510 (6.2), six vectors 1.9.  With 8-bit
+// moments the instructions weigh as much as the memory (390 a warp and 256
+// values, issue 67% active): arithmetic is on pairs, one chunk ahead is in
+// registers (a ring in shared memory filled by cp.async: 550 instead of 454 us,
+// IEEE division and root: 1210).
 #include "rows.cuh"
 
 namespace convrot {
@@ -433,7 +444,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<T, BITS>) adamw_kernel(const _
 }
 
 // ---------------------------------------------------------------------------
-// Sums of squares.  A thread adds 32 squares in float32, in four sums of eight
+// Sums of squares: 62M float32 values in 640 tensors in 40.8 us (6.2 TB/s), 246M
+// bf16 values in 87 (5.7).  A thread adds 32 squares in float32, in four sums of eight
 // and these in pairs, and the total to a 64-bit one; where a sum of eight leaves
 // the range of float32 (not finite, or so small that squares may have been lost)
 // the squares are formed in 64 bits.  Each CTA writes one sum, of a share that depends on the sizes alone.
