@@ -83,6 +83,9 @@ class AdamW(torch.optim.Optimizer):
         self.last_norm: torch.Tensor | None = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, capturable=capturable))
 
+    def __getstate__(self) -> dict:  # of copies and saved optimizers
+        return {**super().__getstate__(), "state_bits": self.state_bits, "max_norm": self.max_norm, "last_norm": None}
+
     def _start(self, p: torch.Tensor) -> dict:
         state = self.state[p]
         if not state:

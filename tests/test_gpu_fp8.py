@@ -333,6 +333,26 @@ def test_other_stream():
         assert torch.equal(got, want)
 
 
+def test_calls_at_once():
+    # products of every kernel on two streams, one after the other without waiting
+    qweight, wscales = _weights(520, 1040, 77)
+    inputs = [[randn((m, 1040), torch.bfloat16, 78 + m + i) for m in (1, 7, 40, 300, 3000)] for i in range(2)]
+    want = [[cr.fp8_linear(x, qweight, wscales) for x in xs] for xs in inputs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        got = [[], []]
+        for j in range(5):
+            for i, stream in enumerate(streams):
+                with torch.cuda.stream(stream):
+                    got[i].append(cr.fp8_linear(inputs[i][j], qweight, wscales))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for xs, ys in zip(got, want) for a, b in zip(xs, ys))
+    assert_no_device_error()
+
+
 def test_captured_forward_and_backward():
     qweight, wscales = _weights(264, 520, 73)
     for m in (2, 64, 1100):

@@ -8,6 +8,7 @@ quotient of two units in the last place: 16 U in all beside m's.  The parameter:
 from __future__ import annotations
 
 import copy
+import io
 import math
 
 import pytest
@@ -369,6 +370,42 @@ def test_optimizer_state_dict(dtype, bits):
     assert all(torch.equal(p, q) for p, q in zip(params, others))
     with pytest.raises(ValueError, match="not kept in"):
         cr.AdamW(others, state_bits=40 - bits).load_state_dict(saved)
+
+
+def test_copies_and_saves_of_the_optimizer():
+    params = _parameters()
+    a = cr.AdamW(params, state_bits=8, max_norm=1.0)
+    _set_grads(params, 450)
+    a.step()
+    file = io.BytesIO()  # pickle alone does not take torch's 8-bit floats
+    torch.save(a, file)
+    file.seek(0)
+    for b in (copy.deepcopy(a), torch.load(file, weights_only=False)):
+        others = b.param_groups[0]["params"]
+        assert (b.state_bits, b.max_norm) == (8, 1.0) and all(torch.equal(p, q) for p, q in zip(params, others))
+        _set_grads(others, 460)
+        b.step()
+    _set_grads(params, 460)
+    a.step()
+    assert all(torch.equal(p, q) for p, q in zip(params, others))
+    assert all(torch.equal(a.state[p]["scales"], b.state[q]["scales"]) for p, q in zip(params, others))
+
+
+def test_two_steps_at_once():
+    # two streams, each with tensors of its own, one after the other without waiting
+    states = [_state([(100_000,), (333, 77)], torch.bfloat16, 8, 1200 + i) for i in range(2)]
+    want = copy.deepcopy(states)
+    for s in want:
+        cr.adamw_step(*s, 7, max_norm=1.0, **HOW)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream())
+    for s, stream in zip(states, streams):
+        with torch.cuda.stream(stream):
+            cr.adamw_step(*s, 7, max_norm=1.0, **HOW)
+    torch.cuda.synchronize()
+    for s, w in zip(states, want):
+        assert all(torch.equal(a, b) for a, b in zip(s[0], w[0])) and all(torch.equal(a, b) for a, b in zip(s[4], w[4]))
 
 
 def test_clipping_over_groups():
