@@ -65,7 +65,7 @@ SIGNATURES: dict[str, tuple] = {
     "convrot_fp8_linear": (_I, [_P, _I, _I64, _P, _I64, _I, _P, _I64, _P, _P, _I, _I64, _I64, _I64, _P, _I64, _P, _I64,
                                 _P]),
     "convrot_square_sums_count": (_I64, [_I64, _P]),
-    "convrot_square_sums": (_I, [_I64, _P, _I, _P, _I64, _P]),
+    "convrot_square_sums": (_I, [_I64, _P, _I, _P, _I64, _P, _P]),
     "convrot_norm_of_sums": (_I, [_P, _I64, _P, _P]),
     "convrot_adamw": (_I, [_I64, _P, _I, _I, _P, _P]),
     "convrot_set_gemm_route": (_I, [_I]),

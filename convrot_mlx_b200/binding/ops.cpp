@@ -667,41 +667,46 @@ int dtype_slot(const Tensor& t) { return dtype_code(t.scalar_type()); }  // 0, 1
 // t where its values are dense in memory in some order, else packed.
 Tensor dense(const Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_and_dense() ? t : t.contiguous(); }
 
-// Partial sums of the squares of gradients of any of the three types, all on
-// one device, in one tensor; None is passed over.
-Tensor square_sums_of(const std::vector<const Tensor*>& grads) {
+// Gradients of one device as the sums of squares take them, by type.
+struct GradLists {
   std::vector<convrot_grad_tensor> by_type[3];
   std::vector<Tensor> held;
-  const Tensor& first = *grads.front();
-  require_cuda({&first});
-  const c10::Device home = first.device();
-  for (const Tensor* g : grads) {
-    if (g->layout() != at::kStrided) refuse("gradients must be dense tensors");
-    if (g->device() != home) refuse("expected all tensors on ", home.str(), ", got one on ", g->device().str());
-    const int slot = dtype_slot(*g);
-    if (g->is_contiguous()) {
-      by_type[slot].push_back({g->data_ptr(), g->numel()});
-    } else {
-      held.push_back(dense(*g));
-      by_type[slot].push_back({held.back().data_ptr(), g->numel()});
+  c10::Device home;
+
+  explicit GradLists(const std::vector<const Tensor*>& grads) : home(grads.front()->device()) {
+    require_cuda({grads.front()});
+    for (const Tensor* g : grads) {
+      if (g->layout() != at::kStrided) refuse("gradients must be dense tensors");
+      if (g->device() != home) refuse("expected all tensors on ", home.str(), ", got one on ", g->device().str());
+      const Tensor* t = g;
+      if (!g->is_contiguous()) {
+        held.push_back(dense(*g));
+        t = &held.back();
+      }
+      by_type[dtype_slot(*g)].push_back({t->data_ptr(), t->numel()});
     }
   }
-  const c10::cuda::OptionalCUDAGuard guard(home);
+  int64_t count(int type) const { return static_cast<int64_t>(by_type[type].size()); }
+};
+
+// Partial sums of the squares of gradients of any of the three types in one
+// tensor.
+Tensor sums_of(const GradLists& lists, const Tensor& like) {
+  const c10::cuda::OptionalCUDAGuard guard(lists.home);
   int64_t counts[3] = {}, total = 0;
   for (int i = 0; i < 3; ++i)
-    if (!by_type[i].empty())
-      total += counts[i] = convrot_square_sums_count(static_cast<int64_t>(by_type[i].size()), by_type[i].data());
-  const Tensor sums = at::empty({total}, first.options().dtype(at::kDouble).requires_grad(false));
+    if (lists.count(i)) total += counts[i] = convrot_square_sums_count(lists.count(i), lists.by_type[i].data());
+  const Tensor sums = at::empty({total}, like.options().dtype(at::kDouble).requires_grad(false));
   auto* at = static_cast<double*>(sums.data_ptr());
   for (int i = 0; i < 3; ++i) {
     if (!counts[i]) continue;
-    check(convrot_square_sums(static_cast<int64_t>(by_type[i].size()), by_type[i].data(), i, at, counts[i],
-                              stream_of(first)),
+    check(convrot_square_sums(lists.count(i), lists.by_type[i].data(), i, at, counts[i], nullptr, stream_of(like)),
           "convrot_square_sums");
     at += counts[i];
   }
   return sums;
 }
+Tensor square_sums_of(const std::vector<const Tensor*>& grads) { return sums_of(GradLists(grads), *grads.front()); }
 
 std::vector<const Tensor*> present(const TensorList& list) {
   std::vector<const Tensor*> out;
@@ -718,15 +723,31 @@ Tensor square_sums(const py::object& grads) {
   return square_sums_of(present(list));
 }
 
+// Chunks of 2048 values whose norm is one launch's: 8 CTAs with 16 each.
+constexpr int64_t kOneLaunch = 128;
+
 Tensor grad_norm(const py::object& grads) {
   const at::NoGradGuard no_grad;
   const TensorList list(grads, "gradients");
   const std::vector<const Tensor*> tensors = present(list);
-  const Tensor sums = square_sums_of(tensors);
-  const c10::cuda::OptionalCUDAGuard guard(sums.device());
-  const Tensor norm = at::empty({}, sums.options().dtype(at::kFloat));
-  check(convrot_norm_of_sums(static_cast<const double*>(sums.data_ptr()), sums.numel(),
-                             static_cast<float*>(norm.data_ptr()), stream_of(sums)),
+  const GradLists lists(tensors);
+  const Tensor& first = *tensors.front();
+  const c10::cuda::OptionalCUDAGuard guard(lists.home);
+  const Tensor norm = at::empty({}, first.options().dtype(at::kFloat).requires_grad(false));
+  auto* to = static_cast<float*>(norm.data_ptr());
+  const int type = dtype_slot(first);
+  if (lists.count(type) == static_cast<int64_t>(tensors.size()) && lists.count(type) <= 1024) {
+    int64_t chunks = 0;
+    for (const convrot_grad_tensor& t : lists.by_type[type]) chunks += (t.numel + 2047) / 2048;
+    if (chunks <= kOneLaunch) {
+      check(convrot_square_sums(lists.count(type), lists.by_type[type].data(), type, nullptr,
+                                std::max<int64_t>(1, std::min<int64_t>(8, (chunks + 3) / 4)), to, stream_of(first)),
+            "convrot_square_sums");
+      return norm;
+    }
+  }
+  const Tensor sums = sums_of(lists, first);
+  check(convrot_norm_of_sums(static_cast<const double*>(sums.data_ptr()), sums.numel(), to, stream_of(sums)),
         "convrot_norm_of_sums");
   return norm;
 }

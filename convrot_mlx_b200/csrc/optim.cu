@@ -445,7 +445,8 @@ __global__ void __launch_bounds__(kThreads, kCtas<T, BITS>) adamw_kernel(const _
 
 // ---------------------------------------------------------------------------
 // Sums of squares: 62M float32 values in 640 tensors in 40.8 us (6.2 TB/s), 246M
-// bf16 values in 87 (5.7).  A thread adds 32 squares in float32, in four sums of eight
+// bf16 values in 87 (5.7).  Up to 262144 values the norm is one launch of a
+// cluster (a call of 3.9 us, 7.2 as two launches).  A thread adds 32 squares in float32, in four sums of eight
 // and these in pairs, and the total to a 64-bit one; where a sum of eight leaves
 // the range of float32 (not finite, or so small that squares may have been lost)
 // the squares are formed in 64 bits.  Each CTA writes one sum, of a share that depends on the sizes alone.
@@ -462,6 +463,7 @@ struct NormTable {
   int count, add;  // add: to what an earlier launch has left
   uint32_t chunks;
   double* sums;
+  float* norm;  // of the sums, where the grid is one cluster
   NormEntry e[CAP];
 };
 
@@ -540,8 +542,22 @@ __global__ void __launch_bounds__(kThreads) square_sums(const __grid_constant__ 
     double v = t.add ? t.sums[blockIdx.x] : 0.0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) v += red[w];
-    t.sums[blockIdx.x] = v;
+    if (t.norm) red[0] = v;
+    else t.sums[blockIdx.x] = v;
   }
+  if (!t.norm) return;
+  // few values: the CTAs are one cluster, whose first adds up the sums of all
+  cluster_sync();
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    double v = 0.0;
+    for (uint32_t r = 0; r < gridDim.x; ++r) {
+      double part;
+      asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(part) : "r"(mapa_shared(&red[0], r)) : "memory");
+      v += part;
+    }
+    *t.norm = static_cast<float>(sqrt(v));
+  }
+  cluster_sync();  // no CTA leaves while its sum may still be read
 }
 
 __global__ void __launch_bounds__(kThreads) norm_kernel(const double* sums, int count, float* norm) {
@@ -561,16 +577,20 @@ constexpr int kSmall = 32, kLarge = 512;        // tensors of a launch
 constexpr int kNormSmall = 64, kNormLarge = 1024;
 
 template <typename K, typename A>
-int launch(K kernel, int64_t ctas, const A& args, cudaStream_t s, const char* what) {
+int launch(K kernel, int64_t ctas, const A& args, cudaStream_t s, const char* what, bool one_cluster = false) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = one_cluster ? 2 : 1;
   CONVROT_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args));
   return check_launch(what);
 }
@@ -626,9 +646,10 @@ int adamw_bits(int bits, const Scalars& s, const convrot_adamw_tensor* tensors, 
 }
 
 template <typename T, int CAP>
-int sums_part(const convrot_grad_tensor* tensors, int count, int64_t ctas, double* sums, bool add, cudaStream_t stream) {
+int sums_part(const convrot_grad_tensor* tensors, int count, int64_t ctas, double* sums, bool add, float* norm,
+              cudaStream_t stream) {
   NormTable<CAP> t;
-  t.count = count, t.add = add, t.sums = sums;
+  t.count = count, t.add = add, t.sums = sums, t.norm = norm;
   int64_t chunks = 0;
   for (int i = 0; i < count; ++i) {
     t.e[i].g = tensors[i].grad, t.e[i].n = tensors[i].numel;
@@ -637,15 +658,16 @@ int sums_part(const convrot_grad_tensor* tensors, int count, int64_t ctas, doubl
   }
   CONVROT_REQUIRE(chunks < (1LL << 31), CONVROT_ERR_UNSUPPORTED, "tensors too large");
   t.chunks = static_cast<uint32_t>(chunks);
-  return launch(square_sums<T, CAP>, ctas, t, stream, "sums of squares");
+  return launch(square_sums<T, CAP>, ctas, t, stream, "sums of squares", norm != nullptr);
 }
 
 template <typename T>
-int sums_all(const convrot_grad_tensor* tensors, int64_t count, int64_t ctas, double* sums, cudaStream_t stream) {
+int sums_all(const convrot_grad_tensor* tensors, int64_t count, int64_t ctas, double* sums, float* norm,
+             cudaStream_t stream) {
   for (int64_t at = 0; at < count || at == 0; at += kNormLarge) {
     const int n = static_cast<int>(count - at < kNormLarge ? count - at : kNormLarge);
-    const int rc = n <= kNormSmall ? sums_part<T, kNormSmall>(tensors + at, n, ctas, sums, at > 0, stream)
-                                   : sums_part<T, kNormLarge>(tensors + at, n, ctas, sums, at > 0, stream);
+    const int rc = n <= kNormSmall ? sums_part<T, kNormSmall>(tensors + at, n, ctas, sums, at > 0, norm, stream)
+                                   : sums_part<T, kNormLarge>(tensors + at, n, ctas, sums, at > 0, norm, stream);
     if (rc != CONVROT_OK) return rc;
   }
   return CONVROT_OK;
@@ -667,21 +689,23 @@ int64_t convrot_square_sums_count(int64_t count, const convrot_grad_tensor* tens
 }
 
 int convrot_square_sums(int64_t count, const convrot_grad_tensor* tensors, int dtype, double* sums, int64_t sums_count,
-                        void* stream) {
+                        float* norm, void* stream) {
   using namespace convrot;
   CONVROT_REQUIRE(valid_dtype(dtype), CONVROT_ERR_INVALID, "unknown dtype %d", dtype);
-  CONVROT_REQUIRE(count >= 0 && (count == 0 || tensors) && sums && aligned_to(sums, 8) && sums_count > 0 &&
+  CONVROT_REQUIRE(count >= 0 && (count == 0 || tensors) && (sums || norm) && aligned_to(sums, 8) && sums_count > 0 &&
                       sums_count <= (1 << 20),
                   CONVROT_ERR_INVALID, "invalid tensor list or sums");
+  CONVROT_REQUIRE(!norm || (sums_count <= 8 && count <= optim::kNormLarge), CONVROT_ERR_INVALID,
+                  "the norm takes at most 8 sums of at most %d tensors", optim::kNormLarge);
   for (int64_t i = 0; i < count; ++i)
     CONVROT_REQUIRE(tensors[i].numel >= 0 &&
                         (tensors[i].numel == 0 || (tensors[i].grad && aligned_to(tensors[i].grad, dtype_size(dtype)))),
                     CONVROT_ERR_INVALID, "tensor %lld: null or misaligned pointer, or negative size", static_cast<long long>(i));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case CONVROT_BF16: return optim::sums_all<__nv_bfloat16>(tensors, count, sums_count, sums, s);
-    case CONVROT_F16: return optim::sums_all<__half>(tensors, count, sums_count, sums, s);
-    default: return optim::sums_all<float>(tensors, count, sums_count, sums, s);
+    case CONVROT_BF16: return optim::sums_all<__nv_bfloat16>(tensors, count, sums_count, sums, norm, s);
+    case CONVROT_F16: return optim::sums_all<__half>(tensors, count, sums_count, sums, norm, s);
+    default: return optim::sums_all<float>(tensors, count, sums_count, sums, norm, s);
   }
 }
 

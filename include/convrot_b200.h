@@ -451,7 +451,9 @@ int convrot_fp8_linear(const void* x, int x_dtype, int64_t x_stride, const uint8
  * total; convrot_square_sums_count gives a good number of them for these
  * tensors.  Which values a sum holds depends on the sizes and sums_count alone.
  * convrot_norm_of_sums: sqrt of the total of sums (of several dtypes, one
- * after another in memory) as float32.  No reference counterpart.
+ * after another in memory) as float32.  With `norm` not NULL (at most 8 sums of at
+ * most 1024 tensors) convrot_square_sums writes the norm itself and no sums,
+ * which may then be NULL.  No reference counterpart.
  */
 typedef struct {
   const void* grad;
@@ -459,7 +461,7 @@ typedef struct {
 } convrot_grad_tensor;
 int64_t convrot_square_sums_count(int64_t count, const convrot_grad_tensor* tensors);
 int convrot_square_sums(int64_t count, const convrot_grad_tensor* tensors, int dtype, double* sums,
-                        int64_t sums_count, void* stream);
+                        int64_t sums_count, float* norm, void* stream);
 int convrot_norm_of_sums(const double* sums, int64_t sums_count, float* norm, void* stream);
 
 /*

@@ -251,7 +251,9 @@ def test_step_and_rate_on_the_device():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shapes", [[(1,)], [(5,), (0,), (256,)], [(1000, 1000)], [(i,) for i in range(1100)], [(3_000_001,)]])
+@pytest.mark.parametrize("shapes", [[(1,)], [(5,), (0,), (256,)], [(1000, 1000)], [(i,) for i in range(1100)], [(3_000_001,)],
+                                    [(2048 * 4 * n + 1,) for n in (0, 1, 2)], [(2048 * 128,)], [(2048 * 127 + 1,), (0,)],
+                                    [(2048 * 128 + 1,)], [(9, 100)] * 64, [(9, 100)] * 65, [(3,)] * 128, [(3,)] * 129])
 def test_grad_norm(dtype, shapes):
     grads = [randn(s, dtype, 31 + i) for i, s in enumerate(shapes)]
     exact = math.sqrt(sum(g.double().square().sum().item() for g in grads))

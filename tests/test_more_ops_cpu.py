@@ -137,10 +137,11 @@ def test_adamw_arguments(lib):
 
 def test_norm_arguments(lib):
     one = (_GradTensor * 1)(_GradTensor(4096, 10))
-    assert lib.convrot_square_sums(1, one, 3, FAKE, 1, None) == -1
-    assert lib.convrot_square_sums(1, one, 0, None, 1, None) == -1 and lib.convrot_square_sums(1, one, 0, FAKE, 0, None) == -1
-    assert lib.convrot_square_sums(1, (_GradTensor * 1)(_GradTensor(None, 10)), 0, FAKE, 1, None) == -1
-    assert lib.convrot_square_sums(1, (_GradTensor * 1)(_GradTensor(4097, 10)), 0, FAKE, 1, None) == -1
+    assert lib.convrot_square_sums(1, one, 3, FAKE, 1, None, None) == -1
+    assert lib.convrot_square_sums(1, one, 0, None, 1, None, None) == -1 and lib.convrot_square_sums(1, one, 0, FAKE, 0, None, None) == -1
+    assert lib.convrot_square_sums(1, (_GradTensor * 1)(_GradTensor(None, 10)), 0, FAKE, 1, None, None) == -1
+    assert lib.convrot_square_sums(1, (_GradTensor * 1)(_GradTensor(4097, 10)), 0, FAKE, 1, None, None) == -1
+    assert lib.convrot_square_sums(1, one, 0, None, 9, FAKE, None) == -1 and "at most 8" in _err(lib)
     assert lib.convrot_norm_of_sums(FAKE, 0, FAKE, None) == -1 and lib.convrot_norm_of_sums(None, 1, FAKE, None) == -1
     assert lib.convrot_square_sums_count(0, None) == 1
     assert lib.convrot_square_sums_count(1, (_GradTensor * 1)(_GradTensor(None, 256 * 8 * 3 + 1))) == 4
