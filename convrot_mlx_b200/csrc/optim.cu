@@ -446,10 +446,11 @@ __global__ void __launch_bounds__(kThreads, kCtas<T, BITS>) adamw_kernel(const _
 // ---------------------------------------------------------------------------
 // Sums of squares: 62M float32 values in 640 tensors in 40.8 us (6.2 TB/s), 246M
 // bf16 values in 87 (5.7).  Up to 262144 values the norm is one launch of a
-// cluster (a call of 3.9 us, 7.2 as two launches).  A thread adds 32 squares in float32, in four sums of eight
-// and these in pairs, and the total to a 64-bit one; where a sum of eight leaves
-// the range of float32 (not finite, or so small that squares may have been lost)
-// the squares are formed in 64 bits.  Each CTA writes one sum, of a share that depends on the sizes alone.
+// cluster (a call of 3.9 us, 7.2 as two launches).  A thread adds 32 squares in
+// float32, in four sums of eight and these in pairs, and the total to a 64-bit
+// one; where a sum of eight leaves the range of float32 (not finite, or so small
+// that squares may have been lost) the squares are formed in 64 bits.  Each CTA
+// writes one sum, of a share that depends on the sizes alone.
 
 struct NormEntry {
   const void* g;

@@ -54,6 +54,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
                                     weight_decay, max_norm, None)
 
 
+def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.shape == b.shape and all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW by ``adamw_step``: all parameters of a group in one launch.
 
@@ -146,21 +150,20 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("this AdamW has neither amsgrad nor maximize")
             if group.get("decoupled_weight_decay") is False and group["weight_decay"] != 0:
                 raise ValueError("this AdamW's weight decay is decoupled, that of the state is not")
-        super().load_state_dict(state_dict)
         ids = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
-        for key, p in zip(ids, params):
-            saved = state_dict["state"].get(key)
-            if not saved:
-                continue
+        loaded = [(p, state_dict["state"][key]) for key, p in zip(ids, params) if state_dict["state"].get(key)]
+        for p, saved in loaded:
             if ("scales" in saved) != (self.state_bits == 8):
                 raise ValueError(f"the state's moments are not kept in {self.state_bits} bits")
-            if self.state_bits == 8 and saved["exp_avg"].stride() != p.stride():
-                raise ValueError("8-bit moments were kept for a parameter of another memory layout")
+            if self.state_bits == 8 and not _same_layout(saved["exp_avg"], p):
+                raise ValueError("8-bit moments were kept for a parameter of another shape or memory layout")
+        super().load_state_dict(state_dict)
+        kind = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
+        for p, saved in loaded:  # the moments again, which the base class casts to the parameter's type
             state = {"step": int(saved["step"])}
             for name in ("exp_avg", "exp_avg_sq"):
                 # the parameter's own layout, whatever that of the saved tensor was
-                kind = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
                 state[name] = torch.empty_like(p, dtype=kind, memory_format=torch.preserve_format).copy_(saved[name])
             if self.state_bits == 8:
                 state["scales"] = saved["scales"].to(p.device, torch.float32, copy=True).contiguous()

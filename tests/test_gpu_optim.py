@@ -372,6 +372,12 @@ def test_optimizer_state_dict(dtype, bits):
     assert all(torch.equal(p, q) for p, q in zip(params, others))
     with pytest.raises(ValueError, match="not kept in"):
         cr.AdamW(others, state_bits=40 - bits).load_state_dict(saved)
+    if bits == 8:
+        turned = [torch.nn.Parameter(v.t().contiguous().t() if v.dim() == 2 else v) for v in values]
+        other = cr.AdamW(turned, state_bits=8)
+        with pytest.raises(ValueError, match="memory layout"):
+            other.load_state_dict(saved)
+        assert not other.state  # nothing is loaded by halves
 
 
 def test_copies_and_saves_of_the_optimizer():
