@@ -1015,10 +1015,10 @@ bool gemv_takes(int layout, int64_t m, int64_t k) {
          m * (2 * k + 2 * kBK + 16 + 4 * (k / kBK + 1)) <= gemv::kMaxBytes;  // no less than smem_of
 }
 
-// x quantized inside the product.
+// x quantized inside the product, which waits for the previous kernel of the
+// stream before it reads anything.
 template <typename T>
-int launch_fused(const void* x, int64_t x_stride, const Operands& o, Params p, cudaStream_t s) {
-  p.early_weights = 0;  // the previous kernel of the stream may have written them
+int launch_fused(const void* x, int64_t x_stride, const Operands& o, const Params& p, cudaStream_t s) {
   return launch_gemv<T, true>({p, x, nullptr, o.weight, x_stride, 0, o.weight_stride}, s);
 }
 
