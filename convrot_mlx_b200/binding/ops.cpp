@@ -809,6 +809,7 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
   std::vector<const Tensor*> used, written;
   std::vector<Tensor> held;
   addresses.reserve(3 * count);
+  for (auto& list : by_type) list.reserve(count);
   used.reserve(count);
   written.reserve(count);
   c10::Device home(c10::DeviceType::CPU);
@@ -819,7 +820,8 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
     if (!pi || !mi || !vi || !si) refuse("parameter ", i, " has a gradient, but a parameter, moment or scale is missing");
     if (used.empty()) home = pi->device();
     for (const Tensor* t : {pi, gi, mi, vi, si}) {
-      if (!t->is_cuda() || t->device() != home) require_cuda({used.empty() ? pi : written.front(), t});
+      const c10::Device at = t->device();
+      if (!at.is_cuda() || at != home) require_cuda({used.empty() ? pi : written.front(), t});
       if (t->layout() != at::kStrided) refuse("the AdamW step takes dense tensors");
     }
     if (gi->scalar_type() != pi->scalar_type() || gi->sizes() != pi->sizes())
@@ -845,9 +847,10 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
       }
     }
     if (n == 0) continue;
-    by_type[dtype_slot(*pi)].push_back({pi->data_ptr(), grad->data_ptr(), mi->data_ptr(), vi->data_ptr(),
-                                        eight ? static_cast<float*>(si->data_ptr()) : nullptr, n});
-    for (const Tensor* t : {pi, mi, vi}) addresses.push_back(t->data_ptr());
+    void *const p_at = pi->data_ptr(), *const m_at = mi->data_ptr(), *const v_at = vi->data_ptr();
+    by_type[dtype_slot(*pi)].push_back(
+        {p_at, grad->const_data_ptr(), m_at, v_at, eight ? static_cast<float*>(si->data_ptr()) : nullptr, n});
+    for (const void* at : {p_at, m_at, v_at}) addresses.push_back(at);
     used.push_back(gi);
     written.push_back(pi);
   }
