@@ -125,20 +125,26 @@ class AdamW(torch.optim.Optimizer):
                     if p.is_cuda and not group["capturable"] and torch.cuda.is_current_stream_capturing():
                         raise RuntimeError("a captured AdamW step needs capturable=True: its count has to be on the device")
                     state = self._start(p)
-                    state["step"] += 1
-                    runs.setdefault(0 if group["capturable"] else state["step"], []).append((p, state))
+                    runs.setdefault(0 if group["capturable"] else state["step"] + 1, []).append((p, state))
             if runs and group["capturable"]:
                 if "step" not in group:
                     first = next(iter(runs.values()))[0]
-                    group["step"] = torch.full((), float(first[1]["step"] - 1), device=first[0].device)
+                    group["step"] = torch.full((), float(first[1]["step"]), device=first[0].device)
                 group["step"].add_(1.0)
             for step, run in runs.items():
                 states = [state for _, state in run]
-                norm = ops.adamw_step([p for p, _ in run], [p.grad for p, _ in run], [s["exp_avg"] for s in states],
-                                      [s["exp_avg_sq"] for s in states],
-                                      [s["scales"] for s in states] if self.state_bits == 8 else None,
-                                      group["step"] if group["capturable"] else step, group["lr"], *group["betas"],
-                                      group["eps"], group["weight_decay"], self.max_norm, sums)
+                try:
+                    norm = ops.adamw_step([p for p, _ in run], [p.grad for p, _ in run], [s["exp_avg"] for s in states],
+                                          [s["exp_avg_sq"] for s in states],
+                                          [s["scales"] for s in states] if self.state_bits == 8 else None,
+                                          group["step"] if group["capturable"] else step, group["lr"], *group["betas"],
+                                          group["eps"], group["weight_decay"], self.max_norm, sums)
+                except (ValueError, NotImplementedError):  # refused: not a step
+                    if group["capturable"]:
+                        group["step"].sub_(1.0)
+                    raise
+                for state in states:
+                    state["step"] += 1
         self.last_norm = norm
         return loss
 

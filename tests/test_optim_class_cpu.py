@@ -1,0 +1,53 @@
+"""The optimizer class's own bookkeeping (no GPU needed): the step itself is a stand-in that records what it is given."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import convrot_mlx_b200 as cr
+from convrot_mlx_b200 import _native
+
+
+class Ops:
+    """What ``AdamW`` calls of the binding."""
+
+    def __init__(self):
+        self.steps = []
+        self.refusal = None
+
+    def square_sums(self, grads):
+        return torch.stack([g.double().square().sum() for g in grads])
+
+    def adamw_step(self, params, grads, exp_avgs, exp_avg_sqs, scales, step, lr, *how):
+        if self.refusal is not None:
+            raise self.refusal
+        self.steps.append(step.clone() if torch.is_tensor(step) else step)
+
+
+@pytest.fixture
+def ops(monkeypatch):
+    stand_in = Ops()
+    monkeypatch.setattr(_native, "ops", lambda: stand_in)
+    return stand_in
+
+
+def _parameters(shapes=((40, 30), (300,))):
+    params = [torch.nn.Parameter(torch.zeros(s)) for s in shapes]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    return params
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_refused_step_is_not_counted(ops, capturable):
+    params = _parameters()
+    optimizer = cr.AdamW(params, capturable=capturable)
+    optimizer.step()
+    ops.refusal = ValueError("refused")
+    with pytest.raises(ValueError, match="refused"):
+        optimizer.step()
+    assert all(optimizer.state[p]["step"] == 1 for p in params)
+    ops.refusal = None
+    optimizer.step()
+    assert [float(s) for s in ops.steps] == [1.0, 2.0] and all(optimizer.state[p]["step"] == 2 for p in params)
