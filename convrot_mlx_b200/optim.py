@@ -67,7 +67,8 @@ class AdamW(torch.optim.Optimizer):
     the norm of all gradients of all groups; ``last_norm`` is that of the last step, on
     the device.  ``capturable``: the step count of a group is on the device
     (``group["step"]``), so that a graph that captured ``step`` counts on as it
-    is replayed; all its parameters share it.  ``lr`` may be one float32 on the
+    is replayed; all its parameters share it, and ``load_state_dict`` takes it from
+    the state, as all options of a group.  ``lr`` may be one float32 on the
     device.  All parameters lie on one CUDA device."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
@@ -104,6 +105,13 @@ class AdamW(torch.optim.Optimizer):
                 state["scales"] = torch.zeros((-(-p.numel() // MOMENT_BLOCK), 2), dtype=torch.float32, device=p.device)
         return state
 
+    def _put_count_on_device(self, group: dict) -> None:
+        started = [p for p in group["params"] if self.state.get(p)]
+        if started[0].is_cuda and torch.cuda.is_current_stream_capturing():  # each replay would set the count again
+            raise RuntimeError("AdamW puts its count on the device in a step of its own: take one before the capture")
+        count = max(self.state[p]["step"] for p in started)
+        group["step"] = torch.full((), float(count), device=started[0].device)
+
     @torch.no_grad()
     def step(self, closure=None):
         """One step; returns the closure's loss, if there is one."""
@@ -127,9 +135,8 @@ class AdamW(torch.optim.Optimizer):
                     state = self._start(p)
                     runs.setdefault(0 if group["capturable"] else state["step"] + 1, []).append((p, state))
             if runs and group["capturable"]:
-                if "step" not in group:
-                    first = next(iter(runs.values()))[0]
-                    group["step"] = torch.full((), float(first[1]["step"]), device=first[0].device)
+                if not torch.is_tensor(group.get("step")):
+                    self._put_count_on_device(group)
                 group["step"].add_(1.0)
             for step, run in runs.items():
                 states = [state for _, state in run]
@@ -178,3 +185,5 @@ class AdamW(torch.optim.Optimizer):
             group.setdefault("capturable", False)
             if torch.is_tensor(group.get("step")):
                 group["step"] = group["step"].to(group["params"][0].device, torch.float32, copy=True)
+            elif group["capturable"] and any(self.state.get(p) for p in group["params"]):
+                self._put_count_on_device(group)

@@ -1,0 +1,73 @@
+"""The optimizer class on the device: counts in captured steps, states loaded and saved between them."""
+
+from __future__ import annotations
+
+import copy
+
+import pytest
+import torch
+
+import convrot_mlx_b200 as cr
+from tests.gpu_util import dev
+from tests.ops64 import U, randn
+
+pytestmark = pytest.mark.gpu
+
+
+def _parameters(seed=1, shapes=((40, 30), (300,), (7, 9, 11))):
+    return [torch.nn.Parameter(randn(s, torch.float32, seed + i)) for i, s in enumerate(shapes)]
+
+
+def _set_grads(params, seed):
+    for i, p in enumerate(params):
+        g = randn(p.shape, p.dtype, seed + i)
+        if p.grad is None:
+            p.grad = g
+        else:
+            p.grad.copy_(g)
+
+
+def _captured(optimizer):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        optimizer.step()
+    return graph
+
+
+def test_capture_right_after_loading():
+    # torch's state has no count of the group: each replay has to count on from the parameters' own
+    params, eager = _parameters(), _parameters()
+    theirs = torch.optim.AdamW(eager, lr=1e-2, weight_decay=0.1, capturable=True)
+    for step in range(3):
+        _set_grads(eager, 50 + 10 * step)
+        theirs.step()
+    optimizer = cr.AdamW(params)
+    optimizer.load_state_dict(theirs.state_dict())
+    with torch.no_grad():
+        for p, q in zip(params, eager):
+            p.copy_(q)
+    _set_grads(params, 90)
+    graph = _captured(optimizer)
+    for step in range(4):
+        for tensors in (params, eager):
+            _set_grads(tensors, 100 + 10 * step)
+        graph.replay()
+        theirs.step()
+        for p, q in zip(params, eager):  # the steps' own bounds: 8 U of the parameter, 64 U of updates of at most 0.1
+            assert ((p - q).abs() <= (step + 1) * (8 * U * q.abs() + 64 * U * 0.1)).all()
+    assert optimizer.param_groups[0]["step"].item() == 7
+
+
+def test_a_capture_that_would_hold_the_count_is_refused():
+    params = _parameters()
+    optimizer = cr.AdamW(params)
+    _set_grads(params, 10)
+    optimizer.step()
+    optimizer.param_groups[0]["capturable"] = True
+    with pytest.raises(RuntimeError, match="before the capture"):
+        _captured(optimizer)
+    optimizer.step()
+    graph = _captured(optimizer)
+    graph.replay()
+    graph.replay()
+    assert optimizer.param_groups[0]["step"].item() == 4

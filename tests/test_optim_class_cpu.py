@@ -51,3 +51,35 @@ def test_a_refused_step_is_not_counted(ops, capturable):
     ops.refusal = None
     optimizer.step()
     assert [float(s) for s in ops.steps] == [1.0, 2.0] and all(optimizer.state[p]["step"] == 2 for p in params)
+
+
+def _torch_state(params, steps=3, **how):
+    other = torch.optim.AdamW(params, **how)
+    for _ in range(steps):
+        other.step()
+    return other.state_dict()
+
+
+def test_a_loaded_count_is_on_the_device_at_once(ops):
+    # a state without the group's own count, whose next step may be a captured one
+    params = _parameters()
+    state = _torch_state(params)
+    state["param_groups"][0]["capturable"] = True
+    optimizer = cr.AdamW(params, capturable=True)
+    optimizer.load_state_dict(state)
+    count = optimizer.param_groups[0]["step"]
+    assert count.item() == 3
+    optimizer.step()
+    assert optimizer.param_groups[0]["step"] is count and count.item() == 4 and ops.steps[0].item() == 4
+
+
+def test_the_count_starts_at_that_of_the_parameters(ops):
+    params = _parameters()
+    optimizer = cr.AdamW(params)
+    optimizer.step()
+    params[0].grad = None
+    optimizer.step()
+    params[0].grad = torch.ones_like(params[0])
+    optimizer.param_groups[0]["capturable"] = True
+    optimizer.step()  # the group has taken two steps, its first parameter one
+    assert optimizer.param_groups[0]["step"].item() == 3
