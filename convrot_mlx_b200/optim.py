@@ -169,8 +169,15 @@ class AdamW(torch.optim.Optimizer):
         for p, saved in loaded:
             if ("scales" in saved) != (self.state_bits == 8):
                 raise ValueError(f"the state's moments are not kept in {self.state_bits} bits")
-            if self.state_bits == 8 and not _same_layout(saved["exp_avg"], p):
-                raise ValueError("8-bit moments were kept for a parameter of another shape or memory layout")
+            if "step" not in saved or not all(torch.is_tensor(saved.get(name)) for name in ("exp_avg", "exp_avg_sq")):
+                raise ValueError(f"the state has no step, exp_avg and exp_avg_sq, but {sorted(saved)}")
+            for moment in (saved["exp_avg"], saved["exp_avg_sq"]):
+                if self.state_bits == 8 and not _same_layout(moment, p):
+                    raise ValueError("8-bit moments were kept for a parameter of another shape or memory layout")
+                if moment.shape != p.shape:
+                    raise ValueError(f"moments of shape {tuple(moment.shape)} are not those of a parameter of shape {tuple(p.shape)}")
+            if self.state_bits == 8 and tuple(saved["scales"].shape) != (-(-p.numel() // MOMENT_BLOCK), 2):
+                raise ValueError(f"scales of shape {tuple(saved['scales'].shape)} are not those of {p.numel()} 8-bit moments")
         super().load_state_dict(state_dict)
         kind = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
         for p, saved in loaded:  # the moments again, which the base class casts to the parameter's type

@@ -83,3 +83,60 @@ def test_the_count_starts_at_that_of_the_parameters(ops):
     optimizer.param_groups[0]["capturable"] = True
     optimizer.step()  # the group has taken two steps, its first parameter one
     assert optimizer.param_groups[0]["step"].item() == 3
+
+
+def _loads_nothing(optimizer, state, match):
+    params = optimizer.param_groups[0]["params"]
+    kept = {p: {k: v.clone() if torch.is_tensor(v) else v for k, v in optimizer.state[p].items()} for p in params}
+    with pytest.raises(ValueError, match=match):
+        optimizer.load_state_dict(state)
+    for p in params:
+        now = optimizer.state[p]
+        assert now.keys() == kept[p].keys()
+        assert all(torch.equal(v, now[k]) if torch.is_tensor(v) else v == now[k] for k, v in kept[p].items())
+
+
+@pytest.mark.parametrize("shape", [(1,), (30,), (40, 1), (30, 40), (1200,), (2, 40, 30)])
+@pytest.mark.parametrize("name", ["exp_avg", "exp_avg_sq"])
+@pytest.mark.parametrize("of", [0, 1])
+def test_moments_of_other_shapes_are_not_loaded(ops, of, name, shape):
+    # also those that would be broadcast, and those of the last parameter
+    params = _parameters(((40, 30), (40, 30)))
+    state = _torch_state(params)
+    state["state"][of][name] = torch.ones(shape)
+    optimizer = cr.AdamW(params)
+    optimizer.step()
+    _loads_nothing(optimizer, state, "shape")
+
+
+def test_states_of_other_rules_are_not_loaded(ops):
+    params = _parameters()
+    other = torch.optim.SGD(params, lr=0.1, momentum=0.9)
+    other.step()
+    optimizer = cr.AdamW(params)
+    optimizer.step()
+    _loads_nothing(optimizer, other.state_dict(), "exp_avg")
+    state = _torch_state(params)
+    del state["state"][1]["step"]
+    _loads_nothing(optimizer, state, "step")
+
+
+def test_8_bit_states_are_checked_whole(ops):
+    params = _parameters()
+    optimizer = cr.AdamW(params, state_bits=8)
+    optimizer.step()
+
+    def changed(name, value):
+        state = optimizer.state_dict()
+        state["state"] = {k: dict(v) for k, v in state["state"].items()}
+        state["state"][1][name] = value
+        return state
+
+    codes = torch.zeros(300, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    for name in ("exp_avg", "exp_avg_sq"):
+        _loads_nothing(optimizer, changed(name, codes[:299]), "shape or memory layout")
+        _loads_nothing(optimizer, changed(name, torch.zeros(600, dtype=torch.uint8).view(torch.float8_e4m3fn)[::2]), "layout")
+    for shape in ((1, 2), (2,), (2, 1), (300, 2)):
+        _loads_nothing(optimizer, changed("scales", torch.ones(shape)), "scales of shape")
+    optimizer.load_state_dict(changed("scales", torch.full((2, 2), 3.0)))
+    assert optimizer.state[params[1]]["scales"].eq(3).all()
