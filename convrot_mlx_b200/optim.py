@@ -190,6 +190,8 @@ class AdamW(torch.optim.Optimizer):
             self.state[p] = state
         for group in self.param_groups:
             group.setdefault("capturable", False)
+            if torch.is_tensor(group["lr"]):  # wherever the state was kept
+                group["lr"] = group["lr"].to(group["params"][0].device, torch.float32, copy=True)
             if torch.is_tensor(group.get("step")):
                 group["step"] = group["step"].to(group["params"][0].device, torch.float32, copy=True)
             elif group["capturable"] and any(self.state.get(p) for p in group["params"]):

@@ -2,7 +2,7 @@
 
 from __future__ import annotations
 
-import copy
+import io
 
 import pytest
 import torch
@@ -71,3 +71,25 @@ def test_a_capture_that_would_hold_the_count_is_refused():
     graph.replay()
     graph.replay()
     assert optimizer.param_groups[0]["step"].item() == 4
+
+
+def test_a_rate_on_the_device_after_loading_from_the_host():
+    params, others = _parameters(), _parameters()
+    optimizer = cr.AdamW(params, lr=torch.tensor(1e-2, device=dev()), state_bits=8, capturable=True)
+    _set_grads(params, 20)
+    optimizer.step()
+    file = io.BytesIO()
+    torch.save(optimizer.state_dict(), file)
+    file.seek(0)
+    state = torch.load(file, map_location="cpu", weights_only=False)
+    assert state["param_groups"][0]["lr"].device.type == "cpu"
+    loaded = cr.AdamW(others, state_bits=8)
+    loaded.load_state_dict(state)
+    with torch.no_grad():
+        for p, q in zip(params, others):
+            q.copy_(p)
+    for tensors, o in ((params, optimizer), (others, loaded)):
+        _set_grads(tensors, 30)
+        o.step()
+    assert loaded.param_groups[0]["lr"].device == dev()
+    assert all(torch.equal(p, q) for p, q in zip(params, others))
