@@ -158,6 +158,26 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict) -> None:
         """Load a state of this class, or with ``state_bits`` 32 of ``torch.optim.AdamW``; moments keep their types."""
 
+        # The state is taken as the pre-hooks leave it, and in place before any post-hook.  The base class loads the
+        # groups alone: it would cast the moments to the parameters' type.
+        loaded: list = []
+
+        def check(_, state: dict) -> dict:
+            loaded.extend(self._checked(state))
+            ids = {key for group in state["param_groups"] for key in group["params"]}
+            return {**state, "state": {key: rest for key, rest in state["state"].items() if key not in ids}}
+
+        before = self.register_load_state_dict_pre_hook(check)
+        after = self.register_load_state_dict_post_hook(lambda _: self._load(loaded), prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            before.remove()
+            after.remove()
+
+    def _checked(self, state_dict: dict) -> list:
+        """The parameters that have a state in ``state_dict``, each with it; refused as a whole."""
+
         for group in state_dict["param_groups"]:
             if group.get("amsgrad") or group.get("maximize"):
                 raise ValueError("this AdamW has neither amsgrad nor maximize")
@@ -178,9 +198,12 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError(f"moments of shape {tuple(moment.shape)} are not those of a parameter of shape {tuple(p.shape)}")
             if self.state_bits == 8 and tuple(saved["scales"].shape) != (-(-p.numel() // MOMENT_BLOCK), 2):
                 raise ValueError(f"scales of shape {tuple(saved['scales'].shape)} are not those of {p.numel()} 8-bit moments")
-        super().load_state_dict(state_dict)
+        return loaded
+
+    @torch.no_grad()
+    def _load(self, loaded: list) -> None:
         kind = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
-        for p, saved in loaded:  # the moments again, which the base class casts to the parameter's type
+        for p, saved in loaded:
             state = {"step": int(saved["step"])}
             for name in ("exp_avg", "exp_avg_sq"):
                 # the parameter's own layout, whatever that of the saved tensor was
@@ -190,6 +213,8 @@ class AdamW(torch.optim.Optimizer):
             self.state[p] = state
         for group in self.param_groups:
             group.setdefault("capturable", False)
+            if not group["params"]:
+                continue
             if torch.is_tensor(group["lr"]):  # wherever the state was kept
                 group["lr"] = group["lr"].to(group["params"][0].device, torch.float32, copy=True)
             if torch.is_tensor(group.get("step")):

@@ -140,3 +140,52 @@ def test_8_bit_states_are_checked_whole(ops):
         _loads_nothing(optimizer, changed("scales", torch.ones(shape)), "scales of shape")
     optimizer.load_state_dict(changed("scales", torch.full((2, 2), 3.0)))
     assert optimizer.state[params[1]]["scales"].eq(3).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_loading_heeds_the_hooks(ops, bits):
+    params = _parameters()
+    optimizer = cr.AdamW(params, state_bits=bits)
+    optimizer.step()
+    saved = optimizer.state_dict()
+    seen = []
+
+    def twice(_, state):  # counts changed on the way in, in a dictionary of the hook's own
+        return {**state, "state": {k: {**v, "step": 2 * v["step"]} for k, v in state["state"].items()}}
+
+    def look(o):
+        seen.append({k: v if k == "step" else v.dtype for k, v in o.state[params[0]].items()})
+
+    hooks = [optimizer.register_load_state_dict_pre_hook(twice), optimizer.register_load_state_dict_post_hook(look)]
+    optimizer.load_state_dict(saved)
+    kind = torch.float32 if bits == 32 else torch.float8_e4m3fn
+    want = {"step": 2, "exp_avg": kind, "exp_avg_sq": kind, **({"scales": torch.float32} if bits == 8 else {})}
+    assert seen == [want] and all(optimizer.state[p]["step"] == 2 for p in params)
+    assert all(v["step"] == 1 for v in saved["state"].values())
+    for hook in hooks:
+        hook.remove()
+    optimizer.load_state_dict(saved)  # and the class leaves none of its own
+    assert optimizer.state[params[0]]["step"] == 1 and len(seen) == 1
+    with pytest.raises(ValueError, match="different"):
+        optimizer.load_state_dict({**saved, "param_groups": saved["param_groups"] * 2})
+    assert optimizer.state[params[0]]["step"] == 1
+
+
+def test_loading_keeps_no_copy_in_another_type(ops):
+    # 8-bit moments of a float32 parameter are loaded as they are: no tensor of four times their size on the way
+    params = _parameters(((1 << 16,),))
+    optimizer = cr.AdamW(params, state_bits=8)
+    optimizer.step()
+    saved = optimizer.state_dict()
+    with torch.profiler.profile(profile_memory=True) as profile:
+        optimizer.load_state_dict(saved)
+    largest = max(event.self_cpu_memory_usage for event in profile.events())
+    assert largest < 4 * (1 << 16), largest
+
+
+def test_a_group_without_parameters_is_loaded(ops):
+    params = _parameters()
+    optimizer = cr.AdamW([dict(params=params), dict(params=[])], lr=torch.tensor(1e-2))
+    optimizer.step()
+    optimizer.load_state_dict(optimizer.state_dict())
+    assert optimizer.state[params[0]]["step"] == 1 and optimizer.param_groups[0]["lr"].item() == torch.tensor(1e-2).item()
