@@ -127,6 +127,9 @@ class AdamW(torch.optim.Optimizer):
                 return loss
             sums = ops.square_sums(grads)
         for group in self.param_groups:
+            if not group["capturable"] and torch.is_tensor(group.get("step")):  # it was until now
+                self._read_counts(group)
+                del group["step"]
             runs: dict = {}  # the parameters by their step, nearly always one
             for p in group["params"]:
                 if p.grad is not None:
@@ -154,6 +157,22 @@ class AdamW(torch.optim.Optimizer):
                     state["step"] += 1
         self.last_norm = norm
         return loss
+
+    def _read_counts(self, group: dict) -> None:
+        """The count on the device, which replays of a captured step advance, as that of the group's parameters."""
+
+        count = int(group["step"].item())
+        for p in group["params"]:
+            if self.state.get(p):
+                self.state[p]["step"] = count
+
+    def state_dict(self) -> dict:
+        """The state, under the names of ``torch.optim.AdamW``; counts that are on the device are read back."""
+
+        for group in self.param_groups:
+            if torch.is_tensor(group.get("step")):
+                self._read_counts(group)
+        return super().state_dict()
 
     def load_state_dict(self, state_dict: dict) -> None:
         """Load a state of this class, or with ``state_bits`` 32 of ``torch.optim.AdamW``; moments keep their types."""

@@ -189,3 +189,29 @@ def test_a_group_without_parameters_is_loaded(ops):
     optimizer.step()
     optimizer.load_state_dict(optimizer.state_dict())
     assert optimizer.state[params[0]]["step"] == 1 and optimizer.param_groups[0]["lr"].item() == torch.tensor(1e-2).item()
+
+
+def test_counts_of_replays_are_saved(ops):
+    params = _parameters()
+    optimizer = cr.AdamW(params, capturable=True)
+    optimizer.step()
+    optimizer.param_groups[0]["step"].add_(6.0)  # as six replays of a captured step do
+    state = optimizer.state_dict()
+    assert [v["step"] for v in state["state"].values()] == [7, 7] and state["param_groups"][0]["step"].item() == 7
+    other = torch.optim.AdamW(params)  # whose steps would be corrected for it
+    state["param_groups"][0]["capturable"] = False
+    other.load_state_dict(state)
+    assert all(int(other.state[p]["step"]) == 7 for p in params)
+
+
+def test_the_count_goes_back_to_the_parameters(ops):
+    params = _parameters()
+    optimizer = cr.AdamW(params, capturable=True)
+    optimizer.step()
+    optimizer.param_groups[0]["step"].add_(6.0)
+    optimizer.param_groups[0]["capturable"] = False
+    optimizer.step()
+    assert ops.steps[-1] == 8 and optimizer.state[params[0]]["step"] == 8
+    optimizer.param_groups[0]["capturable"] = True
+    optimizer.step()
+    assert ops.steps[-1].item() == 9
