@@ -708,6 +708,17 @@ Tensor sums_of(const GradLists& lists, const Tensor& like) {
 }
 Tensor square_sums_of(const std::vector<const Tensor*>& grads) { return sums_of(GradLists(grads), *grads.front()); }
 
+void write_norm(const Tensor& sums, float* to) {
+  check(convrot_norm_of_sums(static_cast<const double*>(sums.data_ptr()), sums.numel(), to, stream_of(sums)),
+        "convrot_norm_of_sums");
+}
+Tensor norm_of(const Tensor& sums) {
+  const c10::cuda::OptionalCUDAGuard guard(sums.device());
+  const Tensor norm = at::empty({}, sums.options().dtype(at::kFloat));
+  write_norm(sums, static_cast<float*>(norm.data_ptr()));
+  return norm;
+}
+
 std::vector<const Tensor*> present(const TensorList& list) {
   std::vector<const Tensor*> out;
   out.reserve(list.size());
@@ -746,9 +757,7 @@ Tensor grad_norm(const py::object& grads) {
       return norm;
     }
   }
-  const Tensor sums = sums_of(lists, first);
-  check(convrot_norm_of_sums(static_cast<const double*>(sums.data_ptr()), sums.numel(), to, stream_of(sums)),
-        "convrot_norm_of_sums");
+  write_norm(sums_of(lists, first), to);
   return norm;
 }
 
@@ -807,6 +816,7 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
   std::vector<convrot_adamw_tensor> by_type[3];
   std::vector<const void*> addresses;
   std::vector<const Tensor*> used, written;
+  const Tensor* given = nullptr;  // a gradient, with values or without
   std::vector<Tensor> held;
   addresses.reserve(3 * count);
   for (auto& list : by_type) list.reserve(count);
@@ -816,6 +826,7 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
   for (int64_t i = 0; i < count; ++i) {
     const Tensor* gi = g.at(i);
     if (!gi) continue;
+    given = gi;
     const Tensor *pi = p.at(i), *mi = m.at(i), *vi = v.at(i), *si = eight ? s.at(i) : mi;
     if (!pi || !mi || !vi || !si) refuse("parameter ", i, " has a gradient, but a parameter, moment or scale is missing");
     if (used.empty()) home = pi->device();
@@ -857,8 +868,10 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
   if (!distinct(addresses)) refuse("a parameter or a moment occurs twice in one AdamW step");
   convrot_adamw_options o = {};
   if (used.empty()) {
-    if (max_norm) refuse("clipping needs at least one gradient");
-    return std::nullopt;
+    if (!max_norm) return std::nullopt;
+    if (!given) refuse("clipping needs at least one gradient");
+    if (sums_in.has_value()) return norm_of(*sums_in);
+    return at::zeros({}, given->options().dtype(at::kFloat).requires_grad(false));  // of no values
   }
   o.step_device = device_scalar(step, "step", home, &o.step);
   o.lr_device = device_scalar(lr, "learning rate", home, &o.lr);

@@ -93,3 +93,27 @@ def test_a_rate_on_the_device_after_loading_from_the_host():
         o.step()
     assert loaded.param_groups[0]["lr"].device == dev()
     assert all(torch.equal(p, q) for p, q in zip(params, others))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_groups_and_steps_of_empty_parameters_are_clipped_too(bits):
+    params, alone = _parameters(), _parameters()
+    empty = [torch.nn.Parameter(torch.zeros((0, 4), device=dev()))]
+    optimizer = cr.AdamW([dict(params=params), dict(params=empty)], state_bits=bits, max_norm=0.5)
+    other = cr.AdamW(alone, state_bits=bits, max_norm=0.5)
+    for step in range(2):
+        for tensors in (params, alone, empty):
+            _set_grads(tensors, 40 + step)
+        optimizer.step()
+        other.step()
+        assert optimizer.last_norm.item() == other.last_norm.item() > 0.5
+        assert all(torch.equal(p, q) for p, q in zip(params, alone))
+        assert optimizer.state[params[0]]["step"] == optimizer.state[empty[0]]["step"] == step + 1
+    only = cr.AdamW(empty, state_bits=bits, max_norm=0.5)
+    only.step()
+    assert only.last_norm.shape == () and only.last_norm.item() == 0
+    p = empty[0].detach()
+    assert cr.adamw_step([p], [p], [p], [p], None, 1, lr=1.0, max_norm=1.0).item() == 0
+    assert cr.adamw_step([p], [p], [p], [p], None, 1, lr=1.0) is None
+    with pytest.raises(ValueError, match="at least one gradient"):
+        cr.adamw_step([p], [None], [p], [p], None, 1, lr=1.0, max_norm=1.0)
