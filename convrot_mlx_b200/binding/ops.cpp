@@ -781,19 +781,111 @@ const float* device_scalar(const py::object& o, const char* what, const c10::Dev
   return static_cast<const float*>(t.data_ptr());
 }
 
-// Whether no address occurs twice (0 aside).
-bool distinct(const std::vector<const void*>& addresses) {
-  size_t size = 64;
-  while (size < 2 * addresses.size()) size *= 2;
-  std::vector<const void*> table(size, nullptr);
-  for (const void* a : addresses) {
-    size_t i = (reinterpret_cast<uintptr_t>(a) >> 2) * 0x9E3779B97F4A7C15ull >> 20 & (size - 1);
-    for (; table[i]; i = (i + 1) & (size - 1))
-      if (table[i] == a) return false;
-    table[i] = a;
+// The tensors of a step in memory: a parameter's gradient may be itself (or its
+// moments), whose values are read before they are written, and two parameters
+// may have one gradient, but nothing that is written may overlap anything else.
+class Spans {
+ public:
+  enum Kind { kParam, kMoment, kRoot, kScales, kGrad, kKinds };
+
+  explicit Spans(int64_t count) { storages_.reserve(kKinds * count); }
+
+  // A tensor whose values are dense in memory; a parameter's own tensors after it.
+  void add(Kind kind, const Tensor& t, const void* at, int64_t bytes) {
+    const auto start = reinterpret_cast<uintptr_t>(at);
+    Range& range = ranges_[kind];
+    range.ascending &= start >= range.end;
+    if (!range.end) range.first = start;
+    range.end = start + bytes;
+    // the lowest bit: only read
+    storages_.push_back(reinterpret_cast<uintptr_t>(t.unsafeGetTensorImpl()->unsafe_storage().data()) & ~uintptr_t(1) |
+                        (kind == kGrad));
   }
-  return true;
-}
+
+  // by_type: the same tensors.
+  bool disjoint(const std::vector<convrot_adamw_tensor> (&by_type)[3], bool eight) const {
+    return in_order() || in_storages_of_their_own() || swept(by_type, eight);
+  }
+
+ private:
+  struct Range {
+    uintptr_t first = 0, end = 0;
+    bool ascending = true;
+  };
+  struct Span {
+    uintptr_t at, end;
+    int64_t index;  // of the parameter
+  };
+
+  // Each kind in a stretch of memory of its own, one tensor after another: packed buffers.
+  bool in_order() const {
+    for (int i = 0; i < kKinds; ++i) {
+      if (!ranges_[i].ascending) return false;
+      for (int j = 0; j < i; ++j)
+        if (ranges_[i].first < ranges_[j].end && ranges_[j].first < ranges_[i].end) return false;
+    }
+    return true;
+  }
+
+  // Tensors allocated one by one, whatever their order.
+  bool in_storages_of_their_own() const {
+    size_t size = 64;
+    while (2 * size < 3 * storages_.size()) size *= 2;
+    std::vector<uintptr_t> table(size, 0);
+    for (const uintptr_t storage : storages_) {
+      const uintptr_t base = storage & ~uintptr_t(1);
+      size_t i = (base >> 4) * 0x9E3779B97F4A7C15ull >> 20 & (size - 1);
+      for (; table[i]; i = (i + 1) & (size - 1))
+        if ((table[i] & ~uintptr_t(1)) == base && !(table[i] & storage & 1)) return false;
+      table[i] = storage;
+    }
+    return true;
+  }
+
+  // In the order of their starts, what is written first: spans that are written
+  // may not overlap, so the last of them is the only one that reaches on.
+  static bool swept(const std::vector<convrot_adamw_tensor> (&by_type)[3], bool eight) {
+    std::vector<Span> spans[kKinds];
+    int64_t index = 0;
+    for (int type = 0; type < 3; ++type) {
+      const int64_t e = type == CONVROT_F32 ? 4 : 2, moment = eight ? 1 : 4;
+      for (const convrot_adamw_tensor& t : by_type[type]) {
+        auto add = [&](Kind kind, const void* at, int64_t bytes) {
+          const auto start = reinterpret_cast<uintptr_t>(at);
+          spans[kind].push_back({start, start + bytes, index});
+        };
+        add(kParam, t.param, e * t.numel);
+        add(kMoment, t.exp_avg, moment * t.numel);
+        add(kRoot, t.exp_avg_sq, moment * t.numel);
+        if (eight) add(kScales, t.scales, (t.numel + 255) / 256 * 8);
+        add(kGrad, t.grad, e * t.numel);
+        ++index;
+      }
+    }
+    for (auto& list : spans) std::sort(list.begin(), list.end(), [](const Span& a, const Span& b) { return a.at < b.at; });
+    size_t next[kKinds] = {};
+    Span written{0, 0, -1};
+    uintptr_t read_end = 0;
+    for (;;) {
+      int kind = -1;
+      for (int k = 0; k < kKinds; ++k)
+        if (next[k] < spans[k].size() && (kind < 0 || spans[k][next[k]].at < spans[kind][next[kind]].at)) kind = k;
+      if (kind < 0) return true;
+      const Span& s = spans[kind][next[kind]++];
+      if (kind == kGrad) {
+        const bool own = s.index == written.index && s.at == written.at && s.end == written.end;
+        if (s.at < written.end && !own) return false;
+        read_end = std::max(read_end, s.end);
+      } else {
+        if (s.at < written.end || s.at < read_end) return false;
+        written = s;
+      }
+    }
+  }
+
+  std::vector<uintptr_t> storages_;
+  Range ranges_[kKinds];
+};
 
 // The step; with max_norm the gradients' norm, else nothing.  sums: of
 // square_sums, where the norm is over more gradients than these.
@@ -814,11 +906,10 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
   if (max_norm && !(*max_norm >= 0)) refuse("the largest norm must be non-negative, got ", *max_norm);
   const at::ScalarType moment = eight ? at::kFloat8_e4m3fn : at::kFloat;
   std::vector<convrot_adamw_tensor> by_type[3];
-  std::vector<const void*> addresses;
   std::vector<const Tensor*> used, written;
   const Tensor* given = nullptr;  // a gradient, with values or without
   std::vector<Tensor> held;
-  addresses.reserve(3 * count);
+  Spans spans(count);
   for (auto& list : by_type) list.reserve(count);
   used.reserve(count);
   written.reserve(count);
@@ -859,13 +950,20 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
     }
     if (n == 0) continue;
     void *const p_at = pi->data_ptr(), *const m_at = mi->data_ptr(), *const v_at = vi->data_ptr();
-    by_type[dtype_slot(*pi)].push_back(
-        {p_at, grad->const_data_ptr(), m_at, v_at, eight ? static_cast<float*>(si->data_ptr()) : nullptr, n});
-    for (const void* at : {p_at, m_at, v_at}) addresses.push_back(at);
+    const void* g_at = grad->const_data_ptr();
+    auto* s_at = eight ? static_cast<float*>(si->data_ptr()) : nullptr;
+    by_type[dtype_slot(*pi)].push_back({p_at, g_at, m_at, v_at, s_at, n});
+    const int64_t bytes = n * pi->element_size(), moment_bytes = n * (eight ? 1 : 4);
+    spans.add(Spans::kParam, *pi, p_at, bytes);
+    spans.add(Spans::kMoment, *mi, m_at, moment_bytes);
+    spans.add(Spans::kRoot, *vi, v_at, moment_bytes);
+    if (eight) spans.add(Spans::kScales, *si, s_at, 8 * blocks);
+    spans.add(Spans::kGrad, *grad, g_at, bytes);
     used.push_back(gi);
     written.push_back(pi);
   }
-  if (!distinct(addresses)) refuse("a parameter or a moment occurs twice in one AdamW step");
+  if (!spans.disjoint(by_type, eight))
+    refuse("a parameter, a moment or its scales overlaps another tensor of the step (or occurs twice)");
   convrot_adamw_options o = {};
   if (used.empty()) {
     if (!max_norm) return std::nullopt;

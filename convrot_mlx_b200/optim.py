@@ -48,7 +48,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     it is replayed.  ``max_norm``: gradients are scaled by
     min(1, max_norm / (norm + 1e-6)) as they are read, with the norm of them all, which
     is returned.  Gradients are not changed.  A parameter that is not contiguous has to be dense, with
-    its moments laid out as it is."""
+    its moments laid out as it is.  Parameters, moments and scales may not overlap one another or another's gradient."""
 
     return _native.ops().adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales, step, lr, betas[0], betas[1], eps,
                                     weight_decay, max_norm, None)
