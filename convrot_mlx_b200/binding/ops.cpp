@@ -912,7 +912,7 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
   Spans spans(count);
   for (auto& list : by_type) list.reserve(count);
   used.reserve(count);
-  written.reserve(count);
+  written.reserve(4 * count);
   c10::Device home(c10::DeviceType::CPU);
   for (int64_t i = 0; i < count; ++i) {
     const Tensor* gi = g.at(i);
@@ -960,7 +960,8 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
     if (eight) spans.add(Spans::kScales, *si, s_at, 8 * blocks);
     spans.add(Spans::kGrad, *grad, g_at, bytes);
     used.push_back(gi);
-    written.push_back(pi);
+    written.insert(written.end(), {pi, mi, vi});
+    if (eight) written.push_back(si);
   }
   if (!spans.disjoint(by_type, eight))
     refuse("a parameter, a moment or its scales overlaps another tensor of the step (or occurs twice)");
@@ -995,7 +996,7 @@ std::optional<Tensor> adamw_step(const py::object& params, const py::object& gra
                         stream_of(*written.front())),
           "convrot_adamw");
   }
-  for (const Tensor* t : written)
+  for (const Tensor* t : written)  // autograd is to see it
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return norm;
 }

@@ -117,3 +117,23 @@ def test_groups_and_steps_of_empty_parameters_are_clipped_too(bits):
     assert cr.adamw_step([p], [p], [p], [p], None, 1, lr=1.0) is None
     with pytest.raises(ValueError, match="at least one gradient"):
         cr.adamw_step([p], [None], [p], [p], None, 1, lr=1.0, max_norm=1.0)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_autograd_sees_every_tensor_that_is_written(bits):
+    params = _parameters()
+    optimizer = cr.AdamW(params, state_bits=bits)
+    _set_grads(params, 60)
+    optimizer.step()
+    tensors = [t for p in params for t in (p, *optimizer.state[p].values()) if torch.is_tensor(t)]
+    assert len(tensors) == len(params) * (4 if bits == 8 else 3)
+    before, grads = [t._version for t in tensors], [p.grad._version for p in params]
+    optimizer.step()
+    assert all(t._version > v for t, v in zip(tensors, before))
+    assert grads == [p.grad._version for p in params]
+    if bits == 32:  # a moment that a graph has saved
+        x = torch.ones((40, 30), device=dev(), requires_grad=True)
+        y = (x * optimizer.state[params[0]]["exp_avg"]).sum()
+        optimizer.step()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
