@@ -26,7 +26,9 @@
 // moments the instructions weigh as much as the memory (390 a warp and 256
 // values, issue 67% active): arithmetic is on pairs, one chunk ahead is in
 // registers (a ring in shared memory filled by cp.async: 550 instead of 454 us,
-// IEEE division and root: 1210).
+// IEEE division and root: 1210).  Roots of subnormal v are a branch of their own
+// (roots_of_any): looking for them takes 1% with 8-bit moments and 16-bit values,
+// nothing otherwise.
 #include "rows.cuh"
 
 namespace convrot {
@@ -178,13 +180,12 @@ __device__ __forceinline__ float rsqrt_approx(float x) {
   return r;
 }
 
-// Square roots: s = v y with y = 1 / sqrt(v) is what divides: 0 has 0 and an
-// infinite v an infinite s, no update.  (v below 2^-126 has too small a root,
-// but eps is what divides there.)
+// Square roots of v from 2^-126 on: s = v y with y = 1 / sqrt(v) is what divides;
+// an infinite v has an infinite s, no update.  roots_of_any takes the others.
+constexpr float kLow = 0x1p-126f, kHigh = 0x1.fffffep127f;
 __device__ __forceinline__ P2 root_of(P2 v, P2& y) {
-  constexpr float kLow = 0x1p-126f, kHigh = 0x1.fffffep127f;
   const float2 f = p2_get(v);
-  y = p2(rsqrt_approx(fminf(fmaxf(f.x, kLow), kHigh)), rsqrt_approx(fminf(fmaxf(f.y, kLow), kHigh)));
+  y = p2(rsqrt_approx(fminf(f.x, kHigh)), rsqrt_approx(fminf(f.y, kHigh)));
   return mul(v, y);
 }
 // What is kept in 8 bits is s after one step of Newton's iteration on s * s = v,
@@ -193,6 +194,25 @@ __device__ __forceinline__ P2 root_of(P2 v, P2& y) {
 __device__ __forceinline__ P2 refined_root(P2 v, P2 y, P2 s) {
   const P2 half_residual = mul(fma(mul(s, p2(-1.0f, -1.0f)), s, v), p2(0.5f, 0.5f));
   return fma(half_residual, y, s);
+}
+// Both of any v: a subnormal one as 2^64 times it, whose root is 2^32 times the
+// root; 0 has 0.  Of all others the same bits as above.
+__device__ __forceinline__ void roots_of_any(P2 v, P2& s, P2& refined) {
+  const float2 f = p2_get(v);
+  const bool x = f.x < kLow, y = f.y < kLow;
+  const P2 down = p2(x ? 0x1p-32f : 1.0f, y ? 0x1p-32f : 1.0f);
+  const float2 up = p2_get(mul(v, p2(x ? 0x1p64f : 1.0f, y ? 0x1p64f : 1.0f)));
+  P2 inverse;
+  root_of(p2(fmaxf(up.x, kLow), fmaxf(up.y, kLow)), inverse);
+  v = p2(up.x, up.y);
+  s = mul(v, inverse);
+  refined = mul(refined_root(v, inverse, s), down);
+  s = mul(s, down);
+}
+__device__ __forceinline__ float smaller(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // A paired product and a paired sum may be compiled to one operation with one
@@ -411,16 +431,30 @@ __global__ void __launch_bounds__(kThreads, kCtas<T, BITS>) adamw_kernel(const _
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) g[i] = mul(g[i], coef2);
     }
+    float least = kHigh;
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
       m[i] = sum_of(mul(m[i], beta1), mul(g[i], rest1));
       v[i] = sum_of(mul(v[i], beta2), mul(mul(g[i], g[i]), rest2));
-      P2 y;
-      r[i] = root_of(v[i], y);
-      const float2 den = p2_get(fma(r[i], root2, eps));
-      if constexpr (BITS == 8) r[i] = refined_root(v[i], y, r[i]);
-      p[i] = fma(mul(m[i], minus_step), p2(rcp_approx(den.x), rcp_approx(den.y)), mul(p[i], decay2));
+      const float2 f = p2_get(v[i]);
+      least = smaller(least, f.x, f.y);
     }
+    auto update = [&](auto any) {
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        P2 s, y;
+        if constexpr (any.value) {
+          roots_of_any(v[i], s, r[i]);
+        } else {
+          s = root_of(v[i], y);
+          if constexpr (BITS == 8) r[i] = refined_root(v[i], y, s);
+        }
+        const float2 den = p2_get(fma(s, root2, eps));
+        p[i] = fma(mul(m[i], minus_step), p2(rcp_approx(den.x), rcp_approx(den.y)), mul(p[i], decay2));
+      }
+    };
+    if (least < kLow) update(std::true_type{});  // zeros too
+    else update(std::false_type{});
     Pack<T, kLane> out;
     out.set_lanes(p);
     uint32_t m_words[kLane * sizeof(M) / 4], v_words[kLane * sizeof(M) / 4];
