@@ -221,12 +221,6 @@ Tensor int8_linear(const Tensor& x, const Tensor& qweight, const Tensor& wscales
 
 constexpr int64_t kSpan = 128;  // values of a row, rows and columns of a weight, that share a scale
 
-// Channels whose products one float32 output sums on the tensor core.  It adds
-// 32 products at a time and cuts what is below the sum's last bit, so its error
-// grows with their number: to 2e-6 of the result over 15360 channels, 8e-7 over
-// 8000.  No 16-bit output shows that; float32 outputs are summed in ranges.
-constexpr int64_t kMaxSum = 8192;
-
 // The quantizer and the product in one call; n columns out.
 Tensor fp8_product(const Tensor& x, const Tensor& qweight, int layout, const Tensor& wscales, const Tensor& bias,
                    int64_t n) {
@@ -244,24 +238,9 @@ Tensor fp8_product(const Tensor& x, const Tensor& qweight, int layout, const Ten
   const auto* weight = static_cast<const uint8_t*>(qweight.data_ptr());
   const auto* ws = static_cast<const uint8_t*>(wscales.data_ptr());
   const auto* b = static_cast<const float*>(address(bias));
-  if (dtype != CONVROT_F32 || k <= kMaxSum) {
-    check(convrot_fp8_linear(r.data_ptr(), dtype, r.stride(0), weight, qweight.stride(0), layout, ws, wscales.size(1), b,
-                             out.data_ptr(), dtype, m, n, k, codes, pitch, scales, scales_pitch, stream_of(x)),
-          "convrot_fp8_linear");
-    return out;
-  }
-  check(convrot_quantize_fp8(r.data_ptr(), dtype, m, k, r.stride(0), codes, pitch, scales, scales_pitch, stream_of(x)),
-        "convrot_quantize_fp8");
-  const bool nk = layout == CONVROT_LAYOUT_NK;
-  for (int64_t at = 0; at < k; at += kMaxSum) {
-    const Tensor part = at ? at::empty(shape, x.options()) : out;
-    const int64_t block = at / kSpan;
-    check(convrot_fp8_gemm(codes + at, pitch, scales + block, scales_pitch, weight + (nk ? at : at * qweight.stride(0)),
-                           qweight.stride(0), layout, ws + (nk ? block : block * wscales.size(1)), wscales.size(1),
-                           at ? nullptr : b, part.data_ptr(), dtype, m, n, std::min(kMaxSum, k - at), stream_of(x)),
-          "convrot_fp8_gemm");
-    if (at) out.add_(part);
-  }
+  check(convrot_fp8_linear(r.data_ptr(), dtype, r.stride(0), weight, qweight.stride(0), layout, ws, wscales.size(1), b,
+                           out.data_ptr(), dtype, m, n, k, codes, pitch, scales, scales_pitch, stream_of(x)),
+        "convrot_fp8_linear");
   return out;
 }
 

@@ -45,7 +45,16 @@ struct Params {
   // the weight copies may be issued before the previous kernel of the stream
   // has completed (it only writes the activation)
   int early_weights;
+  int add;  // float32 outputs: to what `out` holds
 };
+
+// Channels whose products one float32 output sums on the tensor core.  It adds
+// 32 products at a time and cuts what is below the sum's last bit, so its error
+// grows with their number: 5e-7 of the outputs' norm over 8192 channels, 1.1e-6
+// over 15360, 3e-6 over 32768.  No 16-bit output shows that; float32 outputs of
+// the tile kernels are summed in ranges, one launch after another, and the
+// ranges in order (5e-7 over 32768).
+constexpr int kMaxSum = 8192;
 
 // tcgen05 instruction descriptor of kind::mxf8f6f4 with D float32: A and B e4m3
 // (format 0), A M-major for amn, B N-major for bmn, scales ue8m0 (bit 23).  The
@@ -387,6 +396,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int u = 0; u < 4; ++u) v[j + u] = __fadd_rn(__uint_as_float(r[j + u]), bv[u]);
         }
+        if constexpr (sizeof(TOut) == 4) {
+          if (p.add && row0 + lane < p.m) {
+            const float* held = static_cast<const float*>(p.out) + static_cast<int64_t>(row0 + lane) * p.n + col0 + c * 32;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col0 + c * 32 + j < p.n) v[j] = __fadd_rn(held[j], v[j]);
+          }
+        }
         store_rows(v, stage_out + ew * kChunkBytes, static_cast<TOut*>(p.out), row0, col0 + c * 32, p.m, p.n);
       }
       tc_fence_before();
@@ -622,6 +639,13 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = __fadd_rn(__uint_as_float(r[i]), b);
       TOut* dst = out + static_cast<int64_t>(m0 + c) * p.n + n;
+      if constexpr (sizeof(TOut) == 4) {
+        if (p.add) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (i < rows - c && n_ok) v[i] = __fadd_rn(dst[static_cast<int64_t>(i) * p.n], v[i]);
+        }
+      }
       if (rows - c >= 16 && n_ok) {
 #pragma unroll
         for (int i = 0; i < 16; ++i, dst += p.n) *dst = cvt_out<TOut>(v[i]);
@@ -655,6 +679,13 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = __fadd_rn(sum[i], b[i]);
       TOut* dst = out + static_cast<int64_t>(m0 + c) * p.n + n;
+      if constexpr (sizeof(TOut) == 4) {
+        if (p.add) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n + i < p.n) v[i] = __fadd_rn(dst[i], v[i]);
+        }
+      }
       if (whole) {
         Pack<TOut, 4> pk;
         pk.set(v);
@@ -905,7 +936,11 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_kernel(const GemvParams q) {
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) v = __fadd_rn(v, part[turn][w][m][threadIdx.x % kChannels]);
       if (p.bias) v = __fadd_rn(v, ld_f32(p.bias + n));
-      static_cast<TOut*>(p.out)[static_cast<int64_t>(m) * p.n + n] = cvt_out<TOut>(v);
+      TOut* dst = static_cast<TOut*>(p.out) + static_cast<int64_t>(m) * p.n + n;
+      if constexpr (sizeof(TOut) == 4) {
+        if (p.add) v = __fadd_rn(*dst, v);
+      }
+      *dst = cvt_out<TOut>(v);
     }
     set += gridDim.x;
     turn ^= 1;
@@ -1058,7 +1093,7 @@ double swap_time(const Params& p, int bt, int sms, int* ranks) {
 }
 
 template <int LAYOUT, typename TOut>
-int launch(const Operands& o, const Params& p, cudaStream_t s) {
+int launch_range(const Operands& o, const Params& p, cudaStream_t s) {
   const int sms = device_sm_count();
   if (gemv_takes(LAYOUT, p.m, p.k)) {
     const gemv::GemvParams q{p, nullptr, o.act, o.weight, 0, o.act_stride, o.weight_stride};
@@ -1074,6 +1109,25 @@ int launch(const Operands& o, const Params& p, cudaStream_t s) {
     case 64: return launch_swap<LAYOUT, TOut, 64>(o, p, ranks, s);
     default: return launch_swap<LAYOUT, TOut, 128>(o, p, ranks, s);
   }
+}
+
+template <int LAYOUT, typename TOut>
+int launch(const Operands& o, const Params& p, cudaStream_t s) {
+  // the GEMV sums each block from 0, whatever K
+  if (sizeof(TOut) < 4 || p.k <= kMaxSum || gemv_takes(LAYOUT, p.m, p.k)) return launch_range<LAYOUT, TOut>(o, p, s);
+  for (int at = 0; at < p.k; at += kMaxSum) {
+    Operands part = o;
+    part.act += at;
+    part.weight += LAYOUT == CONVROT_LAYOUT_NK ? at : at * o.weight_stride;
+    Params q = p;
+    q.xscales += at / kSpan;
+    q.wscales += at / kSpan * p.ws_k;
+    q.k = std::min(kMaxSum, p.k - at);
+    if (at) q.bias = nullptr, q.early_weights = 0, q.add = 1;
+    const int rc = launch_range<LAYOUT, TOut>(part, q, s);
+    if (rc != CONVROT_OK) return rc;
+  }
+  return CONVROT_OK;
 }
 
 struct Call {
@@ -1122,7 +1176,7 @@ int by_layout(const Call& c, const Params& p, cudaStream_t s) {
 Params params_of(const Call& c, int* err_word, bool early_weights) {
   const bool nk = c.layout == CONVROT_LAYOUT_NK;
   return {c.xscales, c.wscales, c.xs_stride, nk ? c.ws_stride : 1, nk ? 1 : c.ws_stride, c.bias, c.out,
-          static_cast<int>(c.m), static_cast<int>(c.n), static_cast<int>(c.k), err_word, early_weights ? 1 : 0};
+          static_cast<int>(c.m), static_cast<int>(c.n), static_cast<int>(c.k), err_word, early_weights ? 1 : 0, 0};
 }
 
 int run(const Call& c, bool early_weights, cudaStream_t s) {

@@ -424,9 +424,11 @@ int convrot_quantize_fp8_weight(const void* w, int dtype, int64_t rows, int64_t 
  * lies, rows of them at wscales_stride bytes.  Scales are the bytes of the
  * quantizers above.  Row strides of codes are multiples of 16 and cover the
  * rows, and the rows are read in whole 16 bytes, the last one too (what is
- * behind its end is not used); m, n and k are below 2^22.  bias may be NULL (zeros).  The order of
- * the sums is fixed by the shape, the layout and the number of SMs.  No
- * reference counterpart.
+ * behind its end is not used); m, n and k are below 2^22.  bias may be NULL (zeros).  A float32
+ * output over more than 8192 k is summed in ranges of that many, one launch
+ * after another, except where up to 8 tokens of layout NK fit one launch that
+ * adds up blocks.  The order of the sums is fixed by the shape, the layout and the
+ * number of SMs.  No reference counterpart.
  */
 int convrot_fp8_gemm(const uint8_t* act, int64_t act_stride, const uint8_t* xscales, int64_t xscales_stride,
                      const uint8_t* weight, int64_t weight_stride, int layout, const uint8_t* wscales,
