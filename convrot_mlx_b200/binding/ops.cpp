@@ -263,7 +263,8 @@ struct Fp8LinearBackward : torch::autograd::Node {
     once("fp8_linear");
     const std::lock_guard<std::mutex> lock(mutex_);
     if (!grads[0].defined()) return {Tensor()};
-    const Tensor w = qweight.unpack(), ws = wscales.unpack();
+    // hooks of saved tensors may have packed the rows
+    const Tensor w = whole_rows(qweight.unpack()), ws = wscales.unpack().contiguous();
     return {fp8_product(grads[0], w, CONVROT_LAYOUT_KN, ws, {}, w.size(1))};
   }
   void release_variables() override {
