@@ -188,7 +188,7 @@ struct Int8Linear : torch::autograd::Function<Int8Linear> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("int8_linear");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &qweight = saved[0], &wscales = saved[1];
+    const Tensor qweight = padded_rows(saved[0]), wscales = saved[1].contiguous();  // hooks may have packed the rows
     if (qweight.size(0) > kMaxDot) return {i8_gradient_in_ranges(grads[0], wscales, qweight), {}, {}, {}};
     return {i8_product(grads[0], wscales, qweight, CONVROT_LAYOUT_KN, {}, {}, qweight.size(1)), {}, {}, {}};
   }

@@ -11,7 +11,7 @@ from tests.ops64 import DTYPES, randn
 
 pytestmark = pytest.mark.gpu
 
-OPS = {"fp8": (cr.fp8_linear, cr.quantize_fp8_weight)}
+OPS = {"fp8": (cr.fp8_linear, cr.quantize_fp8_weight), "int8": (cr.int8_linear, cr.quantize_int8_weight)}
 
 
 def _apart(t):  # the same values, every stride doubled and the start off any boundary
@@ -44,3 +44,14 @@ def test_gradient_of_a_weight_that_was_moved(op, m, k, n, dtype, hook):
         (dx,) = torch.autograd.grad(y, x, dy, retain_graph=True)
         assert torch.equal(dx, want)
     assert_no_device_error()
+
+
+@pytest.mark.parametrize("hook", list(HOOKS))
+def test_int8_gradient_in_ranges_of_a_weight_that_was_moved(hook):
+    n, k = 131100, 35
+    w, ws = cr.quantize_int8_weight(randn((n, k), torch.float32, 11))
+    x, dy = randn((9, k), torch.bfloat16, 12).requires_grad_(), randn((9, n), torch.bfloat16, 13)
+    (want,) = torch.autograd.grad(cr.int8_linear(x, w, ws), x, dy)
+    with HOOKS[hook]():
+        y = cr.int8_linear(x, w, ws)
+    assert torch.equal(torch.autograd.grad(y, x, dy)[0], want)
