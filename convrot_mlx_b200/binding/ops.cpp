@@ -370,7 +370,7 @@ struct AxialRotary : torch::autograd::Function<AxialRotary> {
     how.interleaved = ctx->saved_data["interleaved"].toBool();
     const Tensor dk = grads.size() > 1 ? grads[1] : Tensor();
     if (!grads[0].defined() && !dk.defined()) return {{}, {}, {}, {}};
-    const auto [gq, gk] = turn(grads[0], dk, ctx->get_saved_variables()[0], how, true,
+    const auto [gq, gk] = turn(grads[0], dk, ctx->get_saved_variables()[0].contiguous(), how, true,
                                ctx->saved_data["heads_inside"].toBool());
     return {gq, gk, {}, {}};
   }
@@ -462,9 +462,14 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     once("layer_norm");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3];
+    // as forward had them, also where hooks of saved tensors have laid them out in another way
+    const Tensor x = saved[0].contiguous(), stats = saved[3].contiguous();
+    Tensor weight = saved[1];
+    const Tensor& bias = saved[2];
     const c10::cuda::OptionalCUDAGuard guard(x.device());
     const NormHow how{ctx->saved_data["segments"].toInt(), ctx->saved_data["add_one"].toBool(), 0.0};
+    if (weight.defined() && (weight.stride(-1) != 1 || (how.segments > 1 && weight.stride(0) < x.size(-1))))
+      weight = weight.contiguous();
     const Tensor dy = grads[0].contiguous();
     const int64_t features = x.size(-1), rows = x.numel() / features, per = std::max<int64_t>(1, rows / how.segments);
     const Tensor dx = at::empty_like(x);
@@ -596,7 +601,8 @@ struct GeluSaved8 : torch::autograd::Function<GeluSaved8> {
     const Tensor dx = at::empty_like(dy);
     const int64_t features = dy.size(-1), rows = dy.numel() / features;
     if (rows == 0) return {dx};
-    const Tensor saved = ctx->get_saved_variables()[0];
+    Tensor saved = ctx->get_saved_variables()[0].contiguous();
+    if (reinterpret_cast<uintptr_t>(saved.data_ptr()) % 16) saved = saved.clone();  // its scales are float32
     const auto* codes = static_cast<const int8_t*>(saved.data_ptr());
     const auto* scales = reinterpret_cast<const float*>(codes + Saved(rows, features).scales_at);
     check(convrot_gelu_saved8_backward(dy.data_ptr(), dtype_code(dy.scalar_type()), rows, features, codes, scales,
