@@ -1161,9 +1161,10 @@ int check_call(const Call& c) {
                   static_cast<long long>(c.xs_stride), static_cast<long long>(c.ws_stride));
   if (c.m == 0) return CONVROT_OK;
   CONVROT_REQUIRE(c.o.act && c.o.weight && c.xscales && c.wscales && c.out, CONVROT_ERR_INVALID, "null pointer");
-  CONVROT_REQUIRE(aligned_to(c.o.act, 16) && aligned_to(c.o.weight, 16) && aligned_to(c.out, 16) && aligned_to(c.xscales, 4),
+  CONVROT_REQUIRE(aligned_to(c.o.act, 16) && aligned_to(c.o.weight, 16) && aligned_to(c.out, 16) &&
+                      aligned_to(c.xscales, 4) && aligned_to(c.bias, 4),
                   CONVROT_ERR_INVALID,
-                  "activation, weight and output must be 16-byte aligned, the activation's scales 4-byte aligned");
+                  "activation, weight and output must be 16-byte aligned, the activation's scales and the bias 4-byte aligned");
   return CONVROT_OK;
 }
 

@@ -288,6 +288,8 @@ int convrot_gelu_saved8(const void* x, int dtype, int64_t rows, int64_t features
   const int rc = check_shape(dtype, rows, features);
   if (rc != CONVROT_OK || rows == 0) return rc;
   CONVROT_REQUIRE(x && y && (codes != nullptr) == (scales != nullptr), CONVROT_ERR_INVALID, "null pointer");
+  CONVROT_REQUIRE(aligned_to(x, dtype_size(dtype)) && aligned_to(y, dtype_size(dtype)) && aligned_to(scales, 4),
+                  CONVROT_ERR_INVALID, "tensors must be aligned to their elements");
   const GeluParams p = params(x, y, codes, scales, rows, features);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
@@ -303,6 +305,8 @@ int convrot_gelu_saved8_backward(const void* dy, int dtype, int64_t rows, int64_
   const int rc = check_shape(dtype, rows, features);
   if (rc != CONVROT_OK || rows == 0) return rc;
   CONVROT_REQUIRE(dy && dx && codes && scales, CONVROT_ERR_INVALID, "null pointer");
+  CONVROT_REQUIRE(aligned_to(dy, dtype_size(dtype)) && aligned_to(dx, dtype_size(dtype)) && aligned_to(scales, 4),
+                  CONVROT_ERR_INVALID, "tensors must be aligned to their elements");
   const GeluParams p =
       params(dy, dx, const_cast<int8_t*>(codes), const_cast<float*>(scales), rows, features);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -727,8 +727,8 @@ int convrot_square_sums(int64_t count, const convrot_grad_tensor* tensors, int d
                         float* norm, void* stream) {
   using namespace convrot;
   CONVROT_REQUIRE(valid_dtype(dtype), CONVROT_ERR_INVALID, "unknown dtype %d", dtype);
-  CONVROT_REQUIRE(count >= 0 && (count == 0 || tensors) && (sums || norm) && aligned_to(sums, 8) && sums_count > 0 &&
-                      sums_count <= (1 << 20),
+  CONVROT_REQUIRE(count >= 0 && (count == 0 || tensors) && (sums || norm) && aligned_to(sums, 8) && aligned_to(norm, 4) &&
+                      sums_count > 0 && sums_count <= (1 << 20),
                   CONVROT_ERR_INVALID, "invalid tensor list or sums");
   CONVROT_REQUIRE(!norm || (sums_count <= 8 && count <= optim::kNormLarge), CONVROT_ERR_INVALID,
                   "the norm takes at most 8 sums of at most %d tensors", optim::kNormLarge);
@@ -746,7 +746,8 @@ int convrot_square_sums(int64_t count, const convrot_grad_tensor* tensors, int d
 
 int convrot_norm_of_sums(const double* sums, int64_t sums_count, float* norm, void* stream) {
   using namespace convrot;
-  CONVROT_REQUIRE(sums && norm && sums_count > 0 && sums_count <= (1 << 24), CONVROT_ERR_INVALID, "invalid sums");
+  CONVROT_REQUIRE(sums && norm && aligned_to(sums, 8) && aligned_to(norm, 4) && sums_count > 0 && sums_count <= (1 << 24),
+                  CONVROT_ERR_INVALID, "invalid sums");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(1, 1, 1);
   cfg.blockDim = dim3(optim::kThreads, 1, 1);
@@ -773,6 +774,9 @@ int convrot_adamw(int64_t count, const convrot_adamw_tensor* tensors, int dtype,
                   "the step counts from 1 and the learning rate is non-negative");
   CONVROT_REQUIRE(!o->sums || (o->sums_count > 0 && o->sums_count <= (1 << 24) && o->max_norm >= 0), CONVROT_ERR_INVALID,
                   "clipping needs sums of squares and a non-negative norm");
+  CONVROT_REQUIRE(aligned_to(o->step_device, 4) && aligned_to(o->lr_device, 4) && aligned_to(o->norm, 4) &&
+                      aligned_to(o->sums, 8),
+                  CONVROT_ERR_INVALID, "step, rate, norm and sums must be aligned to their elements");
   for (int64_t i = 0; i < count; ++i) {
     const convrot_adamw_tensor& t = tensors[i];
     const uintptr_t e = dtype_size(dtype), moment = state_bits == 8 ? 1 : 4;
