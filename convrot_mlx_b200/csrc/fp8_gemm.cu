@@ -802,6 +802,18 @@ __device__ __forceinline__ float scale_of(uint32_t byte) {
   return __uint_as_float(byte == 255u ? 0x7FC00000u : byte == 0u ? 0x00400000u : byte << 23);
 }
 
+// Of two scales; NaN where one is.
+__device__ __forceinline__ float lesser(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float greater(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <typename TOut, bool FUSED>
 __global__ void __launch_bounds__(kThreads, 2) gemv_kernel(const GemvParams q) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -863,8 +875,12 @@ __global__ void __launch_bounds__(kThreads, 2) gemv_kernel(const GemvParams q) {
           const float ws = scale_of(s.scale[i]);
           const float x0 = 2 * t < p.m ? xs[2 * t * k_blocks + block] : 0.0f;
           const float x1 = 2 * t + 1 < p.m ? xs[(2 * t + 1) * k_blocks + block] : 0.0f;
+          // The smaller scale first: a sum of codes, a multiple of 2^-18 below 2^25,
+          // times it is exact however small it is, and too large only where the
+          // result is.
+          const float lo[2] = {lesser(ws, x0), lesser(ws, x1)}, hi[2] = {greater(ws, x0), greater(ws, x1)};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j] = __fmaf_rn(__fmul_rn(sum[j], ws), j & 1 ? x1 : x0, acc[j]);
+          for (int j = 0; j < 4; ++j) acc[j] = __fmaf_rn(__fmul_rn(sum[j], lo[j & 1]), hi[j & 1], acc[j]);
         }
         const int n0 = at_n * kChannels;
         // channels past the last are read as the last, and not written
