@@ -47,4 +47,6 @@ def test_scales_that_are_nan_beside_small_and_large_ones(m):
             y = cr.fp8_matmul(codes, qweight, xs.view(torch.float8_e8m0fnu), ws.view(torch.float8_e8m0fnu),
                               output_dtype=torch.float32)
             assert torch.isnan(y[m - 1]).all()
-            assert which == "w" or not torch.isnan(y[:m - 1]).any()
+            # A weight's scale of 2^127 takes blocks to 2^16 * 2^127 * 2^-8 and more, beyond float32: each is infinite, and two
+            # of opposite signs make a NaN that is not the scale's.
+            assert which == "w" or byte == 254 or not torch.isnan(y[:m - 1]).any()
