@@ -85,7 +85,8 @@ def make_optimizer(kind: str, params, lr: float):
 
     if kind == "adam":
         return torch.optim.Adam(params, lr=lr)
-    return cr.AdamW(params, lr=lr, weight_decay=0.0, state_bits={"adamw32": 32, "adamw8": 8}[kind], max_norm=1.0)
+    how = {"adamw32": dict(state_bits=32), "adamw8": dict(state_bits=8, betas=(0.9, 0.95))}[kind]
+    return cr.AdamW(params, lr=lr, weight_decay=0.0, max_norm=1.0, **how)
 
 
 def train(steps: int, width: int, heads: int, batch: int, frames: int, rows: int, cols: int, device="cuda",

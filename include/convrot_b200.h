@@ -471,8 +471,9 @@ int convrot_norm_of_sums(const double* sums, int64_t sums_count, float* norm, vo
  * one launch for each 512 of them; `tensors` is a host array.  state_bits 32:
  * exp_avg and exp_avg_sq are float32 (m and v).  state_bits 8: they are e4m3
  * codes of m and of sqrt(v), and scales holds {scale of m, scale of sqrt(v)}
- * for each 256 values of the tensor, float32; a block that is not finite gets
- * scales NaN.  Values are taken in memory order, so a tensor and its moments
+ * for each 256 values of the tensor, float32; codes are rounded to nearest, which
+ * roots follow their averages with for beta2 up to 0.95; a block that is not
+ * finite gets scales NaN.  Values are taken in memory order, so a tensor and its moments
  * have to be laid out alike.  step counts from 1; step_device and lr_device, where not NULL, are
  * one float32 each on the device and take the place of step and lr (for a
  * captured step).  With sums (of convrot_square_sums) gradients are scaled by
