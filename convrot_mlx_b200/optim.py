@@ -101,17 +101,16 @@ class AdamW(torch.optim.Optimizer):
         return {**super().__getstate__(), "state_bits": self.state_bits, "max_norm": self.max_norm, "last_norm": None}
 
     def _start(self, p: torch.Tensor) -> dict:
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW starts its moments in its first step: take one before the capture")
+        keep = torch.preserve_format
+        kind = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
         state = self.state[p]
-        if not state:
-            if p.is_cuda and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("AdamW starts its moments in its first step: take one before the capture")
-            keep = torch.preserve_format
-            kind = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
-            state["step"] = 0
-            state["exp_avg"] = torch.zeros_like(p, dtype=kind, memory_format=keep)
-            state["exp_avg_sq"] = torch.zeros_like(p, dtype=kind, memory_format=keep)
-            if self.state_bits == 8:
-                state["scales"] = torch.zeros((-(-p.numel() // MOMENT_BLOCK), 2), dtype=torch.float32, device=p.device)
+        state["step"] = 0
+        state["exp_avg"] = torch.zeros_like(p, dtype=kind, memory_format=keep)
+        state["exp_avg_sq"] = torch.zeros_like(p, dtype=kind, memory_format=keep)
+        if self.state_bits == 8:
+            state["scales"] = torch.zeros((-(-p.numel() // MOMENT_BLOCK), 2), dtype=torch.float32, device=p.device)
         return state
 
     def _put_count_on_device(self, group: dict) -> None:
@@ -139,14 +138,15 @@ class AdamW(torch.optim.Optimizer):
             if not group["capturable"] and torch.is_tensor(group.get("step")):  # it was until now
                 self._read_counts(group)
                 del group["step"]
+            capturable = group["capturable"]
             runs: dict = {}  # the parameters by their step, nearly always one
             for p in group["params"]:
                 if p.grad is not None:
-                    if p.is_cuda and not group["capturable"] and torch.cuda.is_current_stream_capturing():
+                    if not runs and not capturable and p.is_cuda and torch.cuda.is_current_stream_capturing():
                         raise RuntimeError("a captured AdamW step needs capturable=True: its count has to be on the device")
-                    state = self._start(p)
-                    runs.setdefault(0 if group["capturable"] else state["step"] + 1, []).append((p, state))
-            if runs and group["capturable"]:
+                    state = self.state[p] or self._start(p)
+                    runs.setdefault(0 if capturable else state["step"] + 1, []).append((p, state))
+            if runs and capturable:
                 if not torch.is_tensor(group.get("step")):
                     self._put_count_on_device(group)
                 group["step"].add_(1.0)
@@ -156,10 +156,10 @@ class AdamW(torch.optim.Optimizer):
                     norm = ops.adamw_step([p for p, _ in run], [p.grad for p, _ in run], [s["exp_avg"] for s in states],
                                           [s["exp_avg_sq"] for s in states],
                                           [s["scales"] for s in states] if self.state_bits == 8 else None,
-                                          group["step"] if group["capturable"] else step, group["lr"], *group["betas"],
+                                          group["step"] if capturable else step, group["lr"], *group["betas"],
                                           group["eps"], group["weight_decay"], self.max_norm, sums)
                 except (ValueError, NotImplementedError):  # refused: not a step
-                    if group["capturable"]:
+                    if capturable:
                         group["step"].sub_(1.0)
                     raise
                 for state in states:
