@@ -18,8 +18,10 @@
 // for products that fill the GPU with tiles of 256 x 256, swap_kernel between.
 // Times of the product alone, weights from HBM, bf16 out (tokens x K x channels,
 // us): 1 x 5120 x 5120 10.6 (26 MB; 4.0 at a copy's bandwidth), 8 x 5120 x 5120
-// 12.9, 40 x 5120 x 5120 14.1, 451 x 2203 x 1301 13.0, 1536 x 5120 x 5120 46,
-// 4096 x 3072 x 12288 142, 7800 x 5120 x 13824 480 (2300 TFLOP/s), 8192^3 458.
+// 13.4, 40 x 5120 x 5120 14.2, 451 x 2203 x 1301 13.0, 1536 x 5120 x 5120 46,
+// 4096 x 3072 x 12288 142, 7800 x 5120 x 13824 480 (2300 TFLOP/s), 8192^3 458; for
+// the gradient, whose few tokens the GEMV does not take, 1 x 5120 x 5120 12.0, 8
+// 12.6, 40 14.3.
 #include <algorithm>
 
 #include "fp8.cuh"
@@ -143,6 +145,11 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t bar_cluster
 // Tensor memory has 512 columns: two accumulators of 256 that share 32, and
 // two sets of scales of 12 (4 for the tokens, 8 for the channels).  The epilogue
 // reads the shared columns first, and with them free the next tile may begin.
+// In loops of two seconds, which the power limit holds at 1.52 to 1.57 GHz for this
+// kernel and the integer one alike: 8192^3 547 us (at 1552 MHz; the integer kernel
+// 437 at 1522), 7800 x 5120 x 13824 569 (1567; 465 at 1545).  So it takes 1.28 and
+// 1.24 times the integer kernel's cycles, the copies of scales among them, and
+// the clock takes the rest of what a call's loop has over a short run's.
 // ===========================================================================
 namespace pair {
 

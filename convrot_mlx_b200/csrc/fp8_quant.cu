@@ -13,7 +13,7 @@
 // copy's 6.6; 23.9 with a select and a product for each value instead of paired
 // products), 1536 x 5120 in 3.9, 451 x 2203, whose rows start at any byte pair and
 // are read value by value, in 2.5.  Weights: blocks of 128 x 128, a CTA each, once
-// for a layer (13824 x 5120 in 52 us with cold caches).
+// for a layer (13824 x 5120 in 32.5 us, 6.5 TB/s).
 #include "fp8.cuh"
 
 namespace convrot {

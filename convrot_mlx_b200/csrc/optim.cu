@@ -24,7 +24,7 @@
 // values at a time, 8 a lane, so the maximum over a block of 8-bit moments is one
 // exchange in the warp.  A CTA's 2048 values are of one tensor, so that all that
 // depends on the tensor is the same in its threads and costs no instruction of
-// theirs.  Times of the step: 246M bf16 values with 8-bit moments 444 us (5.6
+// theirs.  Times of the step: 246M bf16 values with 8-bit moments 452 us (5.5
 // TB/s of a copy's 6.6), 62M float32 ones in 640 tensors with 8-bit moments 185
 // (5.5), 113M float32 with 32-bit moments 510 (6.2), six vectors 1.9.  With 8-bit
 // moments the instructions weigh as much as the memory (390 a warp and 256
@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, kCtas<T, BITS>) adamw_kernel(const _
 // cluster (a call of 3.9 us, 7.2 as two launches).  A thread adds 32 squares in
 // float32, in four sums of eight and these in pairs, and the total to a 64-bit
 // one; where a sum of eight leaves the range of float32 (not finite, or so small
-// that squares may have been lost) the squares are formed in 64 bits.  Each CTA
+// that squares may have been lost, zeros too) the squares are formed in 64 bits.  Each CTA
 // writes one sum, of a share that depends on the sizes alone.
 
 struct NormEntry {
@@ -658,11 +658,11 @@ int adamw_part(const Scalars& s, const convrot_adamw_tensor* tensors, int count,
   const int64_t most = kCtas<T, BITS> * static_cast<int64_t>(device_sm_count()), ctas = chunks < most ? chunks : most;
   if (chunks > most * count) {
     // large tensors: in the order of the CTAs (246M values in 6 tensors, 8-bit
-    // moments: 434 us, 453 in contiguous shares)
+    // moments: 452 us, 460 in contiguous shares; 113M in 16, 32-bit: 508, 518)
     t.s.share = 1, t.s.span = t.s.chunks, t.s.step_by = static_cast<uint32_t>(ctas);
   } else {
     // tensors that a step over the grid would pass by: in contiguous shares
-    // (62M values in 640: 227 us, 249)
+    // (62M values in 640, 8-bit moments: 185 us, 187)
     t.s.share = t.s.span = static_cast<uint32_t>((chunks + ctas - 1) / ctas), t.s.step_by = 1;
   }
   return launch(adamw_kernel<T, BITS, CAP>, ctas, t, stream, "adamw step");

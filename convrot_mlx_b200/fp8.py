@@ -99,8 +99,9 @@ def fp8_matmul(codes, qweight, xscales, wscales, bias=None, *, output_dtype) -> 
     """The product of ``codes`` (m, k) and ``qweight`` (n, k) transposed, each code times its block's scale, plus bias.
 
     Arguments as ``quantize_fp8_blockwise`` and ``quantize_fp8_weight`` give
-    them; sums are float32, rounded once to ``output_dtype``.  Rows that do not
-    start where the kernel can read them are copied first."""
+    them; sums are float32, rounded once to ``output_dtype`` (float32 outputs over more
+    than 8192 channels are summed in ranges).  Rows that do not start where the kernel can
+    read them are copied first.  No gradients: ``fp8_linear`` has them."""
 
     for t, what in ((codes, "activation"), (qweight, "weight")):
         if t.ndim != 2 or t.dtype != CODES:
